@@ -353,6 +353,58 @@ int xdna_qwen3_stack(const xdna_qwen3_layer* layers, int n_layers, const float* 
                      const int32_t* lens, const uint8_t* mask, int mask_heads, void* out, int out_dtype, int64_t ldo,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ generation
+ * From prompts to the next token (no reference counterpart: the reference answers with the logits of whole
+ * sequences). Head dimensions 64 and 128, bf16 or f16, any number of query heads per key head up to 128;
+ * strides are in elements, positive multiples of 8, bases 16-byte aligned. */
+
+/* Causal attention over packed sequences: out [tokens, hq, d] (contiguous) of q [tokens, hq, d], k and v
+ * [tokens, hkv, d] with the strides *_st of a token and *_sh of a head. Sequence i is the tokens
+ * cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (n_seqs + 1 ascending device words); a token attends to the tokens of its
+ * sequence up to itself. Words outside [0, tokens] or out of order are clamped; tokens of no sequence give zeros.
+ * scale > 0. workspace: xdna_packed_attention_workspace bytes, 256-byte aligned. */
+size_t xdna_packed_attention_workspace(int64_t n_seqs, int64_t tokens, int64_t hq, int64_t hkv);
+int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                          const void* v, int64_t v_st, int64_t v_sh, const int32_t* cu_seqlens, int64_t n_seqs,
+                          int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int dtype, float scale, void* out,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* One decode step's attention of B sequences that share a prefix: out [B, hq, d] (contiguous), row b's softmax over
+ * the P prefix keys pk / pv [P, hkv, d] and the first lens[b] (clamped to 0..S) of its own ck / cv [B, S, hkv, d].
+ * A row without any key gives zeros. workspace: xdna_prefix_attention_workspace bytes, 256-byte aligned. */
+size_t xdna_prefix_attention_workspace(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d);
+int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* pk, int64_t pk_st, int64_t pk_sh,
+                          const void* pv, int64_t pv_st, int64_t pv_sh, const void* ck, int64_t ck_sb, int64_t ck_st,
+                          int64_t ck_sh, const void* cv, int64_t cv_sb, int64_t cv_st, int64_t cv_sh,
+                          const int32_t* lens, int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d,
+                          int dtype, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* 4-bit weights. A weight [N, K] is codes [N, K' / 2] bytes (K' = K rounded up to 128, padded with code 8) and
+ * scales [N, ceil(K / group)] (bf16 or f16; group 32, 64 or 128): w = (code - 8) * scale. A block of 128 columns is
+ * 16 little-endian 32-bit words; the word at place 4 t + w holds columns 32 w + 8 t .. + 7, in the order
+ * 0, 2, 4, 6, 1, 3, 5, 7 from the lowest four bits. xdna_w4_pack quantises w (f32 / bf16 / f16, row pitch ldw):
+ * scale = max |w| of the group / 7, code = clamp(rint(w / scale), -8, 7) + 8. */
+int xdna_w4_pack(const void* w, int w_dtype, int64_t N, int64_t K, int64_t ldw, int group, uint8_t* codes,
+                 void* scales, int scale_dtype, void* stream);
+
+/* y [M, N] = x [M, K] . w^T (+ bias) for such a weight, f32 sums, rounded once to x's type (f32 / bf16 / f16). */
+int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* codes,
+                   const void* scales, int scale_dtype, int group, int64_t N, const void* bias, int bias_dtype,
+                   void* y, int64_t ldy, void* stream);
+
+/* The logits [B, V] of the next token after penalties, bias and mask, in f32 rounded once to their type. For
+ * row b and token v, with `seen` = v is among the row's first lens[b] of tokens [B, T] (32 or 64-bit; ids outside
+ * [0, V) count for nothing) and c = how often it is among those from prompt_lens[b] on:
+ *   l = seen ? (l > 0 ? l / repetition[b] : l * repetition[b]) : l;  l -= frequency[b] * c + (c > 0) * presence[b];
+ *   l += bias[b * ld_bias + v] (ld_bias 0: one for all rows);  l = bit v of mask[b * ld_mask + v / 32] ? l : -inf.
+ * Each of tokens, lens (then T), prompt_lens (then 0), repetition, presence, frequency, bias and mask may be NULL.
+ * out may be logits. */
+int xdna_process_logits(const void* logits, int dtype, int64_t B, int64_t V, int64_t ld_in, const void* tokens,
+                        int token_bytes, int64_t T, int64_t ld_tokens, const int32_t* lens,
+                        const int32_t* prompt_lens, const float* repetition, const float* presence,
+                        const float* frequency, const float* bias, int64_t ld_bias, const uint32_t* mask,
+                        int64_t ld_mask, void* out, int64_t ld_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,6 +87,15 @@ def _load():
         "xdna_ipc_handle": ([P, P], I),
         "xdna_ipc_open": ([P, P], I),
         "xdna_ipc_close": ([P], I),
+        "xdna_packed_attention_workspace": ([I64, I64, I64, I64], ctypes.c_size_t),
+        "xdna_packed_attention": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I64, I64, I64, I,
+                                   ctypes.c_float, P, P, ctypes.c_size_t, P], I),
+        "xdna_prefix_attention_workspace": ([I64, I64, I64, I64, I64, I64], ctypes.c_size_t),
+        "xdna_prefix_attention": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64,
+                                   I64, I64, I64, I64, I64, I, ctypes.c_float, P, P, ctypes.c_size_t, P], I),
+        "xdna_w4_pack": ([P, I, I64, I64, I64, I, P, P, I, P], I),
+        "xdna_linear_w4": ([P, I, I64, I64, I64, P, P, I, I, I64, P, I, P, I64, P], I),
+        "xdna_process_logits": ([P, I, I64, I64, I64, P, I, I64, I64, P, P, P, P, P, P, I64, P, I64, P, I64, P], I),
         "xdna_attention": ([P, P, I64, P, I64, I64, I, P, P, I, P], I),
         "xdna_qwen3_stack_workspace": ([I64, I64], ctypes.c_size_t),
         "xdna_qwen3_stack": ([P, I, P, P, I64, P, I, P, P, ctypes.c_float, P, I64, I64, I, P, P, I, P, I, I64, P,

@@ -8,13 +8,14 @@ conv3x3_int8 as one op, because on the B200 those three steps are kernels of our
 graph ops for the CPU compiler to fuse; xdna::conv3x3_chain, the same for a conv inside a chain of
 convs whose activations between them stay int8 codes; and xdna::conv_int8, the same arithmetic for the
 1x1 and stride-2 convs the reference has no kernel for (offloaded with Config(conv_ext=True)).
+The ops at the end are the generation operators (generate.py), which the reference does not have.
 """
 
 from typing import Optional
 
 import torch
 
-from . import conv, runtime, stack
+from . import conv, generate, runtime, stack
 
 _configs = []  # cfg_id -> Config; op arguments must be plain values (R:torch_xdna/ops.py:14-22)
 
@@ -149,3 +150,56 @@ def qwen3_stack(x: torch.Tensor, mask: torch.Tensor, stack_id: int, cfg_id: int)
 @qwen3_stack.register_fake
 def _(x, mask, stack_id, cfg_id):
     return x.new_empty(*x.shape[:-1], stack.out_features(stack_id))
+
+
+# ------------------------------------------------------------------ generation (generate.py)
+@torch.library.custom_op("xdna::packed_attention", mutates_args=())
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention over packed sequences (generate.packed_attention)."""
+    return generate.packed_attention(q, k, v, cu_seqlens, scale)
+
+
+@packed_attention.register_fake
+def _(q, k, v, cu_seqlens, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("xdna::shared_prefix_attention", mutates_args=())
+def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, cache_lens: torch.Tensor,
+                            scale: Optional[float] = None) -> torch.Tensor:
+    """A decode step's attention for a batch that shares a prefix (generate.shared_prefix_attention)."""
+    return generate.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
+
+
+@shared_prefix_attention.register_fake
+def _(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("xdna::linear_w4", mutates_args=())
+def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int,
+              bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x times a 4-bit weight transposed (generate.linear_w4)."""
+    return generate.linear_w4(x, codes, scales, group, bias)
+
+
+@linear_w4.register_fake
+def _(x, codes, scales, group, bias=None):
+    return x.new_empty(*x.shape[:-1], codes.shape[0])
+
+
+@torch.library.custom_op("xdna::process_logits", mutates_args=())
+def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, lens: Optional[torch.Tensor] = None,
+                   prompt_lens: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                   presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Penalties, bias and grammar mask on the next token's logits (generate.process_logits)."""
+    return generate.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
+
+
+@process_logits.register_fake
+def _(logits, tokens=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None, bias=None,
+      mask=None):
+    return logits.new_empty(logits.shape)
