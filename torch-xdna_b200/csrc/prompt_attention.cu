@@ -6,28 +6,33 @@
 //   prefix   o[b, h]: the same softmax over all P prefix keys and the first lens[b] keys of b's own cache
 //
 // A row with no keys at all is zero.
+//
+// Both read their long axis through one tcgen05 kernel (tile_attention_kernel). The G query heads that share a key
+// head are packed into the rows of a tile: row r is token r / G, head r % G, so a tile of 128 rows holds 128 / G
+// tokens (rounded down) and K and V are read once for all of them. An item is two such tiles (A and B) against a
+// run of key blocks of 128; the kernel is persistent, one CTA per SM, and its roles run across item boundaries:
+//   warp 0      TMA: both Q tiles per item, then K and V blocks in turn into one ring (K_j, V_j, K_j+1, ...). V is
+//               taken as it lies in memory, keys by dimensions: the MN-major B operand of the second product.
+//   warp 1      the MMAs, one thread:  S_A(0) S_B(0) | O_A += P_A(j) V(j), S_A(j+1) | O_B += P_B(j) V(j), S_B(j+1) | ...
+//               While one tile's softmax works, the tensor core does the other's two products.
+//   warps 2..5  softmax of tile A, warps 6..9 of tile B; thread = row. S is read from TMEM once, p = 2^(s - m) is
+//               written as 16 bits over S's own columns and is the A operand of the second product straight from
+//               TMEM, so P costs no shared-memory bandwidth (of which both products together need all there is when
+//               P goes through it). The next S is issued after that product, in order, so it may overwrite P.
+//               The running max m is raised, and O and l rescaled, only when a block exceeds it by more than 2^8.
+//               m, l, O are f32; p is rounded to the operands' type because the tensor core takes one type for both
+//               (its relative error, half an ulp, is that of the output's own rounding).
+// TMEM: S_A | S_B | O_A | O_B, 128 columns each. Shared memory: Q 2 x 128 x D, and as many 128 x D blocks as fit.
+//
+// Keys that are masked for some rows of a tile but not for others carry p = 0; if their V holds an infinity or a NaN
+// the product is NaN. Rows that end non-finite are therefore computed again one by one over exactly their own keys
+// (recompute_row), so that nothing outside a row's keys reaches it.
+#include <algorithm>
+
 #include "host_util.h"
 #include "sm100.cuh"
 
 namespace xdna {
-
-struct PackedArgs {
-  const void *q, *k, *v;
-  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // strides of a token and of a head, in elements
-  const int32_t* cu;
-  int n_seqs, T, hq, hkv;
-  float scale_log2;
-  void* out;
-};
-
-struct PrefixArgs {
-  const void *q, *pk, *pv, *ck, *cv;
-  int64_t q_sb, q_sh, pk_st, pk_sh, pv_st, pv_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh;
-  const int32_t* lens;
-  int B, P, S, hq, hkv;
-  float scale_log2;
-  void* out;
-};
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T x);
@@ -41,68 +46,599 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-
-// One row's running softmax, D / 32 dimensions per lane.
-template <typename T, int D>
-struct Row {
-  float q[D / 32], o[D / 32], m, l;
-  __device__ void init(const T* qp, float sc) {
-    for (int i = 0; i < D / 32; ++i) {
-      q[i] = to_f32(qp[i * 32 + lane_id()]) * sc;
-      o[i] = 0.f;
-    }
-    m = -INFINITY;
-    l = 0.f;
-  }
-  __device__ void key(const T* kp, const T* vp) {
-    float s = 0.f;
-    for (int i = 0; i < D / 32; ++i) s += q[i] * to_f32(kp[i * 32 + lane_id()]);
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s);
-    const float a = exp2f(m - mn), p = exp2f(s - mn);
-    m = mn;
-    l = l * a + p;
-    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * a + p * to_f32(vp[i * 32 + lane_id()]);
-  }
-  __device__ void store(T* dst) const {
-    for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane_id()] = from_f32<T>(l > 0.f ? o[i] / l : 0.f);
-  }
-};
-
-template <typename T, int D>
-__global__ void __launch_bounds__(256) packed_kernel(const PackedArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp_id();
-  if (row >= static_cast<int64_t>(a.T) * a.hq) return;
-  const int t = static_cast<int>(row / a.hq), h = static_cast<int>(row % a.hq), hk = h / (a.hq / a.hkv);
-  int lo = 0, hi = a.n_seqs;  // the last sequence that starts at or before t
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (mid < a.n_seqs && a.cu[mid] <= t) lo = mid; else hi = mid - 1;
-  }
-  Row<T, D> r;
-  r.init(static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh, a.scale_log2);
-  if (a.n_seqs > 0 && t < a.cu[lo + 1])
-    for (int s = max(a.cu[lo], 0); s <= t; ++s)
-      r.key(static_cast<const T*>(a.k) + s * a.k_st + hk * a.k_sh, static_cast<const T*>(a.v) + s * a.v_st + hk * a.v_sh);
-  r.store(static_cast<T*>(a.out) + row * D);
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+enum TileMode { PACKED = 0, PREFIX = 1 };
+
+// What the plan of a packed call says (workspace): a header, then the tile pairs, those with the most key blocks
+// first: {first token, first token of the sequence, end of the sequence, 0}.
+struct PlanHeader {
+  int n_pairs, first, end, pad;  // tokens [0, first) and [end, T) belong to no sequence
+};
+
+struct TileArgs {
+  int hq, hkv, group, tok;  // tok: tokens per tile
+  float scale_log2;
+  int* err;
+  void* out;
+  // PACKED
+  const PlanHeader* plan;  // null: one sequence, cu read here
+  const int32_t* cu;
+  int T;
+  const void *q, *k, *v;  // recompute_row
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  // PREFIX
+  int B, P, pairs, splits, blocks_per_split;
+  float* part_o;   // [split][B * hq][D]
+  float2* part_ml; // [split][B * hq]: m (log2 units), l
+};
+
+constexpr int kTaThreads = 320;
+constexpr int kTaBlock = 128;
+constexpr float kTaRescale = 8.0f;
+
+template <int D>
+struct TaShape {
+  static constexpr int kKB = D / 64;                    // 64-column k-blocks of a row
+  static constexpr int kTile = 128 * D * 2;             // bytes of a Q tile, a K block or a V block
+  static constexpr int kStages = D == 128 ? 5 : 8;      // K / V blocks in the ring
+  static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 256;
+};
+
+struct TileItem {
+  int q_tok, kvh, kv_tok;  // first token of tile A, key head, first key (TMA coordinates)
+  int nb[2];               // key blocks of tiles A and B
+  int len, q_pos;          // PACKED: sequence length, tile A's first place in it
+  int split;               // PREFIX
+};
+
+// One row over exactly its keys [0, n), a warp with D / 32 dimensions per lane.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_kernel(const PrefixArgs a) {
+__device__ __noinline__ void recompute_row(const T* q, const T* k, int64_t k_st, const T* v, int64_t v_st, int n,
+                                           float sc, T* dst) {
+  float qr[D / 32], o[D / 32], m = -INFINITY, l = 0.f;
+  for (int i = 0; i < D / 32; ++i) {
+    qr[i] = to_f32(q[i * 32 + lane_id()]) * sc;
+    o[i] = 0.f;
+  }
+  for (int s = 0; s < n; ++s) {
+    float z = 0.f;
+    for (int i = 0; i < D / 32; ++i) z += qr[i] * to_f32(k[s * k_st + i * 32 + lane_id()]);
+    for (int x = 16; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+    const float mn = fmaxf(m, z);
+    const float a = exp2f(m - mn), p = exp2f(z - mn);
+    m = mn;
+    l = l * a + p;
+    if (__isnanf(l)) break;  // and NaN it stays
+    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * a + p * to_f32(v[s * v_st + i * 32 + lane_id()]);
+  }
+  for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane_id()] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+}
+
+template <typename T, int D, int MODE>
+__global__ void __launch_bounds__(kTaThreads, 1)
+    tile_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                          const __grid_constant__ CUtensorMap tmV, const TileArgs args) {
+  using Shape = TaShape<D>;
+  constexpr int kStages = Shape::kStages, kKB = Shape::kKB, kTile = Shape::kTile, kBlk = 128 * 128;
+  constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+  constexpr uint32_t IDESC_S = idesc_half(kBf16, false, 128, 128);
+  constexpr uint32_t IDESC_O = idesc_half(kBf16, true, 128, D);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smQ = smem;                       // [tile][k-block]
+  uint8_t* smR = smQ + 2 * kTile;            // ring: [stage][k-block]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smR + kStages * kTile);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* r_full = bars + 2;               // [kStages]
+  uint64_t* r_empty = r_full + kStages;      // [kStages]
+  uint64_t* s_full = r_empty + kStages;      // [tile] S ready (and every earlier product of the tile done)
+  uint64_t* p_full = s_full + 2;             // [tile] P written and O rescaled
+  uint64_t* o_full = p_full + 2;             // [tile] the item's last product done
+  uint64_t* drain = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = lane_id();
+  const int cta = static_cast<int>(blockIdx.x), G = static_cast<int>(gridDim.x);
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(r_full + s, 1);
+      mbar_init(r_empty + s, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full + t, 1);
+      mbar_init(p_full + t, 4);
+      mbar_init(o_full + t, 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Items, heaviest first: round n of the G CTAs takes items nG .. nG + G - 1, alternately forwards and backwards,
+  // which balances the CTAs' key blocks. Every role walks the same items.
+  int n_items, one_first = 0, one_end = 0;
+  if constexpr (MODE == PACKED) {
+    if (args.plan) {
+      n_items = args.plan->n_pairs * args.hkv;
+      one_first = args.plan->first;
+      one_end = args.plan->end;
+    } else {
+      one_first = min(max(args.cu[0], 0), args.T);
+      one_end = min(max(args.cu[1], one_first), args.T);
+      n_items = (one_end - one_first + 2 * args.tok - 1) / (2 * args.tok) * args.hkv;
+    }
+  } else {
+    n_items = args.pairs * args.hkv * args.splits;
+  }
+  auto item = [&](int n, TileItem& it) -> bool {
+    const int idx = n * G + ((n & 1) ? G - 1 - cta : cta);
+    if (idx >= n_items) return false;
+    it.kvh = idx % args.hkv;
+    const int rest = idx / args.hkv;
+    if constexpr (MODE == PACKED) {
+      int begin, end;
+      if (args.plan) {
+        const int4 e = reinterpret_cast<const int4*>(args.plan + 1)[rest];
+        it.q_tok = e.x;
+        begin = e.y;
+        end = e.z;
+      } else {
+        begin = one_first;
+        end = one_end;
+        it.q_tok = begin + (n_items / args.hkv - 1 - rest) * 2 * args.tok;
+      }
+      it.kv_tok = begin;
+      it.len = end - begin;
+      it.q_pos = it.q_tok - begin;
+      it.split = 0;
+      for (int t = 0; t < 2; ++t) {  // a tile sees the keys up to its last token
+        const int first = it.q_pos + t * args.tok, last = min(first + args.tok, it.len) - 1;
+        it.nb[t] = last < first ? 0 : last / kTaBlock + 1;
+      }
+    } else {
+      const int pair = rest % args.pairs;
+      it.split = rest / args.pairs;
+      it.q_tok = pair * 2 * args.tok;
+      const int b0 = it.split * args.blocks_per_split;
+      it.kv_tok = b0 * kTaBlock;
+      const int nb = min(args.blocks_per_split, (args.P + kTaBlock - 1) / kTaBlock - b0);
+      it.nb[0] = nb;
+      it.nb[1] = it.q_tok + args.tok < args.B ? nb : 0;
+      it.len = it.q_pos = 0;
+    }
+    return true;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------------------------ TMA
+      int g = 0, q_loads = 0;  // ring blocks and Q loads so far
+      bool ok = true;
+      const uint32_t q_bytes = static_cast<uint32_t>(args.tok * args.group) * D * 2;
+      auto load = [&](const CUtensorMap* map, int kvh, int tok) -> bool {
+        const int st = g % kStages;
+        if (!mbar_wait(r_empty + st, ((g / kStages) & 1) ^ 1, abort_flag, args.err, 40)) return false;
+        mbar_arrive_expect_tx(r_full + st, kTile);
+        for (int kk = 0; kk < kKB; ++kk) tma_load_3d(smR + st * kTile + kk * kBlk, map, r_full + st, kk * 64, kvh, tok);
+        ++g;
+        return true;
+      };
+      TileItem it;
+      for (int n = 0; ok && item(n, it); ++n) {
+        const int tiles = it.nb[1] > 0 ? 2 : 1;
+        if (!mbar_wait(q_empty, (n & 1) ^ 1, abort_flag, args.err, 41)) break;
+        mbar_arrive_expect_tx(q_full, tiles * q_bytes);
+        for (int t = 0; t < tiles; ++t)
+          for (int kk = 0; kk < kKB; ++kk)
+            tma_load_4d(smQ + t * kTile + kk * kBlk, &tmQ, q_full, kk * 64, 0, it.kvh, it.q_tok + t * args.tok);
+        ++q_loads;
+        const int nb = max(it.nb[0], it.nb[1]);
+        for (int j = 0; ok && j < nb; ++j)
+          ok = load(&tmK, it.kvh, it.kv_tok + j * kTaBlock) && load(&tmV, it.kvh, it.kv_tok + j * kTaBlock);
+      }
+      // every load has landed before the CTA may exit
+      volatile int never = 0;
+      if (q_loads > 0) mbar_wait(q_full, static_cast<uint32_t>((q_loads - 1) & 1), &never, args.err, 42);
+      for (int s = 0; s < kStages && s < g; ++s) {
+        const int last = (g - 1 - s) / kStages;  // the last use of stage s
+        mbar_wait(r_full + s, static_cast<uint32_t>(last & 1), &never, args.err, 42);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ------------------------------------------------------------------ MMA
+      bool ok = true, issued = false;
+      int g = 0;             // ring blocks consumed
+      int p_seen[2] = {0, 0};
+      auto ring = [&](int i) { return smR + (i % kStages) * kTile; };
+      auto wait_ring = [&](int i) { return mbar_wait(r_full + i % kStages, (i / kStages) & 1, abort_flag, args.err, 43); };
+      auto issue_s = [&](int t, int i) {
+        const uint32_t tS = tmem + 128 * t;
+#pragma unroll
+        for (int kk = 0; kk < kKB; ++kk) {
+          const uint64_t dQ = smem_desc_k_sw128(smem_u32(smQ + t * kTile + kk * kBlk));
+          const uint64_t dK = smem_desc_k_sw128(smem_u32(ring(i) + kk * kBlk));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16(tS, dQ + 2 * k, dK + 2 * k, IDESC_S, (kk | k) != 0);
+        }
+        umma_commit(s_full + t);
+        issued = true;
+      };
+      auto issue_pv = [&](int t, int i, bool first) -> bool {
+        if (!mbar_wait(p_full + t, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
+        ++p_seen[t];
+        tc_fence_after();
+        const uint32_t tO = tmem + 256 + 128 * t, tP = tmem + 128 * t;
+        const uint64_t dV = smem_desc_mn_sw128(smem_u32(ring(i)), kBlk);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) umma_f16_ts(tO, tP + 8 * k, dV + 128 * k, IDESC_O, (!first || k) != 0);
+        return true;
+      };
+      TileItem it;
+      for (int n = 0; ok && item(n, it); ++n) {
+        const int nb = max(it.nb[0], it.nb[1]);
+        if (!mbar_wait(q_full, n & 1, abort_flag, args.err, 45) || !wait_ring(g)) break;
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (it.nb[t] > 0) issue_s(t, g);
+        umma_commit(r_empty + g % kStages);
+        if (nb == 1) umma_commit(q_empty);
+        for (int j = 0; ok && j < nb; ++j, g += 2) {
+          // ring block g = K_j, g + 1 = V_j, g + 2 = K_{j+1}
+          if (!wait_ring(g + 1) || (j + 1 < nb && !wait_ring(g + 2))) {
+            ok = false;
+            break;
+          }
+          for (int t = 0; ok && t < 2; ++t) {
+            if (j >= it.nb[t]) continue;
+            ok = issue_pv(t, g + 1, j == 0);
+            if (!ok) break;
+            if (j + 1 < it.nb[t])
+              issue_s(t, g + 2);
+            else
+              umma_commit(o_full + t);
+          }
+          if (!ok) break;
+          umma_commit(r_empty + (g + 1) % kStages);
+          if (j + 1 < nb) umma_commit(r_empty + (g + 2) % kStages);
+          if (j + 2 == nb) umma_commit(q_empty);
+        }
+      }
+      if (issued) {
+        umma_commit(drain);
+        volatile int never = 0;
+        mbar_wait(drain, 0, &never, args.err, 46);
+      }
+    }
+  } else {
+    // -------------------------------------------------------------------- softmax (warps 2..9)
+    const int t = (warp - 2) >> 2;           // tile
+    const int qd = warp & 3;                 // TMEM lane quadrant = row block
+    const int r = qd * 32 + lane;            // row of the tile
+    const int r_tok = r / args.group, r_head = r - r_tok * args.group;
+    const bool r_ok = r_tok < args.tok;      // rows past tok * group hold no query
+    const uint32_t lane_off = static_cast<uint32_t>(qd * 32) << 16;
+    const uint32_t tS = tmem + 128 * t + lane_off, tO = tmem + 256 + 128 * t + lane_off;
+    const float sc = args.scale_log2;
+    if constexpr (MODE == PACKED) {
+      // tokens of no sequence
+      const int64_t row = static_cast<int64_t>(args.hq) * D / 8;  // 16-byte pieces of a token
+      const int64_t head = one_first * row, tail = (args.T - one_end) * row;
+      uint4* o = static_cast<uint4*>(args.out);
+      for (int64_t i = static_cast<int64_t>(cta) * 256 + threadIdx.x - 64; i < head + tail; i += static_cast<int64_t>(G) * 256)
+        o[i < head ? i : one_end * row + i - head] = make_uint4(0, 0, 0, 0);
+    }
+    bool ok = true;
+    uint32_t v[128];                         // this row of S
+    int g = 0, items = 0;                    // key blocks and items of this tile so far
+    TileItem it;
+    for (int n = 0; ok && item(n, it); ++n) {
+      const int nb = it.nb[t];
+      if (nb == 0) continue;
+      const int pos = it.q_pos + t * args.tok + r_tok;  // PACKED: place in the sequence
+      float m_use = -INFINITY, l = 0.f;
+      for (int j = 0; j < nb; ++j, ++g) {
+        if (!mbar_wait(s_full + t, g & 1, abort_flag, args.err, 47)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(v + c * 32));
+        tmem_ld_wait();
+        // the last key of this block that the row sees
+        const int last = MODE == PACKED ? pos - j * kTaBlock : args.P - 1 - it.kv_tok - j * kTaBlock;
+        if (__any_sync(0xffffffffu, last < kTaBlock - 1)) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (e > last) v[e] = __float_as_uint(-INFINITY);
+        }
+        float m8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m8[i] = __uint_as_float(v[i]);
+#pragma unroll
+        for (int e = 8; e + 16 <= 128; e += 16) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m8[i] = fmax3(m8[i], __uint_as_float(v[e + i]), __uint_as_float(v[e + 8 + i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(m8[i], __uint_as_float(v[120 + i]));
+        const float m_blk = fmaxf(fmax3(m8[0], m8[1], m8[2]), fmaxf(fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * sc;
+        float alpha = 1.f;
+        const bool raise = m_blk > m_use + kTaRescale;
+        if (raise) {
+          alpha = fast_exp2(m_use - m_blk);  // 0 while m_use is -inf
+          m_use = m_blk;
+        }
+        if (j >= 1 && __any_sync(0xffffffffu, raise)) {
+          // S(j) was issued after O += P(j-1) V(j-1), so O is complete
+          uint32_t o[32];
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            __syncwarp();
+            tmem_ld_32x32b_x32(tO + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x32(tO + c * 32, o);
+          }
+        }
+        l *= alpha;
+        const float neg_m = m_use == -INFINITY ? 0.f : -m_use;
+        float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c * 64 + e]), __uint_as_float(v[c * 64 + e + 1])), sc2, nm2);
+            const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            rs4[(e >> 1) & 3] = __fadd2_rn(rs4[(e >> 1) & 3], pp);
+            w[e / 2] = pack2<T>(pp.x, pp.y);
+          }
+          __syncwarp();
+          tmem_st_32x32b_x32(tS + c * 32, w);
+        }
+        l += ((rs4[0].x + rs4[0].y) + (rs4[1].x + rs4[1].y)) + ((rs4[2].x + rs4[2].y) + (rs4[3].x + rs4[3].y));
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + t);
+      }
+      if (!ok || !mbar_wait(o_full + t, items & 1, abort_flag, args.err, 48)) break;
+      ++items;
+      tc_fence_after();
+      const int tok = it.q_tok + t * args.tok + r_tok;
+      const int head = it.kvh * args.group + r_head;
+      uint32_t o[32];
+      if constexpr (MODE == PACKED) {
+        const bool mine = r_ok && pos < it.len;
+        const float inv = 1.f / l;
+        float bad = 0.f;  // stays 0 over finite values
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(args.out) + (static_cast<int64_t>(tok) * args.hq + head) * D);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          __syncwarp();
+          tmem_ld_32x32b_x32(tO + c * 32, o);
+          tmem_ld_wait();
+          if (mine) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              float x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                x[i] = __uint_as_float(o[e + i]) * inv;
+                bad = fmaf(x[i], 0.f, bad);
+              }
+              dst[(c * 32 + e) / 8] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+            }
+          }
+        }
+        unsigned again = __ballot_sync(0xffffffffu, mine && !(bad == 0.f));
+        while (again) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int w_tok = __shfl_sync(0xffffffffu, tok, who), w_head = __shfl_sync(0xffffffffu, head, who);
+          const int64_t first = it.kv_tok;
+          recompute_row<T, D>(static_cast<const T*>(args.q) + w_tok * args.q_st + w_head * args.q_sh,
+                              static_cast<const T*>(args.k) + first * args.k_st + it.kvh * args.k_sh, args.k_st,
+                              static_cast<const T*>(args.v) + first * args.v_st + it.kvh * args.v_sh, args.v_st,
+                              w_tok - it.kv_tok + 1, sc,
+                              static_cast<T*>(args.out) + (static_cast<int64_t>(w_tok) * args.hq + w_head) * D);
+        }
+      } else {
+        const bool mine = r_ok && tok < args.B;
+        const int64_t row = (static_cast<int64_t>(it.split) * args.B + tok) * args.hq + head;
+        float4* dst = reinterpret_cast<float4*>(args.part_o + row * D);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          __syncwarp();
+          tmem_ld_32x32b_x32(tO + c * 32, o);
+          tmem_ld_wait();
+          if (mine) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              dst[(c * 32 + e) / 4] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
+                                                  __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+          }
+        }
+        if (mine) args.part_ml[row] = make_float2(m_use, l);
+      }
+      // O has been read: the next item's first product (issued after this warp's next P) may overwrite it
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------- the plan of a packed call
+// One block: the sequences' bounds (the running maximum of the clamped words, so they ascend whatever cu holds), and
+// their tile pairs sorted by key blocks, most first, by counting. The order among equals is left to the atomics: it
+// changes which CTA takes a pair, never a result. The list has room for tokens / (2 tok) + n_seqs pairs, which the
+// ascending bounds cannot exceed.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBins = 2048;
+
+__device__ __forceinline__ int warp_scan(int x, bool is_max) {
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane_id() >= o) x = is_max ? max(x, y) : x + y;
+  }
+  return x;
+}
+
+// Inclusive scan over the block; every thread calls it.
+__device__ __forceinline__ int block_scan(int x, bool is_max, int* scratch) {
+  x = warp_scan(x, is_max);
+  if (lane_id() == 31) scratch[warp_id()] = x;
+  __syncthreads();
+  if (warp_id() == 0) scratch[lane_id()] = warp_scan(scratch[lane_id()], is_max);
+  __syncthreads();
+  if (warp_id() > 0) {
+    const int y = scratch[warp_id() - 1];
+    x = is_max ? max(x, y) : x + y;
+  }
+  __syncthreads();
+  return x;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int32_t* cu, int n_seqs, int T, int per_pair,
+                                                                   PlanHeader* plan) {
+  __shared__ int scratch[32], starts[kPlanThreads], ends[kPlanThreads], upto[kPlanThreads], bins[kPlanBins];
+  int4* list = reinterpret_cast<int4*>(plan + 1);
+  auto clamp = [&](int x) { return min(max(x, 0), T); };
+  const int first = clamp(cu[0]);
+  for (int i = threadIdx.x; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
+  __syncthreads();
+  int total = 0, reached = first;
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) {
+      // bins[i] = pairs with more blocks than i: the place of the first pair of bin i
+      const int a = bins[kPlanBins - 1 - 2 * threadIdx.x], b = bins[kPlanBins - 2 - 2 * threadIdx.x];
+      __syncthreads();
+      const int s = block_scan(a + b, false, scratch);
+      bins[kPlanBins - 1 - 2 * threadIdx.x] = s - a - b;
+      bins[kPlanBins - 2 - 2 * threadIdx.x] = s - b;
+      __syncthreads();
+    }
+    reached = first;
+    total = 0;
+    for (int c = 0; c < n_seqs; c += kPlanThreads) {
+      const int i = c + static_cast<int>(threadIdx.x);
+      const int end = max(block_scan(i < n_seqs ? clamp(cu[i + 1]) : 0, true, scratch), reached);
+      ends[threadIdx.x] = end;
+      __syncthreads();
+      const int start = threadIdx.x ? ends[threadIdx.x - 1] : reached;
+      starts[threadIdx.x] = start;
+      const int pairs = block_scan((end - start + per_pair - 1) / per_pair, false, scratch);
+      upto[threadIdx.x] = pairs;
+      __syncthreads();
+      const int here = upto[kPlanThreads - 1];
+      for (int p = threadIdx.x; p < here; p += kPlanThreads) {
+        int lo = 0, hi = kPlanThreads - 1;  // the first sequence with upto > p
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (upto[mid] > p) hi = mid; else lo = mid + 1;
+        }
+        const int at = p - (lo ? upto[lo - 1] : 0), len = ends[lo] - starts[lo];
+        const int blocks = (min(len, (at + 1) * per_pair) + kTaBlock - 1) / kTaBlock;
+        const int bin = min(blocks, kPlanBins - 1);
+        const int place = atomicAdd(&bins[bin], 1);
+        if (pass == 1) list[place] = make_int4(starts[lo] + at * per_pair, starts[lo], ends[lo], 0);
+      }
+      total += here;
+      reached = ends[kPlanThreads - 1];
+      __syncthreads();
+    }
+  }
+  if (threadIdx.x == 0) *plan = PlanHeader{total, first, reached, 0};
+}
+
+// ---------------------------------------------------------------------------- the batch's own keys and the join
+struct OwnArgs {
+  const void *q, *ck, *cv;
+  int64_t q_sb, q_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh;
+  const int32_t* lens;
+  int B, S, hq, hkv, splits;
+  float scale_log2;
+  const float* part_o;
+  const float2* part_ml;
+  void* out;
+};
+
+// One warp per row: its own keys one by one, joined with the prefix's parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) own_keys_kernel(const OwnArgs a) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp_id();
   if (row >= static_cast<int64_t>(a.B) * a.hq) return;
   const int b = static_cast<int>(row / a.hq), h = static_cast<int>(row % a.hq), hk = h / (a.hq / a.hkv);
-  Row<T, D> r;
-  r.init(static_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh, a.scale_log2);
-  for (int s = 0; s < a.P; ++s)
-    r.key(static_cast<const T*>(a.pk) + s * a.pk_st + hk * a.pk_sh, static_cast<const T*>(a.pv) + s * a.pv_st + hk * a.pv_sh);
+  float q[D / 32], o[D / 32], m = -INFINITY, l = 0.f;
+  for (int i = 0; i < D / 32; ++i) {
+    q[i] = to_f32(static_cast<const T*>(a.q)[b * a.q_sb + h * a.q_sh + i * 32 + lane_id()]) * a.scale_log2;
+    o[i] = 0.f;
+  }
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = static_cast<int64_t>(s) * a.B * a.hq + row;
+    const float2 ml = a.part_ml[at];
+    const float mn = fmaxf(m, ml.x), f = exp2f(m - mn), w = exp2f(ml.x - mn);
+    m = mn;
+    l = l * f + ml.y * w;
+    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * f + w * a.part_o[at * D + i * 32 + lane_id()];
+  }
   const int n = min(max(a.lens[b], 0), a.S);
-  for (int s = 0; s < n; ++s)
-    r.key(static_cast<const T*>(a.ck) + b * a.ck_sb + s * a.ck_st + hk * a.ck_sh,
-          static_cast<const T*>(a.cv) + b * a.cv_sb + s * a.cv_st + hk * a.cv_sh);
-  r.store(static_cast<T*>(a.out) + row * D);
+  for (int s = 0; s < n; ++s) {
+    const T* k = static_cast<const T*>(a.ck) + b * a.ck_sb + s * a.ck_st + hk * a.ck_sh;
+    const T* v = static_cast<const T*>(a.cv) + b * a.cv_sb + s * a.cv_st + hk * a.cv_sh;
+    float z = 0.f;
+    for (int i = 0; i < D / 32; ++i) z += q[i] * to_f32(k[i * 32 + lane_id()]);
+    for (int x = 16; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+    const float mn = fmaxf(m, z), f = exp2f(m - mn), p = exp2f(z - mn);
+    m = mn;
+    l = l * f + p;
+    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * f + p * to_f32(v[i * 32 + lane_id()]);
+  }
+  T* dst = static_cast<T*>(a.out) + row * D;
+  for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane_id()] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
 }
 
+// ---------------------------------------------------------------------------- host
 static int check_heads(const char* what, int64_t hq, int64_t hkv, int64_t d, int dtype, float scale) {
   XDNA_CHECK_ARG(hq >= 1 && hkv >= 1 && hq % hkv == 0 && hq / hkv <= 128,
                  "%s: %lld query heads over %lld key heads", what, (long long)hq, (long long)hkv);
@@ -116,6 +652,63 @@ static bool row_ok(const void* p, int64_t a, int64_t b, int64_t c = 8) {
   return p != nullptr && aligned16(p) && a > 0 && b > 0 && c > 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
 }
 
+// q [n, hq, d] as (dimension, head of the group, key head, token): a box is a tile's 64 columns of all its rows.
+static int q_map(CUtensorMap* m, const void* q, int64_t st, int64_t sh, int64_t n, int64_t hkv, int64_t group,
+                 int64_t tok, int64_t d, int dtype) {
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)group, (uint64_t)hkv, (uint64_t)n};
+  const uint64_t strides[3] = {(uint64_t)sh * 2, (uint64_t)(sh * group) * 2, (uint64_t)st * 2};
+  const uint32_t box[4] = {64, (uint32_t)group, 1, (uint32_t)tok};
+  return encode_tma(m, dtype == XDNA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, q, dims,
+                    strides, box, "attention q");
+}
+
+static int kv_map(CUtensorMap* m, const void* k, int64_t st, int64_t sh, int64_t n, int64_t hkv, int64_t d, int dtype) {
+  const uint64_t dims[3] = {(uint64_t)d, (uint64_t)hkv, (uint64_t)n};
+  const uint64_t strides[2] = {(uint64_t)sh * 2, (uint64_t)st * 2};
+  const uint32_t box[3] = {64, 1, kTaBlock};
+  return encode_tma(m, dtype == XDNA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, k, dims,
+                    strides, box, "attention k/v");
+}
+
+template <typename T, int D, int MODE>
+static int launch_tiles_as(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TileArgs& a, int grid,
+                           cudaStream_t s) {
+  static std::atomic<bool> configured[64];  // setting the attribute twice from two threads is harmless
+  int dev = 0;
+  XDNA_CUDA(cudaGetDevice(&dev));
+  auto kern = tile_attention_kernel<T, D, MODE>;
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TaShape<D>::kSmem));
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  kern<<<grid, kTaThreads, TaShape<D>::kSmem, s>>>(q, k, v, a);
+  return check_launch("tile_attention_kernel");
+}
+
+template <int MODE>
+static int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TileArgs& a, int64_t d,
+                        int dtype, int grid, cudaStream_t s) {
+  if (dtype == XDNA_BF16)
+    return d == 128 ? launch_tiles_as<__nv_bfloat16, 128, MODE>(q, k, v, a, grid, s)
+                    : launch_tiles_as<__nv_bfloat16, 64, MODE>(q, k, v, a, grid, s);
+  return d == 128 ? launch_tiles_as<__half, 128, MODE>(q, k, v, a, grid, s)
+                  : launch_tiles_as<__half, 64, MODE>(q, k, v, a, grid, s);
+}
+
+static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { return tokens / (2 * (128 / group)) + n_seqs; }
+
+// Key splits of a prefix: about one item per SM, each at least one block.
+struct PrefixSplit {
+  int64_t pairs, splits, blocks_per_split;
+  PrefixSplit(int64_t B, int64_t P, int64_t hq, int64_t hkv, int sms) {
+    const int64_t tok = 128 / (hq / hkv), blocks = (P + kTaBlock - 1) / kTaBlock;
+    pairs = (B + 2 * tok - 1) / (2 * tok);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(blocks, sms / (pairs * hkv)));
+    blocks_per_split = blocks ? (blocks + want - 1) / want : 0;
+    splits = blocks ? (blocks + blocks_per_split - 1) / blocks_per_split : 0;
+  }
+};
+
 }  // namespace xdna
 
 using namespace xdna;
@@ -123,7 +716,8 @@ using namespace xdna;
 extern "C" {
 
 size_t xdna_packed_attention_workspace(int64_t n_seqs, int64_t tokens, int64_t hq, int64_t hkv) {
-  return 0;
+  if (n_seqs <= 1 || tokens < 0 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
+  return sizeof(PlanHeader) + 16 * static_cast<size_t>(plan_pairs(n_seqs, tokens, hq / hkv));
 }
 
 int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
@@ -134,24 +728,56 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
   if (rc != XDNA_OK) return rc;
   XDNA_CHECK_ARG(tokens >= 0 && n_seqs >= 0 && tokens < (1ll << 31) / hq && n_seqs < (1 << 24),
                  "packed_attention: bad sizes");
-  if ((rc = check_device(nullptr)) != XDNA_OK) return rc;
+  int sms = 0;
+  if ((rc = check_device(&sms)) != XDNA_OK) return rc;
   if (tokens == 0) return XDNA_OK;
   XDNA_CHECK_ARG(row_ok(q, q_st, q_sh) && row_ok(k, k_st, k_sh) && row_ok(v, v_st, v_sh) && cu_seqlens && out &&
                      aligned16(out),
                  "packed_attention: operands must be 16-byte aligned with strides that are positive multiples of 8");
-  const PackedArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu_seqlens, (int)n_seqs, (int)tokens, (int)hq,
-                     (int)hkv, scale * 1.4426950408889634f, out};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned g = static_cast<unsigned>((tokens * hq + 7) / 8);
-  if (dtype == XDNA_BF16)
-    d == 128 ? packed_kernel<__nv_bfloat16, 128><<<g, 256, 0, s>>>(a) : packed_kernel<__nv_bfloat16, 64><<<g, 256, 0, s>>>(a);
-  else
-    d == 128 ? packed_kernel<__half, 128><<<g, 256, 0, s>>>(a) : packed_kernel<__half, 64><<<g, 256, 0, s>>>(a);
-  return check_launch("packed_kernel");
+  if (n_seqs == 0) {
+    XDNA_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(tokens * hq * d * 2), s));
+    return XDNA_OK;
+  }
+  const int64_t group = hq / hkv, tok = 128 / group;
+  TileArgs a{};
+  a.hq = static_cast<int>(hq);
+  a.hkv = static_cast<int>(hkv);
+  a.group = static_cast<int>(group);
+  a.tok = static_cast<int>(tok);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.err = device_error_word();
+  a.out = out;
+  a.cu = cu_seqlens;
+  a.T = static_cast<int>(tokens);
+  a.q = q, a.k = k, a.v = v;
+  a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
+  CUtensorMap tq, tk, tv;
+  if ((rc = q_map(&tq, q, q_st, q_sh, tokens, hkv, group, tok, d, dtype)) != XDNA_OK ||
+      (rc = kv_map(&tk, k, k_st, k_sh, tokens, hkv, d, dtype)) != XDNA_OK ||
+      (rc = kv_map(&tv, v, v_st, v_sh, tokens, hkv, d, dtype)) != XDNA_OK)
+    return rc;
+  int64_t pairs = (tokens + 2 * tok - 1) / (2 * tok);
+  if (n_seqs > 1) {
+    XDNA_CHECK_ARG(workspace && aligned16(workspace) &&
+                       workspace_bytes >= xdna_packed_attention_workspace(n_seqs, tokens, hq, hkv),
+                   "packed_attention: workspace too small or unaligned");
+    auto* plan = static_cast<PlanHeader*>(workspace);
+    packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(cu_seqlens, static_cast<int>(n_seqs), a.T, static_cast<int>(2 * tok), plan);
+    if ((rc = check_launch("packed_plan_kernel")) != XDNA_OK) return rc;
+    a.plan = plan;
+    pairs = plan_pairs(n_seqs, tokens, group);
+  }
+  XDNA_CHECK_ARG(pairs < (1ll << 31) / hkv, "packed_attention: bad sizes");
+  return launch_tiles<PACKED>(tq, tk, tv, a, d, dtype, static_cast<int>(std::min<int64_t>(pairs * hkv, sms)), s);
 }
 
 size_t xdna_prefix_attention_workspace(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d) {
-  return 0;
+  if (B < 1 || P < 1 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
+  int sms = 0;
+  if (check_device(&sms) != XDNA_OK) return 0;
+  const PrefixSplit split(B, P, hq, hkv, sms);
+  return static_cast<size_t>(split.splits * B * hq) * (sizeof(float2) + d * sizeof(float));
 }
 
 int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* pk, int64_t pk_st, int64_t pk_sh,
@@ -161,23 +787,55 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
                           int dtype, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_heads("prefix_attention", hq, hkv, d, dtype, scale);
   if (rc != XDNA_OK) return rc;
-  XDNA_CHECK_ARG(B >= 0 && P >= 0 && S >= 0 && B < (1ll << 31) / hq && P < (1ll << 31) && S < (1ll << 31),
+  XDNA_CHECK_ARG(B >= 0 && P >= 0 && S >= 0 && B < (1ll << 24) / hq && P < (1ll << 31) - kTaBlock && S < (1ll << 31) - kTaBlock,
                  "prefix_attention: bad sizes");
-  if ((rc = check_device(nullptr)) != XDNA_OK) return rc;
+  int sms = 0;
+  if ((rc = check_device(&sms)) != XDNA_OK) return rc;
   if (B == 0) return XDNA_OK;
   XDNA_CHECK_ARG(row_ok(q, q_sb, q_sh) && (P == 0 || (row_ok(pk, pk_st, pk_sh) && row_ok(pv, pv_st, pv_sh))) &&
                      (S == 0 || (row_ok(ck, ck_sb, ck_st, ck_sh) && row_ok(cv, cv_sb, cv_st, cv_sh))) && lens && out &&
                      aligned16(out),
                  "prefix_attention: operands must be 16-byte aligned with strides that are positive multiples of 8");
-  const PrefixArgs a{q, pk, pv, ck, cv, q_sb, q_sh, pk_st, pk_sh, pv_st, pv_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st,
-                     cv_sh, lens, (int)B, (int)P, (int)S, (int)hq, (int)hkv, scale * 1.4426950408889634f, out};
+  XDNA_CHECK_ARG(P == 0 || (workspace && aligned16(workspace) &&
+                            workspace_bytes >= xdna_prefix_attention_workspace(B, P, S, hq, hkv, d)),
+                 "prefix_attention: workspace too small or unaligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t group = hq / hkv, tok = 128 / group;
+  const PrefixSplit split(B, P, hq, hkv, sms);
+  float* part_o = static_cast<float*>(workspace);
+  float2* part_ml = reinterpret_cast<float2*>(part_o + split.splits * B * hq * d);
+  if (P > 0) {
+    TileArgs a{};
+    a.hq = static_cast<int>(hq);
+    a.hkv = static_cast<int>(hkv);
+    a.group = static_cast<int>(group);
+    a.tok = static_cast<int>(tok);
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.err = device_error_word();
+    a.B = static_cast<int>(B);
+    a.P = static_cast<int>(P);
+    a.pairs = static_cast<int>(split.pairs);
+    a.splits = static_cast<int>(split.splits);
+    a.blocks_per_split = static_cast<int>(split.blocks_per_split);
+    a.part_o = part_o;
+    a.part_ml = part_ml;
+    CUtensorMap tq, tk, tv;
+    if ((rc = q_map(&tq, q, q_sb, q_sh, B, hkv, group, tok, d, dtype)) != XDNA_OK ||
+        (rc = kv_map(&tk, pk, pk_st, pk_sh, P, hkv, d, dtype)) != XDNA_OK ||
+        (rc = kv_map(&tv, pv, pv_st, pv_sh, P, hkv, d, dtype)) != XDNA_OK)
+      return rc;
+    const int64_t items = split.pairs * hkv * split.splits;
+    if ((rc = launch_tiles<PREFIX>(tq, tk, tv, a, d, dtype, static_cast<int>(std::min<int64_t>(items, sms)), s)) != XDNA_OK)
+      return rc;
+  }
+  const OwnArgs o{q, ck, cv, q_sb, q_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh, lens, (int)B, (int)S, (int)hq,
+                  (int)hkv, (int)split.splits, scale * 1.4426950408889634f, part_o, part_ml, out};
   const unsigned g = static_cast<unsigned>((B * hq + 7) / 8);
   if (dtype == XDNA_BF16)
-    d == 128 ? prefix_kernel<__nv_bfloat16, 128><<<g, 256, 0, s>>>(a) : prefix_kernel<__nv_bfloat16, 64><<<g, 256, 0, s>>>(a);
+    d == 128 ? own_keys_kernel<__nv_bfloat16, 128><<<g, 256, 0, s>>>(o) : own_keys_kernel<__nv_bfloat16, 64><<<g, 256, 0, s>>>(o);
   else
-    d == 128 ? prefix_kernel<__half, 128><<<g, 256, 0, s>>>(a) : prefix_kernel<__half, 64><<<g, 256, 0, s>>>(a);
-  return check_launch("prefix_kernel");
+    d == 128 ? own_keys_kernel<__half, 128><<<g, 256, 0, s>>>(o) : own_keys_kernel<__half, 64><<<g, 256, 0, s>>>(o);
+  return check_launch("own_keys_kernel");
 }
 
 }  // extern "C"

@@ -163,6 +163,14 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
 // A pair's operand load: written into this CTA's shared memory, completion bytes counted on the
 // barrier at `cluster_bar` (the even CTA's, which its MMA issuer waits on).
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int x,
@@ -271,6 +279,17 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same with A read from TMEM (rows = lanes, two 16-bit K values per 32-bit column).
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -389,6 +408,12 @@ __device__ __forceinline__ uint64_t smem_desc_k_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// Descriptor of an MN-major operand tile written by TMA with 128-byte swizzle: rows of K, 64 MN values of 16 bits
+// (128 bytes) each, 8-row groups 1024 bytes apart (SBO), the next 64 MN values `lbo` bytes on (LBO).
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr, uint32_t lbo) {
+  return (smem_desc_k_sw128(smem_addr) & ~(uint64_t(0x3FFF) << 16)) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16);
+}
+
 // A 128-byte-swizzled matrix that starts some 128-byte rows (and K bytes) into a 1024-byte swizzle atom, as
 // smem_desc_k_sw64_at: the swizzle is a function of the absolute address, which TMA used when it wrote the
 // rows (checked bit for bit against the CPU integers by the conv tests).
@@ -401,6 +426,16 @@ __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
          | (1u << 10)                            // B: signed 8-bit
          | (static_cast<uint32_t>(N >> 3) << 17)  // N >> 3
          | (static_cast<uint32_t>(M >> 4) << 24);  // M >> 4
+}
+
+// Instruction descriptor, kind::f16: D f32, A and B both bf16 or both f16, A K-major, B K-major or MN-major.
+__host__ __device__ constexpr uint32_t idesc_half(bool bf16, bool b_mn_major, int M, int N) {
+  return (1u << 4)                               // D format: F32
+         | ((bf16 ? 1u : 0u) << 7)               // A: BF16 / F16
+         | ((bf16 ? 1u : 0u) << 10)              // B: BF16 / F16
+         | ((b_mn_major ? 1u : 0u) << 16)        // B: MN-major
+         | (static_cast<uint32_t>(N >> 3) << 17)
+         | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
 // Instruction descriptor, kind::f16: D f32, A/B bf16, both K-major, shape M x N.
