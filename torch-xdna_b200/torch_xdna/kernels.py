@@ -93,9 +93,9 @@ def _load():
         "xdna_prefix_attention_workspace": ([I64, I64, I64, I64, I64, I64], ctypes.c_size_t),
         "xdna_prefix_attention": ([P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64,
                                    I64, I64, I64, I64, I64, I, ctypes.c_float, P, P, ctypes.c_size_t, P], I),
-        "xdna_w4_pack": ([P, I, I64, I64, I64, I, P, P, I, P], I),
         "xdna_linear_w4": ([P, I, I64, I64, I64, P, P, I, I, I64, P, I, P, I64, P], I),
         "xdna_process_logits": ([P, I, I64, I64, I64, P, I, I64, I64, P, P, P, P, P, P, I64, P, I64, P, I64, P], I),
+        "xdna_w4_pack": ([P, I, I64, I64, I64, I, P, P, I, P], I),
         "xdna_attention": ([P, P, I64, P, I64, I64, I, P, P, I, P], I),
         "xdna_qwen3_stack_workspace": ([I64, I64], ctypes.c_size_t),
         "xdna_qwen3_stack": ([P, I, P, P, I64, P, I, P, P, ctypes.c_float, P, I64, I64, I, P, P, I, P, I, I64, P,
@@ -472,6 +472,16 @@ def attention(qk, vt, out, B, L_, mask_kind, lens=None, mask=None):
     mh = mask.shape[1] if mask is not None else 1
     _check("xdna_attention", L.xdna_attention(_p(qk), _p(vt), vt.stride(0), _p(out), B, L_, mask_kind, _p(lens),
                                               _p(mask), mh, _stream()))
+
+
+def w4_pack(w, group, codes, scales):
+    """codes, scales = the 4-bit form of w [N, K] (xdna_w4_pack); the other generation entries are called by
+    csrc/binding.cpp."""
+    L = require()
+    _cuda(w, codes, scales)
+    N, K = w.shape
+    _check("xdna_w4_pack", L.xdna_w4_pack(_p(w), DTYPE_CODES[w.dtype], N, K, max(w.stride(0), K), group, _p(codes),
+                                          _p(scales), DTYPE_CODES[scales.dtype], _stream()))
 
 
 def qwen3_stack_workspace(B, L_):
