@@ -23,60 +23,202 @@ struct LogitsArgs {
   int64_t ld_mask;
 };
 
-constexpr int kLogitsChunk = 4096;       // vocabulary entries of a block
+constexpr int kLogitsThreads = 256;
 constexpr uint32_t kSeen = 0x80000000u;  // in the counter of an entry: it is among the row's tokens
 
-__device__ __forceinline__ float logit_in(const float* p) { return *p; }
-__device__ __forceinline__ float logit_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float logit_in(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ void logit_out(float* p, float x) { *p = x; }
-__device__ __forceinline__ void logit_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void logit_out(__half* p, float x) { *p = __float2half_rn(x); }
+template <typename T>
+struct LogitVec;  // 16 bytes of logits
+template <>
+struct LogitVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[4]) {
+    x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ void store(float* p, float x) { *p = x; }
+};
+template <>
+struct LogitVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+};
+template <>
+struct LogitVec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ void store(__half* p, float x) { *p = __float2half_rn(x); }
+};
 
-// A block takes kLogitsChunk entries of one row: it counts the row's tokens that fall into them in shared memory
-// (integer sums, so their order does not matter), then makes one pass over the entries.
-template <typename T, typename Tok>
-__global__ void __launch_bounds__(256) logits_kernel(const LogitsArgs a) {
-  __shared__ uint32_t count[kLogitsChunk];
-  const int64_t row = blockIdx.y, base = static_cast<int64_t>(blockIdx.x) * kLogitsChunk;
-  const int n = static_cast<int>(min(static_cast<int64_t>(kLogitsChunk), a.V - base));
+// A block takes VECS x 256 pieces of 16 bytes of one row. The pieces are loaded first; while they are on their way the
+// block clears its counters and counts the row's tokens that fall into its entries (integer sums in shared memory, so
+// their order does not matter); then each piece is worked on in registers and written. The row is cut at 16-byte
+// boundaries of its own address, so rows of any pitch are read and written in whole pieces except at their two ends.
+// HBM-bound; the history is read once per block, from the L2, so the blocks are as long as still fill the machine.
+template <typename T, typename Tok, int VECS>
+__global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs a) {
+  using Vec = LogitVec<T>;
+  constexpr int N = Vec::N, kChunk = VECS * kLogitsThreads * N;
+  extern __shared__ __align__(16) uint32_t count[];  // [kChunk] (with tokens)
+  const int64_t row = blockIdx.y;
+  const T* in = static_cast<const T*>(a.in) + row * a.ld_in;
+  T* out = static_cast<T*>(a.out) + row * a.ld_out;
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  // entries [base, base + kChunk) of the row, those outside [0, V) left out; in + base is on a 16-byte boundary
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * kChunk - shift;
+  const bool pieces = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(in)) & 15) == 0;
+  auto whole = [&](int v) {
+    const int64_t at = base + (v * kLogitsThreads + threadIdx.x) * N;
+    return pieces && at >= 0 && at + N <= a.V;
+  };
+  uint4 raw[VECS];
+#pragma unroll
+  for (int v = 0; v < VECS; ++v)
+    if (whole(v)) raw[v] = __ldcs(reinterpret_cast<const uint4*>(in + base) + v * kLogitsThreads + threadIdx.x);
   if (a.tokens) {
-    for (int i = threadIdx.x; i < kLogitsChunk; i += 256) count[i] = 0;
+#pragma unroll
+    for (int v = 0; v < VECS * N / 4; ++v) reinterpret_cast<uint4*>(count)[v * kLogitsThreads + threadIdx.x] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const int64_t len = a.lens ? min(static_cast<int64_t>(max(a.lens[row], 0)), a.T) : a.T;
-    const int64_t prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
+    const int len = a.lens ? min(max(a.lens[row], 0), static_cast<int>(a.T)) : static_cast<int>(a.T);
+    const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
     const Tok* tok = static_cast<const Tok*>(a.tokens) + row * a.ld_tokens;
-    for (int64_t i = threadIdx.x; i < len; i += 256) {
-      const int64_t at = static_cast<int64_t>(tok[i]) - base;
-      if (at < 0 || at >= n) continue;
+    auto put = [&](int i, Tok id) {
+      const int64_t at = static_cast<int64_t>(id) - base;
+      if (id < 0 || at < 0 || at >= kChunk) return;
       atomicOr(&count[at], kSeen);
       if (i >= prompt) atomicAdd(&count[at], 1u);
+    };
+    constexpr int M = 16 / sizeof(Tok);
+    const int head = min(len, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(tok) & 15)) % 16 / sizeof(Tok)));
+    if (static_cast<int>(threadIdx.x) < head) put(threadIdx.x, tok[threadIdx.x]);
+    int i = head + static_cast<int>(threadIdx.x) * M;
+#pragma unroll 2
+    for (; i + M <= len; i += kLogitsThreads * M) {
+      Tok id[M];
+      *reinterpret_cast<uint4*>(id) = *reinterpret_cast<const uint4*>(tok + i);
+#pragma unroll
+      for (int e = 0; e < M; ++e) put(i + e, id[e]);
     }
+    for (int e = 0; e < M; ++e)
+      if (i + e < len) put(i + e, tok[i + e]);
     __syncthreads();
   }
   const float rep = a.rep ? a.rep[row] : 1.f, pres = a.pres ? a.pres[row] : 0.f, freq = a.freq ? a.freq[row] : 0.f;
-  const T* in = static_cast<const T*>(a.in) + row * a.ld_in + base;
-  T* out = static_cast<T*>(a.out) + row * a.ld_out + base;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    float l = logit_in(in + i);
-    const uint32_t c = a.tokens ? count[i] : 0u;
+  const float* bias = a.bias ? a.bias + row * a.ld_bias : nullptr;
+  const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  auto penalise = [&](float l, uint32_t c) {
     if (c) {
       l = l > 0.f ? l / rep : l * rep;
       const uint32_t k = c & ~kSeen;
       if (k) l = l - freq * static_cast<float>(k) - pres;
     }
-    if (a.bias) l += a.bias[row * a.ld_bias + base + i];
-    if (a.mask && !((a.mask[row * a.ld_mask + ((base + i) >> 5)] >> ((base + i) & 31)) & 1u)) l = -INFINITY;
-    logit_out(out + i, l);
+    return l;
+  };
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) {
+    const int in_chunk = (v * kLogitsThreads + threadIdx.x) * N;
+    const int64_t at = base + in_chunk;
+    if (whole(v)) {
+      float x[N];
+      Vec::unpack(raw[v], x);
+      if (a.tokens) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const uint4 c = *reinterpret_cast<const uint4*>(count + in_chunk + e);
+          if (c.x | c.y | c.z | c.w) {
+            x[e] = penalise(x[e], c.x);
+            x[e + 1] = penalise(x[e + 1], c.y);
+            x[e + 2] = penalise(x[e + 2], c.z);
+            x[e + 3] = penalise(x[e + 3], c.w);
+          }
+        }
+      }
+      if (bias) {
+        if ((reinterpret_cast<uintptr_t>(bias + at) & 15) == 0) {
+#pragma unroll
+          for (int e = 0; e < N; e += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + at + e);
+            x[e] += b.x, x[e + 1] += b.y, x[e + 2] += b.z, x[e + 3] += b.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[e] += bias[at + e];
+        }
+      }
+      if (mask) {
+        const int64_t w = at >> 5;
+        const int sh = static_cast<int>(at & 31);
+        uint32_t bits = mask[w] >> sh;
+        if (sh + N > 32) bits |= mask[w + 1] << (32 - sh);
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (!((bits >> e) & 1u)) x[e] = -INFINITY;
+      }
+      __stcs(reinterpret_cast<uint4*>(out + at), Vec::pack(x));
+    } else {
+      for (int e = 0; e < N; ++e) {
+        const int64_t i = at + e;
+        if (i < 0 || i >= a.V) continue;
+        float l = penalise(Vec::load(in + i), a.tokens ? count[in_chunk + e] : 0u);
+        if (bias) l += bias[i];
+        if (mask && !((mask[i >> 5] >> (i & 31)) & 1u)) l = -INFINITY;
+        Vec::store(out + i, l);
+      }
+    }
   }
 }
 
+template <typename T, typename Tok, int VECS>
+static void launch_logits(const LogitsArgs& a, int64_t B, cudaStream_t s) {
+  constexpr int N = LogitVec<T>::N, kChunk = VECS * kLogitsThreads * N;
+  // a row that starts off a 16-byte boundary reaches up to N - 1 entries further
+  const dim3 grid(static_cast<unsigned>((a.V + N - 1 + kChunk - 1) / kChunk), static_cast<unsigned>(B));
+  logits_kernel<T, Tok, VECS><<<grid, kLogitsThreads, a.tokens ? kChunk * 4 : 0, s>>>(a);
+}
+
+// The longest blocks (4 pieces a thread) that still make four per SM, since each block reads the row's history.
 template <typename T>
-static void launch_logits(const LogitsArgs& a, int token_bytes, dim3 grid, cudaStream_t s) {
+static void run_logits(const LogitsArgs& a, int64_t B, int token_bytes, int sms, cudaStream_t s) {
+  const int64_t pieces = B * ((a.V + LogitVec<T>::N - 1) / LogitVec<T>::N + kLogitsThreads - 1) / kLogitsThreads;
+  const int vecs = pieces >= 16 * sms ? 4 : pieces >= 8 * sms ? 2 : 1;
   if (token_bytes == 8)
-    logits_kernel<T, int64_t><<<grid, 256, 0, s>>>(a);
+    vecs == 4 ? launch_logits<T, int64_t, 4>(a, B, s) : vecs == 2 ? launch_logits<T, int64_t, 2>(a, B, s) : launch_logits<T, int64_t, 1>(a, B, s);
   else
-    logits_kernel<T, int32_t><<<grid, 256, 0, s>>>(a);
+    vecs == 4 ? launch_logits<T, int32_t, 4>(a, B, s) : vecs == 2 ? launch_logits<T, int32_t, 2>(a, B, s) : launch_logits<T, int32_t, 1>(a, B, s);
 }
 
 }  // namespace xdna
@@ -88,23 +230,23 @@ extern "C" int xdna_process_logits(const void* logits, int dtype, int64_t B, int
                                    const int32_t* lens, const int32_t* prompt_lens, const float* repetition,
                                    const float* presence, const float* frequency, const float* bias, int64_t ld_bias,
                                    const uint32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream) {
-  XDNA_CHECK_ARG(B >= 0 && B < 65536 && V >= 0 && V < (1ll << 31) && T >= 0 && T < (1ll << 31),
+  XDNA_CHECK_ARG(B >= 0 && B < 65536 && V >= 0 && V < (1ll << 31) && T >= 0 && T < (1ll << 30),
                  "process_logits: bad sizes (at most 65535 rows)");
   XDNA_CHECK_ARG(is_float_dtype(dtype), "process_logits: f32, bf16 or f16 logits");
   XDNA_CHECK_ARG(tokens == nullptr || token_bytes == 4 || token_bytes == 8, "process_logits: 32 or 64-bit tokens");
-  int rc = check_device(nullptr);
+  int sms = 0;
+  int rc = check_device(&sms);
   if (rc != XDNA_OK) return rc;
   if (B == 0 || V == 0) return XDNA_OK;
-  XDNA_CHECK_ARG(logits && out && ld_in >= 0 && ld_out >= V, "process_logits: null pointer or bad row pitch");
+  XDNA_CHECK_ARG(logits && out && ld_in >= 0 && ld_out >= V && reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype) == 0, "process_logits: null pointer or bad row pitch");
   const LogitsArgs a{logits, out, ld_in, ld_out, V, tokens, T, ld_tokens, lens, prompt_lens, repetition, presence,
                      frequency, bias, ld_bias, mask, ld_mask};
-  const dim3 grid(static_cast<unsigned>((V + kLogitsChunk - 1) / kLogitsChunk), static_cast<unsigned>(B));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == XDNA_F32)
-    launch_logits<float>(a, token_bytes, grid, s);
+    run_logits<float>(a, B, token_bytes, sms, s);
   else if (dtype == XDNA_BF16)
-    launch_logits<__nv_bfloat16>(a, token_bytes, grid, s);
+    run_logits<__nv_bfloat16>(a, B, token_bytes, sms, s);
   else
-    launch_logits<__half>(a, token_bytes, grid, s);
+    run_logits<__half>(a, B, token_bytes, sms, s);
   return check_launch("logits_kernel");
 }

@@ -596,46 +596,247 @@ struct OwnArgs {
   const void *q, *ck, *cv;
   int64_t q_sb, q_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh;
   const int32_t* lens;
-  int B, S, hq, hkv, splits;
+  int B, S, hq, hkv, group;
+  int parts;   // of the prefix: part_o / part_ml [parts + (splits > 1 ? splits : 0)][B * hq]
+  int splits;  // of the own keys
   float scale_log2;
-  const float* part_o;
-  const float2* part_ml;
+  float* part_o;
+  float2* part_ml;
   void* out;
 };
 
-// One warp per row: its own keys one by one, joined with the prefix's parts.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+constexpr int kOwnWarps = 4;
+constexpr int kOwnStep = 16;  // keys of a warp's step
+
+// A sequence's own keys: few rows (the up to 16 query heads of a tile that share a key head) against a cache of its
+// own, so the time is the reading of the cache. One CTA per (sequence, key head, 16 query heads, split); its warps take
+// steps of 16 keys in turn, each with a running softmax of its own, joined at the end. The products are mma.sync 16 x 8
+// x 16 with the query heads as rows (a step's 16 rows are cheap; tcgen05's 128 would not be filled), and K and V go
+// from global memory straight into fragments in 16-byte pieces: of K, lane (g, t) reads columns 32 c + 8 t .. + 7 of
+// key g, which are B fragments when the query's A fragments are read in the same order; of V, columns 64 e + 8 g .. + 7
+// of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, which are, paired by a byte permute, B fragments of the output columns in
+// the order 64 e + 8 n + i.
+// Keys past the length are not read and count as zeros with score -inf.
+// With one split the CTA also joins the prefix's parts and writes the output; else it leaves a part like theirs.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) own_keys_kernel(const OwnArgs a) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + warp_id();
-  if (row >= static_cast<int64_t>(a.B) * a.hq) return;
-  const int b = static_cast<int>(row / a.hq), h = static_cast<int>(row % a.hq), hk = h / (a.hq / a.hkv);
-  float q[D / 32], o[D / 32], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < D / 32; ++i) {
-    q[i] = to_f32(static_cast<const T*>(a.q)[b * a.q_sb + h * a.q_sh + i * 32 + lane_id()]) * a.scale_log2;
-    o[i] = 0.f;
-  }
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = static_cast<int64_t>(s) * a.B * a.hq + row;
-    const float2 ml = a.part_ml[at];
-    const float mn = fmaxf(m, ml.x), f = exp2f(m - mn), w = exp2f(ml.x - mn);
-    m = mn;
-    l = l * f + ml.y * w;
-    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * f + w * a.part_o[at * D + i * 32 + lane_id()];
-  }
+__global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs a) {
+  constexpr bool kBf16 = !__is_same(T, __half);
+  constexpr int kC = D / 32, kE = D / 64;
+  __shared__ float so[kOwnWarps][16][D + 4];
+  __shared__ float2 sml[kOwnWarps][16];
+  const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
+  const int b = static_cast<int>(blockIdx.x) / a.hkv, kvh = static_cast<int>(blockIdx.x) % a.hkv;
+  const int h0 = kvh * a.group + static_cast<int>(blockIdx.z) * 16;              // the tile's first query head
+  const int rows = min(16, a.group - static_cast<int>(blockIdx.z) * 16);
   const int n = min(max(a.lens[b], 0), a.S);
-  for (int s = 0; s < n; ++s) {
-    const T* k = static_cast<const T*>(a.ck) + b * a.ck_sb + s * a.ck_st + hk * a.ck_sh;
-    const T* v = static_cast<const T*>(a.cv) + b * a.cv_sb + s * a.cv_st + hk * a.cv_sh;
-    float z = 0.f;
-    for (int i = 0; i < D / 32; ++i) z += q[i] * to_f32(k[i * 32 + lane_id()]);
-    for (int x = 16; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
-    const float mn = fmaxf(m, z), f = exp2f(m - mn), p = exp2f(z - mn);
-    m = mn;
-    l = l * f + p;
-    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * f + p * to_f32(v[i * 32 + lane_id()]);
+  const int steps = (n + kOwnStep - 1) / kOwnStep, per = (steps + a.splits - 1) / a.splits;
+  const int s0 = min(steps, static_cast<int>(blockIdx.y) * per), s1 = min(steps, s0 + per);
+
+  uint32_t q[kC][2][4];  // rows g and g + 8
+  {
+    const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(h0) * a.q_sh + 8 * t;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint4 u = g + 8 * r < rows ? *reinterpret_cast<const uint4*>(qp + (g + 8 * r) * a.q_sh + 32 * c) : make_uint4(0, 0, 0, 0);
+        q[c][r][0] = u.x, q[c][r][1] = u.y, q[c][r][2] = u.z, q[c][r][3] = u.w;
+      }
+    }
   }
-  T* dst = static_cast<T*>(a.out) + row * D;
-  for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane_id()] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+  float o[kE][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[e][i][0] = o[e][i][1] = o[e][i][2] = o[e][i][3] = 0.f;
+  }
+  const T* kp = static_cast<const T*>(a.ck) + static_cast<int64_t>(b) * a.ck_sb + static_cast<int64_t>(kvh) * a.ck_sh + 8 * t;
+  const T* vp = static_cast<const T*>(a.cv) + static_cast<int64_t>(b) * a.cv_sb + static_cast<int64_t>(kvh) * a.cv_sh + 8 * g;
+  uint4 k[2][kC], v[kE][4];
+  auto load_k = [&](int step) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int key = step * kOwnStep + 8 * r + g;
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        k[r][c] = step < s1 && key < n ? __ldg(reinterpret_cast<const uint4*>(kp + key * a.ck_st + 32 * c)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto load_v = [&](int step) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int key = step * kOwnStep + 2 * t + (x & 1) + 8 * (x >> 1);
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        v[e][x] = key < n ? __ldg(reinterpret_cast<const uint4*>(vp + key * a.cv_st + 64 * e)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load_k(s0 + warp);
+  for (int step = s0 + warp; step < s1; step += kOwnWarps) {
+    load_v(step);
+    float s[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint32_t a0[4] = {q[c][0][0], q[c][1][0], q[c][0][1], q[c][1][1]};
+        const uint32_t a1[4] = {q[c][0][2], q[c][1][2], q[c][0][3], q[c][1][3]};
+        mma_16816<kBf16>(s[r], a0, k[r][c].x, k[r][c].y);
+        mma_16816<kBf16>(s[r], a1, k[r][c].z, k[r][c].w);
+      }
+    }
+    load_k(step + kOwnWarps);
+    // s[r][e]: row g (+ 8 for e >= 2), key 8 r + 2 t + (e & 1) of the step
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[r][e] = step * kOwnStep + 8 * r + 2 * t + (e & 1) < n ? s[r][e] * a.scale_log2 : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[r][e]);
+      }
+    }
+    float f[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      const float mn = fmaxf(m[h], mx[h]);
+      f[h] = mn == -INFINITY ? 1.f : fast_exp2(m[h] - mn);
+      m[h] = mn;
+      l[h] *= f[h];
+    }
+    uint32_t p[4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float base = m[h] == -INFINITY ? 0.f : m[h];
+        const float p0 = fast_exp2(s[r][2 * h] - base), p1 = fast_exp2(s[r][2 * h + 1] - base);
+        l[h] += p0 + p1;
+        p[2 * r + h] = pack2<T>(p0, p1);
+      }
+    }
+    if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[e][i][0] *= f[0], o[e][i][1] *= f[0], o[e][i][2] *= f[1], o[e][i][3] *= f[1];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&v[e][0]);
+      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&v[e][1]);
+      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&v[e][2]);
+      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&v[e][3]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
+        mma_16816<kBf16>(o[e][i], p, __byte_perm(v0[i / 2], v1[i / 2], sel), __byte_perm(v2[i / 2], v3[i / 2], sel));
+      }
+    }
+  }
+  // the warp's part: rows g, g + 8; column n = 2 t + (x & 1) of product i is dimension 64 e + 8 n + i
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (t == 0) sml[warp][g + 8 * h] = make_float2(m[h], l[h]);
+    if (g + 8 * h < rows) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float* dst = &so[warp][g + 8 * h][64 * e + 8 * (2 * t + x)];
+          *reinterpret_cast<float4*>(dst) = make_float4(o[e][0][2 * h + x], o[e][1][2 * h + x], o[e][2][2 * h + x], o[e][3][2 * h + x]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[e][4][2 * h + x], o[e][5][2 * h + x], o[e][6][2 * h + x], o[e][7][2 * h + x]);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // four dimensions per thread
+  const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kOwnWarps * 32) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    const int64_t row = static_cast<int64_t>(b) * a.hq + h0 + r;
+    const int parts = a.splits == 1 ? a.parts : 0;
+    float mm = -INFINITY, ll = 0.f;
+    for (int w = 0; w < kOwnWarps; ++w) mm = fmaxf(mm, sml[w][r].x);
+    for (int s = 0; s < parts; ++s) mm = fmaxf(mm, a.part_ml[s * n_rows + row].x);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 x) {
+      const float f = fast_exp2(ml.x - base);
+      ll = fmaf(f, ml.y, ll);
+      acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+    };
+    for (int w = 0; w < kOwnWarps; ++w) add(sml[w][r], *reinterpret_cast<const float4*>(&so[w][r][d]));
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s)
+      add(a.part_ml[s * n_rows + row], *reinterpret_cast<const float4*>(a.part_o + (s * n_rows + row) * D + d));
+    if (a.splits == 1) {
+      const float inv = ll > 0.f || __isnanf(ll) ? 1.f / ll : 0.f;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * D + d) =
+          make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+    } else {
+      const int64_t at = (a.parts + blockIdx.y) * n_rows + row;
+      *reinterpret_cast<float4*>(a.part_o + at * D + d) = acc;
+      if (d == 0) a.part_ml[at] = make_float2(mm, ll);
+    }
+  }
+}
+
+// One warp per row: the parts' sums brought to one maximum and added, in the parts' order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const float* part_o, const float2* part_ml, int parts, int64_t n_rows, T* out) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp_id();
+  if (row >= n_rows) return;
+  float mm = -INFINITY, ll = 0.f, acc[D / 32];
+  for (int s = lane_id(); s < parts; s += 32) mm = fmaxf(mm, part_ml[s * n_rows + row].x);
+  for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+  const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = part_ml[s * n_rows + row];
+    const float f = fast_exp2(ml.x - base);
+    ll = fmaf(f, ml.y, ll);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(f, part_o[(s * n_rows + row) * D + i * 32 + lane_id()], acc[i]);
+  }
+  const float inv = ll > 0.f || __isnanf(ll) ? 1.f / ll : 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) out[row * D + i * 32 + lane_id()] = from_f32<T>(acc[i] * inv);
+}
+
+template <typename T, int D>
+static int launch_own(const OwnArgs& a, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(a.B * a.hkv), static_cast<unsigned>(a.splits), static_cast<unsigned>((a.group + 15) / 16));
+  own_keys_kernel<T, D><<<grid, kOwnWarps * 32, 0, s>>>(a);
+  int rc = check_launch("own_keys_kernel");
+  if (rc != XDNA_OK || a.splits == 1) return rc;
+  const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
+  join_kernel<T, D><<<static_cast<unsigned>((n_rows + 3) / 4), 128, 0, s>>>(a.part_o, a.part_ml, a.parts + a.splits, n_rows,
+                                                                            static_cast<T*>(a.out));
+  return check_launch("join_kernel");
 }
 
 // ---------------------------------------------------------------------------- host
@@ -697,16 +898,21 @@ static int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtens
 
 static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { return tokens / (2 * (128 / group)) + n_seqs; }
 
-// Key splits of a prefix: about one item per SM, each at least one block.
+// How a prefix call is split: the prefix's keys into about one item per SM, each at least one block; a sequence's own
+// keys, where the sequences and key heads alone are fewer than two CTAs per SM, into pieces of at least 128 (a CTA's
+// two steps per warp).
 struct PrefixSplit {
-  int64_t pairs, splits, blocks_per_split;
-  PrefixSplit(int64_t B, int64_t P, int64_t hq, int64_t hkv, int sms) {
+  int64_t pairs, parts, blocks_per_part, own;
+  PrefixSplit(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int sms) {
     const int64_t tok = 128 / (hq / hkv), blocks = (P + kTaBlock - 1) / kTaBlock;
     pairs = (B + 2 * tok - 1) / (2 * tok);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(blocks, sms / (pairs * hkv)));
-    blocks_per_split = blocks ? (blocks + want - 1) / want : 0;
-    splits = blocks ? (blocks + blocks_per_split - 1) / blocks_per_split : 0;
+    blocks_per_part = blocks ? (blocks + want - 1) / want : 0;
+    parts = blocks ? (blocks + blocks_per_part - 1) / blocks_per_part : 0;
+    const int64_t ctas = B * hkv * ((hq / hkv + 15) / 16);
+    own = std::max<int64_t>(1, std::min<int64_t>((S + 127) / 128, 2 * sms / ctas));
   }
+  int64_t all() const { return parts + (own > 1 ? own : 0); }
 };
 
 }  // namespace xdna
@@ -773,11 +979,10 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
 }
 
 size_t xdna_prefix_attention_workspace(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d) {
-  if (B < 1 || P < 1 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
+  if (B < 1 || P < 0 || S < 0 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
   int sms = 0;
   if (check_device(&sms) != XDNA_OK) return 0;
-  const PrefixSplit split(B, P, hq, hkv, sms);
-  return static_cast<size_t>(split.splits * B * hq) * (sizeof(float2) + d * sizeof(float));
+  return static_cast<size_t>(PrefixSplit(B, P, S, hq, hkv, sms).all() * B * hq) * (sizeof(float2) + d * sizeof(float));
 }
 
 int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* pk, int64_t pk_st, int64_t pk_sh,
@@ -796,14 +1001,14 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
                      (S == 0 || (row_ok(ck, ck_sb, ck_st, ck_sh) && row_ok(cv, cv_sb, cv_st, cv_sh))) && lens && out &&
                      aligned16(out),
                  "prefix_attention: operands must be 16-byte aligned with strides that are positive multiples of 8");
-  XDNA_CHECK_ARG(P == 0 || (workspace && aligned16(workspace) &&
-                            workspace_bytes >= xdna_prefix_attention_workspace(B, P, S, hq, hkv, d)),
+  const size_t need = xdna_prefix_attention_workspace(B, P, S, hq, hkv, d);
+  XDNA_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                  "prefix_attention: workspace too small or unaligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t group = hq / hkv, tok = 128 / group;
-  const PrefixSplit split(B, P, hq, hkv, sms);
+  const PrefixSplit split(B, P, S, hq, hkv, sms);
   float* part_o = static_cast<float*>(workspace);
-  float2* part_ml = reinterpret_cast<float2*>(part_o + split.splits * B * hq * d);
+  float2* part_ml = reinterpret_cast<float2*>(part_o + split.all() * B * hq * d);
   if (P > 0) {
     TileArgs a{};
     a.hq = static_cast<int>(hq);
@@ -815,8 +1020,8 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
     a.B = static_cast<int>(B);
     a.P = static_cast<int>(P);
     a.pairs = static_cast<int>(split.pairs);
-    a.splits = static_cast<int>(split.splits);
-    a.blocks_per_split = static_cast<int>(split.blocks_per_split);
+    a.splits = static_cast<int>(split.parts);
+    a.blocks_per_split = static_cast<int>(split.blocks_per_part);
     a.part_o = part_o;
     a.part_ml = part_ml;
     CUtensorMap tq, tk, tv;
@@ -824,18 +1029,28 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
         (rc = kv_map(&tk, pk, pk_st, pk_sh, P, hkv, d, dtype)) != XDNA_OK ||
         (rc = kv_map(&tv, pv, pv_st, pv_sh, P, hkv, d, dtype)) != XDNA_OK)
       return rc;
-    const int64_t items = split.pairs * hkv * split.splits;
+    const int64_t items = split.pairs * hkv * split.parts;
     if ((rc = launch_tiles<PREFIX>(tq, tk, tv, a, d, dtype, static_cast<int>(std::min<int64_t>(items, sms)), s)) != XDNA_OK)
       return rc;
   }
-  const OwnArgs o{q, ck, cv, q_sb, q_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh, lens, (int)B, (int)S, (int)hq,
-                  (int)hkv, (int)split.splits, scale * 1.4426950408889634f, part_o, part_ml, out};
-  const unsigned g = static_cast<unsigned>((B * hq + 7) / 8);
-  if (dtype == XDNA_BF16)
-    d == 128 ? own_keys_kernel<__nv_bfloat16, 128><<<g, 256, 0, s>>>(o) : own_keys_kernel<__nv_bfloat16, 64><<<g, 256, 0, s>>>(o);
-  else
-    d == 128 ? own_keys_kernel<__half, 128><<<g, 256, 0, s>>>(o) : own_keys_kernel<__half, 64><<<g, 256, 0, s>>>(o);
-  return check_launch("own_keys_kernel");
+  OwnArgs o{};
+  o.q = q, o.ck = ck, o.cv = cv;
+  o.q_sb = q_sb, o.q_sh = q_sh;
+  o.ck_sb = ck_sb, o.ck_st = ck_st, o.ck_sh = ck_sh, o.cv_sb = cv_sb, o.cv_st = cv_st, o.cv_sh = cv_sh;
+  o.lens = lens;
+  o.B = static_cast<int>(B);
+  o.S = static_cast<int>(S);
+  o.hq = static_cast<int>(hq);
+  o.hkv = static_cast<int>(hkv);
+  o.group = static_cast<int>(group);
+  o.parts = static_cast<int>(split.parts);
+  o.splits = static_cast<int>(split.own);
+  o.scale_log2 = scale * 1.4426950408889634f;
+  o.part_o = part_o;
+  o.part_ml = part_ml;
+  o.out = out;
+  if (dtype == XDNA_BF16) return d == 128 ? launch_own<__nv_bfloat16, 128>(o, s) : launch_own<__nv_bfloat16, 64>(o, s);
+  return d == 128 ? launch_own<__half, 128>(o, s) : launch_own<__half, 64>(o, s);
 }
 
 }  // extern "C"

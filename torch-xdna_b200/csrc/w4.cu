@@ -4,6 +4,8 @@
 // Codes are stored in blocks of 128 columns (64 bytes, K padded with code 8 to whole blocks): the block's runs of
 // eight columns r = 4 w + t lie as 32-bit words at place 4 t + w, and in a word the eight codes lie in the column
 // order 0, 2, 4, 6, 1, 3, 5, 7 from the lowest bits.
+#include <algorithm>
+
 #include "host_util.h"
 #include "sm100.cuh"
 
@@ -36,31 +38,290 @@ struct W4Args {
   const void* scales;
   const void* bias;
   void* y;
-  int64_t ldy, M, N, K, row_bytes, n_groups;
-  int x_dtype, scale_dtype, bias_dtype, group;
+  int64_t ldy;
+  int M, N, K, blocks, n_groups;  // blocks of 128 columns
+  int x_dtype, scale_dtype, bias_dtype;
+  int rows;     // x rows of a pass (blockIdx.y)
+  int ks_log2;  // warps that share a tile, each with every 2^ks-th block
+  int chunk;    // blocks of x in shared memory at a time
 };
 
-// One warp per output: lane l takes the words l, l + 32, ... of the row.
-__global__ void __launch_bounds__(256) w4_kernel(const W4Args a) {
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + warp_id(), m = blockIdx.y;
-  if (n >= a.N) return;
-  const uint32_t* row = reinterpret_cast<const uint32_t*>(a.codes + n * a.row_bytes);
-  float acc = 0.f;
-  for (int64_t i = lane_id(); i < a.row_bytes / 4; i += 32) {
-    const int place = static_cast<int>(i & 15);
-    const int64_t col = (i >> 4) * kW4Block + ((place & 3) * 4 + (place >> 2)) * 8;
-    if (col >= a.K) continue;
-    const uint32_t word = row[i];
-    float part = 0.f;
-    for (int c = 0; c < 8 && col + c < a.K; ++c)
-      part += (static_cast<float>((word >> w4_shift(c)) & 15u) - 8.f) * load_f32(a.x, a.x_dtype, m * a.ldx + col + c);
-    acc += part * load_f32(a.scales, a.scale_dtype, n * a.n_groups + col / a.group);
+// The linear as tensor-core products of 16 weight rows by 8 (NT times) x rows, with the weights as the A operand: a
+// decode step has few x rows, so its time is the reading of the codes, and what has to be kept small is the work per
+// code. A warp takes tiles of 16 weight rows; per block of 128 columns each lane copies 16 bytes (32 codes) of two
+// rows into its own place of a ring in shared memory (cp.async, kW4Stages blocks ahead, so that enough bytes are in
+// flight), and every 32-bit word of them is, after a mask and an or per pair, two registers of A fragments: codes are
+// stored so that a word's pairs are neighbouring columns and the four lanes of a fragment row hold one group of 32.
+// (code - 8) is exact in bf16 and f16, so the products are exact; they are summed in f32 over a group, and then
+// multiplied by the group's scale into the f32 accumulators.
+// f32 x: each value is the exact sum of three bf16 numbers (truncated high, middle and low 8 bits), which take three
+// of the x rows of a product and are added at the end; so the result has the accuracy of f32 sums.
+// x lies in shared memory, 64 bytes off a multiple of 128 per row, which makes the B fragments' loads free of conflicts.
+// Tiles are few for small N: then 2, 4 or 8 warps share one and add their sums in shared memory in a fixed order.
+constexpr int kW4Stages = 6;
+constexpr int kW4Threads = 256;
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The codes at bits 0..3 and 16..19 of w as two exact values code - 8: 128 + code (bf16: ulp 1 at 128) or 1024 + code
+// (f16) by setting the exponent, minus 136 or 1032.
+template <bool BF16>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  const uint32_t u = (w & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
+  if constexpr (BF16) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __floats2bfloat162_rn(136.f, 136.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane_id() == 0) {
-    if (a.bias) acc += load_f32(a.bias, a.bias_dtype, n);
-    store_f32(a.y, a.x_dtype, m * a.ldy + n, acc);
+}
+
+// XT: x's type (XDNA_F32 as three bf16 parts per value).
+template <int XT, int NT, int GROUP>
+__global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
+  constexpr bool kBf16 = XT != XDNA_F16;
+  constexpr int kParts = XT == XDNA_F32 ? 3 : 1, kPer = kW4Block / GROUP;  // groups per block
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
+  const int ks = 1 << a.ks_log2, kslice = warp & (ks - 1), wt = warp >> a.ks_log2, tiles_per_cta = 8 >> a.ks_log2;
+  const int m0 = blockIdx.y * a.rows, m_rows = min(a.rows, a.M - m0), v_rows = m_rows * kParts;
+  const int pitch = a.chunk * kW4Block * 2 + 64;
+  uint8_t* ring = smem + warp * (kW4Stages * 1024);
+  uint8_t* smx = smem + 8 * kW4Stages * 1024;
+  float* red = reinterpret_cast<float*>(smx + ((a.rows * kParts * pitch + 127) & ~127));  // [warp][16][NT * 8]
+  const int n_tiles = (a.N + 15) / 16, n_sets = (n_tiles + tiles_per_cta - 1) / tiles_per_cta;
+  const int64_t row_bytes = static_cast<int64_t>(a.blocks) * 64;
+
+  // this warp's (set of tiles, block) sequence, kW4Stages ahead of its use; the scales of rows g and g + 8 in one
+  // register per stage
+  uint32_t sc[kW4Stages];
+  int p_set = blockIdx.x, p_blk = kslice, p_stage = 0;
+  auto prefetch = [&]() -> uint32_t {
+    uint32_t s = 0;
+    if (p_set < n_sets && p_blk < a.blocks) {
+      const int n = (p_set * tiles_per_cta + wt) * 16 + g;
+      const uint8_t* src = a.codes + n * row_bytes + p_blk * 64 + t * 16;
+      const uint32_t dst = smem_u32(ring + p_stage * 1024 + lane * 16);
+      cp_async_16(dst, n < a.N ? src : a.codes, n < a.N);
+      cp_async_16(dst + 512, n + 8 < a.N ? src + 8 * row_bytes : a.codes, n + 8 < a.N);
+      const int grp = p_blk * kPer + (kPer > 1 ? t % kPer : 0);
+      const uint16_t* sp = static_cast<const uint16_t*>(a.scales) + static_cast<int64_t>(n) * a.n_groups + grp;
+      if (grp < a.n_groups) {
+        if (n < a.N) s = sp[0];
+        if (n + 8 < a.N) s |= static_cast<uint32_t>(sp[static_cast<int64_t>(8) * a.n_groups]) << 16;
+      }
+      p_blk += ks;
+      if (p_blk >= a.blocks) {
+        p_blk = kslice;
+        p_set += gridDim.x;
+      }
+    }
+    p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return s;
+  };
+  if (kslice < a.blocks) {
+#pragma unroll
+    for (int i = 0; i < kW4Stages; ++i) sc[i] = prefetch();
   }
+  int stage = 0;
+
+  auto stage_x = [&](int b0, int nb) {
+    const int cols = nb * kW4Block, k0 = b0 * kW4Block;
+    if constexpr (kParts == 1) {
+      const uint16_t* x = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(m0) * a.ldx + k0;
+      if ((reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx % 8 == 0) {
+        const int per = cols / 8;
+        for (int i = threadIdx.x; i < m_rows * per; i += kW4Threads) {
+          const int r = i / per, c = (i - r * per) * 8;
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (k0 + c + 8 <= a.K) {
+            u = *reinterpret_cast<const uint4*>(x + r * a.ldx + c);
+          } else {
+            uint16_t* h = reinterpret_cast<uint16_t*>(&u);
+            for (int e = 0; e < 8; ++e)
+              if (k0 + c + e < a.K) h[e] = x[r * a.ldx + c + e];
+          }
+          *reinterpret_cast<uint4*>(smx + r * pitch + c * 2) = u;
+        }
+      } else {
+        for (int i = threadIdx.x; i < m_rows * cols; i += kW4Threads) {
+          const int r = i / cols, c = i - r * cols;
+          *reinterpret_cast<uint16_t*>(smx + r * pitch + c * 2) = k0 + c < a.K ? x[r * a.ldx + c] : uint16_t(0);
+        }
+      }
+    } else {
+      const float* x = static_cast<const float*>(a.x) + static_cast<int64_t>(m0) * a.ldx + k0;
+      for (int i = threadIdx.x; i < m_rows * cols; i += kW4Threads) {
+        const int r = i / cols, c = i - r * cols;
+        const float v = k0 + c < a.K ? x[r * a.ldx + c] : 0.f;
+        const bool fin = fabsf(v) < INFINITY;
+        const __nv_bfloat16 hi = fin ? __float2bfloat16_rz(v) : __float2bfloat16_rn(v);
+        const float r1 = fin ? v - __bfloat162float(hi) : 0.f;
+        const __nv_bfloat16 mid = __float2bfloat16_rz(r1);
+        const __nv_bfloat16 lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
+        __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(smx + 3 * r * pitch + c * 2);
+        d[0] = hi;
+        d[pitch / 2] = mid;
+        d[pitch] = lo;
+      }
+    }
+  };
+  auto scale_of = [&](uint32_t bits16) {
+    return a.scale_dtype == XDNA_BF16 ? __uint_as_float(bits16 << 16)
+                                      : __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
+  };
+  auto finish = [&](int m, int n, float v) {
+    if (a.bias) v += load_f32(a.bias, a.bias_dtype, n);
+    store_f32(a.y, XT, (m0 + m) * a.ldy + n, v);
+  };
+
+  bool staged = false;
+  for (int set = blockIdx.x; set < n_sets; set += gridDim.x) {
+    float acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    for (int b0 = 0; b0 < a.blocks; b0 += a.chunk) {
+      const int b1 = min(a.blocks, b0 + a.chunk);
+      if (!staged || a.chunk < a.blocks) {
+        if (staged) __syncthreads();
+        stage_x(b0, b1 - b0);
+        __syncthreads();
+        staged = true;
+      }
+      for (int blk = b0 + kslice; blk < b1; blk += ks) {  // b0 is a multiple of ks
+        asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages - 1) : "memory");
+        const uint8_t* mine = ring + stage * 1024 + lane * 16;
+        const uint4 lo4 = *reinterpret_cast<const uint4*>(mine), hi4 = *reinterpret_cast<const uint4*>(mine + 512);
+        const uint32_t s_now = sc[0];
+#pragma unroll
+        for (int i = 0; i + 1 < kW4Stages; ++i) sc[i] = sc[i + 1];
+        sc[kW4Stages - 1] = prefetch();  // into the stage just read (by this lane alone)
+        stage = stage + 1 == kW4Stages ? 0 : stage + 1;
+        const uint32_t wl[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, wh[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+        const uint8_t* xb = smx + (blk - b0) * (kW4Block * 2) + t * 16;
+        float part[NT][4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if ((w * 32) % GROUP == 0) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
+          }
+          const uint32_t a0[4] = {code_pair<kBf16>(wl[w]), code_pair<kBf16>(wh[w]), code_pair<kBf16>(wl[w] >> 4),
+                                  code_pair<kBf16>(wh[w] >> 4)};
+          const uint32_t a1[4] = {code_pair<kBf16>(wl[w] >> 8), code_pair<kBf16>(wh[w] >> 8),
+                                  code_pair<kBf16>(wl[w] >> 12), code_pair<kBf16>(wh[w] >> 12)};
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            uint4 b = make_uint4(0, 0, 0, 0);
+            if (i * 8 + g < v_rows) b = *reinterpret_cast<const uint4*>(xb + (i * 8 + g) * pitch + w * 64);
+            mma_16816<kBf16>(part[i], a0, b.x, b.y);
+            mma_16816<kBf16>(part[i], a1, b.z, b.w);
+          }
+          if ((w * 32 + 32) % GROUP == 0) {
+            const uint32_t s2 = kPer > 1 ? __shfl_sync(0xffffffffu, s_now, (lane & ~3) + w * 32 / GROUP) : s_now;
+            const float sl = scale_of(s2 & 0xffffu), sh = scale_of(s2 >> 16);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              acc[i][0] = fmaf(part[i][0], sl, acc[i][0]);
+              acc[i][1] = fmaf(part[i][1], sl, acc[i][1]);
+              acc[i][2] = fmaf(part[i][2], sh, acc[i][2]);
+              acc[i][3] = fmaf(part[i][3], sh, acc[i][3]);
+            }
+          }
+        }
+      }
+    }
+    const int n0 = (set * tiles_per_cta + wt) * 16;
+    if (kParts == 1 && ks == 1) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = i * 8 + 2 * t + (e & 1), n = n0 + g + (e >> 1) * 8;
+          if (m < m_rows && n < a.N) finish(m, n, acc[i][e]);
+        }
+      }
+      continue;
+    }
+    float* mine = red + warp * (16 * NT * 8);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(g + (e >> 1) * 8) * (NT * 8) + i * 8 + 2 * t + (e & 1)] = acc[i][e];
+    }
+    const bool alone = ks == 1;
+    if (alone) __syncwarp(); else __syncthreads();
+    // outputs: all warps' tiles, or this warp's alone
+    const int n_out = (alone ? 16 : tiles_per_cta * 16), step = alone ? 32 : kW4Threads;
+    for (int i = alone ? lane : threadIdx.x; i < n_out * m_rows; i += step) {
+      const int r = i % n_out, m = i / n_out;
+      const int tile = alone ? wt : r >> 4, n = (set * tiles_per_cta + tile) * 16 + (r & 15);
+      if (n >= a.N) continue;
+      float v = 0.f;
+      for (int p = kParts - 1; p >= 0; --p)  // small parts first
+        for (int s = 0; s < ks; ++s) v += red[((tile * ks + s) * 16 + (r & 15)) * (NT * 8) + m * kParts + p];
+      finish(m, n, v);
+    }
+    if (alone) __syncwarp(); else __syncthreads();
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <int XT, int NT>
+static int launch_w4(W4Args& a, int group, dim3 grid, int smem, cudaStream_t s) {
+  auto kern = group == 32 ? w4_kernel<XT, NT, 32> : group == 64 ? w4_kernel<XT, NT, 64> : w4_kernel<XT, NT, 128>;
+  static std::atomic<bool> configured[3][64];  // setting the attribute twice from two threads is harmless
+  const int gi = group / 64;
+  int dev = 0;
+  XDNA_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[gi][dev].load(std::memory_order_acquire)) {
+    XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    if (dev >= 0 && dev < 64) configured[gi][dev].store(true, std::memory_order_release);
+  }
+  kern<<<grid, kW4Threads, smem, s>>>(a);
+  return check_launch("w4_kernel");
+}
+
+template <int XT>
+static int run_w4(W4Args& a, int group, int sms, cudaStream_t s) {
+  constexpr int kParts = XT == XDNA_F32 ? 3 : 1;
+  // a pass takes up to 32 x rows (10 of f32); more run as further passes over the codes, which the L2 then holds
+  a.rows = std::min(a.M, 32 / kParts);
+  const int v_rows = a.rows * kParts, nt = v_rows <= 8 ? 1 : v_rows <= 16 ? 2 : 4;
+  // warps per tile: enough warps to fill the SMs (16 each), as long as each has a block
+  const int n_tiles = (a.N + 15) / 16;
+  a.ks_log2 = 0;
+  while (a.ks_log2 < 3 && (n_tiles << a.ks_log2) < 16 * sms && (2 << a.ks_log2) <= a.blocks) ++a.ks_log2;
+  // x in shared memory, whole where it fits in 96 KB (two CTAs per SM)
+  const int ks = 1 << a.ks_log2;
+  a.chunk = std::min(a.blocks, std::max(1, (96 * 1024 / v_rows - 64) / 256));
+  if (a.chunk < a.blocks) a.chunk = std::max(ks, a.chunk / ks * ks);
+  const int pitch = a.chunk * kW4Block * 2 + 64;
+  const int smem = 8 * kW4Stages * 1024 + (v_rows * pitch + 127) / 128 * 128 + 8 * 16 * nt * 8 * 4;
+  const int sets = (n_tiles + (8 >> a.ks_log2) - 1) / (8 >> a.ks_log2);
+  // with one warp per tile the CTAs are persistent, so that x is staged once per CTA
+  const dim3 grid(static_cast<unsigned>(ks == 1 ? std::min(sets, 2 * sms) : sets),
+                  static_cast<unsigned>((a.M + a.rows - 1) / a.rows));
+  return nt == 1 ? launch_w4<XT, 1>(a, group, grid, smem, s)
+                 : nt == 2 ? launch_w4<XT, 2>(a, group, grid, smem, s) : launch_w4<XT, 4>(a, group, grid, smem, s);
 }
 
 // s = max |w| / 7 over the group, rounded to the scales' type; code = clamp(rint(w / s), -8, 7) + 8, 8 where s is 0.
@@ -97,7 +358,7 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const void* w, int dt, int
 }
 
 static int check_w4(const char* what, int64_t N, int64_t K, int group, int scale_dtype) {
-  XDNA_CHECK_ARG(N >= 0 && N < (1ll << 31) && K >= 1 && K < (1ll << 31), "%s: bad sizes", what);
+  XDNA_CHECK_ARG(N >= 0 && N < (1ll << 30) && K >= 1 && K < (1ll << 24), "%s: bad sizes", what);
   XDNA_CHECK_ARG(group == 32 || group == 64 || group == 128, "%s: groups of 32, 64 or 128 columns", what);
   XDNA_CHECK_ARG(scale_dtype == XDNA_BF16 || scale_dtype == XDNA_F16, "%s: scales in bf16 or f16", what);
   return XDNA_OK;
@@ -131,14 +392,29 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
   if (rc != XDNA_OK) return rc;
   XDNA_CHECK_ARG(M >= 0 && M < 65536 && ldx >= K && ldy >= N && is_float_dtype(x_dtype), "linear_w4: bad x or y");
   XDNA_CHECK_ARG(bias == nullptr || is_float_dtype(bias_dtype), "linear_w4: bad bias type");
-  if ((rc = check_device(nullptr)) != XDNA_OK) return rc;
+  int sms = 0;
+  if ((rc = check_device(&sms)) != XDNA_OK) return rc;
   if (M == 0 || N == 0) return XDNA_OK;
   XDNA_CHECK_ARG(x && codes && scales && y && aligned16(codes), "linear_w4: null pointer or unaligned codes");
-  const W4Args a{x, ldx, codes, scales, bias, y, ldy, M, N, K, (K + kW4Block - 1) / kW4Block * 64,
-                 (K + group - 1) / group, x_dtype, scale_dtype, bias_dtype, group};
-  w4_kernel<<<dim3(static_cast<unsigned>((N + 7) / 8), static_cast<unsigned>(M)), 256, 0,
-              static_cast<cudaStream_t>(stream)>>>(a);
-  return check_launch("w4_kernel");
+  W4Args a{};
+  a.x = x;
+  a.ldx = ldx;
+  a.codes = codes;
+  a.scales = scales;
+  a.bias = bias;
+  a.y = y;
+  a.ldy = ldy;
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.blocks = static_cast<int>((K + kW4Block - 1) / kW4Block);
+  a.n_groups = static_cast<int>((K + group - 1) / group);
+  a.x_dtype = x_dtype;
+  a.scale_dtype = scale_dtype;
+  a.bias_dtype = bias_dtype;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return x_dtype == XDNA_F32 ? run_w4<XDNA_F32>(a, group, sms, s)
+                             : x_dtype == XDNA_BF16 ? run_w4<XDNA_BF16>(a, group, sms, s) : run_w4<XDNA_F16>(a, group, sms, s);
 }
 
 }  // extern "C"
