@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   uint64_t* r_full = bars + 2;               // [kStages]
   uint64_t* r_empty = r_full + kStages;      // [kStages]
   uint64_t* s_full = r_empty + kStages;      // [tile] S ready (and every earlier product of the tile done)
-  uint64_t* p_full = s_full + 2;             // [tile] P written and O rescaled
-  uint64_t* o_full = p_full + 2;             // [tile] the item's last product done
+  uint64_t* p_full = s_full + 2;             // [tile][half] 64 columns of P written, and O rescaled
+  uint64_t* o_full = p_full + 4;             // [tile] the item's last product done
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + t, 1);
-      mbar_init(p_full + t, 4);
+      mbar_init(p_full + 2 * t, 4);
+      mbar_init(p_full + 2 * t + 1, 4);
       mbar_init(o_full + t, 1);
     }
     mbar_init(drain, 1);
@@ -295,13 +296,16 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         issued = true;
       };
       auto issue_pv = [&](int t, int i, bool first) -> bool {
-        if (!mbar_wait(p_full + t, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
-        ++p_seen[t];
-        tc_fence_after();
         const uint32_t tO = tmem + 256 + 128 * t, tP = tmem + 128 * t;
         const uint64_t dV = smem_desc_mn_sw128(smem_u32(ring(i)), kBlk);
+        for (int h = 0; h < 2; ++h) {
+          if (!mbar_wait(p_full + 2 * t + h, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
+          tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < 8; ++k) umma_f16_ts(tO, tP + 8 * k, dV + 128 * k, IDESC_O, (!first || k) != 0);
+          for (int k = 4 * h; k < 4 * h + 4; ++k) umma_f16_ts(tO, tP + 8 * k, dV + 128 * k, IDESC_O, (!first || k) != 0);
+          issued = true;
+        }
+        ++p_seen[t];
         return true;
       };
       TileItem it;
@@ -359,7 +363,6 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         o[i < head ? i : one_end * row + i - head] = make_uint4(0, 0, 0, 0);
     }
     bool ok = true;
-    uint32_t v[128];                         // this row of S
     int g = 0, items = 0;                    // key blocks and items of this tile so far
     TileItem it;
     for (int n = 0; ok && item(n, it); ++n) {
@@ -374,26 +377,34 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         tc_fence_after();
         __syncwarp();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(v + c * 32));
-        tmem_ld_wait();
         // the last key of this block that the row sees
         const int last = MODE == PACKED ? pos - j * kTaBlock : args.P - 1 - it.kv_tok - j * kTaBlock;
-        if (__any_sync(0xffffffffu, last < kTaBlock - 1)) {
+        const bool masked = __any_sync(0xffffffffu, last < kTaBlock - 1);
+        // S is read twice, 32 columns at a time and one piece ahead, rather than kept in 128 registers
+        uint32_t v[2][32];
+        auto mask = [&](uint32_t(&x)[32], int c) {
+          if (masked) {
 #pragma unroll
-          for (int e = 0; e < 128; ++e)
-            if (e > last) v[e] = __float_as_uint(-INFINITY);
-        }
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e > last) x[e] = __float_as_uint(-INFINITY);
+          }
+        };
         float m8[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = __uint_as_float(v[i]);
+        for (int i = 0; i < 8; ++i) m8[i] = -INFINITY;
+        tmem_ld_32x32b_x32(tS, v[0]);
 #pragma unroll
-        for (int e = 8; e + 16 <= 128; e += 16) {
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait(v[c & 1]);
+          tmem_ld_32x32b_x32(tS + (c < 3 ? c + 1 : 0) * 32, v[(c + 1) & 1]);
+          uint32_t(&x)[32] = v[c & 1];
+          mask(x, c);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m8[i] = fmax3(m8[i], __uint_as_float(v[e + i]), __uint_as_float(v[e + 8 + i]));
+          for (int e = 0; e < 32; e += 16) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m8[i] = fmax3(m8[i], __uint_as_float(x[e + i]), __uint_as_float(x[e + 8 + i]));
+          }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(m8[i], __uint_as_float(v[120 + i]));
         const float m_blk = fmaxf(fmax3(m8[0], m8[1], m8[2]), fmaxf(fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * sc;
         float alpha = 1.f;
         const bool raise = m_blk > m_use + kTaRescale;
@@ -403,15 +414,15 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         if (j >= 1 && __any_sync(0xffffffffu, raise)) {
           // S(j) was issued after O += P(j-1) V(j-1), so O is complete
-          uint32_t o[32];
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
             __syncwarp();
-            tmem_ld_32x32b_x32(tO + c * 32, o);
+            tmem_ld_32x32b_x16(tO + c * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32b_x32(tO + c * 32, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32b_x16(tO + c * 16, o);
           }
         }
         l *= alpha;
@@ -419,23 +430,30 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[32];
+        for (int c = 0; c < 4; ++c) {
+          __syncwarp();
+          tmem_ld_wait(v[c & 1]);  // piece c (the first was asked for above)
+          if (c < 3) tmem_ld_32x32b_x32(tS + (c + 1) * 32, v[(c + 1) & 1]);
+          uint32_t(&x)[32] = v[c & 1];
+          mask(x, c);
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[c * 64 + e]), __uint_as_float(v[c * 64 + e + 1])), sc2, nm2);
-            const float2 pp = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          for (int e = 0; e < 32; e += 2) {
+            const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, nm2);
+            const float2 pp = make_float2(fast_exp2(z.x), fast_exp2(z.y));
             rs4[(e >> 1) & 3] = __fadd2_rn(rs4[(e >> 1) & 3], pp);
             w[e / 2] = pack2<T>(pp.x, pp.y);
           }
-          __syncwarp();
-          tmem_st_32x32b_x32(tS + c * 32, w);
+          tmem_st_32x32b_x16(tS + c * 16, w);  // over columns of S already read
+          if (c & 1) {
+            // half of P is ready: its share of the product may start
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 2 * t + (c >> 1));
+          }
         }
         l += ((rs4[0].x + rs4[0].y) + (rs4[1].x + rs4[1].y)) + ((rs4[2].x + rs4[2].y) + (rs4[3].x + rs4[3].y));
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + t);
       }
       if (!ok || !mbar_wait(o_full + t, items & 1, abort_flag, args.err, 48)) break;
       ++items;
