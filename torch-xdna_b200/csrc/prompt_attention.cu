@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   uint8_t* smR = smQ + 2 * kTile;            // ring: [stage][k-block]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smR + kStages * kTile);
   uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
+  uint64_t* q_empty = bars + 1;              // the softmaxes have seen the item's last S: Q may be reloaded
   uint64_t* r_full = bars + 2;               // [kStages]
-  uint64_t* r_empty = r_full + kStages;      // [kStages]
+  uint64_t* r_empty = r_full + kStages;      // [kStages] likewise, 2 arrivals
   uint64_t* s_full = r_empty + kStages;      // [tile] S ready (and every earlier product of the tile done)
   uint64_t* p_full = s_full + 2;             // [tile][half] 64 columns of P written, and O rescaled
   uint64_t* o_full = p_full + 4;             // [tile] the item's last product done
@@ -156,10 +156,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(r_full + s, 1);
-      mbar_init(r_empty + s, 1);
+      mbar_init(r_empty + s, 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + t, 1);
@@ -279,16 +279,14 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     if (lane == 0) {
       // ------------------------------------------------------------------ MMA
       bool ok = true, issued = false;
-      int g = 0;             // ring blocks consumed
-      int p_seen[2] = {0, 0};
-      auto ring = [&](int i) { return smR + (i % kStages) * kTile; };
+      int g = 0, p_seen[2] = {0, 0};  // ring blocks, and each tile's P so far
       auto wait_ring = [&](int i) { return mbar_wait(r_full + i % kStages, (i / kStages) & 1, abort_flag, args.err, 43); };
       auto issue_s = [&](int t, int i) {
         const uint32_t tS = tmem + 128 * t;
+        const uint32_t block = smem_u32(smR + (i % kStages) * kTile), q = smem_u32(smQ + t * kTile);
 #pragma unroll
         for (int kk = 0; kk < kKB; ++kk) {
-          const uint64_t dQ = smem_desc_k_sw128(smem_u32(smQ + t * kTile + kk * kBlk));
-          const uint64_t dK = smem_desc_k_sw128(smem_u32(ring(i) + kk * kBlk));
+          const uint64_t dQ = smem_desc_k_sw128(q + kk * kBlk), dK = smem_desc_k_sw128(block + kk * kBlk);
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_f16(tS, dQ + 2 * k, dK + 2 * k, IDESC_S, (kk | k) != 0);
         }
@@ -297,13 +295,13 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       };
       auto issue_pv = [&](int t, int i, bool first) -> bool {
         const uint32_t tO = tmem + 256 + 128 * t, tP = tmem + 128 * t;
-        const uint64_t dV = smem_desc_mn_sw128(smem_u32(ring(i)), kBlk);
+        const uint64_t dV = smem_desc_mn_sw128(smem_u32(smR + (i % kStages) * kTile), kBlk);
         for (int h = 0; h < 2; ++h) {
           if (!mbar_wait(p_full + 2 * t + h, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
           tc_fence_after();
 #pragma unroll
-          for (int k = 4 * h; k < 4 * h + 4; ++k) umma_f16_ts(tO, tP + 8 * k, dV + 128 * k, IDESC_O, (!first || k) != 0);
-          issued = true;
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tO, tP + 32 * h + 8 * k, dV + 512 * h + 128 * k, IDESC_O, (!first || h || k) != 0);
         }
         ++p_seen[t];
         return true;
@@ -315,27 +313,20 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         tc_fence_after();
         for (int t = 0; t < 2; ++t)
           if (it.nb[t] > 0) issue_s(t, g);
-        umma_commit(r_empty + g % kStages);
-        if (nb == 1) umma_commit(q_empty);
         for (int j = 0; ok && j < nb; ++j, g += 2) {
           // ring block g = K_j, g + 1 = V_j, g + 2 = K_{j+1}
           if (!wait_ring(g + 1) || (j + 1 < nb && !wait_ring(g + 2))) {
             ok = false;
             break;
           }
-          for (int t = 0; ok && t < 2; ++t) {
+          for (int t = 0; t < 2; ++t) {
             if (j >= it.nb[t]) continue;
-            ok = issue_pv(t, g + 1, j == 0);
-            if (!ok) break;
+            if (!(ok = issue_pv(t, g + 1, j == 0))) break;
             if (j + 1 < it.nb[t])
               issue_s(t, g + 2);
             else
               umma_commit(o_full + t);
           }
-          if (!ok) break;
-          umma_commit(r_empty + (g + 1) % kStages);
-          if (j + 1 < nb) umma_commit(r_empty + (g + 2) % kStages);
-          if (j + 2 == nb) umma_commit(q_empty);
         }
       }
       if (issued) {
@@ -363,11 +354,16 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         o[i < head ? i : one_end * row + i - head] = make_uint4(0, 0, 0, 0);
     }
     bool ok = true;
-    int g = 0, items = 0;                    // key blocks and items of this tile so far
+    int g = 0, items = 0, ring = 0;          // key blocks and items of this tile, ring blocks before this item
     TileItem it;
-    for (int n = 0; ok && item(n, it); ++n) {
-      const int nb = it.nb[t];
+    for (int n = 0; ok && item(n, it); ring += 2 * max(it.nb[0], it.nb[1]), ++n) {
+      const int nb = it.nb[t], other = it.nb[t ^ 1];
       if (nb == 0) continue;
+      // one arrival of the two for this tile, both where the other tile has no part
+      auto release = [&](uint64_t* bar, bool both) {
+        if (qd == 0 && lane == 0) mbar_arrive_n(bar, both ? 2u : 1u);
+      };
+      auto stage = [&](int i) { return r_empty + (ring + i) % kStages; };
       const int pos = it.q_pos + t * args.tok + r_tok;  // PACKED: place in the sequence
       float m_use = -INFINITY, l = 0.f;
       for (int j = 0; j < nb; ++j, ++g) {
@@ -377,6 +373,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         tc_fence_after();
         __syncwarp();
+        // S(j) is done, and with it the product with V_{j-1}: K_j and V_{j-1} may be overwritten, after the last S Q too
+        release(stage(2 * j), j >= other);
+        if (j > 0) release(stage(2 * j - 1), j - 1 >= other);
+        if (j + 1 == nb) release(q_empty, other == 0);
         // the last key of this block that the row sees
         const int last = MODE == PACKED ? pos - j * kTaBlock : args.P - 1 - it.kv_tok - j * kTaBlock;
         const bool masked = __any_sync(0xffffffffu, last < kTaBlock - 1);
@@ -457,6 +457,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       }
       if (!ok || !mbar_wait(o_full + t, items & 1, abort_flag, args.err, 48)) break;
       ++items;
+      release(stage(2 * nb - 1), nb - 1 >= other);
       tc_fence_after();
       const int tok = it.q_tok + t * args.tok + r_tok;
       const int head = it.kvh * args.group + r_head;
