@@ -200,13 +200,14 @@ at::Tensor linear_w4(PyObject* const* a) {
   REQUIRE(!bias || (bias->dim() == 1 && bias->size(0) == N && code(bias->scalar_type()) >= 0), XDNA_ERR_INVALID,
           "bias: [N] in f32, bf16 or f16");
   Place place(name, x, {&codes, &scales, in(bias)});
+  const at::Tensor sc = reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4 ? scales.clone() : scales;
   at::Tensor x2 = x.dim() == 2 ? x : x.reshape({x.numel() / K, K});
   const int64_t M = x2.size(0);
   if (x2.stride(1) != 1 || (M > 1 && x2.stride(0) < K)) x2 = x2.clone(at::MemoryFormat::Contiguous);
   if (bias && !bias->is_contiguous()) bias = bias->contiguous();
   at::Tensor y = at::empty({M, N}, x.options());
   check(name, xdna_linear_w4(x2.data_ptr(), code(x.scalar_type()), M, K, M > 1 ? x2.stride(0) : K,
-                             codes.data_ptr<uint8_t>(), scales.data_ptr(), code(scales.scalar_type()),
+                             codes.data_ptr<uint8_t>(), sc.data_ptr(), code(scales.scalar_type()),
                              static_cast<int>(group), N, ptr(bias), bias ? code(bias->scalar_type()) : XDNA_F32,
                              y.data_ptr(), N, place.stream));
   if (x.dim() == 2) return y;

@@ -24,7 +24,6 @@ struct LogitsArgs {
 };
 
 constexpr int kLogitsThreads = 256;
-constexpr uint32_t kSeen = 0x80000000u;  // in the counter of an entry: it is among the row's tokens
 
 template <typename T>
 struct LogitVec;  // 16 bytes of logits
@@ -84,116 +83,144 @@ struct LogitVec<__half> {
   static __device__ __forceinline__ void store(__half* p, float x) { *p = __float2half_rn(x); }
 };
 
-// A block takes VECS x 256 pieces of 16 bytes of one row. The pieces are loaded first; while they are on their way the
-// block clears its counters and counts the row's tokens that fall into its entries (integer sums in shared memory, so
-// their order does not matter); then each piece is worked on in registers and written. The row is cut at 16-byte
-// boundaries of its own address, so rows of any pitch are read and written in whole pieces except at their two ends.
+// A block takes VECS x 256 pieces of 16 bytes of one row. The loads go out first: the thread's first tokens, its
+// logits, bias and mask words. While they are on their way the block clears a bitmap and its counters; then it marks
+// and counts the row's tokens that fall into its entries (integer sums in shared memory, so their order does not
+// matter), and each piece is worked on in registers and written; only pieces with a marked entry look at the counters.
+// The row is cut at 16-byte boundaries of its own address, so rows of any pitch are read and written in whole pieces
+// except at their two ends.
 // HBM-bound; the history is read once per block, from the L2, so the blocks are as long as still fill the machine.
 template <typename T, typename Tok, int VECS>
-__global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const LogitsArgs a) {
   using Vec = LogitVec<T>;
   constexpr int N = Vec::N, kChunk = VECS * kLogitsThreads * N;
+  constexpr int M = 16 / sizeof(Tok), kAhead = 2;    // tokens of a piece, pieces of the history loaded ahead
   extern __shared__ __align__(16) uint32_t count[];  // [kChunk] (with tokens)
+  __shared__ uint32_t marked[kChunk / 32];
   const int64_t row = blockIdx.y;
   const T* in = static_cast<const T*>(a.in) + row * a.ld_in;
   T* out = static_cast<T*>(a.out) + row * a.ld_out;
+  const int V = static_cast<int>(a.V), tid = threadIdx.x;
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
   // entries [base, base + kChunk) of the row, those outside [0, V) left out; in + base is on a 16-byte boundary
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kChunk - shift;
+  const int base = static_cast<int>(blockIdx.x) * kChunk - shift;
   const bool pieces = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(in)) & 15) == 0;
-  auto whole = [&](int v) {
-    const int64_t at = base + (v * kLogitsThreads + threadIdx.x) * N;
-    return pieces && at >= 0 && at + N <= a.V;
-  };
-  uint4 raw[VECS];
-#pragma unroll
-  for (int v = 0; v < VECS; ++v)
-    if (whole(v)) raw[v] = __ldcs(reinterpret_cast<const uint4*>(in + base) + v * kLogitsThreads + threadIdx.x);
+
+  // the history up to T, whatever the row's length: it is cut when counting
+  const Tok* tok = static_cast<const Tok*>(a.tokens) + row * a.ld_tokens;
+  const int T_ = static_cast<int>(a.T);
+  const int head = min(T_, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(tok) & 15)) % 16 / sizeof(Tok)));
+  uint4 ahead[kAhead];
+  int len = T_, prompt = 0;
   if (a.tokens) {
 #pragma unroll
-    for (int v = 0; v < VECS * N / 4; ++v) reinterpret_cast<uint4*>(count)[v * kLogitsThreads + threadIdx.x] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    const int len = a.lens ? min(max(a.lens[row], 0), static_cast<int>(a.T)) : static_cast<int>(a.T);
-    const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
-    const Tok* tok = static_cast<const Tok*>(a.tokens) + row * a.ld_tokens;
-    auto put = [&](int i, Tok id) {
-      const int64_t at = static_cast<int64_t>(id) - base;
-      if (id < 0 || at < 0 || at >= kChunk) return;
-      atomicOr(&count[at], kSeen);
-      if (i >= prompt) atomicAdd(&count[at], 1u);
-    };
-    constexpr int M = 16 / sizeof(Tok);
-    const int head = min(len, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(tok) & 15)) % 16 / sizeof(Tok)));
-    if (static_cast<int>(threadIdx.x) < head) put(threadIdx.x, tok[threadIdx.x]);
-    int i = head + static_cast<int>(threadIdx.x) * M;
-#pragma unroll 2
-    for (; i + M <= len; i += kLogitsThreads * M) {
-      Tok id[M];
-      *reinterpret_cast<uint4*>(id) = *reinterpret_cast<const uint4*>(tok + i);
-#pragma unroll
-      for (int e = 0; e < M; ++e) put(i + e, id[e]);
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = head + (i * kLogitsThreads + tid) * M;
+      if (at + M <= T_) ahead[i] = *reinterpret_cast<const uint4*>(tok + at);
     }
-    for (int e = 0; e < M; ++e)
-      if (i + e < len) put(i + e, tok[i + e]);
-    __syncthreads();
+    if (a.lens) len = min(max(a.lens[row], 0), T_);
+    if (a.prompt_lens) prompt = a.prompt_lens[row];
   }
   const float rep = a.rep ? a.rep[row] : 1.f, pres = a.pres ? a.pres[row] : 0.f, freq = a.freq ? a.freq[row] : 0.f;
+  auto whole = [&](int at) { return pieces && at >= 0 && at + N <= V; };
+  uint4 raw[VECS];
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) {
+    const int at = base + (v * kLogitsThreads + tid) * N;
+    if (whole(at)) raw[v] = __ldcs(reinterpret_cast<const uint4*>(in + at));
+  }
   const float* bias = a.bias ? a.bias + row * a.ld_bias : nullptr;
-  const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
-  auto penalise = [&](float l, uint32_t c) {
-    if (c) {
-      l = l > 0.f ? l / rep : l * rep;
-      const uint32_t k = c & ~kSeen;
-      if (k) l = l - freq * static_cast<float>(k) - pres;
+  const bool wide_bias = bias && (reinterpret_cast<uintptr_t>(bias + base) & 15) == 0;
+  float4 b[VECS][N / 4];
+  if (wide_bias) {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = base + (v * kLogitsThreads + tid) * N;
+#pragma unroll
+      for (int e = 0; e < N / 4; ++e)
+        if (whole(at)) b[v][e] = reinterpret_cast<const float4*>(bias + at)[e];
     }
-    return l;
+  }
+  const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  uint32_t allowed[VECS];
+  if (mask) {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int at = base + (v * kLogitsThreads + tid) * N, sh = at & 31;
+      if (whole(at)) {
+        allowed[v] = mask[at >> 5] >> sh;
+        if (sh + N > 32) allowed[v] |= mask[(at >> 5) + 1] << (32 - sh);
+      }
+    }
+  }
+  if (a.tokens) {
+#pragma unroll
+    for (int i = 0; i < kChunk / 4 / kLogitsThreads; ++i) reinterpret_cast<uint4*>(count)[i * kLogitsThreads + tid] = make_uint4(0, 0, 0, 0);
+    if (tid < kChunk / 32) marked[tid] = 0;
+    __syncthreads();
+    auto put = [&](int i, Tok id) {
+      if (i >= len || id < 0 || id >= V) return;
+      const int at = static_cast<int>(id) - base;
+      if (at < 0 || at >= kChunk) return;
+      atomicOr(&marked[at >> 5], 1u << (at & 31));
+      if (i >= prompt) atomicAdd(&count[at], 1u);
+    };
+    if (tid < head) put(tid, tok[tid]);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = head + (i * kLogitsThreads + tid) * M;
+      if (at + M > T_) continue;
+#pragma unroll
+      for (int e = 0; e < M; ++e) put(at + e, reinterpret_cast<const Tok*>(&ahead[i])[e]);
+    }
+    const int rest = head + (T_ - head) / M * M;
+    for (int at = head + (kAhead * kLogitsThreads + tid) * M; at < min(len, rest); at += kLogitsThreads * M) {
+      const uint4 u = *reinterpret_cast<const uint4*>(tok + at);
+#pragma unroll
+      for (int e = 0; e < M; ++e) put(at + e, reinterpret_cast<const Tok*>(&u)[e]);
+    }
+    if (rest + tid < T_) put(rest + tid, tok[rest + tid]);  // fewer than M
+    __syncthreads();
+  }
+  auto penalise = [&](float l, int at) {
+    l = l > 0.f ? l / rep : l * rep;
+    const uint32_t c = count[at];
+    return c ? l - freq * static_cast<float>(c) - pres : l;
   };
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
-    const int in_chunk = (v * kLogitsThreads + threadIdx.x) * N;
-    const int64_t at = base + in_chunk;
-    if (whole(v)) {
+    const int in_chunk = (v * kLogitsThreads + tid) * N, at = base + in_chunk;
+    const uint32_t hit = a.tokens ? marked[in_chunk >> 5] >> (in_chunk & 31) & ((1u << N) - 1) : 0;
+    if (whole(at)) {
       float x[N];
       Vec::unpack(raw[v], x);
-      if (a.tokens) {
-#pragma unroll
-        for (int e = 0; e < N; e += 4) {
-          const uint4 c = *reinterpret_cast<const uint4*>(count + in_chunk + e);
-          if (c.x | c.y | c.z | c.w) {
-            x[e] = penalise(x[e], c.x);
-            x[e + 1] = penalise(x[e + 1], c.y);
-            x[e + 2] = penalise(x[e + 2], c.z);
-            x[e + 3] = penalise(x[e + 3], c.w);
-          }
-        }
-      }
-      if (bias) {
-        if ((reinterpret_cast<uintptr_t>(bias + at) & 15) == 0) {
-#pragma unroll
-          for (int e = 0; e < N; e += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(bias + at + e);
-            x[e] += b.x, x[e + 1] += b.y, x[e + 2] += b.z, x[e + 3] += b.w;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) x[e] += bias[at + e];
-        }
-      }
-      if (mask) {
-        const int64_t w = at >> 5;
-        const int sh = static_cast<int>(at & 31);
-        uint32_t bits = mask[w] >> sh;
-        if (sh + N > 32) bits |= mask[w + 1] << (32 - sh);
+      if (hit) {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (!((bits >> e) & 1u)) x[e] = -INFINITY;
+          if (hit >> e & 1) x[e] = penalise(x[e], in_chunk + e);
+      }
+      if (wide_bias) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const float4 f = b[v][e / 4];
+          x[e] += f.x, x[e + 1] += f.y, x[e + 2] += f.z, x[e + 3] += f.w;
+        }
+      } else if (bias) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] += bias[at + e];
+      }
+      if (mask) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (!(allowed[v] >> e & 1)) x[e] = -INFINITY;
       }
       __stcs(reinterpret_cast<uint4*>(out + at), Vec::pack(x));
     } else {
       for (int e = 0; e < N; ++e) {
-        const int64_t i = at + e;
-        if (i < 0 || i >= a.V) continue;
-        float l = penalise(Vec::load(in + i), a.tokens ? count[in_chunk + e] : 0u);
+        const int i = at + e;
+        if (i < 0 || i >= V) continue;
+        float l = Vec::load(in + i);
+        if (hit >> e & 1) l = penalise(l, in_chunk + e);
         if (bias) l += bias[i];
         if (mask && !((mask[i >> 5] >> (i & 31)) & 1u)) l = -INFINITY;
         Vec::store(out + i, l);
@@ -230,7 +257,7 @@ extern "C" int xdna_process_logits(const void* logits, int dtype, int64_t B, int
                                    const int32_t* lens, const int32_t* prompt_lens, const float* repetition,
                                    const float* presence, const float* frequency, const float* bias, int64_t ld_bias,
                                    const uint32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream) {
-  XDNA_CHECK_ARG(B >= 0 && B < 65536 && V >= 0 && V < (1ll << 31) && T >= 0 && T < (1ll << 30),
+  XDNA_CHECK_ARG(B >= 0 && B < 65536 && V >= 0 && V < (1ll << 30) && T >= 0 && T < (1ll << 30),
                  "process_logits: bad sizes (at most 65535 rows)");
   XDNA_CHECK_ARG(is_float_dtype(dtype), "process_logits: f32, bf16 or f16 logits");
   XDNA_CHECK_ARG(tokens == nullptr || token_bytes == 4 || token_bytes == 8, "process_logits: 32 or 64-bit tokens");

@@ -638,12 +638,18 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
 constexpr int kOwnWarps = 4;
-constexpr int kOwnStep = 16;  // keys of a warp's step
+constexpr int kOwnStep = 16;   // keys of a warp's step
+constexpr int kOwnStages = 3;  // steps under way per warp
 
 // A sequence's own keys: few rows (the up to 16 query heads of a tile that share a key head) against a cache of its
 // own, so the time is the reading of the cache. One CTA per (sequence, key head, 16 query heads, split); its warps take
-// steps of 16 keys in turn, each with a running softmax of its own, joined at the end. The products are mma.sync 16 x 8
+// steps of 16 keys in turn, with three steps' copies under way (cp.async: 24 KB per warp, 192 KB per SM), each with a
+// running softmax of its own, joined at the end. The products are mma.sync 16 x 8
 // x 16 with the query heads as rows (a step's 16 rows are cheap; tcgen05's 128 would not be filled), and K and V go
 // from global memory straight into fragments in 16-byte pieces: of K, lane (g, t) reads columns 32 c + 8 t .. + 7 of
 // key g, which are B fragments when the query's A fragments are read in the same order; of V, columns 64 e + 8 g .. + 7
@@ -655,7 +661,10 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs a) {
   constexpr bool kBf16 = !__is_same(T, __half);
   constexpr int kC = D / 32, kE = D / 64;
-  __shared__ float so[kOwnWarps][16][D + 4];
+  constexpr int kStageBytes = 2 * kC * 2 * 512;  // a step's K and V, 16 bytes of each lane per piece
+  extern __shared__ __align__(16) uint8_t own_smem[];
+  uint8_t* ring = own_smem + warp_id() * (kOwnStages * kStageBytes);
+  float(*so)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(own_smem);  // the warps' sums, once the ring is done
   __shared__ float2 sml[kOwnWarps][16];
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
   const int b = static_cast<int>(blockIdx.x) / a.hkv, kvh = static_cast<int>(blockIdx.x) % a.hkv;
@@ -685,28 +694,33 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
   }
   const T* kp = static_cast<const T*>(a.ck) + static_cast<int64_t>(b) * a.ck_sb + static_cast<int64_t>(kvh) * a.ck_sh + 8 * t;
   const T* vp = static_cast<const T*>(a.cv) + static_cast<int64_t>(b) * a.cv_sb + static_cast<int64_t>(kvh) * a.cv_sh + 8 * g;
-  uint4 k[2][kC], v[kE][4];
-  auto load_k = [&](int step) {
+  // Each lane copies its pieces of K (8 r + g, c) and V (x, e) and reads back just them: no barrier is needed.
+  auto fetch = [&](int step, int st) {
+    if (step < s1) {
+      const uint32_t dst = smem_u32(ring + st * kStageBytes + lane * 16);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int key = step * kOwnStep + 8 * r + g;
+      for (int r = 0; r < 2; ++r) {
+        const int key = step * kOwnStep + 8 * r + g;
+        const T* src = kp + (key < n ? key : 0) * a.ck_st;
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-        k[r][c] = step < s1 && key < n ? __ldg(reinterpret_cast<const uint4*>(kp + key * a.ck_st + 32 * c)) : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < kC; ++c) cp_async_16(dst + (r * kC + c) * 512, src + 32 * c, key < n);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int key = step * kOwnStep + 2 * t + (x & 1) + 8 * (x >> 1);
+        const T* src = vp + (key < n ? key : 0) * a.cv_st;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) cp_async_16(dst + (2 * kC + e * 4 + x) * 512, src + 64 * e, key < n);
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto load_v = [&](int step) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int key = step * kOwnStep + 2 * t + (x & 1) + 8 * (x >> 1);
-#pragma unroll
-      for (int e = 0; e < kE; ++e)
-        v[e][x] = key < n ? __ldg(reinterpret_cast<const uint4*>(vp + key * a.cv_st + 64 * e)) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  load_k(s0 + warp);
-  for (int step = s0 + warp; step < s1; step += kOwnWarps) {
-    load_v(step);
+  for (int i = 0; i < kOwnStages; ++i) fetch(s0 + warp + i * kOwnWarps, i);
+  int st = 0;
+  for (int step = s0 + warp; step < s1; step += kOwnWarps, st = st + 1 == kOwnStages ? 0 : st + 1) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kOwnStages - 1) : "memory");
+    const uint4* mine = reinterpret_cast<const uint4*>(ring + st * kStageBytes) + lane;
     float s[2][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -715,11 +729,11 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
       for (int c = 0; c < kC; ++c) {
         const uint32_t a0[4] = {q[c][0][0], q[c][1][0], q[c][0][1], q[c][1][1]};
         const uint32_t a1[4] = {q[c][0][2], q[c][1][2], q[c][0][3], q[c][1][3]};
-        mma_16816<kBf16>(s[r], a0, k[r][c].x, k[r][c].y);
-        mma_16816<kBf16>(s[r], a1, k[r][c].z, k[r][c].w);
+        const uint4 k = mine[(r * kC + c) * 32];
+        mma_16816<kBf16>(s[r], a0, k.x, k.y);
+        mma_16816<kBf16>(s[r], a1, k.z, k.w);
       }
     }
-    load_k(step + kOwnWarps);
     // s[r][e]: row g (+ 8 for e >= 2), key 8 r + 2 t + (e & 1) of the step
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -760,17 +774,20 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
     }
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&v[e][0]);
-      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&v[e][1]);
-      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&v[e][2]);
-      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&v[e][3]);
+      const uint4 u0 = mine[(2 * kC + e * 4) * 32], u1 = mine[(2 * kC + e * 4 + 1) * 32], u2 = mine[(2 * kC + e * 4 + 2) * 32],
+                  u3 = mine[(2 * kC + e * 4 + 3) * 32];
+      const uint32_t v0[4] = {u0.x, u0.y, u0.z, u0.w}, v1[4] = {u1.x, u1.y, u1.z, u1.w}, v2[4] = {u2.x, u2.y, u2.z, u2.w},
+                     v3[4] = {u3.x, u3.y, u3.z, u3.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
         mma_16816<kBf16>(o[e][i], p, __byte_perm(v0[i / 2], v1[i / 2], sel), __byte_perm(v2[i / 2], v3[i / 2], sel));
       }
     }
+    fetch(step + kOwnStages * kOwnWarps, st);  // into the stage just read
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
   // the warp's part: rows g, g + 8; column n = 2 t + (x & 1) of product i is dimension 64 e + 8 n + i
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -849,7 +866,17 @@ __global__ void __launch_bounds__(128) join_kernel(const float* part_o, const fl
 template <typename T, int D>
 static int launch_own(const OwnArgs& a, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.B * a.hkv), static_cast<unsigned>(a.splits), static_cast<unsigned>((a.group + 15) / 16));
-  own_keys_kernel<T, D><<<grid, kOwnWarps * 32, 0, s>>>(a);
+  constexpr int kSmem = kOwnWarps * kOwnStages * (D / 32) * 2048;
+  static_assert(kSmem >= kOwnWarps * 16 * (D + 4) * 4, "the sums lie where the ring was");
+  auto kern = own_keys_kernel<T, D>;
+  static std::atomic<bool> configured[64];  // setting the attribute twice from two threads is harmless
+  int dev = 0;
+  XDNA_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  kern<<<grid, kOwnWarps * 32, kSmem, s>>>(a);
   int rc = check_launch("own_keys_kernel");
   if (rc != XDNA_OK || a.splits == 1) return rc;
   const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;

@@ -42,27 +42,37 @@ struct W4Args {
   int M, N, K, blocks, n_groups;  // blocks of 128 columns
   int x_dtype, scale_dtype, bias_dtype;
   int rows;     // x rows of a pass (blockIdx.y)
-  int ks_log2;  // warps that share a tile, each with every 2^ks-th block
+  int ks_log2;  // warps that share a tile
   int chunk;    // blocks of x in shared memory at a time
+  int run;      // of these, a warp's
 };
 
 // The linear as tensor-core products of 16 weight rows by 8 (NT times) x rows, with the weights as the A operand: a
 // decode step has few x rows, so its time is the reading of the codes, and what has to be kept small is the work per
-// code. A warp takes tiles of 16 weight rows; per block of 128 columns each lane copies 16 bytes (32 codes) of two
-// rows into its own place of a ring in shared memory (cp.async, kW4Stages blocks ahead, so that enough bytes are in
-// flight), and every 32-bit word of them is, after a mask and an or per pair, two registers of A fragments: codes are
-// stored so that a word's pairs are neighbouring columns and the four lanes of a fragment row hold one group of 32.
+// code. A warp takes tiles of 16 weight rows. Each lane copies its codes (16 bytes, 32 codes, of each block of the rows
+// g and g + 8) and its share of the scales into the warp's ring in shared memory, kW4Blocks blocks to a stage and
+// kW4Stages stages ahead (cp.async), so that the addresses are worked out once per stage. Every 32-bit word of the
+// codes is, after a shift, a mask-and-or and a subtraction per pair, two registers of A fragments: codes are stored so
+// that a word's pairs are neighbouring columns and the four lanes of a fragment row hold one group of 32.
 // (code - 8) is exact in bf16 and f16, so the products are exact; they are summed in f32 over a group, and then
 // multiplied by the group's scale into the f32 accumulators.
 // f32 x: each value is the exact sum of three bf16 numbers (truncated high, middle and low 8 bits), which take three
 // of the x rows of a product and are added at the end; so the result has the accuracy of f32 sums.
 // x lies in shared memory, 64 bytes off a multiple of 128 per row, which makes the B fragments' loads free of conflicts.
-// Tiles are few for small N: then 2, 4 or 8 warps share one and add their sums in shared memory in a fixed order.
-constexpr int kW4Stages = 6;
+// Tiles are few for small N: then 2, 4 or 8 warps share one, each with a run of its blocks, and add their sums in
+// shared memory in a fixed order.
+constexpr int kW4Blocks = 4;
+constexpr int kW4Stages = 2;
 constexpr int kW4Threads = 256;
+constexpr int w4_stage_bytes(int group) { return kW4Blocks * 1024 + kW4Block / group * 256; }  // a warp's codes and scales
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// 4 bytes, of which the first n (2 or 4) are read and the others are zeros.
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
 template <bool BF16>
@@ -83,14 +93,13 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
 // (f16) by setting the exponent, minus 136 or 1032.
 template <bool BF16>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  const uint32_t u = (w & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u);
-  if constexpr (BF16) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __floats2bfloat162_rn(136.f, 136.f));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
+  uint32_t u, r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(u) : "r"(w), "r"(0x000f000fu), "r"(BF16 ? 0x43004300u : 0x64006400u));  // (w & mask) | exponent
+  if constexpr (BF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0x3f803f80u), "r"(0xc308c308u));  // u * 1 - 136
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0x3c003c00u), "r"(0xe408e408u));  // u * 1 - 1032
+  return r;
 }
 
 // XT: x's type (XDNA_F32 as three bf16 parts per value).
@@ -98,49 +107,90 @@ template <int XT, int NT, int GROUP>
 __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
   constexpr bool kBf16 = XT != XDNA_F16;
   constexpr int kParts = XT == XDNA_F32 ? 3 : 1, kPer = kW4Block / GROUP;  // groups per block
+  constexpr int kStageBytes = w4_stage_bytes(GROUP);
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
   const int ks = 1 << a.ks_log2, kslice = warp & (ks - 1), wt = warp >> a.ks_log2, tiles_per_cta = 8 >> a.ks_log2;
   const int m0 = blockIdx.y * a.rows, m_rows = min(a.rows, a.M - m0), v_rows = m_rows * kParts;
   const int pitch = a.chunk * kW4Block * 2 + 64;
-  uint8_t* ring = smem + warp * (kW4Stages * 1024);
-  uint8_t* smx = smem + 8 * kW4Stages * 1024;
+  uint8_t* ring = smem + warp * (kW4Stages * kStageBytes);
+  uint8_t* smx = smem + 8 * kW4Stages * kStageBytes;
   float* red = reinterpret_cast<float*>(smx + ((a.rows * kParts * pitch + 127) & ~127));  // [warp][16][NT * 8]
   const int n_tiles = (a.N + 15) / 16, n_sets = (n_tiles + tiles_per_cta - 1) / tiles_per_cta;
   const int64_t row_bytes = static_cast<int64_t>(a.blocks) * 64;
 
-  // this warp's (set of tiles, block) sequence, kW4Stages ahead of its use; the scales of rows g and g + 8 in one
-  // register per stage
-  uint32_t sc[kW4Stages];
-  int p_set = blockIdx.x, p_blk = kslice, p_stage = 0;
-  auto prefetch = [&]() -> uint32_t {
-    uint32_t s = 0;
-    if (p_set < n_sets && p_blk < a.blocks) {
-      const int n = (p_set * tiles_per_cta + wt) * 16 + g;
-      const uint8_t* src = a.codes + n * row_bytes + p_blk * 64 + t * 16;
-      const uint32_t dst = smem_u32(ring + p_stage * 1024 + lane * 16);
-      cp_async_16(dst, n < a.N ? src : a.codes, n < a.N);
-      cp_async_16(dst + 512, n + 8 < a.N ? src + 8 * row_bytes : a.codes, n + 8 < a.N);
-      const int grp = p_blk * kPer + (kPer > 1 ? t % kPer : 0);
-      const uint16_t* sp = static_cast<const uint16_t*>(a.scales) + static_cast<int64_t>(n) * a.n_groups + grp;
-      if (grp < a.n_groups) {
-        if (n < a.N) s = sp[0];
-        if (n + 8 < a.N) s |= static_cast<uint32_t>(sp[static_cast<int64_t>(8) * a.n_groups]) << 16;
-      }
-      p_blk += ks;
-      if (p_blk >= a.blocks) {
-        p_blk = kslice;
-        p_set += gridDim.x;
-      }
-    }
-    p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    return s;
+  // What a warp does, in order: its tile of each set of tiles, of it its run of each chunk of blocks, of it stages of
+  // kW4Blocks blocks. prefetch() walks this order kW4Stages ahead of the use.
+  int p_set = blockIdx.x, p_b0 = 0, p_blk = kslice * a.run, p_stage = 0;
+  const uint8_t *p_lo = nullptr, *p_hi = nullptr;
+  int64_t p_slo = 0, p_shi = 0;  // where the rows' scales start, plus t: lane t copies every fourth scale of a row
+  bool p_inner = false;          // there are rows after these
+  auto start_tile = [&]() {
+    // rows past N repeat the last one: their results are not used
+    const int n = min((p_set * tiles_per_cta + wt) * 16 + g, a.N - 1), n8 = min(n + 8, a.N - 1);
+    p_lo = a.codes + n * row_bytes + t * 16;
+    p_hi = a.codes + n8 * row_bytes + t * 16;
+    p_slo = static_cast<int64_t>(n) * a.n_groups + t;
+    p_shi = static_cast<int64_t>(n8) * a.n_groups + t;
+    p_inner = n8 < a.N - 1;
   };
-  if (kslice < a.blocks) {
+  if (p_set < n_sets) start_tile();
+  auto prefetch = [&]() {
+    // the next stage with blocks, if there is one
+    int end = 0;
+    while (p_set < n_sets && p_blk >= (end = min(a.blocks, p_b0 + min(a.chunk, (kslice + 1) * a.run)))) {
+      p_b0 += a.chunk;
+      if (p_b0 >= a.blocks) {
+        p_b0 = 0;
+        p_set += gridDim.x;
+        if (p_set < n_sets) start_tile();
+      }
+      p_blk = p_b0 + kslice * a.run;
+    }
+    if (p_set < n_sets) {
+      const uint32_t dst = smem_u32(ring + p_stage * kStageBytes) + lane * 16;
+      const uint32_t dst_s = smem_u32(ring + p_stage * kStageBytes) + kW4Blocks * 1024 + lane * 4;
+      const uint8_t *lo = p_lo + p_blk * 64, *hi = p_hi + p_blk * 64;
+      // a scale is copied as the aligned 4 bytes that hold it
+      const uint16_t* sc = static_cast<const uint16_t*>(a.scales);
+      const uint16_t *slo = sc + ((p_slo + p_blk * kPer) & ~int64_t(1)), *shi = sc + ((p_shi + p_blk * kPer) & ~int64_t(1));
+      if (p_blk + kW4Blocks <= end && (p_inner || p_blk + kW4Blocks < a.blocks)) {
 #pragma unroll
-    for (int i = 0; i < kW4Stages; ++i) sc[i] = prefetch();
-  }
+        for (int u = 0; u < kW4Blocks; ++u) {
+          cp_async_16(dst + u * 1024, lo + u * 64);
+          cp_async_16(dst + u * 1024 + 512, hi + u * 64);
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          cp_async_4(dst_s + j * 256, slo + 4 * j, 4);
+          cp_async_4(dst_s + j * 256 + 128, shi + 4 * j, 4);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < kW4Blocks; ++u) {
+          if (p_blk + u < end) {
+            cp_async_16(dst + u * 1024, lo + u * 64);
+            cp_async_16(dst + u * 1024 + 512, hi + u * 64);
+          }
+        }
+        const uint16_t* sc_last = sc + (static_cast<int64_t>(a.N) * a.n_groups - 1);
+        const int groups = min(a.n_groups, end * kPer);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (p_blk * kPer + 4 * j + t < groups) {  // the array's last scale may stand alone in its word
+            cp_async_4(dst_s + j * 256, slo + 4 * j, slo + 4 * j < sc_last ? 4 : 2);
+            cp_async_4(dst_s + j * 256 + 128, shi + 4 * j, shi + 4 * j < sc_last ? 4 : 2);
+          }
+        }
+      }
+      p_blk += kW4Blocks;
+    }
+    p_stage ^= 1;
+    static_assert(kW4Stages == 2, "two stages");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kW4Stages; ++i) prefetch();
   int stage = 0;
 
   auto stage_x = [&](int b0, int nb) {
@@ -162,91 +212,119 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
           *reinterpret_cast<uint4*>(smx + r * pitch + c * 2) = u;
         }
       } else {
-        for (int i = threadIdx.x; i < m_rows * cols; i += kW4Threads) {
-          const int r = i / cols, c = i - r * cols;
-          *reinterpret_cast<uint16_t*>(smx + r * pitch + c * 2) = k0 + c < a.K ? x[r * a.ldx + c] : uint16_t(0);
+        for (int r = 0; r < m_rows; ++r) {
+#pragma unroll 8
+          for (int c = threadIdx.x; c < cols; c += kW4Threads)
+            *reinterpret_cast<uint16_t*>(smx + r * pitch + c * 2) = k0 + c < a.K ? x[r * a.ldx + c] : uint16_t(0);
         }
       }
     } else {
       const float* x = static_cast<const float*>(a.x) + static_cast<int64_t>(m0) * a.ldx + k0;
-      for (int i = threadIdx.x; i < m_rows * cols; i += kW4Threads) {
-        const int r = i / cols, c = i - r * cols;
-        const float v = k0 + c < a.K ? x[r * a.ldx + c] : 0.f;
-        const bool fin = fabsf(v) < INFINITY;
-        const __nv_bfloat16 hi = fin ? __float2bfloat16_rz(v) : __float2bfloat16_rn(v);
-        const float r1 = fin ? v - __bfloat162float(hi) : 0.f;
-        const __nv_bfloat16 mid = __float2bfloat16_rz(r1);
-        const __nv_bfloat16 lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
-        __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(smx + 3 * r * pitch + c * 2);
-        d[0] = hi;
-        d[pitch / 2] = mid;
-        d[pitch] = lo;
+      // four values per thread at a time, so that their loads are under way together
+      for (int r = 0; r < m_rows; ++r) {
+        for (int c0 = threadIdx.x; c0 < cols; c0 += 4 * kW4Threads) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = c0 + e * kW4Threads;
+            v[e] = c < cols && k0 + c < a.K ? x[r * a.ldx + c] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = c0 + e * kW4Threads;
+            if (c >= cols) break;
+            const bool fin = fabsf(v[e]) < INFINITY;
+            const __nv_bfloat16 hi = fin ? __float2bfloat16_rz(v[e]) : __float2bfloat16_rn(v[e]);
+            const float r1 = fin ? v[e] - __bfloat162float(hi) : 0.f;
+            const __nv_bfloat16 mid = __float2bfloat16_rz(r1);
+            const __nv_bfloat16 lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
+            __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(smx + 3 * r * pitch + c * 2);
+            d[0] = hi;
+            d[pitch / 2] = mid;
+            d[pitch] = lo;
+          }
+        }
       }
     }
   };
-  auto scale_of = [&](uint32_t bits16) {
-    return a.scale_dtype == XDNA_BF16 ? __uint_as_float(bits16 << 16)
-                                      : __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
+  auto scale_of = [&](uint32_t word, uint32_t upper) {
+    const uint32_t top = __byte_perm(word, 0, upper ? 0x3244 : 0x1044);  // the scale in the upper half
+    return a.scale_dtype == XDNA_BF16 ? __uint_as_float(top) : __half2float(__ushort_as_half(static_cast<unsigned short>(top >> 16)));
   };
   auto finish = [&](int m, int n, float v) {
     if (a.bias) v += load_f32(a.bias, a.bias_dtype, n);
     store_f32(a.y, XT, (m0 + m) * a.ldy + n, v);
   };
 
+  int x_row[NT];  // columns of a product past the last x row repeat it: their sums are not used
+#pragma unroll
+  for (int i = 0; i < NT; ++i) x_row[i] = min(i * 8 + g, v_rows - 1) * pitch;
   bool staged = false;
   for (int set = blockIdx.x; set < n_sets; set += gridDim.x) {
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    // a scale is the upper half of its word where it stands at an odd place of the array
+    const int row_lo = min((set * tiles_per_cta + wt) * 16 + g, a.N - 1);
+    const uint32_t odd_lo = row_lo & a.n_groups & 1, odd_hi = min(row_lo + 8, a.N - 1) & a.n_groups & 1;
     for (int b0 = 0; b0 < a.blocks; b0 += a.chunk) {
-      const int b1 = min(a.blocks, b0 + a.chunk);
       if (!staged || a.chunk < a.blocks) {
         if (staged) __syncthreads();
-        stage_x(b0, b1 - b0);
+        stage_x(b0, min(a.blocks, b0 + a.chunk) - b0);
         __syncthreads();
         staged = true;
       }
-      for (int blk = b0 + kslice; blk < b1; blk += ks) {  // b0 is a multiple of ks
+      const int first = b0 + kslice * a.run, last = min(a.blocks, min(b0 + a.chunk, first + a.run));
+      for (int blk = first; blk < last; blk += kW4Blocks) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages - 1) : "memory");
-        const uint8_t* mine = ring + stage * 1024 + lane * 16;
-        const uint4 lo4 = *reinterpret_cast<const uint4*>(mine), hi4 = *reinterpret_cast<const uint4*>(mine + 512);
-        const uint32_t s_now = sc[0];
-#pragma unroll
-        for (int i = 0; i + 1 < kW4Stages; ++i) sc[i] = sc[i + 1];
-        sc[kW4Stages - 1] = prefetch();  // into the stage just read (by this lane alone)
-        stage = stage + 1 == kW4Stages ? 0 : stage + 1;
-        const uint32_t wl[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, wh[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+        __syncwarp();  // a fragment row's scales come from its four lanes
+        const uint8_t* mine = ring + stage * kStageBytes + lane * 16;
+        const uint8_t* scales = ring + stage * kStageBytes + kW4Blocks * 1024 + g * 16;
         const uint8_t* xb = smx + (blk - b0) * (kW4Block * 2) + t * 16;
-        float part[NT][4];
+        const uint32_t up_lo = odd_lo ^ (blk * kPer & 1), up_hi = odd_hi ^ (blk * kPer & 1);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          if ((w * 32) % GROUP == 0) {
+        for (int u = 0; u < kW4Blocks; ++u) {
+          if (blk + u >= last) break;
+          const uint4 lo4 = *reinterpret_cast<const uint4*>(mine + u * 1024), hi4 = *reinterpret_cast<const uint4*>(mine + u * 1024 + 512);
+          const uint32_t wl[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, wh[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+          float part[NT][4];
 #pragma unroll
-            for (int i = 0; i < NT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
-          }
-          const uint32_t a0[4] = {code_pair<kBf16>(wl[w]), code_pair<kBf16>(wh[w]), code_pair<kBf16>(wl[w] >> 4),
-                                  code_pair<kBf16>(wh[w] >> 4)};
-          const uint32_t a1[4] = {code_pair<kBf16>(wl[w] >> 8), code_pair<kBf16>(wh[w] >> 8),
-                                  code_pair<kBf16>(wl[w] >> 12), code_pair<kBf16>(wh[w] >> 12)};
+          for (int w = 0; w < 4; ++w) {
+            if ((w * 32) % GROUP == 0) {
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (i * 8 + g < v_rows) b = *reinterpret_cast<const uint4*>(xb + (i * 8 + g) * pitch + w * 64);
-            mma_16816<kBf16>(part[i], a0, b.x, b.y);
-            mma_16816<kBf16>(part[i], a1, b.z, b.w);
-          }
-          if ((w * 32 + 32) % GROUP == 0) {
-            const uint32_t s2 = kPer > 1 ? __shfl_sync(0xffffffffu, s_now, (lane & ~3) + w * 32 / GROUP) : s_now;
-            const float sl = scale_of(s2 & 0xffffu), sh = scale_of(s2 >> 16);
+              for (int i = 0; i < NT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
+            }
+            const uint32_t a0[4] = {code_pair<kBf16>(wl[w]), code_pair<kBf16>(wh[w]), code_pair<kBf16>(wl[w] >> 4),
+                                    code_pair<kBf16>(wh[w] >> 4)};
+            const uint32_t a1[4] = {code_pair<kBf16>(wl[w] >> 8), code_pair<kBf16>(wh[w] >> 8),
+                                    code_pair<kBf16>(wl[w] >> 12), code_pair<kBf16>(wh[w] >> 12)};
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-              acc[i][0] = fmaf(part[i][0], sl, acc[i][0]);
-              acc[i][1] = fmaf(part[i][1], sl, acc[i][1]);
-              acc[i][2] = fmaf(part[i][2], sh, acc[i][2]);
-              acc[i][3] = fmaf(part[i][3], sh, acc[i][3]);
+              const uint4 b = *reinterpret_cast<const uint4*>(xb + x_row[i] + u * (kW4Block * 2) + w * 64);
+              mma_16816<kBf16>(part[i], a0, b.x, b.y);
+              mma_16816<kBf16>(part[i], a1, b.z, b.w);
+            }
+            if ((w * 32 + 32) % GROUP == 0) {
+              const int idx = u * kPer + w * 32 / GROUP, j = idx >> 2, lane_t = idx & 3;
+              // groups past the last hold padding columns alone
+              const bool there = kPer == 1 || (blk + u) * kPer + w * 32 / GROUP < a.n_groups;
+              const uint32_t s_lo = *reinterpret_cast<const uint32_t*>(scales + j * 256 + lane_t * 4);
+              const uint32_t s_hi = *reinterpret_cast<const uint32_t*>(scales + j * 256 + 128 + lane_t * 4);
+              const float sl = there ? scale_of(s_lo, (up_lo ^ lane_t) & 1) : 0.f;
+              const float sh = there ? scale_of(s_hi, (up_hi ^ lane_t) & 1) : 0.f;
+#pragma unroll
+              for (int i = 0; i < NT; ++i) {
+                acc[i][0] = fmaf(part[i][0], sl, acc[i][0]);
+                acc[i][1] = fmaf(part[i][1], sl, acc[i][1]);
+                acc[i][2] = fmaf(part[i][2], sh, acc[i][2]);
+                acc[i][3] = fmaf(part[i][3], sh, acc[i][3]);
+              }
             }
           }
         }
+        __syncwarp();
+        prefetch();  // into the stage just read
+        stage ^= 1;
       }
     }
     const int n0 = (set * tiles_per_cta + wt) * 16;
@@ -310,12 +388,18 @@ static int run_w4(W4Args& a, int group, int sms, cudaStream_t s) {
   const int n_tiles = (a.N + 15) / 16;
   a.ks_log2 = 0;
   while (a.ks_log2 < 3 && (n_tiles << a.ks_log2) < 16 * sms && (2 << a.ks_log2) <= a.blocks) ++a.ks_log2;
-  // x in shared memory, whole where it fits in 96 KB (two CTAs per SM)
+  // x in shared memory, whole where it fits in 96 KB, else in chunks of a whole stage per warp
   const int ks = 1 << a.ks_log2;
-  a.chunk = std::min(a.blocks, std::max(1, (96 * 1024 / v_rows - 64) / 256));
-  if (a.chunk < a.blocks) a.chunk = std::max(ks, a.chunk / ks * ks);
+  a.chunk = std::max(1, (96 * 1024 / v_rows - 64) / 256);
+  if (a.chunk >= a.blocks) {
+    a.chunk = a.blocks;
+    a.run = (a.blocks + ks - 1) / ks;
+  } else {
+    a.run = std::max(1, a.chunk / ks / kW4Blocks * kW4Blocks);
+    a.chunk = a.run * ks;
+  }
   const int pitch = a.chunk * kW4Block * 2 + 64;
-  const int smem = 8 * kW4Stages * 1024 + (v_rows * pitch + 127) / 128 * 128 + 8 * 16 * nt * 8 * 4;
+  const int smem = 8 * kW4Stages * w4_stage_bytes(group) + (v_rows * pitch + 127) / 128 * 128 + 8 * 16 * nt * 8 * 4;
   const int sets = (n_tiles + (8 >> a.ks_log2) - 1) / (8 >> a.ks_log2);
   // with one warp per tile the CTAs are persistent, so that x is staged once per CTA
   const dim3 grid(static_cast<unsigned>(ks == 1 ? std::min(sets, 2 * sms) : sets),
@@ -395,7 +479,8 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
   int sms = 0;
   if ((rc = check_device(&sms)) != XDNA_OK) return rc;
   if (M == 0 || N == 0) return XDNA_OK;
-  XDNA_CHECK_ARG(x && codes && scales && y && aligned16(codes), "linear_w4: null pointer or unaligned codes");
+  XDNA_CHECK_ARG(x && codes && scales && y && aligned16(codes) && reinterpret_cast<uintptr_t>(scales) % 4 == 0,
+                 "linear_w4: null pointer or unaligned codes or scales");
   W4Args a{};
   a.x = x;
   a.ldx = ldx;
