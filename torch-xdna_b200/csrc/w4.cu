@@ -42,9 +42,7 @@ struct W4Args {
   int M, N, K, blocks, n_groups;  // blocks of 128 columns
   int x_dtype, scale_dtype, bias_dtype;
   int rows;     // x rows of a pass (blockIdx.y)
-  int ks_log2;  // warps that share a tile
   int chunk;    // blocks of x in shared memory at a time
-  int run;      // of these, a warp's
 };
 
 // The linear as tensor-core products of 16 weight rows by 8 (NT times) x rows, with the weights as the A operand: a
@@ -59,12 +57,15 @@ struct W4Args {
 // f32 x: each value is the exact sum of three bf16 numbers (truncated high, middle and low 8 bits), which take three
 // of the x rows of a product and are added at the end; so the result has the accuracy of f32 sums.
 // x lies in shared memory, 64 bytes off a multiple of 128 per row, which makes the B fragments' loads free of conflicts.
-// Tiles are few for small N: then 2, 4 or 8 warps share one, each with a run of its blocks, and add their sums in
-// shared memory in a fixed order.
+// A CTA has an equal share of the tiles, to one, eight at a time; where fewer are left, or there are fewer from the
+// start, 2, 4 or 8 warps share one, each with a run of its blocks, and add their sums in shared memory in a fixed order.
+// (Whole rounds of eight alone left the 9496 tiles of a 151936-row head at 4.01 rounds: a fifth with three CTAs.)
 constexpr int kW4Blocks = 4;
 constexpr int kW4Stages = 2;
 constexpr int kW4Threads = 256;
-constexpr int w4_stage_bytes(int group) { return kW4Blocks * 1024 + kW4Block / group * 256; }  // a warp's codes and scales
+// a warp's codes and scales: of each row four lanes' words as often as the stage's groups need
+constexpr int w4_scale_words(int group) { return (kW4Blocks * (kW4Block / group) + 3) / 4; }
+constexpr int w4_stage_bytes(int group) { return kW4Blocks * 1024 + w4_scale_words(group) * 256; }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -107,61 +108,79 @@ template <int XT, int NT, int GROUP>
 __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
   constexpr bool kBf16 = XT != XDNA_F16;
   constexpr int kParts = XT == XDNA_F32 ? 3 : 1, kPer = kW4Block / GROUP;  // groups per block
-  constexpr int kStageBytes = w4_stage_bytes(GROUP);
+  constexpr int kStageBytes = w4_stage_bytes(GROUP), kWords = w4_scale_words(GROUP);
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
-  const int ks = 1 << a.ks_log2, kslice = warp & (ks - 1), wt = warp >> a.ks_log2, tiles_per_cta = 8 >> a.ks_log2;
   const int m0 = blockIdx.y * a.rows, m_rows = min(a.rows, a.M - m0), v_rows = m_rows * kParts;
   const int pitch = a.chunk * kW4Block * 2 + 64;
   uint8_t* ring = smem + warp * (kW4Stages * kStageBytes);
   uint8_t* smx = smem + 8 * kW4Stages * kStageBytes;
   float* red = reinterpret_cast<float*>(smx + ((a.rows * kParts * pitch + 127) & ~127));  // [warp][16][NT * 8]
-  const int n_tiles = (a.N + 15) / 16, n_sets = (n_tiles + tiles_per_cta - 1) / tiles_per_cta;
+  const int64_t n_tiles = (a.N + 15) / 16;
+  const int tile0 = static_cast<int>(n_tiles * blockIdx.x / gridDim.x), tile1 = static_cast<int>(n_tiles * (blockIdx.x + 1) / gridDim.x);
   const int64_t row_bytes = static_cast<int64_t>(a.blocks) * 64;
 
-  // What a warp does, in order: its tile of each set of tiles, of it its run of each chunk of blocks, of it stages of
-  // kW4Blocks blocks. prefetch() walks this order kW4Stages ahead of the use.
-  int p_set = blockIdx.x, p_b0 = 0, p_blk = kslice * a.run, p_stage = 0;
+  // What a warp does, in order: its tile of each round, of it its run of each chunk of blocks, of it stages of kW4Blocks
+  // blocks. prefetch() walks this order kW4Stages ahead of the use.
+  struct Round {
+    int tile, ks, slice, run;  // tile -1: no part in it
+  };
+  auto round_of = [&](int i) -> Round {
+    const int left = tile1 - tile0 - 8 * i;
+    int log2 = left >= 5 ? 0 : left >= 3 ? 1 : left == 2 ? 2 : 3;
+    while ((1 << log2) > a.blocks) --log2;
+    Round r;
+    r.ks = 1 << log2;
+    r.slice = warp & (r.ks - 1);
+    r.run = (a.chunk + r.ks - 1) >> log2;
+    r.tile = (warp >> log2) < left ? tile0 + 8 * i + (warp >> log2) : -1;
+    return r;
+  };
+  const int n_rounds = (tile1 - tile0 + 7) / 8;
+  Round p = n_rounds > 0 ? round_of(0) : Round{-1, 1, 0, 0};
+  int p_round = 0, p_b0 = 0, p_blk = p.slice * p.run, p_stage = 0;
   const uint8_t *p_lo = nullptr, *p_hi = nullptr;
   int64_t p_slo = 0, p_shi = 0;  // where the rows' scales start, plus t: lane t copies every fourth scale of a row
   bool p_inner = false;          // there are rows after these
   auto start_tile = [&]() {
     // rows past N repeat the last one: their results are not used
-    const int n = min((p_set * tiles_per_cta + wt) * 16 + g, a.N - 1), n8 = min(n + 8, a.N - 1);
+    const int n = min(max(p.tile, 0) * 16 + g, a.N - 1), n8 = min(n + 8, a.N - 1);
     p_lo = a.codes + n * row_bytes + t * 16;
     p_hi = a.codes + n8 * row_bytes + t * 16;
     p_slo = static_cast<int64_t>(n) * a.n_groups + t;
     p_shi = static_cast<int64_t>(n8) * a.n_groups + t;
     p_inner = n8 < a.N - 1;
   };
-  if (p_set < n_sets) start_tile();
+  start_tile();
   auto prefetch = [&]() {
     // the next stage with blocks, if there is one
     int end = 0;
-    while (p_set < n_sets && p_blk >= (end = min(a.blocks, p_b0 + min(a.chunk, (kslice + 1) * a.run)))) {
+    while (p_round < n_rounds && (p.tile < 0 || p_blk >= (end = min(a.blocks, p_b0 + min(a.chunk, (p.slice + 1) * p.run))))) {
       p_b0 += a.chunk;
-      if (p_b0 >= a.blocks) {
+      if (p_b0 >= a.blocks || p.tile < 0) {
         p_b0 = 0;
-        p_set += gridDim.x;
-        if (p_set < n_sets) start_tile();
+        if (++p_round < n_rounds) {
+          p = round_of(p_round);
+          start_tile();
+        }
       }
-      p_blk = p_b0 + kslice * a.run;
+      p_blk = p_b0 + p.slice * p.run;
     }
-    if (p_set < n_sets) {
+    if (p_round < n_rounds) {
       const uint32_t dst = smem_u32(ring + p_stage * kStageBytes) + lane * 16;
       const uint32_t dst_s = smem_u32(ring + p_stage * kStageBytes) + kW4Blocks * 1024 + lane * 4;
       const uint8_t *lo = p_lo + p_blk * 64, *hi = p_hi + p_blk * 64;
       // a scale is copied as the aligned 4 bytes that hold it
       const uint16_t* sc = static_cast<const uint16_t*>(a.scales);
       const uint16_t *slo = sc + ((p_slo + p_blk * kPer) & ~int64_t(1)), *shi = sc + ((p_shi + p_blk * kPer) & ~int64_t(1));
-      if (p_blk + kW4Blocks <= end && (p_inner || p_blk + kW4Blocks < a.blocks)) {
+      if (p_blk + kW4Blocks <= end && (p_inner || p_blk + std::max(kW4Blocks, 4 / kPer) < a.blocks)) {
 #pragma unroll
         for (int u = 0; u < kW4Blocks; ++u) {
           cp_async_16(dst + u * 1024, lo + u * 64);
           cp_async_16(dst + u * 1024 + 512, hi + u * 64);
         }
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
+        for (int j = 0; j < kWords; ++j) {
           cp_async_4(dst_s + j * 256, slo + 4 * j, 4);
           cp_async_4(dst_s + j * 256 + 128, shi + 4 * j, 4);
         }
@@ -176,7 +195,7 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
         const uint16_t* sc_last = sc + (static_cast<int64_t>(a.N) * a.n_groups - 1);
         const int groups = min(a.n_groups, end * kPer);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
+        for (int j = 0; j < kWords; ++j) {
           if (p_blk * kPer + 4 * j + t < groups) {  // the array's last scale may stand alone in its word
             cp_async_4(dst_s + j * 256, slo + 4 * j, slo + 4 * j < sc_last ? 4 : 2);
             cp_async_4(dst_s + j * 256 + 128, shi + 4 * j, shi + 4 * j < sc_last ? 4 : 2);
@@ -185,8 +204,7 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
       }
       p_blk += kW4Blocks;
     }
-    p_stage ^= 1;
-    static_assert(kW4Stages == 2, "two stages");
+    p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
@@ -260,12 +278,13 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) x_row[i] = min(i * 8 + g, v_rows - 1) * pitch;
   bool staged = false;
-  for (int set = blockIdx.x; set < n_sets; set += gridDim.x) {
+  for (int round = 0; round < n_rounds; ++round) {
+    const Round now = round_of(round);
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     // a scale is the upper half of its word where it stands at an odd place of the array
-    const int row_lo = min((set * tiles_per_cta + wt) * 16 + g, a.N - 1);
+    const int row_lo = min(max(now.tile, 0) * 16 + g, a.N - 1);
     const uint32_t odd_lo = row_lo & a.n_groups & 1, odd_hi = min(row_lo + 8, a.N - 1) & a.n_groups & 1;
     for (int b0 = 0; b0 < a.blocks; b0 += a.chunk) {
       if (!staged || a.chunk < a.blocks) {
@@ -274,7 +293,8 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
         __syncthreads();
         staged = true;
       }
-      const int first = b0 + kslice * a.run, last = min(a.blocks, min(b0 + a.chunk, first + a.run));
+      const int first = b0 + now.slice * now.run;
+      const int last = now.tile < 0 ? 0 : min(a.blocks, b0 + min(a.chunk, (now.slice + 1) * now.run));
       for (int blk = first; blk < last; blk += kW4Blocks) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages - 1) : "memory");
         __syncwarp();  // a fragment row's scales come from its four lanes
@@ -324,17 +344,18 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
         }
         __syncwarp();
         prefetch();  // into the stage just read
-        stage ^= 1;
+        stage = stage + 1 == kW4Stages ? 0 : stage + 1;
       }
     }
-    const int n0 = (set * tiles_per_cta + wt) * 16;
-    if (kParts == 1 && ks == 1) {
+    if (kParts == 1 && now.ks == 1) {
+      if (now.tile >= 0) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = i * 8 + 2 * t + (e & 1), n = n0 + g + (e >> 1) * 8;
-          if (m < m_rows && n < a.N) finish(m, n, acc[i][e]);
+          for (int e = 0; e < 4; ++e) {
+            const int m = i * 8 + 2 * t + (e & 1), n = now.tile * 16 + g + (e >> 1) * 8;
+            if (m < m_rows && n < a.N) finish(m, n, acc[i][e]);
+          }
         }
       }
       continue;
@@ -345,17 +366,19 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) mine[(g + (e >> 1) * 8) * (NT * 8) + i * 8 + 2 * t + (e & 1)] = acc[i][e];
     }
-    const bool alone = ks == 1;
+    const bool alone = now.ks == 1;
     if (alone) __syncwarp(); else __syncthreads();
-    // outputs: all warps' tiles, or this warp's alone
-    const int n_out = (alone ? 16 : tiles_per_cta * 16), step = alone ? 32 : kW4Threads;
+    // outputs: those of the round's tiles, or of this warp's alone
+    const int here = alone ? now.tile >= 0 : min(8 / now.ks, tile1 - tile0 - 8 * round);
+    const int n_out = here * 16, step = alone ? 32 : kW4Threads;
     for (int i = alone ? lane : threadIdx.x; i < n_out * m_rows; i += step) {
       const int r = i % n_out, m = i / n_out;
-      const int tile = alone ? wt : r >> 4, n = (set * tiles_per_cta + tile) * 16 + (r & 15);
+      const int n = (alone ? now.tile : tile0 + 8 * round + (r >> 4)) * 16 + (r & 15);
       if (n >= a.N) continue;
+      const float* sums = red + ((alone ? warp : (r >> 4) * now.ks) * 16 + (r & 15)) * (NT * 8) + m * kParts;
       float v = 0.f;
-      for (int p = kParts - 1; p >= 0; --p)  // small parts first
-        for (int s = 0; s < ks; ++s) v += red[((tile * ks + s) * 16 + (r & 15)) * (NT * 8) + m * kParts + p];
+      for (int q = kParts - 1; q >= 0; --q)  // small parts first
+        for (int k = 0; k < now.ks; ++k) v += sums[k * 16 * (NT * 8) + q];
       finish(m, n, v);
     }
     if (alone) __syncwarp(); else __syncthreads();
@@ -384,26 +407,12 @@ static int run_w4(W4Args& a, int group, int sms, cudaStream_t s) {
   // a pass takes up to 32 x rows (10 of f32); more run as further passes over the codes, which the L2 then holds
   a.rows = std::min(a.M, 32 / kParts);
   const int v_rows = a.rows * kParts, nt = v_rows <= 8 ? 1 : v_rows <= 16 ? 2 : 4;
-  // warps per tile: enough warps to fill the SMs (16 each), as long as each has a block
-  const int n_tiles = (a.N + 15) / 16;
-  a.ks_log2 = 0;
-  while (a.ks_log2 < 3 && (n_tiles << a.ks_log2) < 16 * sms && (2 << a.ks_log2) <= a.blocks) ++a.ks_log2;
-  // x in shared memory, whole where it fits in 96 KB, else in chunks of a whole stage per warp
-  const int ks = 1 << a.ks_log2;
-  a.chunk = std::max(1, (96 * 1024 / v_rows - 64) / 256);
-  if (a.chunk >= a.blocks) {
-    a.chunk = a.blocks;
-    a.run = (a.blocks + ks - 1) / ks;
-  } else {
-    a.run = std::max(1, a.chunk / ks / kW4Blocks * kW4Blocks);
-    a.chunk = a.run * ks;
-  }
+  // x in shared memory, whole where it fits in 96 KB (with one or two x rows it fits for any K in use)
+  a.chunk = std::min(a.blocks, std::max(1, (96 * 1024 / v_rows - 64) / 256));
   const int pitch = a.chunk * kW4Block * 2 + 64;
   const int smem = 8 * kW4Stages * w4_stage_bytes(group) + (v_rows * pitch + 127) / 128 * 128 + 8 * 16 * nt * 8 * 4;
-  const int sets = (n_tiles + (8 >> a.ks_log2) - 1) / (8 >> a.ks_log2);
-  // with one warp per tile the CTAs are persistent, so that x is staged once per CTA
-  const dim3 grid(static_cast<unsigned>(ks == 1 ? std::min(sets, 2 * sms) : sets),
-                  static_cast<unsigned>((a.M + a.rows - 1) / a.rows));
+  // two CTAs per SM, which the registers and the shared memory of most shapes allow
+  const dim3 grid(static_cast<unsigned>(std::min((a.N + 15) / 16, 2 * sms)), static_cast<unsigned>((a.M + a.rows - 1) / a.rows));
   return nt == 1 ? launch_w4<XT, 1>(a, group, grid, smem, s)
                  : nt == 2 ? launch_w4<XT, 2>(a, group, grid, smem, s) : launch_w4<XT, 4>(a, group, grid, smem, s);
 }
