@@ -398,7 +398,7 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
  *   l = seen ? (l > 0 ? l / repetition[b] : l * repetition[b]) : l;  l -= frequency[b] * c + (c > 0) * presence[b];
  *   l += bias[b * ld_bias + v] (ld_bias 0: one for all rows);  l = bit v of mask[b * ld_mask + v / 32] ? l : -inf.
  * Each of tokens, lens (then T), prompt_lens (then 0), repetition, presence, frequency, bias and mask may be NULL.
- * out may be logits. */
+ * out must not overlap logits. */
 int xdna_process_logits(const void* logits, int dtype, int64_t B, int64_t V, int64_t ld_in, const void* tokens,
                         int token_bytes, int64_t T, int64_t ld_tokens, const int32_t* lens,
                         const int32_t* prompt_lens, const float* repetition, const float* presence,

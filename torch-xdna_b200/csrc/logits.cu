@@ -24,6 +24,7 @@ struct LogitsArgs {
 };
 
 constexpr int kLogitsThreads = 256;
+constexpr int kLogitsCtas = 6;  // per SM: what covers the blocks' two barriers is other blocks
 
 template <typename T>
 struct LogitVec;  // 16 bytes of logits
@@ -84,14 +85,14 @@ struct LogitVec<__half> {
 };
 
 // A block takes VECS x 256 pieces of 16 bytes of one row. The loads go out first: the thread's first tokens, its
-// logits, bias and mask words. While they are on their way the block clears a bitmap and its counters; then it marks
+// logits and mask words. While they are on their way the block clears a bitmap and its counters; then it marks
 // and counts the row's tokens that fall into its entries (integer sums in shared memory, so their order does not
 // matter), and each piece is worked on in registers and written; only pieces with a marked entry look at the counters.
 // The row is cut at 16-byte boundaries of its own address, so rows of any pitch are read and written in whole pieces
 // except at their two ends.
 // HBM-bound; the history is read once per block, from the L2, so the blocks are as long as still fill the machine.
 template <typename T, typename Tok, int VECS>
-__global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(kLogitsThreads, kLogitsCtas) logits_kernel(const LogitsArgs a) {
   using Vec = LogitVec<T>;
   constexpr int N = Vec::N, kChunk = VECS * kLogitsThreads * N;
   constexpr int M = 16 / sizeof(Tok), kAhead = 2;    // tokens of a piece, pieces of the history loaded ahead
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const LogitsA
     if (a.lens) len = min(max(a.lens[row], 0), T_);
     if (a.prompt_lens) prompt = a.prompt_lens[row];
   }
-  const float rep = a.rep ? a.rep[row] : 1.f, pres = a.pres ? a.pres[row] : 0.f, freq = a.freq ? a.freq[row] : 0.f;
+  const float rep = a.rep ? a.rep[row] : 1.f, inv_rep = 1.f / rep, pres = a.pres ? a.pres[row] : 0.f, freq = a.freq ? a.freq[row] : 0.f;
   auto whole = [&](int at) { return pieces && at >= 0 && at + N <= V; };
   uint4 raw[VECS];
 #pragma unroll
@@ -131,16 +132,6 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const LogitsA
   }
   const float* bias = a.bias ? a.bias + row * a.ld_bias : nullptr;
   const bool wide_bias = bias && (reinterpret_cast<uintptr_t>(bias + base) & 15) == 0;
-  float4 b[VECS][N / 4];
-  if (wide_bias) {
-#pragma unroll
-    for (int v = 0; v < VECS; ++v) {
-      const int at = base + (v * kLogitsThreads + tid) * N;
-#pragma unroll
-      for (int e = 0; e < N / 4; ++e)
-        if (whole(at)) b[v][e] = reinterpret_cast<const float4*>(bias + at)[e];
-    }
-  }
   const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
   uint32_t allowed[VECS];
   if (mask) {
@@ -158,32 +149,46 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const LogitsA
     for (int i = 0; i < kChunk / 4 / kLogitsThreads; ++i) reinterpret_cast<uint4*>(count)[i * kLogitsThreads + tid] = make_uint4(0, 0, 0, 0);
     if (tid < kChunk / 32) marked[tid] = 0;
     __syncthreads();
+    // entries [first, first + range) of the row are this block's: one subtraction and one comparison per token
+    const uint32_t first = static_cast<uint32_t>(max(base, 0));
+    const uint32_t range = static_cast<uint32_t>(max(min(base + kChunk, V) - max(base, 0), 0));  // 0 in a block past V
+    auto here = [&](Tok id) {
+      if constexpr (sizeof(Tok) == 8)
+        return static_cast<uint64_t>(id) - first < range;
+      else
+        return static_cast<uint32_t>(id) - first < range;
+    };
     auto put = [&](int i, Tok id) {
-      if (i >= len || id < 0 || id >= V) return;
+      if (!here(id) || i >= len) return;
       const int at = static_cast<int>(id) - base;
-      if (at < 0 || at >= kChunk) return;
       atomicOr(&marked[at >> 5], 1u << (at & 31));
       if (i >= prompt) atomicAdd(&count[at], 1u);
+    };
+    auto put_piece = [&](int at, const uint4& u) {
+      Tok id[M];
+      *reinterpret_cast<uint4*>(id) = u;
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < M; ++e) any |= here(id[e]);
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < M; ++e) put(at + e, id[e]);
+      }
     };
     if (tid < head) put(tid, tok[tid]);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int at = head + (i * kLogitsThreads + tid) * M;
-      if (at + M > T_) continue;
-#pragma unroll
-      for (int e = 0; e < M; ++e) put(at + e, reinterpret_cast<const Tok*>(&ahead[i])[e]);
+      if (at + M <= T_) put_piece(at, ahead[i]);
     }
     const int rest = head + (T_ - head) / M * M;
-    for (int at = head + (kAhead * kLogitsThreads + tid) * M; at < min(len, rest); at += kLogitsThreads * M) {
-      const uint4 u = *reinterpret_cast<const uint4*>(tok + at);
-#pragma unroll
-      for (int e = 0; e < M; ++e) put(at + e, reinterpret_cast<const Tok*>(&u)[e]);
-    }
+    for (int at = head + (kAhead * kLogitsThreads + tid) * M; at < min(len, rest); at += kLogitsThreads * M)
+      put_piece(at, *reinterpret_cast<const uint4*>(tok + at));
     if (rest + tid < T_) put(rest + tid, tok[rest + tid]);  // fewer than M
     __syncthreads();
   }
   auto penalise = [&](float l, int at) {
-    l = l > 0.f ? l / rep : l * rep;
+    l *= l > 0.f ? inv_rep : rep;
     const uint32_t c = count[at];
     return c ? l - freq * static_cast<float>(c) - pres : l;
   };
@@ -202,7 +207,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const LogitsA
       if (wide_bias) {
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
-          const float4 f = b[v][e / 4];
+          const float4 f = *reinterpret_cast<const float4*>(bias + at + e);
           x[e] += f.x, x[e + 1] += f.y, x[e + 2] += f.z, x[e + 3] += f.w;
         }
       } else if (bias) {
@@ -237,15 +242,15 @@ static void launch_logits(const LogitsArgs& a, int64_t B, cudaStream_t s) {
   logits_kernel<T, Tok, VECS><<<grid, kLogitsThreads, a.tokens ? kChunk * 4 : 0, s>>>(a);
 }
 
-// The longest blocks (4 pieces a thread) that still make four per SM, since each block reads the row's history.
+// Two pieces a thread, or one where that leaves SMs without enough blocks.
 template <typename T>
 static void run_logits(const LogitsArgs& a, int64_t B, int token_bytes, int sms, cudaStream_t s) {
   const int64_t pieces = B * ((a.V + LogitVec<T>::N - 1) / LogitVec<T>::N + kLogitsThreads - 1) / kLogitsThreads;
-  const int vecs = pieces >= 16 * sms ? 4 : pieces >= 8 * sms ? 2 : 1;
+  const bool two = pieces >= 8 * sms;
   if (token_bytes == 8)
-    vecs == 4 ? launch_logits<T, int64_t, 4>(a, B, s) : vecs == 2 ? launch_logits<T, int64_t, 2>(a, B, s) : launch_logits<T, int64_t, 1>(a, B, s);
+    two ? launch_logits<T, int64_t, 2>(a, B, s) : launch_logits<T, int64_t, 1>(a, B, s);
   else
-    vecs == 4 ? launch_logits<T, int32_t, 4>(a, B, s) : vecs == 2 ? launch_logits<T, int32_t, 2>(a, B, s) : launch_logits<T, int32_t, 1>(a, B, s);
+    two ? launch_logits<T, int32_t, 2>(a, B, s) : launch_logits<T, int32_t, 1>(a, B, s);
 }
 
 }  // namespace xdna
