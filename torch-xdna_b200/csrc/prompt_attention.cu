@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  if constexpr (MODE == PREFIX) asm volatile("griddepcontrol.launch_dependents;");
   const int warp = warp_id(), lane = lane_id();
   const int cta = static_cast<int>(blockIdx.x), G = static_cast<int>(gridDim.x);
 
@@ -644,57 +645,42 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool 
 
 constexpr int kOwnWarps = 4;
 constexpr int kOwnStep = 16;   // keys of a warp's step
-constexpr int kOwnStages = 3;  // steps under way per warp
+constexpr int kOwnStages = 2;  // steps under way per warp
+constexpr int kOwnMinSteps = 8;  // of a split, two per warp
 
-// A sequence's own keys: few rows (the up to 16 query heads of a tile that share a key head) against a cache of its
-// own, so the time is the reading of the cache. One CTA per (sequence, key head, 16 query heads, split); its warps take
-// steps of 16 keys in turn, with three steps' copies under way (cp.async: 24 KB per warp, 192 KB per SM), each with a
-// running softmax of its own, joined at the end. The products are mma.sync 16 x 8
-// x 16 with the query heads as rows (a step's 16 rows are cheap; tcgen05's 128 would not be filled), and K and V go
-// from global memory straight into fragments in 16-byte pieces: of K, lane (g, t) reads columns 32 c + 8 t .. + 7 of
-// key g, which are B fragments when the query's A fragments are read in the same order; of V, columns 64 e + 8 g .. + 7
-// of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, which are, paired by a byte permute, B fragments of the output columns in
-// the order 64 e + 8 n + i.
+// A sequence's own keys: few rows (the query heads that share a key head) against a cache of its own, so the time is
+// the reading of the cache. One CTA per (sequence, key head, 8 query heads, split); its warps take steps of 16 keys in
+// turn, two steps' copies under way each (cp.async: 16 KB per warp, 192 KB per SM), each with a running softmax of its
+// own, joined at the end. The products are mma.sync 16 x 8 x 16 with keys, then dimensions, as rows and the query heads
+// as columns (tcgen05's 128 rows would not be filled): S^T = K Q^T, O^T = V^T P^T. K and V are copied in 16-byte pieces
+// that are fragments as they are: of K, lane (g, t) takes dimensions 32 c + 8 t .. + 7 of keys g and g + 8, which are A
+// fragments when the queries' B fragments are read in the same order; of V, dimensions 64 e + 8 g .. + 7 of keys 2 t,
+// 2 t + 1, 2 t + 8, 2 t + 9, which are, paired by a byte permute, A fragments of output rows in the order of dimensions
+// 64 e + 8 g + 2 i (row g of product i) and 64 e + 8 g + 2 i + 1 (row g + 8). P^T is S^T's fragment, transposed by
+// movmatrix. Every lane reads back just what it copied, so no barrier is needed.
 // Keys past the length are not read and count as zeros with score -inf.
 // With one split the CTA also joins the prefix's parts and writes the output; else it leaves a part like theirs.
 template <typename T, int D>
-__global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs a) {
+__global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnArgs a) {
   constexpr bool kBf16 = !__is_same(T, __half);
   constexpr int kC = D / 32, kE = D / 64;
   constexpr int kStageBytes = 2 * kC * 2 * 512;  // a step's K and V, 16 bytes of each lane per piece
   extern __shared__ __align__(16) uint8_t own_smem[];
   uint8_t* ring = own_smem + warp_id() * (kOwnStages * kStageBytes);
-  float(*so)[16][D + 4] = reinterpret_cast<float(*)[16][D + 4]>(own_smem);  // the warps' sums, once the ring is done
-  __shared__ float2 sml[kOwnWarps][16];
+  float(*so)[8][D + 4] = reinterpret_cast<float(*)[8][D + 4]>(own_smem);  // the warps' sums, once the ring is done
+  __shared__ float2 sml[kOwnWarps][8];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
   const int b = static_cast<int>(blockIdx.x) / a.hkv, kvh = static_cast<int>(blockIdx.x) % a.hkv;
-  const int h0 = kvh * a.group + static_cast<int>(blockIdx.z) * 16;              // the tile's first query head
-  const int rows = min(16, a.group - static_cast<int>(blockIdx.z) * 16);
+  const int h0 = kvh * a.group + static_cast<int>(blockIdx.z) * 8;              // the tile's first query head
+  const int rows = min(8, a.group - static_cast<int>(blockIdx.z) * 8);
   const int n = min(max(a.lens[b], 0), a.S);
-  const int steps = (n + kOwnStep - 1) / kOwnStep, per = (steps + a.splits - 1) / a.splits;
+  const int steps = (n + kOwnStep - 1) / kOwnStep;
+  const int per = max((steps + a.splits - 1) / a.splits, kOwnMinSteps);
   const int s0 = min(steps, static_cast<int>(blockIdx.y) * per), s1 = min(steps, s0 + per);
 
-  uint32_t q[kC][2][4];  // rows g and g + 8
-  {
-    const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.q_sb + static_cast<int64_t>(h0) * a.q_sh + 8 * t;
-#pragma unroll
-    for (int c = 0; c < kC; ++c) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint4 u = g + 8 * r < rows ? *reinterpret_cast<const uint4*>(qp + (g + 8 * r) * a.q_sh + 32 * c) : make_uint4(0, 0, 0, 0);
-        q[c][r][0] = u.x, q[c][r][1] = u.y, q[c][r][2] = u.z, q[c][r][3] = u.w;
-      }
-    }
-  }
-  float o[kE][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-  for (int e = 0; e < kE; ++e) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[e][i][0] = o[e][i][1] = o[e][i][2] = o[e][i][3] = 0.f;
-  }
   const T* kp = static_cast<const T*>(a.ck) + static_cast<int64_t>(b) * a.ck_sb + static_cast<int64_t>(kvh) * a.ck_sh + 8 * t;
   const T* vp = static_cast<const T*>(a.cv) + static_cast<int64_t>(b) * a.cv_sb + static_cast<int64_t>(kvh) * a.cv_sh + 8 * g;
-  // Each lane copies its pieces of K (8 r + g, c) and V (x, e) and reads back just them: no barrier is needed.
   auto fetch = [&](int step, int st) {
     if (step < s1) {
       const uint32_t dst = smem_u32(ring + st * kStageBytes + lane * 16);
@@ -717,59 +703,58 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
   };
 #pragma unroll
   for (int i = 0; i < kOwnStages; ++i) fetch(s0 + warp + i * kOwnWarps, i);
+
+  uint4 q[kC];  // query head g, dimensions 32 c + 8 t .. + 7
+#pragma unroll
+  for (int c = 0; c < kC; ++c)
+    q[c] = g < rows ? *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<int64_t>(b) * a.q_sb +
+                                                      static_cast<int64_t>(h0 + g) * a.q_sh + 8 * t + 32 * c)
+                    : make_uint4(0, 0, 0, 0);
+  float o[kE][4][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m, l: of query heads 2 t, 2 t + 1
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[e][i][0] = o[e][i][1] = o[e][i][2] = o[e][i][3] = 0.f;
+  }
   int st = 0;
   for (int step = s0 + warp; step < s1; step += kOwnWarps, st = st + 1 == kOwnStages ? 0 : st + 1) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kOwnStages - 1) : "memory");
     const uint4* mine = reinterpret_cast<const uint4*>(ring + st * kStageBytes) + lane;
-    float s[2][4];
+    float s2[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // two sums, so that the products are two chains
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        const uint32_t a0[4] = {q[c][0][0], q[c][1][0], q[c][0][1], q[c][1][1]};
-        const uint32_t a1[4] = {q[c][0][2], q[c][1][2], q[c][0][3], q[c][1][3]};
-        const uint4 k = mine[(r * kC + c) * 32];
-        mma_16816<kBf16>(s[r], a0, k.x, k.y);
-        mma_16816<kBf16>(s[r], a1, k.z, k.w);
-      }
+    for (int c = 0; c < kC; ++c) {
+      const uint4 k0 = mine[c * 32], k1 = mine[(kC + c) * 32];
+      const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+      mma_16816<kBf16>(s2[0], a0, q[c].x, q[c].y);
+      mma_16816<kBf16>(s2[1], a1, q[c].z, q[c].w);
     }
-    // s[r][e]: row g (+ 8 for e >= 2), key 8 r + 2 t + (e & 1) of the step
-    float mx[2] = {-INFINITY, -INFINITY};
+    // s[e]: key g (g + 8 for e >= 2) of the step, query head 2 t + (e & 1)
+    float s[4], f[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[r][e] = step * kOwnStep + 8 * r + 2 * t + (e & 1) < n ? s[r][e] * a.scale_log2 : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[r][e]);
-      }
-    }
-    float f[2];
+    for (int e = 0; e < 4; ++e)
+      s[e] = step * kOwnStep + g + 8 * (e >> 1) < n ? (s2[0][e] + s2[1][e]) * a.scale_log2 : -INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      const float mn = fmaxf(m[h], mx[h]);
+      float mx = fmaxf(s[h], s[2 + h]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float mn = fmaxf(m[h], mx);
       f[h] = mn == -INFINITY ? 1.f : fast_exp2(m[h] - mn);
       m[h] = mn;
-      l[h] *= f[h];
+      const float base = mn == -INFINITY ? 0.f : mn;
+      s[h] = fast_exp2(s[h] - base);
+      s[2 + h] = fast_exp2(s[2 + h] - base);
+      l[h] = l[h] * f[h] + (s[h] + s[2 + h]);  // this lane's keys; the lanes' sums are added at the end
     }
-    uint32_t p[4];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float base = m[h] == -INFINITY ? 0.f : m[h];
-        const float p0 = fast_exp2(s[r][2 * h] - base), p1 = fast_exp2(s[r][2 * h + 1] - base);
-        l[h] += p0 + p1;
-        p[2 * r + h] = pack2<T>(p0, p1);
-      }
-    }
+    uint32_t p0, p1;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p0) : "r"(pack2<T>(s[0], s[1])));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p1) : "r"(pack2<T>(s[2], s[3])));
     if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[e][i][0] *= f[0], o[e][i][1] *= f[0], o[e][i][2] *= f[1], o[e][i][3] *= f[1];
+        for (int i = 0; i < 4; ++i) o[e][i][0] *= f[0], o[e][i][1] *= f[1], o[e][i][2] *= f[0], o[e][i][3] *= f[1];
       }
     }
 #pragma unroll
@@ -779,34 +764,34 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
       const uint32_t v0[4] = {u0.x, u0.y, u0.z, u0.w}, v1[4] = {u1.x, u1.y, u1.z, u1.w}, v2[4] = {u2.x, u2.y, u2.z, u2.w},
                      v3[4] = {u3.x, u3.y, u3.z, u3.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
-        mma_16816<kBf16>(o[e][i], p, __byte_perm(v0[i / 2], v1[i / 2], sel), __byte_perm(v2[i / 2], v3[i / 2], sel));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t av[4] = {__byte_perm(v0[i], v1[i], 0x5410), __byte_perm(v0[i], v1[i], 0x7632),
+                                __byte_perm(v2[i], v3[i], 0x5410), __byte_perm(v2[i], v3[i], 0x7632)};
+        mma_16816<kBf16>(o[e][i], av, p0, p1);
       }
     }
     fetch(step + kOwnStages * kOwnWarps, st);  // into the stage just read
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  // the warp's part: rows g, g + 8; column n = 2 t + (x & 1) of product i is dimension 64 e + 8 n + i
+  // the warp's part
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (t == 0) sml[warp][g + 8 * h] = make_float2(m[h], l[h]);
-    if (g + 8 * h < rows) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+    if (g == 0) sml[warp][2 * t + h] = make_float2(m[h], l[h]);
+    if (2 * t + h < rows) {
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float* dst = &so[warp][g + 8 * h][64 * e + 8 * (2 * t + x)];
-          *reinterpret_cast<float4*>(dst) = make_float4(o[e][0][2 * h + x], o[e][1][2 * h + x], o[e][2][2 * h + x], o[e][3][2 * h + x]);
-          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[e][4][2 * h + x], o[e][5][2 * h + x], o[e][6][2 * h + x], o[e][7][2 * h + x]);
-        }
+        float* dst = &so[warp][2 * t + h][64 * e + 8 * g];
+        *reinterpret_cast<float4*>(dst) = make_float4(o[e][0][h], o[e][0][2 + h], o[e][1][h], o[e][1][2 + h]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[e][2][h], o[e][2][2 + h], o[e][3][h], o[e][3][2 + h]);
       }
     }
   }
   __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's parts (also where only the join reads them)
   // four dimensions per thread
   const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
   for (int i = threadIdx.x; i < rows * (D / 4); i += kOwnWarps * 32) {
@@ -815,6 +800,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
     const int parts = a.splits == 1 ? a.parts : 0;
     float mm = -INFINITY, ll = 0.f;
     for (int w = 0; w < kOwnWarps; ++w) mm = fmaxf(mm, sml[w][r].x);
+#pragma unroll 8
     for (int s = 0; s < parts; ++s) mm = fmaxf(mm, a.part_ml[s * n_rows + row].x);
     const float base = mm == -INFINITY ? 0.f : mm;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -824,7 +810,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
       acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
     };
     for (int w = 0; w < kOwnWarps; ++w) add(sml[w][r], *reinterpret_cast<const float4*>(&so[w][r][d]));
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s < parts; ++s)
       add(a.part_ml[s * n_rows + row], *reinterpret_cast<const float4*>(a.part_o + (s * n_rows + row) * D + d));
     if (a.splits == 1) {
@@ -843,31 +829,56 @@ __global__ void __launch_bounds__(kOwnWarps * 32) own_keys_kernel(const OwnArgs 
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const float* part_o, const float2* part_ml, int parts, int64_t n_rows, T* out) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp_id();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (row >= n_rows) return;
-  float mm = -INFINITY, ll = 0.f, acc[D / 32];
+  constexpr int kV = D / 32;  // dimensions of a lane
+  float mm = -INFINITY, ll = 0.f, acc[kV];
   for (int s = lane_id(); s < parts; s += 32) mm = fmaxf(mm, part_ml[s * n_rows + row].x);
   for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
   const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-#pragma unroll 4
+  for (int i = 0; i < kV; ++i) acc[i] = 0.f;
+#pragma unroll 8
   for (int s = 0; s < parts; ++s) {
     const float2 ml = part_ml[s * n_rows + row];
     const float f = fast_exp2(ml.x - base);
     ll = fmaf(f, ml.y, ll);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(f, part_o[(s * n_rows + row) * D + i * 32 + lane_id()], acc[i]);
+    const float* x = part_o + (s * n_rows + row) * D + lane_id() * kV;
+    if constexpr (kV == 4) {
+      const float4 u = *reinterpret_cast<const float4*>(x);
+      acc[0] = fmaf(f, u.x, acc[0]), acc[1] = fmaf(f, u.y, acc[1]), acc[2] = fmaf(f, u.z, acc[2]), acc[3] = fmaf(f, u.w, acc[3]);
+    } else {
+      const float2 u = *reinterpret_cast<const float2*>(x);
+      acc[0] = fmaf(f, u.x, acc[0]), acc[1] = fmaf(f, u.y, acc[1]);
+    }
   }
   const float inv = ll > 0.f || __isnanf(ll) ? 1.f / ll : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out + row * D + lane_id() * kV);
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) out[row * D + i * 32 + lane_id()] = from_f32<T>(acc[i] * inv);
+  for (int i = 0; i < kV; i += 2) dst[i / 2] = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+}
+
+// A launch that may start while the kernel before it still runs (and waits for it itself, griddepcontrol.wait).
+template <typename... Params, typename... Args>
+static cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
 }
 
 template <typename T, int D>
 static int launch_own(const OwnArgs& a, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(a.B * a.hkv), static_cast<unsigned>(a.splits), static_cast<unsigned>((a.group + 15) / 16));
+  const dim3 grid(static_cast<unsigned>(a.B * a.hkv), static_cast<unsigned>(a.splits), static_cast<unsigned>((a.group + 7) / 8));
   constexpr int kSmem = kOwnWarps * kOwnStages * (D / 32) * 2048;
-  static_assert(kSmem >= kOwnWarps * 16 * (D + 4) * 4, "the sums lie where the ring was");
+  static_assert(kSmem >= kOwnWarps * 8 * (D + 4) * 4, "the sums lie where the ring was");
   auto kern = own_keys_kernel<T, D>;
   static std::atomic<bool> configured[64];  // setting the attribute twice from two threads is harmless
   int dev = 0;
@@ -876,13 +887,19 @@ static int launch_own(const OwnArgs& a, cudaStream_t s) {
     XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
-  kern<<<grid, kOwnWarps * 32, kSmem, s>>>(a);
-  int rc = check_launch("own_keys_kernel");
-  if (rc != XDNA_OK || a.splits == 1) return rc;
+  // after the prefix's kernel it may start early; alone it is an ordinary launch
+  if (a.parts > 0) {
+    XDNA_CUDA(launch_early(kern, grid, kOwnWarps * 32, kSmem, s, a));
+  } else {
+    kern<<<grid, kOwnWarps * 32, kSmem, s>>>(a);
+    int rc = check_launch("own_keys_kernel");
+    if (rc != XDNA_OK) return rc;
+  }
+  if (a.splits == 1) return XDNA_OK;
   const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
-  join_kernel<T, D><<<static_cast<unsigned>((n_rows + 3) / 4), 128, 0, s>>>(a.part_o, a.part_ml, a.parts + a.splits, n_rows,
-                                                                            static_cast<T*>(a.out));
-  return check_launch("join_kernel");
+  XDNA_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>((n_rows + 3) / 4)), 128, 0, s, a.part_o, a.part_ml,
+                         a.parts + a.splits, n_rows, a.out));
+  return XDNA_OK;
 }
 
 // ---------------------------------------------------------------------------- host
@@ -945,8 +962,8 @@ static int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtens
 static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { return tokens / (2 * (128 / group)) + n_seqs; }
 
 // How a prefix call is split: the prefix's keys into about one item per SM, each at least one block; a sequence's own
-// keys, where the sequences and key heads alone are fewer than two CTAs per SM, into pieces of at least 128 (a CTA's
-// two steps per warp).
+// keys, where the sequences and key heads alone are few CTAs for an SM, into pieces of at least 128 (a CTA's two steps
+// per warp): lengths differ, and the longest would be waited for.
 struct PrefixSplit {
   int64_t pairs, parts, blocks_per_part, own;
   PrefixSplit(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int sms) {
@@ -955,8 +972,8 @@ struct PrefixSplit {
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(blocks, sms / (pairs * hkv)));
     blocks_per_part = blocks ? (blocks + want - 1) / want : 0;
     parts = blocks ? (blocks + blocks_per_part - 1) / blocks_per_part : 0;
-    const int64_t ctas = B * hkv * ((hq / hkv + 15) / 16);
-    own = std::max<int64_t>(1, std::min<int64_t>((S + 127) / 128, 2 * sms / ctas));
+    const int64_t ctas = B * hkv * ((hq / hkv + 7) / 8);
+    own = std::max<int64_t>(1, std::min<int64_t>((S + 127) / 128, 8 * sms / ctas));
   }
   int64_t all() const { return parts + (own > 1 ? own : 0); }
 };
