@@ -15,7 +15,7 @@
 //               taken as it lies in memory, keys by dimensions: the MN-major B operand of the second product.
 //   warp 1      the MMAs, one thread:  S_A(0) S_B(0) | O_A += P_A(j) V(j), S_A(j+1) | O_B += P_B(j) V(j), S_B(j+1) | ...
 //               While one tile's softmax works, the tensor core does the other's two products.
-//   warps 2..5  softmax of tile A, warps 6..9 of tile B; thread = row. S is read from TMEM once, p = 2^(s - m) is
+//   warps 4..7  softmax of tile A, warps 8..11 of tile B; thread = row. S is read from TMEM once, p = 2^(s - m) is
 //               written as 16 bits over S's own columns and is the A operand of the second product straight from
 //               TMEM, so P costs no shared-memory bandwidth (of which both products together need all there is when
 //               P goes through it). The next S is issued after that product, in order, so it may overwrite P.
@@ -84,7 +84,10 @@ struct TileArgs {
   float2* part_ml; // [split][B * hq]: m (log2 units), l
 };
 
-constexpr int kTaThreads = 320;
+constexpr int kTaThreads = 384;  // three warpgroups: issue (TMA, MMA), softmax of tile A, of tile B
+// Registers per thread after setmaxnreg: together what the launch gives, 384 x 168.
+constexpr int kTaRegsLaunch = 168, kTaRegsIssue = 72, kTaRegsSoftmax = 216;
+static_assert(128 * kTaRegsIssue + 256 * kTaRegsSoftmax <= kTaThreads * kTaRegsLaunch, "more registers than the launch has");
 constexpr int kTaBlock = 128;
 constexpr float kTaRescale = 8.0f;
 
@@ -241,6 +244,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     return true;
   };
 
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTaRegsIssue));
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------------------------ TMA
@@ -336,9 +340,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         mbar_wait(drain, 0, &never, args.err, 46);
       }
     }
-  } else {
-    // -------------------------------------------------------------------- softmax (warps 2..9)
-    const int t = (warp - 2) >> 2;           // tile
+  } else if (warp >= 4) {
+    // -------------------------------------------------------------------- softmax (warps 4..11)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTaRegsSoftmax));
+    const int t = (warp - 4) >> 2;           // tile
     const int qd = warp & 3;                 // TMEM lane quadrant = row block
     const int r = qd * 32 + lane;            // row of the tile
     const int r_tok = r / args.group, r_head = r - r_tok * args.group;
@@ -351,7 +356,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const int64_t row = static_cast<int64_t>(args.hq) * D / 8;  // 16-byte pieces of a token
       const int64_t head = one_first * row, tail = (args.T - one_end) * row;
       uint4* o = static_cast<uint4*>(args.out);
-      for (int64_t i = static_cast<int64_t>(cta) * 256 + threadIdx.x - 64; i < head + tail; i += static_cast<int64_t>(G) * 256)
+      for (int64_t i = static_cast<int64_t>(cta) * 256 + threadIdx.x - 128; i < head + tail; i += static_cast<int64_t>(G) * 256)
         o[i < head ? i : one_end * row + i - head] = make_uint4(0, 0, 0, 0);
     }
     bool ok = true;
@@ -381,31 +386,28 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         // the last key of this block that the row sees
         const int last = MODE == PACKED ? pos - j * kTaBlock : args.P - 1 - it.kv_tok - j * kTaBlock;
         const bool masked = __any_sync(0xffffffffu, last < kTaBlock - 1);
-        // S is read twice, 32 columns at a time and one piece ahead, rather than kept in 128 registers
-        uint32_t v[2][32];
-        auto mask = [&](uint32_t(&x)[32], int c) {
-          if (masked) {
+        uint32_t v[4][32];                   // this row of S
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e > last) x[e] = __float_as_uint(-INFINITY);
-          }
-        };
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + c * 32, v[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(v[c]);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 128; ++e)
+            if (e > last) v[e >> 5][e & 31] = __float_as_uint(-INFINITY);
+        }
+        // eight partial maxima, so that the reduction is not one long chain; two keys per instruction
         float m8[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = -INFINITY;
-        tmem_ld_32x32b_x32(tS, v[0]);
+        for (int i = 0; i < 8; ++i) m8[i] = __uint_as_float(v[0][i]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait(v[c & 1]);
-          tmem_ld_32x32b_x32(tS + (c < 3 ? c + 1 : 0) * 32, v[(c + 1) & 1]);
-          uint32_t(&x)[32] = v[c & 1];
-          mask(x, c);
+        for (int e = 8; e + 16 <= 128; e += 16) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 16) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m8[i] = fmax3(m8[i], __uint_as_float(x[e + i]), __uint_as_float(x[e + 8 + i]));
-          }
+          for (int i = 0; i < 8; ++i)
+            m8[i] = fmax3(m8[i], __uint_as_float(v[(e + i) >> 5][(e + i) & 31]), __uint_as_float(v[(e + 8 + i) >> 5][(e + 8 + i) & 31]));
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(m8[i], __uint_as_float(v[3][24 + i]));
         const float m_blk = fmaxf(fmax3(m8[0], m8[1], m8[2]), fmaxf(fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * sc;
         float alpha = 1.f;
         const bool raise = m_blk > m_use + kTaRescale;
@@ -432,11 +434,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          __syncwarp();
-          tmem_ld_wait(v[c & 1]);  // piece c (the first was asked for above)
-          if (c < 3) tmem_ld_32x32b_x32(tS + (c + 1) * 32, v[(c + 1) & 1]);
-          uint32_t(&x)[32] = v[c & 1];
-          mask(x, c);
+          uint32_t(&x)[32] = v[c];
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -445,6 +443,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             rs4[(e >> 1) & 3] = __fadd2_rn(rs4[(e >> 1) & 3], pp);
             w[e / 2] = pack2<T>(pp.x, pp.y);
           }
+          __syncwarp();
           tmem_st_32x32b_x16(tS + c * 16, w);  // over columns of S already read
           if (c & 1) {
             // half of P is ready: its share of the product may start
@@ -942,6 +941,10 @@ static int launch_tiles_as(const CUtensorMap& q, const CUtensorMap& k, const CUt
   XDNA_CUDA(cudaGetDevice(&dev));
   auto kern = tile_attention_kernel<T, D, MODE>;
   if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    // setmaxnreg shares out the launch's registers: with fewer its warps would wait for good
+    cudaFuncAttributes attr;
+    XDNA_CUDA(cudaFuncGetAttributes(&attr, kern));
+    if (attr.numRegs < kTaRegsLaunch) return fail(XDNA_ERR_UNSUPPORTED, "tile_attention_kernel: built with %d registers", attr.numRegs);
     XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TaShape<D>::kSmem));
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
