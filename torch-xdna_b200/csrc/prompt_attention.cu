@@ -281,64 +281,83 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ------------------------------------------------------------------ MMA
-      bool ok = true, issued = false;
-      int g = 0, p_seen[2] = {0, 0};  // ring blocks, and each tile's P so far
-      auto wait_ring = [&](int i) { return mbar_wait(r_full + i % kStages, (i / kStages) & 1, abort_flag, args.err, 43); };
-      auto issue_s = [&](int t, int i) {
+    // -------------------------------------------------------------------- MMA
+    // The whole warp walks the loop, so that addresses and descriptors are warp-uniform values, and one elected lane
+    // issues: from divergent code (lane 0 alone) an MMA went out every 85 to 90 cycles, and it takes 64.
+    const bool leader = elect_one();
+    bool ok = true, issued = false;
+    int p_seen[2] = {0, 0};         // each tile's P so far
+    uint32_t stage = 0, phase = 0;  // of the ring's next block
+    const uint32_t ring0 = smem_u32(smR), q0 = smem_u32(smQ);
+    // the stage i blocks on (i < kStages), and its phase
+    auto stage_of = [&](uint32_t i) { return stage + i >= kStages ? stage + i - kStages : stage + i; };
+    auto wait_ring = [&](uint32_t i) {
+      const uint32_t st = stage_of(i);
+      return mbar_wait(r_full + st, phase ^ (stage + i >= kStages ? 1u : 0u), abort_flag, args.err, 43);
+    };
+    auto issue_s = [&](int t, uint32_t i) {
+      tc_fence_after();
+      if (leader) {
         const uint32_t tS = tmem + 128 * t;
-        const uint32_t block = smem_u32(smR + (i % kStages) * kTile), q = smem_u32(smQ + t * kTile);
+        const uint64_t dQ = smem_desc_k_sw128(q0 + t * kTile), dK = smem_desc_k_sw128(ring0 + stage_of(i) * kTile);
 #pragma unroll
         for (int kk = 0; kk < kKB; ++kk) {
-          const uint64_t dQ = smem_desc_k_sw128(q + kk * kBlk), dK = smem_desc_k_sw128(block + kk * kBlk);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tS, dQ + 2 * k, dK + 2 * k, IDESC_S, (kk | k) != 0);
-        }
-        umma_commit(s_full + t);
-        issued = true;
-      };
-      auto issue_pv = [&](int t, int i, bool first) -> bool {
-        const uint32_t tO = tmem + 256 + 128 * t, tP = tmem + 128 * t;
-        const uint64_t dV = smem_desc_mn_sw128(smem_u32(smR + (i % kStages) * kTile), kBlk);
-        for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait(p_full + 2 * t + h, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
-          tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tO, tP + 32 * h + 8 * k, dV + 512 * h + 128 * k, IDESC_O, (!first || h || k) != 0);
+            umma_f16(tS, dQ + (kk * (kBlk >> 4) + 2 * k), dK + (kk * (kBlk >> 4) + 2 * k), IDESC_S, (kk | k) != 0);
         }
-        ++p_seen[t];
-        return true;
-      };
-      TileItem it;
-      for (int n = 0; ok && item(n, it); ++n) {
-        const int nb = max(it.nb[0], it.nb[1]);
-        if (!mbar_wait(q_full, n & 1, abort_flag, args.err, 45) || !wait_ring(g)) break;
+        umma_commit(s_full + t);
+      }
+      __syncwarp();
+      issued = true;
+    };
+    auto issue_pv = [&](int t, uint32_t i, bool first) -> bool {
+      const uint32_t tO = tmem + 256 + 128 * t, tP = tmem + 128 * t;
+      const uint64_t dV = smem_desc_mn_sw128(ring0 + stage_of(i) * kTile, kBlk);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!mbar_wait(p_full + 2 * t + h, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
         tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (it.nb[t] > 0) issue_s(t, g);
-        for (int j = 0; ok && j < nb; ++j, g += 2) {
-          // ring block g = K_j, g + 1 = V_j, g + 2 = K_{j+1}
-          if (!wait_ring(g + 1) || (j + 1 < nb && !wait_ring(g + 2))) {
-            ok = false;
-            break;
-          }
-          for (int t = 0; t < 2; ++t) {
-            if (j >= it.nb[t]) continue;
-            if (!(ok = issue_pv(t, g + 1, j == 0))) break;
-            if (j + 1 < it.nb[t])
-              issue_s(t, g + 2);
-            else
-              umma_commit(o_full + t);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tO, tP + 32 * h + 8 * k, dV + (512 * h + 128 * k), IDESC_O, h || k ? 1u : first ? 0u : 1u);
+        }
+        __syncwarp();
+      }
+      ++p_seen[t];
+      return true;
+    };
+    TileItem it;
+    for (int n = 0; ok && item(n, it); ++n) {
+      const int nb = max(it.nb[0], it.nb[1]);
+      if (!mbar_wait(q_full, n & 1, abort_flag, args.err, 45) || !wait_ring(0)) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (it.nb[t] > 0) issue_s(t, 0);
+      for (int j = 0; ok && j < nb; ++j) {
+        // the ring's next blocks: K_j, V_j, K_{j+1}
+        ok = wait_ring(1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && j < it.nb[t]) {
+            ok = issue_pv(t, 1, j == 0);
+            // K_{j+1} is waited for no earlier than it is used: its stage was released late
+            if (ok && j + 1 < it.nb[t] && (ok = wait_ring(2))) issue_s(t, 2);
+            if (ok && j + 1 == it.nb[t]) {
+              if (leader) umma_commit(o_full + t);
+              __syncwarp();
+            }
           }
         }
+        if (stage + 2 >= kStages) phase ^= 1;
+        stage = stage_of(2);
       }
-      if (issued) {
-        umma_commit(drain);
-        volatile int never = 0;
-        mbar_wait(drain, 0, &never, args.err, 46);
-      }
+    }
+    if (issued) {
+      if (leader) umma_commit(drain);
+      volatile int never = 0;
+      mbar_wait(drain, 0, &never, args.err, 46);
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------------- softmax (warps 4..11)
