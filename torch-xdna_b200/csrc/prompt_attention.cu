@@ -59,6 +59,34 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 2^x of two values on the FMA pipe, to relieve the MUFU unit, whose rate (16 a clock and SM) is as tight here as the
+// tensor core's: x = n + f with n whole and |f| <= 1/2, by adding and taking off 1.5 * 2^23; 2^f by the polynomial
+// 1 + c1 f + ... of least largest relative error on [-1/2, 1/2] (a linear program over 4001 points): 1.0e-4 of degree
+// 3, 2.8e-6 of degree 4, against roundings to 2^-9 (bf16) and 2^-12 (f16) that follow. x <= -126, and -inf with it,
+// gives exactly 0 (2^-126 is taken off at the end, where it is otherwise lost), NaN gives NaN. x < 128.
+template <int DEG>
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  constexpr float kC[4] = {DEG == 3 ? 0.6932829f : 0.6931242f, DEG == 3 ? 0.24221097f : 0.24024038f,
+                           DEG == 3 ? 0.055008933f : 0.055906627f, 0.009585382f};
+  auto both = [](float a) { return make_float2(a, a); };
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  const float2 t = __fadd2_rn(x, both(12582912.f)), n = __fadd2_rn(t, both(-12582912.f));
+  const float2 f = __ffma2_rn(n, both(-1.f), x);
+  float2 p = both(kC[DEG - 1]);
+#pragma unroll
+  for (int i = DEG - 2; i >= 0; --i) p = __ffma2_rn(p, f, both(kC[i]));
+  p = __ffma2_rn(p, f, both(1.f));
+  const float2 two_n = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+  return __ffma2_rn(p, two_n, both(-1.17549435e-38f));
+}
+
+// Of every four pairs of exponentials, those computed by exp2_fma. With heads of 64 the exponentials are twice as many
+// per MMA: one of four 208 us, none 226, two 238 (one prompt of 8191, 16 heads of 64). With heads of 128 the issue
+// slots it takes cost as much as it saves: 232, 229 and 249 us (16 heads over 8).
+constexpr int ta_fma_of_4(int d) { return d == 64 ? 1 : 0; }
+
 enum TileMode { PACKED = 0, PREFIX = 1 };
 
 // What the plan of a packed call says (workspace): a header, then the tile pairs, those with the most key blocks
@@ -95,8 +123,11 @@ template <int D>
 struct TaShape {
   static constexpr int kKB = D / 64;                    // 64-column k-blocks of a row
   static constexpr int kTile = 128 * D * 2;             // bytes of a Q tile, a K block or a V block
-  static constexpr int kStages = D == 128 ? 5 : 8;      // K / V blocks in the ring
-  static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 256;
+  static constexpr int kStages = D == 128 ? 4 : 8;      // K / V blocks in the ring (a fifth of 128 gained nothing)
+  static constexpr int kStaging = 8 * 4096;             // a warp's 32 rows of 128 bytes on their way out
+  static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 1;  // mbarriers
+  static constexpr int kSmem = (2 + kStages) * kTile + kStaging + kBars * 8 + 8 /*TMEM address, abort flag*/ + 1024 /*alignment*/;
+  static_assert(kSmem <= 227 * 1024, "more shared memory than a CTA may have");
 };
 
 struct TileItem {
@@ -136,13 +167,15 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   using Shape = TaShape<D>;
   constexpr int kStages = Shape::kStages, kKB = Shape::kKB, kTile = Shape::kTile, kBlk = 128 * 128;
   constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+  constexpr int kDeg = kBf16 ? 3 : 4;  // of exp2_fma
   constexpr uint32_t IDESC_S = idesc_half(kBf16, false, 128, 128);
   constexpr uint32_t IDESC_O = idesc_half(kBf16, true, 128, D);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smQ = smem;                       // [tile][k-block]
   uint8_t* smR = smQ + 2 * kTile;            // ring: [stage][k-block]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smR + kStages * kTile);
+  uint8_t* smO = smR + kStages * kTile;      // staging
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smO + Shape::kStaging);
   uint64_t* q_full = bars;
   uint64_t* q_empty = bars + 1;              // the softmaxes have seen the item's last S: Q may be reloaded
   uint64_t* r_full = bars + 2;               // [kStages]
@@ -458,7 +491,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, nm2);
-            const float2 pp = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+            const float2 pp = ((e >> 1) & 3) < ta_fma_of_4(D) ? exp2_fma<kDeg>(z) : make_float2(fast_exp2(z.x), fast_exp2(z.y));
             rs4[(e >> 1) & 3] = __fadd2_rn(rs4[(e >> 1) & 3], pp);
             w[e / 2] = pack2<T>(pp.x, pp.y);
           }
@@ -480,18 +513,34 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       tc_fence_after();
       const int tok = it.q_tok + t * args.tok + r_tok;
       const int head = it.kvh * args.group + r_head;
+      const bool mine = r_ok && (MODE == PACKED ? pos < it.len : tok < args.B);
+      const int row = mine ? tok * args.hq + head : -1;
+      // The rows go out through shared memory, 128 bytes of each at a time, so that a store of the warp writes four
+      // whole lines; the threads' own rows, 16 bytes each, were 32 half sectors apart (128 us instead of 113 for 16
+      // ragged prompts). put() takes 16-byte piece p of the thread's row, flush() writes the pieces to base + row * pitch.
+      uint8_t* staging = smO + (warp - 4) * 4096;
+      auto put = [&](int p, uint4 u) { *reinterpret_cast<uint4*>(staging + lane * 128 + ((p ^ lane) & 7) * 16) = u; };
+      auto flush = [&](uint8_t* base, int pitch) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int from = i * 4 + (lane >> 3), to = __shfl_sync(0xffffffffu, row, from);
+          const uint4 u = *reinterpret_cast<const uint4*>(staging + from * 128 + ((lane ^ from) & 7) * 16);
+          if (to >= 0) *reinterpret_cast<uint4*>(base + static_cast<int64_t>(to) * pitch + (lane & 7) * 16) = u;
+        }
+        __syncwarp();
+      };
       uint32_t o[32];
       if constexpr (MODE == PACKED) {
-        const bool mine = r_ok && pos < it.len;
         const float inv = 1.f / l;
         float bad = 0.f;  // stays 0 over finite values
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(args.out) + (static_cast<int64_t>(tok) * args.hq + head) * D);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          __syncwarp();
-          tmem_ld_32x32b_x32(tO + c * 32, o);
-          tmem_ld_wait();
-          if (mine) {
+        for (int c = 0; c < D / 64; ++c) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            __syncwarp();
+            tmem_ld_32x32b_x32(tO + c * 64 + h * 32, o);
+            tmem_ld_wait(o);
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               float x[8];
@@ -500,9 +549,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
                 x[i] = __uint_as_float(o[e + i]) * inv;
                 bad = fmaf(x[i], 0.f, bad);
               }
-              dst[(c * 32 + e) / 8] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+              put(h * 4 + e / 8, make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])));
             }
           }
+          flush(static_cast<uint8_t*>(args.out) + c * 128, D * 2);
         }
         unsigned again = __ballot_sync(0xffffffffu, mine && !(bad == 0.f));
         while (again) {
@@ -517,22 +567,17 @@ __global__ void __launch_bounds__(kTaThreads, 1)
                               static_cast<T*>(args.out) + (static_cast<int64_t>(w_tok) * args.hq + w_head) * D);
         }
       } else {
-        const bool mine = r_ok && tok < args.B;
-        const int64_t row = (static_cast<int64_t>(it.split) * args.B + tok) * args.hq + head;
-        float4* dst = reinterpret_cast<float4*>(args.part_o + row * D);
+        const int64_t part = static_cast<int64_t>(it.split) * args.B * args.hq;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           __syncwarp();
           tmem_ld_32x32b_x32(tO + c * 32, o);
-          tmem_ld_wait();
-          if (mine) {
+          tmem_ld_wait(o);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              dst[(c * 32 + e) / 4] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
-                                                  __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-          }
+          for (int e = 0; e < 32; e += 4) put(e / 4, make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+          flush(reinterpret_cast<uint8_t*>(args.part_o + part * D) + c * 128, D * 4);
         }
-        if (mine) args.part_ml[row] = make_float2(m_use, l);
+        if (mine) args.part_ml[part + row] = make_float2(m_use, l);
       }
       // O has been read: the next item's first product (issued after this warp's next P) may overwrite it
       tc_fence_before();
