@@ -101,9 +101,9 @@ struct TileArgs {
   int* err;
   void* out;
   // PACKED
-  const PlanHeader* plan;  // null: one sequence, cu read here
+  const PlanHeader* plan;  // null: at most 32 sequences, cu read here
   const int32_t* cu;
-  int T;
+  int T, n_seqs;
   const void *q, *k, *v;  // recompute_row
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
   // PREFIX
@@ -223,17 +223,36 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   // Items, heaviest first: round n of the G CTAs takes items nG .. nG + G - 1, alternately forwards and backwards,
-  // which balances the CTAs' key blocks. Every role walks the same items.
-  int n_items, one_first = 0, one_end = 0;
+  // which balances the CTAs' key blocks. Every warp walks the same items, all its lanes together.
+  // PACKED, up to 32 sequences: no plan is made. Lane i holds sequence i, and an item's place in the order of falling
+  // weight (key blocks) is found from counts: a sequence of len tokens has min(pairs, 128 w / (tokens of a pair)) pairs
+  // of weight w or less (all of them where len <= 128 w), so walking the weights down and adding these up over the
+  // lanes says which weight item number x has, and a scan over the lanes which sequence's and which pair.
+  const int per_pair = 2 * args.tok;
+  int n_items, one_first = 0, one_end = 0, seq_start = 0, seq_len = 0, level = 0, level_base = 0, level_count = 0;
+  auto pairs_upto = [&](int w) { return seq_len <= kTaBlock * w ? (seq_len + per_pair - 1) / per_pair : kTaBlock * w / per_pair; };
   if constexpr (MODE == PACKED) {
     if (args.plan) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       n_items = args.plan->n_pairs * args.hkv;
       one_first = args.plan->first;
       one_end = args.plan->end;
     } else {
-      one_first = min(max(args.cu[0], 0), args.T);
-      one_end = min(max(args.cu[1], one_first), args.T);
-      n_items = (one_end - one_first + 2 * args.tok - 1) / (2 * args.tok) * args.hkv;
+      auto clamp = [&](int x) { return min(max(x, 0), args.T); };
+      one_first = clamp(args.cu[0]);
+      int end = lane < args.n_seqs ? clamp(args.cu[lane + 1]) : 0;  // ascending whatever cu holds
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end = max(end, y);
+      }
+      end = max(end, one_first);
+      seq_start = __shfl_up_sync(0xffffffffu, end, 1);
+      if (lane == 0) seq_start = one_first;
+      seq_len = end - seq_start;
+      one_end = __shfl_sync(0xffffffffu, end, 31);
+      n_items = __reduce_add_sync(0xffffffffu, (seq_len + per_pair - 1) / per_pair) * args.hkv;
+      level = __reduce_max_sync(0xffffffffu, (seq_len + kTaBlock - 1) / kTaBlock);
+      level_count = __reduce_add_sync(0xffffffffu, pairs_upto(level) - pairs_upto(level - 1));
     }
   } else {
     n_items = args.pairs * args.hkv * args.splits;
@@ -251,9 +270,21 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         begin = e.y;
         end = e.z;
       } else {
-        begin = one_first;
-        end = one_end;
-        it.q_tok = begin + (n_items / args.hkv - 1 - rest) * 2 * args.tok;
+        while (rest >= level_base + level_count) {  // weights down to 1 hold all pairs
+          level_base += level_count;
+          --level;
+          level_count = __reduce_add_sync(0xffffffffu, pairs_upto(level) - pairs_upto(level - 1));
+        }
+        const int below = pairs_upto(level - 1), mine = pairs_upto(level) - below, at = rest - level_base;
+        int upto = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        const int who = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
+        begin = __shfl_sync(0xffffffffu, seq_start, who);
+        end = begin + __shfl_sync(0xffffffffu, seq_len, who);
+        it.q_tok = begin + __shfl_sync(0xffffffffu, below + at - (upto - mine), who) * per_pair;
       }
       it.kv_tok = begin;
       it.len = end - begin;
@@ -266,7 +297,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     } else {
       const int pair = rest % args.pairs;
       it.split = rest / args.pairs;
-      it.q_tok = pair * 2 * args.tok;
+      it.q_tok = pair * per_pair;
       const int b0 = it.split * args.blocks_per_split;
       it.kv_tok = b0 * kTaBlock;
       const int nb = min(args.blocks_per_split, (args.P + kTaBlock - 1) / kTaBlock - b0);
@@ -279,39 +310,44 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTaRegsIssue));
   if (warp == 0) {
-    if (lane == 0) {
-      // ------------------------------------------------------------------ TMA
-      int g = 0, q_loads = 0;  // ring blocks and Q loads so far
-      bool ok = true;
-      const uint32_t q_bytes = static_cast<uint32_t>(args.tok * args.group) * D * 2;
-      auto load = [&](const CUtensorMap* map, int kvh, int tok) -> bool {
-        const int st = g % kStages;
-        if (!mbar_wait(r_empty + st, ((g / kStages) & 1) ^ 1, abort_flag, args.err, 40)) return false;
+    // -------------------------------------------------------------------- TMA
+    const bool leader = elect_one();
+    int g = 0, q_loads = 0;  // ring blocks and Q loads so far
+    bool ok = true;
+    const uint32_t q_bytes = static_cast<uint32_t>(args.tok * args.group) * D * 2;
+    auto load = [&](const CUtensorMap* map, int kvh, int tok) -> bool {
+      const int st = g % kStages;
+      if (!mbar_wait_warp(r_empty + st, ((g / kStages) & 1) ^ 1, abort_flag, args.err, 40)) return false;
+      if (leader) {
         mbar_arrive_expect_tx(r_full + st, kTile);
         for (int kk = 0; kk < kKB; ++kk) tma_load_3d(smR + st * kTile + kk * kBlk, map, r_full + st, kk * 64, kvh, tok);
-        ++g;
-        return true;
-      };
-      TileItem it;
-      for (int n = 0; ok && item(n, it); ++n) {
-        const int tiles = it.nb[1] > 0 ? 2 : 1;
-        if (!mbar_wait(q_empty, (n & 1) ^ 1, abort_flag, args.err, 41)) break;
+      }
+      __syncwarp();
+      ++g;
+      return true;
+    };
+    TileItem it;
+    for (int n = 0; ok && item(n, it); ++n) {
+      const int tiles = it.nb[1] > 0 ? 2 : 1;
+      if (!mbar_wait_warp(q_empty, (n & 1) ^ 1, abort_flag, args.err, 41)) break;
+      if (leader) {
         mbar_arrive_expect_tx(q_full, tiles * q_bytes);
         for (int t = 0; t < tiles; ++t)
           for (int kk = 0; kk < kKB; ++kk)
             tma_load_4d(smQ + t * kTile + kk * kBlk, &tmQ, q_full, kk * 64, 0, it.kvh, it.q_tok + t * args.tok);
-        ++q_loads;
-        const int nb = max(it.nb[0], it.nb[1]);
-        for (int j = 0; ok && j < nb; ++j)
-          ok = load(&tmK, it.kvh, it.kv_tok + j * kTaBlock) && load(&tmV, it.kvh, it.kv_tok + j * kTaBlock);
       }
-      // every load has landed before the CTA may exit
-      volatile int never = 0;
-      if (q_loads > 0) mbar_wait(q_full, static_cast<uint32_t>((q_loads - 1) & 1), &never, args.err, 42);
-      for (int s = 0; s < kStages && s < g; ++s) {
-        const int last = (g - 1 - s) / kStages;  // the last use of stage s
-        mbar_wait(r_full + s, static_cast<uint32_t>(last & 1), &never, args.err, 42);
-      }
+      __syncwarp();
+      ++q_loads;
+      const int nb = max(it.nb[0], it.nb[1]);
+      for (int j = 0; ok && j < nb; ++j)
+        ok = load(&tmK, it.kvh, it.kv_tok + j * kTaBlock) && load(&tmV, it.kvh, it.kv_tok + j * kTaBlock);
+    }
+    // every load has landed before the CTA may exit
+    volatile int never = 0;
+    if (q_loads > 0) mbar_wait_warp(q_full, static_cast<uint32_t>((q_loads - 1) & 1), &never, args.err, 42);
+    for (int s = 0; s < kStages && s < g; ++s) {
+      const int last = (g - 1 - s) / kStages;  // the last use of stage s
+      mbar_wait_warp(r_full + s, static_cast<uint32_t>(last & 1), &never, args.err, 42);
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------------- MMA
@@ -326,7 +362,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     auto stage_of = [&](uint32_t i) { return stage + i >= kStages ? stage + i - kStages : stage + i; };
     auto wait_ring = [&](uint32_t i) {
       const uint32_t st = stage_of(i);
-      return mbar_wait(r_full + st, phase ^ (stage + i >= kStages ? 1u : 0u), abort_flag, args.err, 43);
+      return mbar_wait_warp(r_full + st, phase ^ (stage + i >= kStages ? 1u : 0u), abort_flag, args.err, 43);
     };
     auto issue_s = [&](int t, uint32_t i) {
       tc_fence_after();
@@ -349,7 +385,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const uint64_t dV = smem_desc_mn_sw128(ring0 + stage_of(i) * kTile, kBlk);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!mbar_wait(p_full + 2 * t + h, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
+        if (!mbar_wait_warp(p_full + 2 * t + h, p_seen[t] & 1, abort_flag, args.err, 44)) return false;
         tc_fence_after();
         if (leader) {
 #pragma unroll
@@ -364,7 +400,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     TileItem it;
     for (int n = 0; ok && item(n, it); ++n) {
       const int nb = max(it.nb[0], it.nb[1]);
-      if (!mbar_wait(q_full, n & 1, abort_flag, args.err, 45) || !wait_ring(0)) break;
+      if (!mbar_wait_warp(q_full, n & 1, abort_flag, args.err, 45) || !wait_ring(0)) break;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if (it.nb[t] > 0) issue_s(t, 0);
@@ -390,7 +426,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     if (issued) {
       if (leader) umma_commit(drain);
       volatile int never = 0;
-      mbar_wait(drain, 0, &never, args.err, 46);
+      mbar_wait_warp(drain, 0, &never, args.err, 46);
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------------- softmax (warps 4..11)
@@ -425,7 +461,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const int pos = it.q_pos + t * args.tok + r_tok;  // PACKED: place in the sequence
       float m_use = -INFINITY, l = 0.f;
       for (int j = 0; j < nb; ++j, ++g) {
-        if (!mbar_wait(s_full + t, g & 1, abort_flag, args.err, 47)) {
+        if (!mbar_wait_warp(s_full + t, g & 1, abort_flag, args.err, 47)) {
           ok = false;
           break;
         }
@@ -507,7 +543,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
         l += ((rs4[0].x + rs4[0].y) + (rs4[1].x + rs4[1].y)) + ((rs4[2].x + rs4[2].y) + (rs4[3].x + rs4[3].y));
       }
-      if (!ok || !mbar_wait(o_full + t, items & 1, abort_flag, args.err, 48)) break;
+      if (!ok || !mbar_wait_warp(o_full + t, items & 1, abort_flag, args.err, 48)) break;
       ++items;
       release(stage(2 * nb - 1), nb - 1 >= other);
       tc_fence_after();
@@ -596,6 +632,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 // their tile pairs sorted by key blocks, most first, by counting. The order among equals is left to the atomics: it
 // changes which CTA takes a pair, never a result. The list has room for tokens / (2 tok) + n_seqs pairs, which the
 // ascending bounds cannot exceed.
+constexpr int kPlanFree = 32;  // up to so many sequences no plan is made (one lane each)
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBins = 2048;
 
@@ -624,6 +661,7 @@ __device__ __forceinline__ int block_scan(int x, bool is_max, int* scratch) {
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int32_t* cu, int n_seqs, int T, int per_pair,
                                                                    PlanHeader* plan) {
+  asm volatile("griddepcontrol.launch_dependents;");
   __shared__ int scratch[32], starts[kPlanThreads], ends[kPlanThreads], upto[kPlanThreads], bins[kPlanBins];
   int4* list = reinterpret_cast<int4*>(plan + 1);
   auto clamp = [&](int x) { return min(max(x, 0), T); };
@@ -1012,6 +1050,10 @@ static int launch_tiles_as(const CUtensorMap& q, const CUtensorMap& k, const CUt
     XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TaShape<D>::kSmem));
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
+  if (a.plan) {  // it may start while the plan is made
+    XDNA_CUDA(launch_early(kern, dim3(grid), kTaThreads, TaShape<D>::kSmem, s, q, k, v, a));
+    return XDNA_OK;
+  }
   kern<<<grid, kTaThreads, TaShape<D>::kSmem, s>>>(q, k, v, a);
   return check_launch("tile_attention_kernel");
 }
@@ -1052,7 +1094,7 @@ using namespace xdna;
 extern "C" {
 
 size_t xdna_packed_attention_workspace(int64_t n_seqs, int64_t tokens, int64_t hq, int64_t hkv) {
-  if (n_seqs <= 1 || tokens < 0 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
+  if (n_seqs <= kPlanFree || tokens < 0 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
   return sizeof(PlanHeader) + 16 * static_cast<size_t>(plan_pairs(n_seqs, tokens, hq / hkv));
 }
 
@@ -1086,6 +1128,7 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
   a.out = out;
   a.cu = cu_seqlens;
   a.T = static_cast<int>(tokens);
+  a.n_seqs = static_cast<int>(n_seqs);
   a.q = q, a.k = k, a.v = v;
   a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
   CUtensorMap tq, tk, tv;
@@ -1093,8 +1136,8 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
       (rc = kv_map(&tk, k, k_st, k_sh, tokens, hkv, d, dtype)) != XDNA_OK ||
       (rc = kv_map(&tv, v, v_st, v_sh, tokens, hkv, d, dtype)) != XDNA_OK)
     return rc;
-  int64_t pairs = (tokens + 2 * tok - 1) / (2 * tok);
-  if (n_seqs > 1) {
+  const int64_t pairs = plan_pairs(n_seqs, tokens, group);
+  if (n_seqs > kPlanFree) {
     XDNA_CHECK_ARG(workspace && aligned16(workspace) &&
                        workspace_bytes >= xdna_packed_attention_workspace(n_seqs, tokens, hq, hkv),
                    "packed_attention: workspace too small or unaligned");
@@ -1102,7 +1145,6 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
     packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(cu_seqlens, static_cast<int>(n_seqs), a.T, static_cast<int>(2 * tok), plan);
     if ((rc = check_launch("packed_plan_kernel")) != XDNA_OK) return rc;
     a.plan = plan;
-    pairs = plan_pairs(n_seqs, tokens, group);
   }
   XDNA_CHECK_ARG(pairs < (1ll << 31) / hkv, "packed_attention: bad sizes");
   return launch_tiles<PACKED>(tq, tk, tv, a, d, dtype, static_cast<int>(std::min<int64_t>(pairs * hkv, sms)), s);

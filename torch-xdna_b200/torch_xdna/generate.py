@@ -61,7 +61,7 @@ def packed_attention(q, k, v, cu_seqlens, scale=None):
     kernels cannot read them); cu_seqlens [N + 1] int32 on the GPU: sequence i is tokens cu_seqlens[i] ..
     cu_seqlens[i + 1] - 1. Tokens of no sequence (padding past the last one) give zeros. scale: 1 / sqrt(D) unless
     given. Returns [T, Hq, D]."""
-    return _call("packed_attention", 1 if cu_seqlens.shape[0] <= 2 else 2, q, k, v, cu_seqlens, scale)
+    return _call("packed_attention", 1 if cu_seqlens.shape[0] <= 33 else 2, q, k, v, cu_seqlens, scale)
 
 
 def shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale=None):
