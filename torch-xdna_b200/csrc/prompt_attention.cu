@@ -114,7 +114,7 @@ struct TileArgs {
 
 constexpr int kTaThreads = 384;  // three warpgroups: issue (TMA, MMA), softmax of tile A, of tile B
 // Registers per thread after setmaxnreg: together what the launch gives, 384 x 168.
-constexpr int kTaRegsLaunch = 168, kTaRegsIssue = 72, kTaRegsSoftmax = 216;
+constexpr int kTaRegsLaunch = 168, kTaRegsIssue = 120, kTaRegsSoftmax = 192;
 static_assert(128 * kTaRegsIssue + 256 * kTaRegsSoftmax <= kTaThreads * kTaRegsLaunch, "more registers than the launch has");
 constexpr int kTaBlock = 128;
 constexpr float kTaRescale = 8.0f;
@@ -466,7 +466,6 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           break;
         }
         tc_fence_after();
-        __syncwarp();
         // S(j) is done, and with it the product with V_{j-1}: K_j and V_{j-1} may be overwritten, after the last S Q too
         release(stage(2 * j), j >= other);
         if (j > 0) release(stage(2 * j - 1), j - 1 >= other);
@@ -714,10 +713,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int32_t
 
 // ---------------------------------------------------------------------------- the batch's own keys and the join
 struct OwnArgs {
-  const void *q, *ck, *cv;
-  int64_t q_sb, q_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh;
+  const void *q, *ck, *cv, *pk, *pv;
+  int64_t q_sb, q_sh, ck_sb, ck_st, ck_sh, cv_sb, cv_st, cv_sh, pk_st, pk_sh, pv_st, pv_sh;
   const int32_t* lens;
   int B, S, hq, hkv, group;
+  int P;       // prefix keys read here, before the own ones (few sequences); else 0
   int parts;   // of the prefix: part_o / part_ml [parts + (splits > 1 ? splits : 0)][B * hq]
   int splits;  // of the own keys
   float scale_log2;
@@ -775,27 +775,31 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnAr
   const int b = static_cast<int>(blockIdx.x) / a.hkv, kvh = static_cast<int>(blockIdx.x) % a.hkv;
   const int h0 = kvh * a.group + static_cast<int>(blockIdx.z) * 8;              // the tile's first query head
   const int rows = min(8, a.group - static_cast<int>(blockIdx.z) * 8);
-  const int n = min(max(a.lens[b], 0), a.S);
+  const int n = a.P + min(max(a.lens[b], 0), a.S);
   const int steps = (n + kOwnStep - 1) / kOwnStep;
   const int per = max((steps + a.splits - 1) / a.splits, kOwnMinSteps);
   const int s0 = min(steps, static_cast<int>(blockIdx.y) * per), s1 = min(steps, s0 + per);
 
   const T* kp = static_cast<const T*>(a.ck) + static_cast<int64_t>(b) * a.ck_sb + static_cast<int64_t>(kvh) * a.ck_sh + 8 * t;
   const T* vp = static_cast<const T*>(a.cv) + static_cast<int64_t>(b) * a.cv_sb + static_cast<int64_t>(kvh) * a.cv_sh + 8 * g;
+  const T* pkp = static_cast<const T*>(a.pk) + static_cast<int64_t>(kvh) * a.pk_sh + 8 * t;
+  const T* pvp = static_cast<const T*>(a.pv) + static_cast<int64_t>(kvh) * a.pv_sh + 8 * g;
+  auto key_row = [&](int key) { return key < a.P ? pkp + key * a.pk_st : kp + (key - a.P) * a.ck_st; };
+  auto value_row = [&](int key) { return key < a.P ? pvp + key * a.pv_st : vp + (key - a.P) * a.cv_st; };
   auto fetch = [&](int step, int st) {
     if (step < s1) {
       const uint32_t dst = smem_u32(ring + st * kStageBytes + lane * 16);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = step * kOwnStep + 8 * r + g;
-        const T* src = kp + (key < n ? key : 0) * a.ck_st;
+        const T* src = key_row(min(key, n - 1));
 #pragma unroll
         for (int c = 0; c < kC; ++c) cp_async_16(dst + (r * kC + c) * 512, src + 32 * c, key < n);
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int key = step * kOwnStep + 2 * t + (x & 1) + 8 * (x >> 1);
-        const T* src = vp + (key < n ? key : 0) * a.cv_st;
+        const T* src = value_row(min(key, n - 1));
 #pragma unroll
         for (int e = 0; e < kE; ++e) cp_async_16(dst + (2 * kC + e * 4 + x) * 512, src + 64 * e, key < n);
       }
@@ -926,21 +930,23 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnAr
   }
 }
 
-// One warp per row: the parts' sums brought to one maximum and added, in the parts' order.
+// One block per row, its warps with every fourth part each: the parts' sums brought to one maximum and added, in a
+// fixed order.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const float* part_o, const float2* part_ml, int parts, int64_t n_rows, T* out) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp_id();
+  const int64_t row = blockIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= n_rows) return;
   constexpr int kV = D / 32;  // dimensions of a lane
+  __shared__ float sums[4][D];
+  __shared__ float2 sml[4];
   float mm = -INFINITY, ll = 0.f, acc[kV];
   for (int s = lane_id(); s < parts; s += 32) mm = fmaxf(mm, part_ml[s * n_rows + row].x);
   for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
   const float base = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
   for (int i = 0; i < kV; ++i) acc[i] = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < parts; ++s) {
+#pragma unroll 4
+  for (int s = warp_id(); s < parts; s += 4) {
     const float2 ml = part_ml[s * n_rows + row];
     const float f = fast_exp2(ml.x - base);
     ll = fmaf(f, ml.y, ll);
@@ -953,10 +959,18 @@ __global__ void __launch_bounds__(128) join_kernel(const float* part_o, const fl
       acc[0] = fmaf(f, u.x, acc[0]), acc[1] = fmaf(f, u.y, acc[1]);
     }
   }
-  const float inv = ll > 0.f || __isnanf(ll) ? 1.f / ll : 0.f;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(out + row * D + lane_id() * kV);
 #pragma unroll
-  for (int i = 0; i < kV; i += 2) dst[i / 2] = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
+  for (int i = 0; i < kV; ++i) sums[warp_id()][lane_id() * kV + i] = acc[i];
+  if (lane_id() == 0) sml[warp_id()].y = ll;
+  __syncthreads();
+  if (threadIdx.x < D / 2) {
+    const int d = threadIdx.x * 2;
+    float x = 0.f, y = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x += sums[w][d], y += sums[w][d + 1], l += sml[w].y;
+    const float inv = l > 0.f || __isnanf(l) ? 1.f / l : 0.f;
+    reinterpret_cast<uint32_t*>(out + row * D)[threadIdx.x] = pack2<T>(x * inv, y * inv);
+  }
 }
 
 // A launch that may start while the kernel before it still runs (and waits for it itself, griddepcontrol.wait).
@@ -998,7 +1012,7 @@ static int launch_own(const OwnArgs& a, cudaStream_t s) {
   }
   if (a.splits == 1) return XDNA_OK;
   const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
-  XDNA_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>((n_rows + 3) / 4)), 128, 0, s, a.part_o, a.part_ml,
+  XDNA_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>(n_rows)), 128, 0, s, a.part_o, a.part_ml,
                          a.parts + a.splits, n_rows, a.out));
   return XDNA_OK;
 }
@@ -1070,19 +1084,23 @@ static int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtens
 
 static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { return tokens / (2 * (128 / group)) + n_seqs; }
 
-// How a prefix call is split: the prefix's keys into about one item per SM, each at least one block; a sequence's own
-// keys, where the sequences and key heads alone are few CTAs for an SM, into pieces of at least 128 (a CTA's two steps
-// per warp): lengths differ, and the longest would be waited for.
+// How a prefix call is split. One sequence, and few with a short prefix, read the prefix themselves, before their own
+// keys (direct): the tile kernel and its parts take about 11 us for any prefix, the reading 0.8 us per thousand keys and
+// sequence (8 key heads of 128). Else the prefix's keys are split into about one item per SM, each at least one block.
+// A sequence's keys, where the sequences and key heads alone are few CTAs for an SM, are split into pieces of at least
+// 128 (a CTA's two steps per warp), at most 32: lengths differ, and the longest would be waited for.
 struct PrefixSplit {
+  bool direct;
   int64_t pairs, parts, blocks_per_part, own;
   PrefixSplit(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int sms) {
-    const int64_t tok = 128 / (hq / hkv), blocks = (P + kTaBlock - 1) / kTaBlock;
+    direct = B == 1 || B * P <= 8192;
+    const int64_t tok = 128 / (hq / hkv), blocks = direct ? 0 : (P + kTaBlock - 1) / kTaBlock;
     pairs = (B + 2 * tok - 1) / (2 * tok);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(blocks, sms / (pairs * hkv)));
     blocks_per_part = blocks ? (blocks + want - 1) / want : 0;
     parts = blocks ? (blocks + blocks_per_part - 1) / blocks_per_part : 0;
-    const int64_t ctas = B * hkv * ((hq / hkv + 7) / 8);
-    own = std::max<int64_t>(1, std::min<int64_t>((S + 127) / 128, 8 * sms / ctas));
+    const int64_t ctas = B * hkv * ((hq / hkv + 7) / 8), keys = S + (direct ? P : 0);
+    own = std::max<int64_t>(1, std::min<int64_t>({(keys + 127) / 128, 8 * sms / ctas, 32}));
   }
   int64_t all() const { return parts + (own > 1 ? own : 0); }
 };
@@ -1164,7 +1182,7 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
                           int dtype, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_heads("prefix_attention", hq, hkv, d, dtype, scale);
   if (rc != XDNA_OK) return rc;
-  XDNA_CHECK_ARG(B >= 0 && P >= 0 && S >= 0 && B < (1ll << 24) / hq && P < (1ll << 31) - kTaBlock && S < (1ll << 31) - kTaBlock,
+  XDNA_CHECK_ARG(B >= 0 && P >= 0 && S >= 0 && B < (1ll << 24) / hq && P < (1ll << 30) && S < (1ll << 30),
                  "prefix_attention: bad sizes");
   int sms = 0;
   if ((rc = check_device(&sms)) != XDNA_OK) return rc;
@@ -1181,7 +1199,7 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
   const PrefixSplit split(B, P, S, hq, hkv, sms);
   float* part_o = static_cast<float*>(workspace);
   float2* part_ml = reinterpret_cast<float2*>(part_o + split.all() * B * hq * d);
-  if (P > 0) {
+  if (split.parts > 0) {
     TileArgs a{};
     a.hq = static_cast<int>(hq);
     a.hkv = static_cast<int>(hkv);
@@ -1209,6 +1227,11 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
   o.q = q, o.ck = ck, o.cv = cv;
   o.q_sb = q_sb, o.q_sh = q_sh;
   o.ck_sb = ck_sb, o.ck_st = ck_st, o.ck_sh = ck_sh, o.cv_sb = cv_sb, o.cv_st = cv_st, o.cv_sh = cv_sh;
+  if (split.direct) {
+    o.P = static_cast<int>(P);
+    o.pk = pk, o.pv = pv;
+    o.pk_st = pk_st, o.pk_sh = pk_sh, o.pv_st = pv_st, o.pv_sh = pv_sh;
+  }
   o.lens = lens;
   o.B = static_cast<int>(B);
   o.S = static_cast<int>(S);

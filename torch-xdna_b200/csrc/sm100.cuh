@@ -130,20 +130,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 
 // mbar_wait by a whole converged warp, which gets one answer, so that it stays converged also where the wait gives up.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int site) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  const uint64_t t0 = global_timer();
-  while (true) {
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    bool stop = *abort != 0;
-    if (!stop && global_timer() - t0 > XDNA_WAIT_LIMIT_NS) {
-      if (lane_id() == 0) record_error(err, XDNA_ERR_TIMEOUT, site);
-      *abort = 1;
-      stop = true;
-    }
-    if (__any_sync(0xffffffffu, stop)) return false;
-  }
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, site));
 }
 
 // ------------------------------------------------------------------ CTA pairs (clusters of 2)

@@ -217,50 +217,59 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
       const uint16_t* x = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(m0) * a.ldx + k0;
       if ((reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx % 8 == 0) {
         const int per = cols / 8;
-        for (int i = threadIdx.x; i < m_rows * per; i += kW4Threads) {
-          const int r = i / per, c = (i - r * per) * 8;
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (k0 + c + 8 <= a.K) {
-            u = *reinterpret_cast<const uint4*>(x + r * a.ldx + c);
-          } else {
-            uint16_t* h = reinterpret_cast<uint16_t*>(&u);
-            for (int e = 0; e < 8; ++e)
-              if (k0 + c + e < a.K) h[e] = x[r * a.ldx + c + e];
+        // four pieces per thread at a time, so that their loads are under way together
+        for (int i0 = threadIdx.x; i0 < m_rows * per; i0 += 4 * kW4Threads) {
+          uint4 u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = i0 + e * kW4Threads, r = i / per, c = (i - r * per) * 8;
+            u[e] = make_uint4(0, 0, 0, 0);
+            if (i < m_rows * per && k0 + c + 8 <= a.K) {
+              u[e] = *reinterpret_cast<const uint4*>(x + r * a.ldx + c);
+            } else if (i < m_rows * per) {
+              uint16_t* h = reinterpret_cast<uint16_t*>(&u[e]);
+              for (int k = 0; k < 8; ++k)
+                if (k0 + c + k < a.K) h[k] = x[r * a.ldx + c + k];
+            }
           }
-          *reinterpret_cast<uint4*>(smx + r * pitch + c * 2) = u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = i0 + e * kW4Threads, r = i / per, c = (i - r * per) * 8;
+            if (i < m_rows * per) *reinterpret_cast<uint4*>(smx + r * pitch + c * 2) = u[e];
+          }
         }
-      } else {
-        for (int r = 0; r < m_rows; ++r) {
-#pragma unroll 8
-          for (int c = threadIdx.x; c < cols; c += kW4Threads)
-            *reinterpret_cast<uint16_t*>(smx + r * pitch + c * 2) = k0 + c < a.K ? x[r * a.ldx + c] : uint16_t(0);
-        }
+        return;
       }
-    } else {
-      const float* x = static_cast<const float*>(a.x) + static_cast<int64_t>(m0) * a.ldx + k0;
-      // four values per thread at a time, so that their loads are under way together
-      for (int r = 0; r < m_rows; ++r) {
-        for (int c0 = threadIdx.x; c0 < cols; c0 += 4 * kW4Threads) {
-          float v[4];
+    }
+    // single values: a warp takes runs of 512 columns of a row, 16 loads per lane under way together
+    const int runs = (cols + 511) / 512;
+    for (int job = warp; job < m_rows * runs; job += kW4Threads / 32) {
+      const int r = job / runs, c0 = (job - r * runs) * 512 + lane;
+      if constexpr (kParts == 1) {
+        const uint16_t* x = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(m0 + r) * a.ldx + k0;
+        uint16_t v[16];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = c0 + e * kW4Threads;
-            v[e] = c < cols && k0 + c < a.K ? x[r * a.ldx + c] : 0.f;
-          }
+        for (int e = 0; e < 16; ++e) v[e] = c0 + 32 * e < cols && k0 + c0 + 32 * e < a.K ? x[c0 + 32 * e] : uint16_t(0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = c0 + e * kW4Threads;
-            if (c >= cols) break;
-            const bool fin = fabsf(v[e]) < INFINITY;
-            const __nv_bfloat16 hi = fin ? __float2bfloat16_rz(v[e]) : __float2bfloat16_rn(v[e]);
-            const float r1 = fin ? v[e] - __bfloat162float(hi) : 0.f;
-            const __nv_bfloat16 mid = __float2bfloat16_rz(r1);
-            const __nv_bfloat16 lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
-            __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(smx + 3 * r * pitch + c * 2);
-            d[0] = hi;
-            d[pitch / 2] = mid;
-            d[pitch] = lo;
-          }
+        for (int e = 0; e < 16; ++e)
+          if (c0 + 32 * e < cols) *reinterpret_cast<uint16_t*>(smx + r * pitch + (c0 + 32 * e) * 2) = v[e];
+      } else {
+        const float* x = static_cast<const float*>(a.x) + static_cast<int64_t>(m0 + r) * a.ldx + k0;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = c0 + 32 * e < cols && k0 + c0 + 32 * e < a.K ? x[c0 + 32 * e] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (c0 + 32 * e >= cols) break;
+          const bool fin = fabsf(v[e]) < INFINITY;
+          const __nv_bfloat16 hi = fin ? __float2bfloat16_rz(v[e]) : __float2bfloat16_rn(v[e]);
+          const float r1 = fin ? v[e] - __bfloat162float(hi) : 0.f;
+          const __nv_bfloat16 mid = __float2bfloat16_rz(r1);
+          const __nv_bfloat16 lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
+          __nv_bfloat16* d = reinterpret_cast<__nv_bfloat16*>(smx + 3 * r * pitch + (c0 + 32 * e) * 2);
+          d[0] = hi;
+          d[pitch / 2] = mid;
+          d[pitch] = lo;
         }
       }
     }
