@@ -100,6 +100,9 @@ const char* xdna_last_error(void);
 /* ABI version of this library (bumped when a signature changes). */
 int xdna_abi_version(void);
 
+/* Kernels of this library that the calling thread has enqueued so far. */
+int64_t xdna_launch_count(void);
+
 /* XDNA_OK when `device` is an sm_100 GPU this library's kernels run on. */
 int xdna_device_check(int device);
 

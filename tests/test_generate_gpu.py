@@ -600,3 +600,119 @@ def test_report_counts_the_calls(cuda):
     for c in calls:
         c(pkg)
     assert pkg.stats.calls["gpu"] == 4 and pkg.stats.launches >= 4
+
+
+def test_launches_are_counted(cuda):
+    """One kernel each where one is enough; the plan of many sequences, the prefix's tiles and the join are more."""
+    import torch_xdna
+
+    def launches(f):
+        before = torch_xdna.stats.launches
+        f()
+        return torch_xdna.stats.launches - before
+
+    q, k = randn(100, 4, 64), randn(100, 2, 64)
+    assert launches(lambda: torch_xdna.packed_attention(q, k, k, cu_of((60, 40)))) == 1
+    assert launches(lambda: torch_xdna.packed_attention(q, k, k, cu_of([2] * 50))) == 2
+    x = prefix_inputs(3, 50, 20, 4, 2, 64)
+    assert launches(lambda: torch_xdna.shared_prefix_attention(*x, int32([1, 2, 3]))) == 1
+    x = prefix_inputs(70, 257, 20, 4, 2, 64)
+    assert launches(lambda: torch_xdna.shared_prefix_attention(*x, int32([5] * 70))) == 2
+    codes, scales = w4_inputs(64, 128, 32)
+    assert launches(lambda: torch_xdna.linear_w4(randn(1, 128), codes, scales, 32)) == 1
+    assert launches(lambda: torch_xdna.w4_pack(randn(4, 128))) == 1
+    assert launches(lambda: torch_xdna.process_logits(randn(2, 100))) == 1
+
+
+# ------------------------------------------------------------------ values at the ends of the types, both paths
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_large_and_special_values(cuda, d):
+    import torch_xdna
+
+    lens = (130, 170)
+    q, k, v = randn(300, 4, d, seed=1), randn(300, 2, d, seed=2), randn(300, 2, d, seed=3)
+    clean = packed_want(q, k, v, [(0, 130)])
+    v[130:] = 3e38                                       # finite, of another sequence
+    got = torch_xdna.packed_attention(q, k, v, cu_of(lens))
+    close(got[:130], *(x[:130] for x in clean))
+    # a NaN key reaches every later token of its sequence and no earlier one
+    v[130:] = 1.0
+    k[40, 0] = float("nan")
+    got = torch_xdna.packed_attention(q, k, v, cu_of(lens))
+    assert bool(torch.isnan(got[40:130, :2]).all()) and not bool(torch.isnan(got[:40]).any())
+    assert not bool(torch.isnan(got[130:]).any()) and not bool(torch.isnan(got[:, 2:]).any())
+    # a NaN value: only its own dimension
+    k[40, 0] = 0.0
+    v[41, 0, 3] = float("nan")
+    got = torch_xdna.packed_attention(q, k, v, cu_of(lens))
+    assert bool(torch.isnan(got[41:130, :2, 3]).all()) and not bool(torch.isnan(got[41:130, :2, 4:]).any())
+    assert not bool(torch.isnan(got[:41]).any())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b", [3, 90])
+def test_prefix_peaked_special_and_far(cuda, b, d):
+    """b = 3: few sequences read the prefix themselves; 90: it goes through the tiles."""
+    import torch_xdna
+
+    p, s = 1000, 40
+    q, pk, pv, ck, cv = prefix_inputs(b, p, s, 4, 2, d)
+    q = q.abs()
+    lens = [(11 * i) % (s + 1) for i in range(b)]
+    for x, y in ((0.1, 4.0), (4.0, 0.1), (-3.0, 3.0), (3.0, -3.0)):
+        kp = (pk.abs().float() * torch.linspace(0, x, p, device="cuda")[:, None, None]).bfloat16()
+        kc = (ck.abs().float() * y).bfloat16()
+        o, tol = prefix_want(q, kp, pv, kc, cv, lens)
+        close(torch_xdna.shared_prefix_attention(q, kp, pv, kc, cv, int32(lens)), o, tol * 2)
+    bad = pk.clone()
+    bad[77, 1] = float("nan")
+    got = torch_xdna.shared_prefix_attention(q, bad, pv, ck, cv, int32(lens))
+    assert bool(torch.isnan(got[:, 2:]).all()) and not bool(torch.isnan(got[:, :2]).any())
+    heads_first = [t.transpose(-3, -2).contiguous().transpose(-3, -2) for t in (q, pk, pv, ck, cv)]
+    close(torch_xdna.shared_prefix_attention(*heads_first, int32(lens)), *prefix_want(q, pk, pv, ck, cv, lens))
+    base = torch.empty(2 ** 31 + 2 ** 20, dtype=torch.bfloat16, device="cuda")
+    far = base.as_strided((p, 2, d), (2 ** 21, d, 1))
+    far.copy_(pk)
+    close(torch_xdna.shared_prefix_attention(q, far, far, ck, cv, int32(lens)), *prefix_want(q, pk, pk, ck, cv, lens))
+
+
+def test_linear_w4_scales_at_odd_places(cuda):
+    """Views of larger weights: scales that start on two bytes, rows of an odd number of them, the array's last one."""
+    import torch_xdna
+
+    for k, group in ((300, 128), (1100, 128), (1500, 64), (900, 32)):
+        codes, scales = w4_inputs(41, k, group)
+        x = randn(3, k, seed=2)
+        for i in (0, 1, 40):
+            close(torch_xdna.linear_w4(x, codes[i:], scales[i:], group), *w4_want(x, codes[i:], scales[i:], group, None))
+
+
+# ------------------------------------------------------------------ the operators together
+def test_example_decode_agrees_with_prefill(cuda):
+    """The example's decode (4-bit linears, caches, shared prefix) against its own packed prefill of the same tokens with
+    the weights those bits stand for: the logits after the last step, within the 5e-2 (relative norm) that the package
+    allows its bf16 linears, and tokens that obey the mask."""
+    import importlib.util
+
+    from conftest import ROOT
+
+    spec = importlib.util.spec_from_file_location("generate_example", ROOT / "examples" / "generate.py")
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    gen = torch.Generator().manual_seed(3)
+    vocab, shared, steps = 1000, 140, 5
+    system = torch.randint(0, vocab, (shared,), generator=gen)
+    prompts = [torch.cat((system, torch.randint(0, vocab, (n,), generator=gen))).cuda() for n in (1, 30, 77)]
+    model = ex.Model(2, vocab, torch.device("cuda"))
+    session = ex.Session(model, prompts, shared, steps)
+    mask = torch.full((1, -(-vocab // 32)), -1, dtype=torch.int32, device="cuda")
+    mask[0, :16] = 0                                                     # only tokens from 512 on
+    for _ in range(steps):
+        token = session.choose(mask=mask)
+        assert bool((token >= 512).all())
+        session.step(token)
+    whole = [session.tokens[j, :int(session.prompt_lens[j]) + steps].long() for j in range(3)]
+    logits, _, cu = model.prefill(whole)
+    want = logits[cu[1:].long() - 1].float()
+    got = session.logits.float()
+    assert float((got - want).norm() / want.norm()) < 5e-2

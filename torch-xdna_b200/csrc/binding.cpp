@@ -262,6 +262,8 @@ at::Tensor process_logits(PyObject* const* a) {
   return out;
 }
 
+thread_local int64_t t_launches = 0;  // kernels of the last call
+
 template <at::Tensor (*F)(PyObject* const*), int N>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -270,12 +272,17 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
   }
   try {
-    return THPVariable_Wrap(F(args));
+    const int64_t before = xdna_launch_count();
+    at::Tensor out = F(args);
+    t_launches = xdna_launch_count() - before;
+    return THPVariable_Wrap(std::move(out));
   } catch (const Raised&) {
     return nullptr;
   }
   END_HANDLE_TH_ERRORS
 }
+
+PyObject* launches(PyObject*, PyObject*) { return PyLong_FromLongLong(t_launches); }
 
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 2) {
@@ -292,6 +299,7 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f))
 PyMethodDef kMethods[] = {
     {"init", FAST(init), METH_FASTCALL, "the exception types"},
+    {"launches", launches, METH_NOARGS, "kernels that this thread's last call enqueued"},
     {"packed_attention", FAST((call<packed_attention, 5>)), METH_FASTCALL, nullptr},
     {"shared_prefix_attention", FAST((call<shared_prefix_attention, 7>)), METH_FASTCALL, nullptr},
     {"linear_w4", FAST((call<linear_w4, 5>)), METH_FASTCALL, nullptr},

@@ -16,6 +16,7 @@ namespace xdna {
 __device__ int g_device_error[4];
 
 static thread_local std::string t_last_error;
+static thread_local int64_t t_launches = 0;
 
 int fail(int code, const char* fmt, ...) {
   char buf[1024];
@@ -93,6 +94,7 @@ int* device_error_word() {
 int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(XDNA_ERR_CUDA, "launch of %s failed: %s", what, cudaGetErrorString(e));
+  ++t_launches;
   return XDNA_OK;
 }
 
@@ -145,6 +147,8 @@ extern "C" {
 const char* xdna_last_error(void) { return xdna::t_last_error.c_str(); }
 
 int xdna_abi_version(void) { return 1; }
+
+int64_t xdna_launch_count(void) { return xdna::t_launches; }
 
 int xdna_ipc_alloc(size_t bytes, void** dev_ptr) {
   XDNA_CHECK_ARG(dev_ptr != nullptr && bytes > 0, "ipc_alloc: bad arguments");

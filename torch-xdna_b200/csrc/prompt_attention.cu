@@ -137,6 +137,23 @@ struct TileItem {
   int split;               // PREFIX
 };
 
+// A launch that may start while the kernel before it still runs (and waits for it itself, griddepcontrol.wait).
+template <typename... Params, typename... Args>
+static int launch_early(const char* what, void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  XDNA_CUDA(cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...));
+  return check_launch(what);
+}
+
 // One row over exactly its keys [0, n), a warp with D / 32 dimensions per lane.
 template <typename T, int D>
 __device__ __noinline__ void recompute_row(const T* q, const T* k, int64_t k_st, const T* v, int64_t v_st, int n,
@@ -973,22 +990,6 @@ __global__ void __launch_bounds__(128) join_kernel(const float* part_o, const fl
   }
 }
 
-// A launch that may start while the kernel before it still runs (and waits for it itself, griddepcontrol.wait).
-template <typename... Params, typename... Args>
-static cudaError_t launch_early(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
-}
-
 template <typename T, int D>
 static int launch_own(const OwnArgs& a, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.B * a.hkv), static_cast<unsigned>(a.splits), static_cast<unsigned>((a.group + 7) / 8));
@@ -1003,18 +1004,17 @@ static int launch_own(const OwnArgs& a, cudaStream_t s) {
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
   // after the prefix's kernel it may start early; alone it is an ordinary launch
+  int rc;
   if (a.parts > 0) {
-    XDNA_CUDA(launch_early(kern, grid, kOwnWarps * 32, kSmem, s, a));
+    rc = launch_early("own_keys_kernel", kern, grid, kOwnWarps * 32, kSmem, s, a);
   } else {
     kern<<<grid, kOwnWarps * 32, kSmem, s>>>(a);
-    int rc = check_launch("own_keys_kernel");
-    if (rc != XDNA_OK) return rc;
+    rc = check_launch("own_keys_kernel");
   }
-  if (a.splits == 1) return XDNA_OK;
+  if (rc != XDNA_OK || a.splits == 1) return rc;
   const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
-  XDNA_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>(n_rows)), 128, 0, s, a.part_o, a.part_ml,
-                         a.parts + a.splits, n_rows, a.out));
-  return XDNA_OK;
+  return launch_early("join_kernel", join_kernel<T, D>, dim3(static_cast<unsigned>(n_rows)), 128, 0, s, a.part_o, a.part_ml,
+                      a.parts + a.splits, n_rows, a.out);
 }
 
 // ---------------------------------------------------------------------------- host
@@ -1065,8 +1065,7 @@ static int launch_tiles_as(const CUtensorMap& q, const CUtensorMap& k, const CUt
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
   if (a.plan) {  // it may start while the plan is made
-    XDNA_CUDA(launch_early(kern, dim3(grid), kTaThreads, TaShape<D>::kSmem, s, q, k, v, a));
-    return XDNA_OK;
+    return launch_early("tile_attention_kernel", kern, dim3(grid), kTaThreads, TaShape<D>::kSmem, s, q, k, v, a);
   }
   kern<<<grid, kTaThreads, TaShape<D>::kSmem, s>>>(q, k, v, a);
   return check_launch("tile_attention_kernel");

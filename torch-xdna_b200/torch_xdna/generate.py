@@ -24,33 +24,39 @@ from .runtime import DEVICE, stats
 ERR_INVALID = -1
 W4_BLOCK = 128          # columns per block of the stored codes
 BINDING_PATH = Path(__file__).resolve().parent / "lib" / "_xdna_generate.so"
-_native = None          # the binding (csrc/binding.cpp): argument checks, allocation and the C calls
 
 
-def _load():
-    global _native
-    kernels.lib()
-    if not BINDING_PATH.exists():
-        raise kernels.XdnaUnavailable(
-            f"{BINDING_PATH} is not built (run __graft_entry__.build() or make -C torch-xdna_b200/csrc)")
-    loader = importlib.machinery.ExtensionFileLoader("_xdna_generate", str(BINDING_PATH))
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
-    loader.exec_module(module)
-    module.init(kernels.XdnaError, kernels.XdnaUnavailable)
-    _native = module
-    return module
+class _NotLoaded:
+    """Stands for the binding (csrc/binding.cpp: argument checks, allocation and the C calls) until its first use."""
+
+    def __getattr__(self, name):
+        global _native
+        kernels.lib()
+        if not BINDING_PATH.exists():
+            raise kernels.XdnaUnavailable(
+                f"{BINDING_PATH} is not built (run __graft_entry__.build() or make -C torch-xdna_b200/csrc)")
+        loader = importlib.machinery.ExtensionFileLoader("_xdna_generate", str(BINDING_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+        loader.exec_module(module)
+        module.init(kernels.XdnaError, kernels.XdnaUnavailable)
+        _native = module
+        return getattr(module, name)
 
 
-def _call(fn, launches, *args):
-    """fn of the binding on args, accounted in stats."""
-    t0 = time.perf_counter()
-    if not kernels._state["ok"] and getattr(args[0], "is_cuda", False):
+_native = _NotLoaded()
+
+
+def _ready(x):
+    """Raises XdnaUnavailable where the kernels cannot run; CPU tensors are left to the binding, after its checks."""
+    if not kernels._state["ok"] and getattr(x, "is_cuda", False):
         kernels.require()
-    out = getattr(_native or _load(), fn)(*args)
+    return time.perf_counter()
+
+
+def _account(t0, launches=None):
     stats.calls[DEVICE] += 1
-    stats.launches += launches
+    stats.launches += _native.launches() if launches is None else launches
     stats.seconds[DEVICE] += time.perf_counter() - t0
-    return out
 
 
 def packed_attention(q, k, v, cu_seqlens, scale=None):
@@ -61,7 +67,10 @@ def packed_attention(q, k, v, cu_seqlens, scale=None):
     kernels cannot read them); cu_seqlens [N + 1] int32 on the GPU: sequence i is tokens cu_seqlens[i] ..
     cu_seqlens[i + 1] - 1. Tokens of no sequence (padding past the last one) give zeros. scale: 1 / sqrt(D) unless
     given. Returns [T, Hq, D]."""
-    return _call("packed_attention", 1 if cu_seqlens.shape[0] <= 33 else 2, q, k, v, cu_seqlens, scale)
+    t0 = _ready(q)
+    out = _native.packed_attention(q, k, v, cu_seqlens, scale)
+    _account(t0)
+    return out
 
 
 def shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale=None):
@@ -71,8 +80,10 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens,
     cache_lens[b] (int32 on the GPU, clamped to 0..S) are its own keys (bf16 or f16, D 64 or 128, Hq a multiple of
     Hkv; any strides, copied where the kernels cannot read them). Row b attends to the prefix and its own keys; with
     neither it is zero. scale: 1 / sqrt(D) unless given. Returns [B, Hq, D]."""
-    return _call("shared_prefix_attention", 1 if prefix_k.shape[0] == 0 else 2, q, prefix_k, prefix_v, k_cache, v_cache,
-                 cache_lens, scale)
+    t0 = _ready(q)
+    out = _native.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
+    _account(t0)
+    return out
 
 
 def w4_pack(w, group=128, scale_dtype=None):
@@ -80,7 +91,7 @@ def w4_pack(w, group=128, scale_dtype=None):
     rounded up to 128, w ~= (code - 8) * scale with scale = max |w| of the group / 7. group: 32, 64 or 128;
     scale_dtype: bf16 or f16, by default w's where it is one of them, else f16. The layout of the codes is described
     in include/xdna_b200.h."""
-    t0 = time.perf_counter()
+    t0 = _ready(w)
     bad = None
     if w.dim() != 2 or w.shape[1] < 1 or w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         bad = f"a [N, K] weight in f32, bf16 or f16, not {tuple(w.shape)} {w.dtype}"
@@ -101,17 +112,17 @@ def w4_pack(w, group=128, scale_dtype=None):
     scales = torch.empty((N, -(-K // group)), dtype=scale_dtype, device=w.device)
     with torch.cuda.device(w.device):
         kernels.w4_pack(w, group, codes, scales)
-    stats.calls[DEVICE] += 1
-    stats.launches += 1
-    stats.seconds[DEVICE] += time.perf_counter() - t0
+    _account(t0, 1)
     return codes, scales
 
 
 def linear_w4(x, codes, scales, group, bias=None):
     """x [..., K] times a 4-bit weight (w4_pack) transposed, plus bias [N]: [..., N] in x's type (f32, bf16 or f16),
     summed in 32 bits and rounded once. Meant for the few rows of a decode step; any number is right."""
-    y = _call("linear_w4", 1, x, codes, scales, group, bias)
-    stats.macs[DEVICE] += x.numel() * codes.shape[0]
+    t0 = _ready(x)
+    y = _native.linear_w4(x, codes, scales, group, bias)
+    stats.macs[DEVICE] += x.numel() * len(codes)
+    _account(t0)
     return y
 
 
@@ -125,4 +136,7 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=
     (taken off a generated token's logit once, and once for each time it occurs). bias: f32 [V] or [B, V], added.
     mask: int32 [B, ceil(V / 32)] or [1, ...], bit v % 32 of word v / 32 set where v is allowed; others become -inf,
     whatever stood there. Each may be None. Returns new logits in the same type."""
-    return _call("process_logits", 1, logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
+    t0 = _ready(logits)
+    out = _native.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
+    _account(t0)
+    return out

@@ -58,6 +58,7 @@ def _load():
     sig = {
         "xdna_last_error": ([], ctypes.c_char_p),
         "xdna_abi_version": ([], I),
+        "xdna_launch_count": ([], I64),
         "xdna_device_check": ([I], I),
         "xdna_take_device_error": ([P, P, P], I),
         "xdna_quant_rows_i8": ([P, I, I64, I64, I64, P, I64, P, P], I),
