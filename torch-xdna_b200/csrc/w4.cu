@@ -138,71 +138,79 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
   };
   const int n_rounds = (tile1 - tile0 + 7) / 8;
   Round p = n_rounds > 0 ? round_of(0) : Round{-1, 1, 0, 0};
-  int p_round = 0, p_b0 = 0, p_blk = p.slice * p.run, p_stage = 0;
+  int p_round = 0, p_b0 = 0, p_blk = 0, p_end = 0, p_stage = 0;  // of the run under way, blocks p_blk .. p_end - 1 are left
+  // where its next stage's codes of rows g and g + 8 lie, and the aligned 4 bytes that hold their scales: lane t copies
+  // every fourth scale of a row (a stage's scales are an even number, so they stay aligned)
   const uint8_t *p_lo = nullptr, *p_hi = nullptr;
-  int64_t p_slo = 0, p_shi = 0;  // where the rows' scales start, plus t: lane t copies every fourth scale of a row
-  bool p_inner = false;          // there are rows after these
-  auto start_tile = [&]() {
-    // rows past N repeat the last one: their results are not used
-    const int n = min(max(p.tile, 0) * 16 + g, a.N - 1), n8 = min(n + 8, a.N - 1);
-    p_lo = a.codes + n * row_bytes + t * 16;
-    p_hi = a.codes + n8 * row_bytes + t * 16;
-    p_slo = static_cast<int64_t>(n) * a.n_groups + t;
-    p_shi = static_cast<int64_t>(n8) * a.n_groups + t;
-    p_inner = n8 < a.N - 1;
-  };
-  start_tile();
-  auto prefetch = [&]() {
-    // the next stage with blocks, if there is one
-    int end = 0;
-    while (p_round < n_rounds && (p.tile < 0 || p_blk >= (end = min(a.blocks, p_b0 + min(a.chunk, (p.slice + 1) * p.run))))) {
-      p_b0 += a.chunk;
-      if (p_b0 >= a.blocks || p.tile < 0) {
-        p_b0 = 0;
-        if (++p_round < n_rounds) {
-          p = round_of(p_round);
-          start_tile();
+  const uint16_t *p_slo = nullptr, *p_shi = nullptr;
+  bool p_inner = false;  // there are rows after these
+  static_assert(kW4Blocks * kPer % 2 == 0, "a stage's scales are an even number");
+  // the next run with blocks, if there is one
+  auto next_run = [&](bool first) {
+    while (p_round < n_rounds) {
+      if (!first) {
+        p_b0 += a.chunk;
+        if (p_b0 >= a.blocks || p.tile < 0) {
+          p_b0 = 0;
+          if (++p_round < n_rounds) p = round_of(p_round);
         }
       }
+      first = false;
+      if (p_round >= n_rounds || p.tile < 0) continue;
       p_blk = p_b0 + p.slice * p.run;
-    }
-    if (p_round < n_rounds) {
-      const uint32_t dst = smem_u32(ring + p_stage * kStageBytes) + lane * 16;
-      const uint32_t dst_s = smem_u32(ring + p_stage * kStageBytes) + kW4Blocks * 1024 + lane * 4;
-      const uint8_t *lo = p_lo + p_blk * 64, *hi = p_hi + p_blk * 64;
-      // a scale is copied as the aligned 4 bytes that hold it
+      p_end = min(a.blocks, p_b0 + min(a.chunk, (p.slice + 1) * p.run));
+      if (p_blk >= p_end) continue;
+      // rows past N repeat the last one: their results are not used
+      const int n = min(p.tile * 16 + g, a.N - 1), n8 = min(n + 8, a.N - 1);
+      p_lo = a.codes + n * row_bytes + p_blk * 64 + t * 16;
+      p_hi = a.codes + n8 * row_bytes + p_blk * 64 + t * 16;
       const uint16_t* sc = static_cast<const uint16_t*>(a.scales);
-      const uint16_t *slo = sc + ((p_slo + p_blk * kPer) & ~int64_t(1)), *shi = sc + ((p_shi + p_blk * kPer) & ~int64_t(1));
-      if (p_blk + kW4Blocks <= end && (p_inner || p_blk + std::max(kW4Blocks, 4 / kPer) < a.blocks)) {
+      p_slo = sc + ((static_cast<int64_t>(n) * a.n_groups + p_blk * kPer + t) & ~int64_t(1));
+      p_shi = sc + ((static_cast<int64_t>(n8) * a.n_groups + p_blk * kPer + t) & ~int64_t(1));
+      p_inner = n8 < a.N - 1;
+      return;
+    }
+  };
+  next_run(true);
+  const uint32_t ring_lane = smem_u32(ring) + lane * 16, ring_scale = smem_u32(ring) + kW4Blocks * 1024 + lane * 4;
+  auto prefetch = [&]() {
+    if (p_round < n_rounds) {
+      const uint32_t dst = ring_lane + p_stage * kStageBytes, dst_s = ring_scale + p_stage * kStageBytes;
+      if (p_blk + kW4Blocks <= p_end && (p_inner || p_blk + std::max(kW4Blocks, 4 / kPer) < a.blocks)) {
 #pragma unroll
         for (int u = 0; u < kW4Blocks; ++u) {
-          cp_async_16(dst + u * 1024, lo + u * 64);
-          cp_async_16(dst + u * 1024 + 512, hi + u * 64);
+          cp_async_16(dst + u * 1024, p_lo + u * 64);
+          cp_async_16(dst + u * 1024 + 512, p_hi + u * 64);
         }
 #pragma unroll
         for (int j = 0; j < kWords; ++j) {
-          cp_async_4(dst_s + j * 256, slo + 4 * j, 4);
-          cp_async_4(dst_s + j * 256 + 128, shi + 4 * j, 4);
+          cp_async_4(dst_s + j * 256, p_slo + 4 * j, 4);
+          cp_async_4(dst_s + j * 256 + 128, p_shi + 4 * j, 4);
         }
       } else {
 #pragma unroll
         for (int u = 0; u < kW4Blocks; ++u) {
-          if (p_blk + u < end) {
-            cp_async_16(dst + u * 1024, lo + u * 64);
-            cp_async_16(dst + u * 1024 + 512, hi + u * 64);
+          if (p_blk + u < p_end) {
+            cp_async_16(dst + u * 1024, p_lo + u * 64);
+            cp_async_16(dst + u * 1024 + 512, p_hi + u * 64);
           }
         }
-        const uint16_t* sc_last = sc + (static_cast<int64_t>(a.N) * a.n_groups - 1);
-        const int groups = min(a.n_groups, end * kPer);
+        const uint16_t* sc_last = static_cast<const uint16_t*>(a.scales) + (static_cast<int64_t>(a.N) * a.n_groups - 1);
+        const int groups = min(a.n_groups, p_end * kPer);
 #pragma unroll
         for (int j = 0; j < kWords; ++j) {
           if (p_blk * kPer + 4 * j + t < groups) {  // the array's last scale may stand alone in its word
-            cp_async_4(dst_s + j * 256, slo + 4 * j, slo + 4 * j < sc_last ? 4 : 2);
-            cp_async_4(dst_s + j * 256 + 128, shi + 4 * j, shi + 4 * j < sc_last ? 4 : 2);
+            cp_async_4(dst_s + j * 256, p_slo + 4 * j, p_slo + 4 * j < sc_last ? 4 : 2);
+            cp_async_4(dst_s + j * 256 + 128, p_shi + 4 * j, p_shi + 4 * j < sc_last ? 4 : 2);
           }
         }
       }
       p_blk += kW4Blocks;
+      p_lo += kW4Blocks * 64;
+      p_hi += kW4Blocks * 64;
+      p_slo += kW4Blocks * kPer;
+      p_shi += kW4Blocks * kPer;
+      if (p_blk >= p_end) next_run(false);
     }
     p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -274,8 +282,8 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
       }
     }
   };
-  auto scale_of = [&](uint32_t word, uint32_t upper) {
-    const uint32_t top = __byte_perm(word, 0, upper ? 0x3244 : 0x1044);  // the scale in the upper half
+  auto scale_of = [&](uint32_t word, uint32_t selector) {
+    const uint32_t top = __byte_perm(word, 0, selector);  // the scale in the upper half
     return a.scale_dtype == XDNA_BF16 ? __uint_as_float(top) : __half2float(__ushort_as_half(static_cast<unsigned short>(top >> 16)));
   };
   auto finish = [&](int m, int n, float v) {
@@ -310,7 +318,10 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
         const uint8_t* mine = ring + stage * kStageBytes + lane * 16;
         const uint8_t* scales = ring + stage * kStageBytes + kW4Blocks * 1024 + g * 16;
         const uint8_t* xb = smx + (blk - b0) * (kW4Block * 2) + t * 16;
-        const uint32_t up_lo = odd_lo ^ (blk * kPer & 1), up_hi = odd_hi ^ (blk * kPer & 1);
+        // byte selectors that bring a word's scale to the upper half: of the scales of even and of odd lanes
+        const bool up_lo = (odd_lo ^ (blk * kPer)) & 1, up_hi = (odd_hi ^ (blk * kPer)) & 1;
+        const uint32_t sel_lo[2] = {up_lo ? 0x3244u : 0x1044u, up_lo ? 0x1044u : 0x3244u};
+        const uint32_t sel_hi[2] = {up_hi ? 0x3244u : 0x1044u, up_hi ? 0x1044u : 0x3244u};
 #pragma unroll
         for (int u = 0; u < kW4Blocks; ++u) {
           if (blk + u >= last) break;
@@ -339,8 +350,8 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
               const bool there = kPer == 1 || (blk + u) * kPer + w * 32 / GROUP < a.n_groups;
               const uint32_t s_lo = *reinterpret_cast<const uint32_t*>(scales + j * 256 + lane_t * 4);
               const uint32_t s_hi = *reinterpret_cast<const uint32_t*>(scales + j * 256 + 128 + lane_t * 4);
-              const float sl = there ? scale_of(s_lo, (up_lo ^ lane_t) & 1) : 0.f;
-              const float sh = there ? scale_of(s_hi, (up_hi ^ lane_t) & 1) : 0.f;
+              const float sl = there ? scale_of(s_lo, sel_lo[lane_t & 1]) : 0.f;
+              const float sh = there ? scale_of(s_hi, sel_hi[lane_t & 1]) : 0.f;
 #pragma unroll
               for (int i = 0; i < NT; ++i) {
                 acc[i][0] = fmaf(part[i][0], sl, acc[i][0]);
