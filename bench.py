@@ -75,7 +75,8 @@ def parse():
                          "TMA straight from peer memory, after an NCCL all-gather; or data-parallel with the sequences")
     ap.add_argument("--kernel", default=None,
                     choices=["gemm_i8", "quant_rows", "conv3x3", "conv3x3_chain", "conv_quant_codes", "attention",
-                             "gemm_bf16", "gemm_bf16_qkv"],
+                             "gemm_bf16", "gemm_bf16_qkv", "packed_attention", "shared_prefix_attention", "linear_w4",
+                             "process_logits"],
                     help="time one kernel on --shape instead of a workload (profiling)")
     ap.add_argument("--shape", default="8192,6144,1024", help="--kernel shape, comma-separated")
     return ap.parse_args()
@@ -1291,6 +1292,41 @@ def run_kernel(args):
         fn = lambda: kernels.gemm_bf16(h, w, kernels.GEMM_QKV, out=qk, vt=vt, rope_cos=cos, rope_sin=sin,  # noqa
                                        q_norm=qn, k_norm=kn, seq_len=L)
         work, unit = 2 * T * 4096 * 1024, "TFLOP/s"
+    elif args.kernel == "packed_attention":          # lengths: causal, 16 q heads / 8 kv heads of 128, bf16
+        import torch_xdna
+
+        qkv = torch.randn(sum(shp), 32, 128, device=dev, generator=g).to(torch.bfloat16)
+        cu = torch.tensor([0] + shp, device=dev).cumsum(0).to(torch.int32)
+        fn = lambda: torch_xdna.packed_attention(qkv[:, :16], qkv[:, 16:24], qkv[:, 24:], cu)  # noqa
+        work, unit = sum(2 * 2 * 16 * 128 * (n * (n + 1) // 2) for n in shp), "TFLOP/s"
+    elif args.kernel == "shared_prefix_attention":   # B, P, S: S own keys behind P shared ones, same heads
+        import torch_xdna
+
+        B, P, S = shp
+        q = torch.randn(B, 16, 128, device=dev, generator=g).to(torch.bfloat16)
+        pk, ck = (torch.randn(*n, 8, 128, device=dev, generator=g).to(torch.bfloat16) for n in ((P,), (B, S)))
+        pv, cv, lens = torch.rand_like(pk), torch.rand_like(ck), torch.full((B,), S, dtype=torch.int32, device=dev)
+        fn = lambda: torch_xdna.shared_prefix_attention(q, pk, pv, ck, cv, lens)  # noqa
+        work, unit = 2 * 2 * 8 * 128 * (P + B * S) + 2 * 2 * B * 16 * 128, "GB/s"
+    elif args.kernel == "linear_w4":                 # M, N, K: bf16 x, groups of 128
+        import torch_xdna
+
+        M, N, K = shp
+        x = torch.randn(M, K, device=dev, generator=g).to(torch.bfloat16)
+        codes, scales = torch_xdna.w4_pack((torch.randn(N, K, device=dev, generator=g) * 0.02).to(torch.bfloat16))
+        fn = lambda: torch_xdna.linear_w4(x, codes, scales, 128)  # noqa
+        work, unit = codes.numel() + 2 * scales.numel() + 2 * M * (N + K), "GB/s"
+    elif args.kernel == "process_logits":            # B, V, T: bf16, T tokens so far, a shared bias, a mask per row
+        import torch_xdna
+
+        B, V, T = shp
+        x = torch.randn(B, V, device=dev, generator=g).to(torch.bfloat16)
+        tokens = (float(V) ** torch.rand(B, T, device=dev, generator=g) - 1).to(torch.int32)
+        bias, one = torch.zeros(V, device=dev), torch.ones(B, device=dev)
+        mask = torch.full((B, -(-V // 32)), 0x55555555, dtype=torch.int32, device=dev)
+        fn = lambda: torch_xdna.process_logits(x, tokens, repetition=one, presence=one, frequency=one, bias=bias,  # noqa
+                                               mask=mask)
+        work, unit = 4 * B * V + 4 * V + 4 * mask.numel() + 4 * B * T, "GB/s"
     else:
         raise SystemExit(f"unknown kernel {args.kernel}")
     for _ in range(5):
