@@ -388,6 +388,17 @@ def test_linear_w4_large(cuda, m, n, k):
         close(torch_xdna.linear_w4(x, codes, scales, 64, bias), *w4_want(x, codes, scales, 64, bias))
 
 
+@pytest.mark.parametrize("m,n,k", [(32, 20000, 2500), (31, 21000, 2240), (33, 5000, 4300), (11, 3000, 5001)])
+def test_linear_w4_x_in_runs(cuda, m, n, k):
+    """x does not fit in shared memory: it is copied run by run, for each round of tiles again."""
+    import torch_xdna
+
+    for dtype, group in ((torch.float16, 32), (torch.bfloat16, 128), (torch.float32, 64)):
+        codes, scales = w4_inputs(n, k, group)
+        x = randn(m, k, seed=4, dtype=dtype)
+        close(torch_xdna.linear_w4(x, codes, scales, group), *w4_want(x, codes, scales, group, None))
+
+
 def test_linear_w4_strides_shapes_and_specials(cuda):
     import torch_xdna
 

@@ -63,12 +63,18 @@ struct W4Args {
 constexpr int kW4Blocks = 4;
 constexpr int kW4Stages = 2;
 constexpr int kW4Threads = 256;
+constexpr int kW4Smem = 227 * 1024;  // what a CTA may have; two on an SM lose 1 KB each of its 228
 // a warp's codes and scales: of each row four lanes' words as often as the stage's groups need
 constexpr int w4_scale_words(int group) { return (kW4Blocks * (kW4Block / group) + 3) / 4; }
 constexpr int w4_stage_bytes(int group) { return kW4Blocks * 1024 + w4_scale_words(group) * 256; }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// 16 bytes, of which the first n are read and the others are zeros.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
 // 4 bytes, of which the first n (2 or 4) are read and the others are zeros.
@@ -215,39 +221,20 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
     p_stage = p_stage + 1 == kW4Stages ? 0 : p_stage + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll
-  for (int i = 0; i < kW4Stages; ++i) prefetch();
-  int stage = 0;
-
-  auto stage_x = [&](int b0, int nb) {
-    const int cols = nb * kW4Block, k0 = b0 * kW4Block;
-    if constexpr (kParts == 1) {
+  // x of 16 bits on 16-byte boundaries is copied as the codes are, and before the first of them; else it is read value
+  // by value after they are on their way.
+  const bool copy_x = kParts == 1 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx % 8 == 0;
+  auto stage_x = [&](int b0) {
+    const int cols = min(a.blocks - b0, a.chunk) * kW4Block, k0 = b0 * kW4Block;
+    if (kParts == 1 && copy_x) {
       const uint16_t* x = static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(m0) * a.ldx + k0;
-      if ((reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx % 8 == 0) {
-        const int per = cols / 8;
-        // four pieces per thread at a time, so that their loads are under way together
-        for (int i0 = threadIdx.x; i0 < m_rows * per; i0 += 4 * kW4Threads) {
-          uint4 u[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = i0 + e * kW4Threads, r = i / per, c = (i - r * per) * 8;
-            u[e] = make_uint4(0, 0, 0, 0);
-            if (i < m_rows * per && k0 + c + 8 <= a.K) {
-              u[e] = *reinterpret_cast<const uint4*>(x + r * a.ldx + c);
-            } else if (i < m_rows * per) {
-              uint16_t* h = reinterpret_cast<uint16_t*>(&u[e]);
-              for (int k = 0; k < 8; ++k)
-                if (k0 + c + k < a.K) h[k] = x[r * a.ldx + c + k];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = i0 + e * kW4Threads, r = i / per, c = (i - r * per) * 8;
-            if (i < m_rows * per) *reinterpret_cast<uint4*>(smx + r * pitch + c * 2) = u[e];
-          }
-        }
-        return;
+      const int per = cols / 8;
+      for (int i = threadIdx.x; i < m_rows * per; i += kW4Threads) {
+        const int r = i / per, c = (i - r * per) * 8, n = min(max(a.K - k0 - c, 0), 8) * 2;  // zeros past K
+        cp_async_16(smem_u32(smx) + r * pitch + c * 2, n ? x + r * a.ldx + c : x, n);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      return;
     }
     // single values: a warp takes runs of 512 columns of a row, 16 loads per lane under way together
     const int runs = (cols + 511) / 512;
@@ -282,6 +269,14 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
       }
     }
   };
+  if (copy_x) stage_x(0);
+#pragma unroll
+  for (int i = 0; i < kW4Stages; ++i) prefetch();
+  if (!copy_x) stage_x(0);
+  asm volatile("cp.async.wait_group %0;" ::"n"(kW4Stages) : "memory");  // x, where it is copied
+  __syncthreads();
+  int stage = 0;
+
   auto scale_of = [&](uint32_t word, uint32_t selector) {
     const uint32_t top = __byte_perm(word, 0, selector);  // the scale in the upper half
     return a.scale_dtype == XDNA_BF16 ? __uint_as_float(top) : __half2float(__ushort_as_half(static_cast<unsigned short>(top >> 16)));
@@ -294,7 +289,6 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
   int x_row[NT];  // columns of a product past the last x row repeat it: their sums are not used
 #pragma unroll
   for (int i = 0; i < NT; ++i) x_row[i] = min(i * 8 + g, v_rows - 1) * pitch;
-  bool staged = false;
   for (int round = 0; round < n_rounds; ++round) {
     const Round now = round_of(round);
     float acc[NT][4];
@@ -304,11 +298,11 @@ __global__ void __launch_bounds__(kW4Threads) w4_kernel(const W4Args a) {
     const int row_lo = min(max(now.tile, 0) * 16 + g, a.N - 1);
     const uint32_t odd_lo = row_lo & a.n_groups & 1, odd_hi = min(row_lo + 8, a.N - 1) & a.n_groups & 1;
     for (int b0 = 0; b0 < a.blocks; b0 += a.chunk) {
-      if (!staged || a.chunk < a.blocks) {
-        if (staged) __syncthreads();
-        stage_x(b0, min(a.blocks, b0 + a.chunk) - b0);
+      if (a.chunk < a.blocks && (b0 > 0 || round > 0)) {
         __syncthreads();
-        staged = true;
+        stage_x(b0);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
       }
       const int first = b0 + now.slice * now.run;
       const int last = now.tile < 0 ? 0 : min(a.blocks, b0 + min(a.chunk, (now.slice + 1) * now.run));
@@ -414,7 +408,7 @@ static int launch_w4(W4Args& a, int group, dim3 grid, int smem, cudaStream_t s) 
   int dev = 0;
   XDNA_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !configured[gi][dev].load(std::memory_order_acquire)) {
-    XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4Smem));
     if (dev >= 0 && dev < 64) configured[gi][dev].store(true, std::memory_order_release);
   }
   kern<<<grid, kW4Threads, smem, s>>>(a);
@@ -425,14 +419,19 @@ template <int XT>
 static int run_w4(W4Args& a, int group, int sms, cudaStream_t s) {
   constexpr int kParts = XT == XDNA_F32 ? 3 : 1;
   // a pass takes up to 32 x rows (10 of f32); more run as further passes over the codes, which the L2 then holds
-  a.rows = std::min(a.M, 32 / kParts);
+  const int passes = (a.M + 32 / kParts - 1) / (32 / kParts);
+  a.rows = (a.M + passes - 1) / passes;
   const int v_rows = a.rows * kParts, nt = v_rows <= 8 ? 1 : v_rows <= 16 ? 2 : 4;
-  // x in shared memory, whole where it fits in 96 KB (with one or two x rows it fits for any K in use)
-  a.chunk = std::min(a.blocks, std::max(1, (96 * 1024 / v_rows - 64) / 256));
-  const int pitch = a.chunk * kW4Block * 2 + 64;
-  const int smem = 8 * kW4Stages * w4_stage_bytes(group) + (v_rows * pitch + 127) / 128 * 128 + 8 * 16 * nt * 8 * 4;
-  // two CTAs per SM, which the registers and the shared memory of most shapes allow
-  const dim3 grid(static_cast<unsigned>(std::min((a.N + 15) / 16, 2 * sms)), static_cast<unsigned>((a.M + a.rows - 1) / a.rows));
+  // x in shared memory, whole where it fits beside the ring and the sums, else in runs of blocks
+  const int others = 8 * kW4Stages * w4_stage_bytes(group) + 8 * 16 * nt * 8 * 4;
+  a.chunk = std::min(a.blocks, ((kW4Smem - others - 128) / v_rows - 64) / (kW4Block * 2));
+  const int smem = others + (v_rows * (a.chunk * kW4Block * 2 + 64) + 127) / 128 * 128;
+  // One wave: the CTAs of all passes together are as many as run at a time, two per SM where the shared memory allows it,
+  // so x is copied once per CTA and pass. (Two per SM of each pass whatever the shared memory, 20000 rows of 4096: 79 us
+  // for 32 x rows, 44 for 16, against 52 and 24; 6144 rows of 1024 and 40 x rows 24.9 against 8.1; x in shorter runs so
+  // that two CTAs always fit took 134 and 31.)
+  const int at_once = sms * (smem <= kW4Smem / 2 - 512 ? 2 : 1);
+  const dim3 grid(static_cast<unsigned>(std::min((a.N + 15) / 16, std::max(1, at_once / passes))), static_cast<unsigned>(passes));
   return nt == 1 ? launch_w4<XT, 1>(a, group, grid, smem, s)
                  : nt == 2 ? launch_w4<XT, 2>(a, group, grid, smem, s) : launch_w4<XT, 4>(a, group, grid, smem, s);
 }
