@@ -1,6 +1,6 @@
 // The generation operators' calls from Python: argument checks, output and workspace allocation and the current
 // stream, in C++, because a decode step's kernels are shorter than the same work done in Python (a call of
-// linear_w4 for one row: 4 us of host time instead of 20). Everything else is in the C ABI's entries, which these
+// linear_w4 for one row: 5 us of host time, as torch.add takes, instead of 20). Everything else is in the C ABI's entries, which these
 // call. Module torch_xdna.lib._xdna_generate; generate.py documents the arguments.
 #include <Python.h>
 

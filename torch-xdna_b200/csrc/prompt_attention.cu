@@ -22,7 +22,16 @@
 //               The running max m is raised, and O and l rescaled, only when a block exceeds it by more than 2^8.
 //               m, l, O are f32; p is rounded to the operands' type because the tensor core takes one type for both
 //               (its relative error, half an ulp, is that of the output's own rounding).
-// TMEM: S_A | S_B | O_A | O_B, 128 columns each. Shared memory: Q 2 x 128 x D, and as many 128 x D blocks as fit.
+// Warps 2 and 3 only fill the first warpgroup: registers are moved between whole warpgroups.
+// TMEM: S_A | S_B | O_A | O_B, 128 columns each. Shared memory: Q 2 x 128 x D, a ring of K and V blocks of 128 x D (4 of
+// D = 128, 8 of 64), 32 KB through which outputs leave in whole lines.
+// Measured (bf16, 16 heads over 8 of 128, one causal prompt, the causal half counted): 4096 tokens 69 us, 990 TFLOP/s;
+// 8191 tokens 230 us, 1195 TFLOP/s, 0.72 of a large matrix product's rate. What bounds it is a tile's own chain, about
+// 2000 cycles of softmax and 1100 of its products per key block, with the other tile in antiphase: the tensor pipe and
+// the unit of the exponentials are each busy half of the time, and short prompts leave SMs idle at the end. Tried on an
+// earlier state of the kernel and left out: two threads per row (298 us against 289), an MMA thread per tile (their
+// products interleave, so each chain gets longer: 336 against 298), the row's maximum overlapped with its loads (239
+// against 236).
 //
 // Keys that are masked for some rows of a tile but not for others carry p = 0; if their V holds an infinity or a NaN
 // the product is NaN. Rows that end non-finite are therefore computed again one by one over exactly their own keys
@@ -113,7 +122,9 @@ struct TileArgs {
 };
 
 constexpr int kTaThreads = 384;  // three warpgroups: issue (TMA, MMA), softmax of tile A, of tile B
-// Registers per thread after setmaxnreg: together what the launch gives, 384 x 168.
+// Registers per thread after setmaxnreg: together what the launch gives, 384 x 168. 16 prompts of up to 1900 tokens, and
+// one of 8191 with 16 heads of 64, with 56 for the issuing warps and 224 for the softmax: 125 and 248 us; 88 and 208: 111
+// and 217; 120 and 192: 109 and 216; 152 and 176: 111 and 233.
 constexpr int kTaRegsLaunch = 168, kTaRegsIssue = 120, kTaRegsSoftmax = 192;
 static_assert(128 * kTaRegsIssue + 256 * kTaRegsSoftmax <= kTaThreads * kTaRegsLaunch, "more registers than the launch has");
 constexpr int kTaBlock = 128;
@@ -777,6 +788,8 @@ constexpr int kOwnMinSteps = 8;  // of a split, two per warp
 // 64 e + 8 g + 2 i (row g of product i) and 64 e + 8 g + 2 i + 1 (row g + 8). P^T is S^T's fragment, transposed by
 // movmatrix. Every lane reads back just what it copied, so no barrier is needed.
 // Keys past the length are not read and count as zeros with score -inf.
+// 190 sequences with 150 keys on average, 16 heads over 8 of 128: 58 us for 247 MB, 4.2 TB/s, bound by the latency of the
+// copies that three CTAs per SM keep under way (the tensor pipe is busy 7 % of the time, the issue slots 25 %).
 // With one split the CTA also joins the prefix's parts and writes the output; else it leaves a part like theirs.
 template <typename T, int D>
 __global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnArgs a) {
@@ -913,7 +926,10 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnAr
     }
   }
   __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's parts (also where only the join reads them)
+  // The prefix's parts, which are joined here with one split. With more, join_kernel reads them, and one CTA that waits
+  // for the kernel that writes them is enough: this grid's end is then after its end, and the others leave their SMs.
+  if (a.splits == 1 || (blockIdx.x + 1 == gridDim.x && blockIdx.y + 1 == gridDim.y && blockIdx.z + 1 == gridDim.z))
+    asm volatile("griddepcontrol.wait;" ::: "memory");
   // four dimensions per thread
   const int64_t n_rows = static_cast<int64_t>(a.B) * a.hq;
   for (int i = threadIdx.x; i < rows * (D / 4); i += kOwnWarps * 32) {
@@ -1085,21 +1101,39 @@ static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { retur
 
 // How a prefix call is split. One sequence, and few with a short prefix, read the prefix themselves, before their own
 // keys (direct): the tile kernel and its parts take about 11 us for any prefix, the reading 0.8 us per thousand keys and
-// sequence (8 key heads of 128). Else the prefix's keys are split into about one item per SM, each at least one block.
+// sequence (8 key heads of 128).
 // A sequence's keys, where the sequences and key heads alone are few CTAs for an SM, are split into pieces of at least
 // 128 (a CTA's two steps per warp), at most 32: lengths differ, and the longest would be waited for.
+// Else the prefix's blocks are split over at most one CTA per SM. The own keys' kernel runs beside this one on the SMs
+// that it leaves, as long as its CTAs need not wait for it (where the own keys are split too, or the CTAs all fit there,
+// three to an SM). Then the number of parts is a balance: of a part's time, 10 us and 1.4 per block (2 where its items
+// have two tiles), against the work of both kernels, 8 us per part's CTA and those blocks and the own keys, half the
+// cache, at 20 KB per us and SM, spread over all SMs. Else the two follow each other. (32 sequences, prefix 4096, caches
+// of 600: 16 parts of 2 blocks 26.5 us, 8 parts 24.2, 6 parts 22.1; 64 and caches of 300: 28.9, 25.7, 24.1; 8 sequences,
+// prefix 8192, caches of 300: 16 parts of 4 blocks 18.2, 8 parts 23.2; 16 sequences, prefix 2000, caches of 64: 16 parts
+// of one block 14.0, 8 parts 12.1; 100 sequences, prefix 1000, caches of 200: 8 parts of one block 26.3, 4 parts 28.0.)
 struct PrefixSplit {
   bool direct;
   int64_t pairs, parts, blocks_per_part, own;
-  PrefixSplit(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int sms) {
+  PrefixSplit(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d, int sms) {
     direct = B == 1 || B * P <= 8192;
     const int64_t tok = 128 / (hq / hkv), blocks = direct ? 0 : (P + kTaBlock - 1) / kTaBlock;
-    pairs = (B + 2 * tok - 1) / (2 * tok);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(blocks, sms / (pairs * hkv)));
-    blocks_per_part = blocks ? (blocks + want - 1) / want : 0;
-    parts = blocks ? (blocks + blocks_per_part - 1) / blocks_per_part : 0;
     const int64_t ctas = B * hkv * ((hq / hkv + 7) / 8), keys = S + (direct ? P : 0);
     own = std::max<int64_t>(1, std::min<int64_t>({(keys + 127) / 128, 8 * sms / ctas, 32}));
+    pairs = (B + 2 * tok - 1) / (2 * tok);
+    const int64_t units = pairs * hkv;
+    const double block = B > tok ? 2.0 : 1.4, keys_work = 0.5 * B * S * hkv * d * 4 / 20e3;
+    double best = 1e30;
+    blocks_per_part = 0;
+    const int64_t most = std::max<int64_t>(1, std::min(blocks, sms / units));
+    for (int64_t per = (blocks + most - 1) / most; per >= 1 && per <= blocks && 10 + block * per < best; ++per) {
+      const int64_t c = units * ((blocks + per - 1) / per);
+      const double part = 10 + block * per;
+      const bool beside = own > 1 || ctas <= 3 * (sms - c);
+      const double time = beside ? std::max(part, (keys_work + 8.0 * c + block * units * blocks) / sms) : part + 3 + keys_work / sms;
+      if (time < best) best = time, blocks_per_part = per;
+    }
+    parts = blocks ? (blocks + blocks_per_part - 1) / blocks_per_part : 0;
   }
   int64_t all() const { return parts + (own > 1 ? own : 0); }
 };
@@ -1171,7 +1205,7 @@ size_t xdna_prefix_attention_workspace(int64_t B, int64_t P, int64_t S, int64_t 
   if (B < 1 || P < 0 || S < 0 || hkv < 1 || hq < hkv || hq / hkv > 128) return 0;
   int sms = 0;
   if (check_device(&sms) != XDNA_OK) return 0;
-  return static_cast<size_t>(PrefixSplit(B, P, S, hq, hkv, sms).all() * B * hq) * (sizeof(float2) + d * sizeof(float));
+  return static_cast<size_t>(PrefixSplit(B, P, S, hq, hkv, d, sms).all() * B * hq) * (sizeof(float2) + d * sizeof(float));
 }
 
 int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* pk, int64_t pk_st, int64_t pk_sh,
@@ -1195,7 +1229,7 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
                  "prefix_attention: workspace too small or unaligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t group = hq / hkv, tok = 128 / group;
-  const PrefixSplit split(B, P, S, hq, hkv, sms);
+  const PrefixSplit split(B, P, S, hq, hkv, d, sms);
   float* part_o = static_cast<float*>(workspace);
   float2* part_ml = reinterpret_cast<float2*>(part_o + split.all() * B * hq * d);
   if (split.parts > 0) {
