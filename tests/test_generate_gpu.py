@@ -246,6 +246,25 @@ def test_prefix_long_and_wide(cuda, b, p, s, hq, hkv, d):
     close(torch_xdna.shared_prefix_attention(*x, int32(lens)), *prefix_want(*x, lens))
 
 
+@pytest.mark.parametrize("b,p,s,hq,hkv,d", [(20, 1500, 300, 8, 4, 128), (12, 2100, 500, 14, 2, 64), (40, 333, 700, 16, 8, 128),
+                                            (9, 1025, 129, 4, 4, 64)])
+def test_prefix_beside_split_caches(cuda, b, p, s, hq, hkv, d):
+    """The prefix's kernel and the own keys' run side by side and are joined; calls in a row use the same memory."""
+    import torch_xdna
+
+    x = prefix_inputs(b, p, s, hq, hkv, d)
+    y = [x[0].flip(0).contiguous(), x[2], x[1], x[4], x[3]]
+    lens = [(i * i * 31 + 5) % (s + 1) if i % 4 else 0 for i in range(b)]
+    a, z = int32(lens), int32(lens[::-1])
+    first = torch_xdna.shared_prefix_attention(*x, a)
+    close(first, *prefix_want(*x, lens))
+    other = torch_xdna.shared_prefix_attention(*y, z)
+    close(other, *prefix_want(*y, lens[::-1]))
+    for _ in range(50):
+        got, got2 = torch_xdna.shared_prefix_attention(*x, a), torch_xdna.shared_prefix_attention(*y, z)
+        assert torch.equal(got, first) and torch.equal(got2, other)
+
+
 def test_prefix_empty_rows_and_clamped_lengths(cuda):
     import torch_xdna
 

@@ -436,7 +436,17 @@ static int run_w4(W4Args& a, int group, int sms, cudaStream_t s) {
   // for 32 x rows, 44 for 16, against 52 and 24; 6144 rows of 1024 and 40 x rows 24.9 against 8.1; x in shorter runs so
   // that two CTAs always fit took 134 and 31.)
   const int at_once = sms * (smem <= kW4Smem / 2 - 512 ? 2 : 1);
-  const dim3 grid(static_cast<unsigned>(std::min((a.N + 15) / 16, std::max(1, at_once / passes))), static_cast<unsigned>(passes));
+  // Many passes may leave SMs idle: another wave where it fills a fifth more of them (4096 rows of 1024: 2400 x rows 142
+  // us in one wave, 102 in two; 3300: 142 and 114; 1800, a quarter more: 73 and 70; but 1000, a ninth more: 39 and 44).
+  const int tiles = (a.N + 15) / 16;
+  int across = 1;
+  double best = 0;
+  for (int waves = 1; waves <= 4; ++waves) {
+    const int x = std::min(tiles, waves * at_once / passes);
+    const double filled = static_cast<double>(x) * passes / (waves * at_once);
+    if (filled > 1.2 * best) best = filled, across = std::max(1, x);
+  }
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(passes));
   return nt == 1 ? launch_w4<XT, 1>(a, group, grid, smem, s)
                  : nt == 2 ? launch_w4<XT, 2>(a, group, grid, smem, s) : launch_w4<XT, 4>(a, group, grid, smem, s);
 }
