@@ -788,7 +788,7 @@ constexpr int kOwnMinSteps = 8;  // of a split, two per warp
 // 64 e + 8 g + 2 i (row g of product i) and 64 e + 8 g + 2 i + 1 (row g + 8). P^T is S^T's fragment, transposed by
 // movmatrix. Every lane reads back just what it copied, so no barrier is needed.
 // Keys past the length are not read and count as zeros with score -inf.
-// 190 sequences with 150 keys on average, 16 heads over 8 of 128: 58 us for 247 MB, 4.2 TB/s, bound by the latency of the
+// 190 sequences of 300 keys, 16 heads over 8 of 128, alone: 58 us for 247 MB, 4.2 TB/s, bound by the latency of the
 // copies that three CTAs per SM keep under way (the tensor pipe is busy 7 % of the time, the issue slots 25 %).
 // With one split the CTA also joins the prefix's parts and writes the output; else it leaves a part like theirs.
 template <typename T, int D>
@@ -1105,13 +1105,16 @@ static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { retur
 // A sequence's keys, where the sequences and key heads alone are few CTAs for an SM, are split into pieces of at least
 // 128 (a CTA's two steps per warp), at most 32: lengths differ, and the longest would be waited for.
 // Else the prefix's blocks are split over at most one CTA per SM. The own keys' kernel runs beside this one on the SMs
-// that it leaves, as long as its CTAs need not wait for it (where the own keys are split too, or the CTAs all fit there,
-// three to an SM). Then the number of parts is a balance: of a part's time, 10 us and 1.4 per block (2 where its items
-// have two tiles), against the work of both kernels, 8 us per part's CTA and those blocks and the own keys, half the
-// cache, at 20 KB per us and SM, spread over all SMs. Else the two follow each other. (32 sequences, prefix 4096, caches
-// of 600: 16 parts of 2 blocks 26.5 us, 8 parts 24.2, 6 parts 22.1; 64 and caches of 300: 28.9, 25.7, 24.1; 8 sequences,
-// prefix 8192, caches of 300: 16 parts of 4 blocks 18.2, 8 parts 23.2; 16 sequences, prefix 2000, caches of 64: 16 parts
-// of one block 14.0, 8 parts 12.1; 100 sequences, prefix 1000, caches of 200: 8 parts of one block 26.3, 4 parts 28.0.)
+// that it leaves, as long as its CTAs need not wait for it (where the own keys are split too, or the CTAs all fit
+// there, three to an SM). Then the number of parts is a balance: of a part's time, 10 us and 1.4 per block (2 where
+// its items have two tiles), against the work of both kernels, 8 us per part's CTA and those blocks and the own keys,
+// half the cache, at 20 KB per us and SM, spread over all SMs. Else the two follow each other, or, where that is
+// shorter, caches of two pieces or more are split too, for a join's 3 us. (32 sequences, prefix 4096, caches of 600:
+// 16 parts of 2 blocks 26.5 us, 8 parts 24.2, 6 parts 22.1; 64 and caches of 300: 28.9, 25.7, 24.1; 8 sequences,
+// prefix 8192, caches of 300: 16 parts of 4 blocks 18.2, 8 parts 23.2; 16 sequences, prefix 2000, caches of 64: 16
+// parts of one block 14.0, 8 parts 12.1; 100 sequences, prefix 1000, caches of 200: 8 parts of one block 26.3, 4 parts
+// 28.0. Split caches against whole ones: 300 sequences, prefix 9000, caches of 300: 81 us against 100; 190 and 16381:
+// 69 against 73; 190 and 4096: 49 against 51.)
 struct PrefixSplit {
   bool direct;
   int64_t pairs, parts, blocks_per_part, own;
@@ -1125,13 +1128,14 @@ struct PrefixSplit {
     const double block = B > tok ? 2.0 : 1.4, keys_work = 0.5 * B * S * hkv * d * 4 / 20e3;
     double best = 1e30;
     blocks_per_part = 0;
-    const int64_t most = std::max<int64_t>(1, std::min(blocks, sms / units));
+    const int64_t most = std::max<int64_t>(1, std::min(blocks, sms / units)), whole = own;
     for (int64_t per = (blocks + most - 1) / most; per >= 1 && per <= blocks && 10 + block * per < best; ++per) {
       const int64_t c = units * ((blocks + per - 1) / per);
-      const double part = 10 + block * per;
-      const bool beside = own > 1 || ctas <= 3 * (sms - c);
-      const double time = beside ? std::max(part, (keys_work + 8.0 * c + block * units * blocks) / sms) : part + 3 + keys_work / sms;
-      if (time < best) best = time, blocks_per_part = per;
+      const double part = 10 + block * per, beside = std::max(part, (keys_work + 8.0 * c + block * units * blocks) / sms);
+      const bool fits = whole > 1 || ctas <= 3 * (sms - c);
+      const double time = fits ? beside : part + 3 + keys_work / sms;
+      if (time < best) best = time, blocks_per_part = per, own = whole;
+      if (!fits && S >= 256 && beside + 3 < best) best = beside + 3, blocks_per_part = per, own = 2;
     }
     parts = blocks ? (blocks + blocks_per_part - 1) / blocks_per_part : 0;
   }
