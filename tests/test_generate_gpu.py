@@ -247,7 +247,7 @@ def test_prefix_long_and_wide(cuda, b, p, s, hq, hkv, d):
 
 
 @pytest.mark.parametrize("b,p,s,hq,hkv,d", [(20, 1500, 300, 8, 4, 128), (12, 2100, 500, 14, 2, 64), (40, 333, 700, 16, 8, 128),
-                                            (9, 1025, 129, 4, 4, 64)])
+                                            (9, 1025, 129, 4, 4, 64), (50, 1100, 300, 14, 2, 64), (60, 513, 129, 4, 4, 64)])
 def test_prefix_beside_split_caches(cuda, b, p, s, hq, hkv, d):
     """The prefix's kernel and the own keys' run side by side and are joined; calls in a row use the same memory."""
     import torch_xdna
@@ -263,6 +263,18 @@ def test_prefix_beside_split_caches(cuda, b, p, s, hq, hkv, d):
     for _ in range(50):
         got, got2 = torch_xdna.shared_prefix_attention(*x, a), torch_xdna.shared_prefix_attention(*y, z)
         assert torch.equal(got, first) and torch.equal(got2, other)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,p,s,hq,hkv,d", [(130, 1001, 9, 3, 1, 64), (50, 1025, 1, 4, 2, 64), (65, 255, 33, 12, 4, 128),
+                                            (33, 1537, 0, 8, 1, 128), (129, 513, 270, 10, 2, 128), (3, 33000, 17, 4, 1, 64)])
+def test_prefix_through_the_tiles(cuda, dtype, b, p, s, hq, hkv, d):
+    """Prefixes too long for the sequences to read each by itself, odd ends, groups that do not divide 128."""
+    import torch_xdna
+
+    x = prefix_inputs(b, p, s, hq, hkv, d, dtype)
+    lens = [(5 * i * i + i) % (s + 1) for i in range(b)]
+    close(torch_xdna.shared_prefix_attention(*x, int32(lens)), *prefix_want(*x, lens))
 
 
 def test_prefix_empty_rows_and_clamped_lengths(cuda):

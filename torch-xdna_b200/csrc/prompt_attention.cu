@@ -1100,8 +1100,9 @@ static int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtens
 static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { return tokens / (2 * (128 / group)) + n_seqs; }
 
 // How a prefix call is split. One sequence, and few with a short prefix, read the prefix themselves, before their own
-// keys (direct): the tile kernel and its parts take about 11 us for any prefix, the reading 0.8 us per thousand keys and
-// sequence (8 key heads of 128).
+// keys (direct). With 8 key heads of 128, direct against the tile kernel: 2 sequences and a prefix of 3000 10.9 us and
+// 14.7, of 8000 22.1 and 17.1; 4 and 1000 8.7 and 9.2, and 2000 14.3 and 11.2; 8 and 500 8.7 and 10.4, and 1000 16.3 and
+// 11.3; with 2 of 64, 8 and 1000 6.3 and 8.0, 16 and 1500 8.8 and 9.5.
 // A sequence's keys, where the sequences and key heads alone are few CTAs for an SM, are split into pieces of at least
 // 128 (a CTA's two steps per warp), at most 32: lengths differ, and the longest would be waited for.
 // Else the prefix's blocks are split over at most one CTA per SM. The own keys' kernel runs beside this one on the SMs
@@ -1119,7 +1120,7 @@ struct PrefixSplit {
   bool direct;
   int64_t pairs, parts, blocks_per_part, own;
   PrefixSplit(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d, int sms) {
-    direct = B == 1 || B * P <= 8192;
+    direct = B == 1 || B * P * hkv * d <= 6 << 20;
     const int64_t tok = 128 / (hq / hkv), blocks = direct ? 0 : (P + kTaBlock - 1) / kTaBlock;
     const int64_t ctas = B * hkv * ((hq / hkv + 7) / 8), keys = S + (direct ? P : 0);
     own = std::max<int64_t>(1, std::min<int64_t>({(keys + 127) / 128, 8 * sms / ctas, 32}));
