@@ -5,7 +5,7 @@
 //            scale * q[t, h] . k[s, h / G]                                  (G = Hq / Hkv query heads per key head)
 //   prefix   o[b, h]: the same softmax over all P prefix keys and the first lens[b] keys of b's own cache
 //
-// A row with no keys at all is zero.
+// A row with no keys at all, or with scores of -inf alone, is zero.
 //
 // Both read their long axis through one tcgen05 kernel (tile_attention_kernel). The G query heads that share a key
 // head are packed into the rows of a tile: row r is token r / G, head r % G, so a tile of 128 rows holds 128 / G
@@ -179,7 +179,8 @@ __device__ __noinline__ void recompute_row(const T* q, const T* k, int64_t k_st,
     for (int i = 0; i < D / 32; ++i) z += qr[i] * to_f32(k[s * k_st + i * 32 + lane_id()]);
     for (int x = 16; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
     const float mn = fmaxf(m, z);
-    const float a = exp2f(m - mn), p = exp2f(z - mn);
+    const bool none = mn == -INFINITY;  // no key so far weighs anything
+    const float a = none ? 1.f : exp2f(m - mn), p = none ? 0.f : exp2f(z - mn);
     m = mn;
     l = l * a + p;
     if (__isnanf(l)) break;  // and NaN it stays
