@@ -55,3 +55,62 @@ def test_packed_infinite_key_at_the_start(cuda, dtype, d):
     want, tol = packed_rows(q, k, v, lens)
     assert bool(torch.isfinite(want[:40]).all()) and not want[:first, :2].any()
     close(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_non_finite_values_everywhere(cuda, dtype, d):
+    """Infinities and NaN all over V, of keys that rows see and of keys that they do not, under weights from large to
+    far below what 16 bits hold: each row is that of exactly its own keys."""
+    import torch_xdna
+
+    lens = (300, 1, 129, 260)
+    q = randn(690, 4, d, seed=1, dtype=dtype, scale=6.0)
+    k, v = randn(690, 2, d, seed=2, dtype=dtype), randn(690, 2, d, seed=3, dtype=dtype)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    kind = torch.randint(0, 3, v.shape, generator=g, device="cuda")
+    special = torch.tensor([math.inf, -math.inf, math.nan], device="cuda")[kind].to(dtype)
+    v = torch.where(torch.rand(v.shape, generator=g, device="cuda") < 0.002, special, v)
+    close(torch_xdna.packed_attention(q, k, v, cu_of(lens)), *packed_rows(q, k, v, lens))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_packed_non_finite_values_of_a_long_prompt(cuda, dtype):
+    """One NaN and two infinities in the values of a prompt of 200000 tokens: the rows that see them, the rows that only
+    share a tile with them, and all else, which keeps its bits."""
+    import torch_xdna
+
+    t, d = 200_000, 64
+    q, k, v = (randn(t, h, d, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2)))
+    k[7, 0] *= 24                                        # weights of the first infinity from large to nothing
+    clean = torch_xdna.packed_attention(q, k, v, cu_of((t,)))
+    v[7, 0, 1], v[100_003, 0, 2], v[9, 0, 3] = math.inf, -math.inf, math.nan
+    got = torch_xdna.packed_attention(q, k, v, cu_of((t,)))
+    assert torch.equal(got[:, 2:], clean[:, 2:]) and torch.equal(got[:, :2, 4:], clean[:, :2, 4:])
+    for dim, first, value in ((1, 7, math.inf), (2, 100_003, -math.inf)):
+        assert bool((got[first:, :2, dim] == value).all())
+    assert bool(torch.isnan(got[9:, :2, 3]).all())
+    rows = [0, 6, 7, 8, 9, 10, 63, 64, 127, 128, 99_999, 100_002, 100_003, 100_004, 100_095, 100_096, t - 1]
+    close(got[rows], *packed_rows(q, k, v, (t,), rows))
+
+
+def test_packed_non_finite_value_costs_little(cuda):
+    """A NaN or an infinity in the values of each head is looked into once per tile, not once per row and key."""
+    import torch_xdna
+
+    def ms(fn):
+        fn()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        fn()
+        b.record()
+        b.synchronize()
+        return a.elapsed_time(b)
+
+    for dtype in HALF:
+        q, k, v = (randn(8191, h, 128, seed=i, dtype=dtype) for i, h in enumerate((16, 8, 8)))
+        cu = cu_of((8191,))
+        clean = ms(lambda: torch_xdna.packed_attention(q, k, v, cu))
+        for value in (math.nan, math.inf):
+            v[50, :, 9] = value
+            assert ms(lambda: torch_xdna.packed_attention(q, k, v, cu)) < 20 * clean + 1.0

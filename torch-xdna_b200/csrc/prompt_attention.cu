@@ -34,8 +34,10 @@
 // against 236).
 //
 // Keys that are masked for some rows of a tile but not for others carry p = 0; if their V holds an infinity or a NaN
-// the product is NaN. Rows that end non-finite are therefore computed again one by one over exactly their own keys
-// (recompute_row), so that nothing outside a row's keys reaches it.
+// the product is NaN. So it is where a weight that a row does see is too small for 16 bits, and sums of values near the
+// end of f32 overflow. A warp that has written non-finite results therefore looks at them again once it has done all its
+// items (repair_rows), when no other role waits for it: the values of V that a row sees say which of its results
+// stand, and the others are summed again over exactly its keys, in f32.
 #include <algorithm>
 
 #include "host_util.h"
@@ -113,7 +115,7 @@ struct TileArgs {
   const PlanHeader* plan;  // null: at most 32 sequences, cu read here
   const int32_t* cu;
   int T, n_seqs;
-  const void *q, *k, *v;  // recompute_row
+  const void *q, *k, *v;  // repair_rows
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
   // PREFIX
   int B, P, pairs, splits, blocks_per_split;
@@ -129,6 +131,7 @@ constexpr int kTaRegsLaunch = 168, kTaRegsIssue = 120, kTaRegsSoftmax = 192;
 static_assert(128 * kTaRegsIssue + 256 * kTaRegsSoftmax <= kTaThreads * kTaRegsLaunch, "more registers than the launch has");
 constexpr int kTaBlock = 128;
 constexpr float kTaRescale = 8.0f;
+constexpr int kRepairRows = 8;  // rows that repair_rows sums together: the columns of a product
 
 template <int D>
 struct TaShape {
@@ -137,7 +140,7 @@ struct TaShape {
   static constexpr int kStages = D == 128 ? 4 : 8;      // K / V blocks in the ring (a fifth of 128 gained nothing)
   static constexpr int kStaging = 8 * 4096;             // a warp's 32 rows of 128 bytes on their way out
   static constexpr int kBars = 2 + 2 * kStages + 2 + 4 + 2 + 1;  // mbarriers
-  static constexpr int kSmem = (2 + kStages) * kTile + kStaging + kBars * 8 + 8 /*TMEM address, abort flag*/ + 1024 /*alignment*/;
+  static constexpr int kSmem = (2 + kStages) * kTile + kStaging + kBars * 8 + 16 /*TMEM address, abort flag, repair flags*/ + 1024 /*alignment*/;
   static_assert(kSmem <= 227 * 1024, "more shared memory than a CTA may have");
 };
 
@@ -165,28 +168,283 @@ static int launch_early(const char* what, void (*kern)(Params...), dim3 grid, in
   return check_launch(what);
 }
 
-// One row over exactly its keys [0, n), a warp with D / 32 dimensions per lane.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// N consecutive values of T as they are (N * 2 bytes, aligned to as many) and as floats.
+template <int N>
+struct Raw {
+  uint32_t w[N / 2];
+};
+template <int N>
+__device__ __forceinline__ Raw<N> load_raw(const void* p) {
+  Raw<N> x;
+  if constexpr (N == 8) {
+    const uint4 u = *static_cast<const uint4*>(p);
+    x.w[0] = u.x, x.w[1] = u.y, x.w[2] = u.z, x.w[3] = u.w;
+  } else if constexpr (N == 4) {
+    const uint2 u = *static_cast<const uint2*>(p);
+    x.w[0] = u.x, x.w[1] = u.y;
+  } else {
+    x.w[0] = *static_cast<const uint32_t*>(p);
+  }
+  return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Raw<N>& u, float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint16_t h = static_cast<uint16_t>(u.w[i / 2] >> (16 * (i & 1)));
+    x[i] = to_f32(*reinterpret_cast<const T*>(&h));
+  }
+}
+
+// Looks again at a warp's rows of an item whose results, already in dst, hold an infinity or a NaN. Per lane: its row's
+// place pos in the sequence (not falling from lane to lane), query q, result dst, and whether it has one (mine). k, v:
+// the sequence's first key and value. A lane owns D / 32 dimensions. Per dimension, the sum of the non-finite values of V that the row sees is 0, an infinity or NaN:
+//   NaN       so is the result, and it stands;
+//   infinite  the result is that infinity where it stands, and NaN where a weight was lost to 16 bits or a masked value
+//             came in: summed again. Where the row's scores are known to be sound, because another of its results is
+//             finite, the keys between the first and the last non-finite value are enough;
+//   0         the result is finite (a masked value came in, or sums overflowed) or a score is not: summed again over
+//             all keys.
+// The sums over V's non-finite values run on from row to row, so a warp reads V once for all of its rows, and up to
+// kRepairRows rows are summed again in one pass over K and V, 32 keys at a time, by running averages: with weights
+// divided by the sum of the weights so far they stay within the range of V.
+// One prompt of 8191 tokens (16 heads over 8 of 128, 235 us) with one NaN or infinity in V per head: 1.3 ms at its first
+// token, 2.7 ms in the middle, 5.7 ms at the last one, whose tile's other rows are summed again over everything. The
+// number of rows of V under way (kAhead) is what needs no spills here: with 16, and so with this called inside the loop
+// over items, the kernel's own loops lost 1 to 8 % to the registers.
 template <typename T, int D>
-__device__ __noinline__ void recompute_row(const T* q, const T* k, int64_t k_st, const T* v, int64_t v_st, int n,
-                                           float sc, T* dst) {
-  float qr[D / 32], o[D / 32], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < D / 32; ++i) {
-    qr[i] = to_f32(q[i * 32 + lane_id()]) * sc;
-    o[i] = 0.f;
+__device__ __noinline__ void repair_rows(bool mine, int pos, const T* q, T* dst, const T* k, int64_t k_st, const T* v,
+                                         int64_t v_st, float sc) {
+  constexpr bool kBf16 = !__is_same(T, __half);
+  constexpr int kV = D / 32, kC = D / 32, kAhead = 8;  // rows of V under way
+  constexpr unsigned kAll = 0xffffffffu;
+  const int d0 = lane_id() * kV;
+  auto of_lane = [](auto* p, int who) {
+    return reinterpret_cast<decltype(p)>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(p), who));
+  };
+  const unsigned there = __ballot_sync(kAll, mine);
+  unsigned again = 0;
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    const T* row = of_lane(dst, r);
+    bool odd = false;
+    if (there >> r & 1) {
+      float x[kV];
+      unpack<T>(load_raw<kV>(row + d0), x);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) odd |= !(fabsf(x[i]) < INFINITY);
+    }
+    if (__any_sync(kAll, odd)) again |= 1u << r;
   }
-  for (int s = 0; s < n; ++s) {
-    float z = 0.f;
-    for (int i = 0; i < D / 32; ++i) z += qr[i] * to_f32(k[s * k_st + i * 32 + lane_id()]);
-    for (int x = 16; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
-    const float mn = fmaxf(m, z);
-    const bool none = mn == -INFINITY;  // no key so far weighs anything
-    const float a = none ? 1.f : exp2f(m - mn), p = none ? 0.f : exp2f(z - mn);
-    m = mn;
-    l = l * a + p;
-    if (__isnanf(l)) break;  // and NaN it stays
-    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * a + p * to_f32(v[s * v_st + i * 32 + lane_id()]);
+  float seen[kV];
+  int scanned = 0, first = INT_MAX, last = -1;  // of the keys scanned, those with a non-finite value in these dimensions
+#pragma unroll
+  for (int i = 0; i < kV; ++i) seen[i] = 0.f;
+  while (again) {
+    // the next rows to sum again: their lanes and numbers of keys, and per lane the dimensions (bits)
+    int count = 0, s0 = INT_MAX, s1 = 0, n_least = INT_MAX, lane_of[kRepairRows], n_of[kRepairRows];
+    uint32_t redo[kRepairRows];
+#pragma unroll
+    for (int r = 0; r < kRepairRows; ++r) lane_of[r] = n_of[r] = 0, redo[r] = 0;
+    while (again && count < kRepairRows) {
+      const int who = __ffs(again) - 1;
+      again &= again - 1;
+      const int n = __shfl_sync(kAll, pos, who) + 1;
+      const T* row_dst = of_lane(dst, who);
+#pragma unroll 1
+      for (; scanned < n; scanned = min(scanned + kAhead, n)) {
+        Raw<kV> u[kAhead];
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) u[e] = load_raw<kV>(v + min(scanned + e, n - 1) * v_st + d0);
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          float x[kV];
+          unpack<T>(u[e], x);
+          bool odd = false;
+#pragma unroll
+          for (int i = 0; i < kV; ++i) odd |= !(fabsf(x[i]) < INFINITY);
+          if (odd && scanned + e < n) {
+#pragma unroll
+            for (int i = 0; i < kV; ++i)
+              if (!(fabsf(x[i]) < INFINITY)) seen[i] += x[i];
+            first = min(first, scanned + e);
+            last = scanned + e;
+          }
+        }
+      }
+      float x[kV];
+      unpack<T>(load_raw<kV>(row_dst + d0), x);
+      uint32_t finite = 0, infinite = 0;
+      bool sound = false;
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        if (fabsf(x[i]) < INFINITY)
+          sound = true;
+        else if (seen[i] == 0.f)
+          finite |= 1u << i;
+        else if (!__isnanf(seen[i]) && x[i] != seen[i])
+          infinite |= 1u << i;
+      }
+      if (!__any_sync(kAll, finite | infinite)) continue;
+      sound = __any_sync(kAll, sound);
+      if (__any_sync(kAll, finite) || !sound) {
+        s0 = 0;
+        s1 = max(s1, n);
+      } else {
+        s0 = min(s0, __reduce_min_sync(kAll, infinite ? first : INT_MAX));
+        s1 = max(s1, __reduce_max_sync(kAll, infinite ? last : -1) + 1);
+      }
+      n_least = min(n_least, n);
+#pragma unroll
+      for (int r = 0; r < kRepairRows; ++r)
+        if (r == count) lane_of[r] = who, n_of[r] = n, redo[r] = finite | infinite;
+      ++count;
+    }
+    if (count == 0) return;
+    // as in own_keys_kernel: the rows' queries are the columns of S^T = K Q^T, lane (g, t) holds the scores of keys g
+    // and g + 8 against rows 2 t and 2 t + 1
+    const int g = lane_id() >> 2, t = lane_id() & 3;
+    Raw<8> qf[kC];
+    int sees[2] = {0, 0};
+    {
+      int from = -1;
+#pragma unroll
+      for (int r = 0; r < kRepairRows; ++r) {
+        if (r < count && r == g) from = lane_of[r];
+        if (r == 2 * t) sees[0] = n_of[r];
+        if (r == 2 * t + 1) sees[1] = n_of[r];
+      }
+      const T* row_q = of_lane(q, max(from, 0));
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        qf[c] = load_raw<8>(row_q + 32 * c + 8 * t);
+        if (from < 0) qf[c].w[0] = qf[c].w[1] = qf[c].w[2] = qf[c].w[3] = 0;
+      }
+    }
+    float o[kRepairRows][kV], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < kRepairRows; ++r) {
+#pragma unroll
+      for (int i = 0; i < kV; ++i) o[r][i] = 0.f;
+    }
+    auto values = [&](Raw<kV>(&u)[8], int from) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] = load_raw<kV>(v + min(from + e, s1 - 1) * v_st + d0);
+    };
+#pragma unroll 1
+    for (; s0 < s1; s0 += 32) {
+      Raw<kV> u[8];
+      values(u, s0);
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        Raw<8> x[kC], y[kC];
+        const T* kx = k + min(s0 + 16 * b + g, s1 - 1) * k_st + 8 * t;
+        const T* ky = k + min(s0 + 16 * b + 8 + g, s1 - 1) * k_st + 8 * t;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) x[c] = load_raw<8>(kx + 32 * c), y[c] = load_raw<8>(ky + 32 * c);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          const uint32_t a0[4] = {x[c].w[0], y[c].w[0], x[c].w[1], y[c].w[1]};
+          const uint32_t a1[4] = {x[c].w[2], y[c].w[2], x[c].w[3], y[c].w[3]};
+          mma_16816<kBf16>(s[b], a0, qf[c].w[0], qf[c].w[1]);
+          mma_16816<kBf16>(s[b], a1, qf[c].w[2], qf[c].w[3]);
+        }
+      }
+      float keep[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // rows 2 t + h: scores of keys 16 b + 8 j + g, then weights
+        float top = m[h], sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float& z = s[x >> 1][2 * (x & 1) + h];
+          z = s0 + 8 * x + g < min(sees[h], s1) ? z * sc : -INFINITY;
+          top = fmaxf(top, z);
+        }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, x));
+        const float base = top == -INFINITY ? 0.f : top;
+        float p[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum += p[x] = exp2f(s[x >> 1][2 * (x & 1) + h] - base);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(kAll, sum, x);
+        const bool any = l[h] > 0.f;
+        const float before = l[h] * exp2f(m[h] - base);
+        m[h] = top;
+        l[h] = before + sum;
+        const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+        keep[h] = before * inv;
+        // a weight is zero for a score of -inf alone, which an infinity in V tells from one that is only small
+        if (any && keep[h] < 1.4e-45f) keep[h] = 1.4e-45f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float& z = s[x >> 1][2 * (x & 1) + h];
+          p[x] *= inv;
+          z = z > -INFINITY && p[x] < 1.4e-45f ? 1.4e-45f : p[x];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kRepairRows; ++r) {
+        const float f = __shfl_sync(kAll, keep[r & 1], r >> 1);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) o[r][i] *= f;
+      }
+#pragma unroll 1
+      for (int x = 0; x < 4; ++x) {
+        const int at = s0 + 8 * x;
+        const bool whole = at + 8 <= min(n_least, s1);
+        float w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = x < 2 ? (x ? s[0][2 + h] : s[0][h]) : (x == 3 ? s[1][2 + h] : s[1][h]);
+        Raw<kV> next[8];
+        values(next, at + 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float f[kV];
+          unpack<T>(u[e], f);
+#pragma unroll
+          for (int r = 0; r < kRepairRows; ++r) {
+            const float p = __shfl_sync(kAll, w[r & 1], 4 * e + (r >> 1));
+            if (whole || at + e < min(n_of[r], s1)) {  // a key that the row does not see may hold anything
+#pragma unroll
+              for (int i = 0; i < kV; ++i) o[r][i] = fmaf(p, f[i], o[r][i]);
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = next[e];
+      }
+      bool open = false;  // what is NaN stays NaN
+#pragma unroll
+      for (int r = 0; r < kRepairRows; ++r) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) open |= (redo[r] >> i & 1) && !__isnanf(o[r][i]);
+      }
+      if (!__any_sync(kAll, open)) break;
+    }
+#pragma unroll
+    for (int r = 0; r < kRepairRows; ++r) {
+      T* row_dst = of_lane(dst, lane_of[r]);
+#pragma unroll
+      for (int i = 0; i < kV; ++i)
+        if (redo[r] >> i & 1) row_dst[d0 + i] = from_f32<T>(o[r][i]);
+    }
   }
-  for (int i = 0; i < D / 32; ++i) dst[i * 32 + lane_id()] = from_f32<T>(l == 0.f ? 0.f : o[i] / l);
 }
 
 template <typename T, int D, int MODE>
@@ -215,6 +473,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* repair = reinterpret_cast<uint8_t*>(tmem_slot + 2);  // [softmax warp] has written non-finite results
 
   if constexpr (MODE == PREFIX) asm volatile("griddepcontrol.launch_dependents;");
   const int warp = warp_id(), lane = lane_id();
@@ -235,6 +494,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
+    for (int w = 0; w < 8; ++w) repair[w] = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -280,12 +540,16 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       seq_len = end - seq_start;
       one_end = __shfl_sync(0xffffffffu, end, 31);
       n_items = __reduce_add_sync(0xffffffffu, (seq_len + per_pair - 1) / per_pair) * args.hkv;
-      level = __reduce_max_sync(0xffffffffu, (seq_len + kTaBlock - 1) / kTaBlock);
-      level_count = __reduce_add_sync(0xffffffffu, pairs_upto(level) - pairs_upto(level - 1));
     }
   } else {
     n_items = args.pairs * args.hkv * args.splits;
   }
+  auto first_level = [&]() {
+    level = __reduce_max_sync(0xffffffffu, (seq_len + kTaBlock - 1) / kTaBlock);
+    level_base = 0;
+    level_count = __reduce_add_sync(0xffffffffu, pairs_upto(level) - pairs_upto(level - 1));
+  };
+  if (MODE == PACKED && !args.plan) first_level();
   auto item = [&](int n, TileItem& it) -> bool {
     const int idx = n * G + ((n & 1) ? G - 1 - cta : cta);
     if (idx >= n_items) return false;
@@ -596,7 +860,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       };
       uint32_t o[32];
       if constexpr (MODE == PACKED) {
-        const float inv = 1.f / l;
+        const float inv = l > 0.f || __isnanf(l) ? 1.f / l : 0.f;
         float bad = 0.f;  // stays 0 over finite values
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
@@ -618,18 +882,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
           flush(static_cast<uint8_t*>(args.out) + c * 128, D * 2);
         }
-        unsigned again = __ballot_sync(0xffffffffu, mine && !(bad == 0.f));
-        while (again) {
-          const int who = __ffs(again) - 1;
-          again &= again - 1;
-          const int w_tok = __shfl_sync(0xffffffffu, tok, who), w_head = __shfl_sync(0xffffffffu, head, who);
-          const int64_t first = it.kv_tok;
-          recompute_row<T, D>(static_cast<const T*>(args.q) + w_tok * args.q_st + w_head * args.q_sh,
-                              static_cast<const T*>(args.k) + first * args.k_st + it.kvh * args.k_sh, args.k_st,
-                              static_cast<const T*>(args.v) + first * args.v_st + it.kvh * args.v_sh, args.v_st,
-                              w_tok - it.kv_tok + 1, sc,
-                              static_cast<T*>(args.out) + (static_cast<int64_t>(w_tok) * args.hq + w_head) * D);
-        }
+        if (mine && !(bad == 0.f)) repair[warp - 4] = 1;
       } else {
         const int64_t part = static_cast<int64_t>(it.split) * args.B * args.hq;
 #pragma unroll 1
@@ -645,6 +898,22 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       }
       // O has been read: the next item's first product (issued after this warp's next P) may overwrite it
       tc_fence_before();
+    }
+    if constexpr (MODE == PACKED) {
+      __syncwarp();
+      if (ok && repair[warp - 4]) {
+        if (!args.plan) first_level();
+        for (int n = 0; item(n, it); ++n) {
+          if (it.nb[t] == 0) continue;
+          const int pos = it.q_pos + t * args.tok + r_tok;
+          const bool mine = r_ok && pos < it.len;
+          const int64_t first = it.kv_tok, tok = mine ? it.q_tok + t * args.tok + r_tok : first, head = it.kvh * args.group + r_head;
+          repair_rows<T, D>(mine, pos, static_cast<const T*>(args.q) + tok * args.q_st + head * args.q_sh,
+                            static_cast<T*>(args.out) + (tok * args.hq + head) * D,
+                            static_cast<const T*>(args.k) + first * args.k_st + it.kvh * args.k_sh, args.k_st,
+                            static_cast<const T*>(args.v) + first * args.v_st + it.kvh * args.v_sh, args.v_st, sc);
+        }
+      }
     }
   }
   __syncthreads();
@@ -754,20 +1023,6 @@ struct OwnArgs {
   float2* part_ml;
   void* out;
 };
-
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
