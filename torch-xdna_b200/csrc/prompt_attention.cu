@@ -802,7 +802,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             uint32_t o[16];
             __syncwarp();
             tmem_ld_32x32b_x16(tO + c * 16, o);
-            tmem_ld_wait();
+            tmem_ld_wait(o);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
             tmem_st_32x32b_x16(tO + c * 16, o);
