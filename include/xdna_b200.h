@@ -387,7 +387,9 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
  * scales [N, ceil(K / group)] (bf16 or f16; group 32, 64 or 128): w = (code - 8) * scale. A block of 128 columns is
  * 16 little-endian 32-bit words; the word at place 4 t + w holds columns 32 w + 8 t .. + 7, in the order
  * 0, 2, 4, 6, 1, 3, 5, 7 from the lowest four bits. xdna_w4_pack quantises w (f32 / bf16 / f16, row pitch ldw):
- * scale = max |w| of the group / 7, code = clamp(rint(w / scale), -8, 7) + 8. */
+ * scale = max |w| of the group / 7, code = clamp(rint(w / scale), -8, 7) + 8. A group with a NaN or an infinity has the
+ * scale NaN, so it shows in the results; f16 scales hold groups of max |w| from 2e-7 (below: zeros) to 4.5e5 (above: an
+ * infinite scale, whose results are NaN). */
 int xdna_w4_pack(const void* w, int w_dtype, int64_t N, int64_t K, int64_t ldw, int group, uint8_t* codes,
                  void* scales, int scale_dtype, void* stream);
 

@@ -5,7 +5,7 @@ import math
 
 import pytest
 import torch
-from test_generate_gpu import U, _clean, close, cu_of, randn  # noqa: F401 (_clean: autouse)
+from test_generate_gpu import U, _clean, close, cu_of, randn, unpack, w4_inputs, w4_want  # noqa: F401 (_clean: autouse)
 
 pytestmark = pytest.mark.gpu
 HALF = [torch.bfloat16, torch.float16]
@@ -114,3 +114,38 @@ def test_packed_non_finite_value_costs_little(cuda):
         for value in (math.nan, math.inf):
             v[50, :, 9] = value
             assert ms(lambda: torch_xdna.packed_attention(q, k, v, cu)) < 20 * clean + 1.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_pack_shows_non_finite_weights(cuda, dtype, group):
+    """A group with a NaN or an infinity among its weights has a scale of NaN and codes of zero, and so its row's results
+    are NaN; every other group is what it is without."""
+    import torch_xdna
+
+    n, k = 6, 300
+    w = randn(n, k, seed=1, dtype=dtype, scale=0.05)
+    clean_codes, clean_scales = torch_xdna.w4_pack(w, group)
+    for row, col, value in ((0, 5, math.nan), (1, 200, math.inf), (2, 299, -math.inf), (3, 0, math.nan), (3, 1, math.inf)):
+        w[row, col] = value
+    codes, scales = torch_xdna.w4_pack(w, group)
+    bad = torch.zeros(n, -(-k // group), dtype=torch.bool, device="cuda")
+    bad[[0, 1, 2, 3], [5 // group, 200 // group, 299 // group, 0]] = True
+    assert torch.equal(torch.isnan(scales), bad) and torch.equal(scales[~bad], clean_scales[~bad])
+    hit = bad.repeat_interleave(group, 1)[:, :k].cpu()
+    assert torch.equal(unpack(codes, k), torch.where(hit, 8, unpack(clean_codes, k)))
+    x = randn(3, k, seed=2, dtype=dtype)
+    y, clean = torch_xdna.linear_w4(x, codes, scales, group), torch_xdna.linear_w4(x, clean_codes, clean_scales, group)
+    assert bool(torch.isnan(y[:, :4]).all()) and torch.equal(y[:, 4:], clean[:, 4:])
+
+
+def test_w4_pack_past_the_range_of_f16_scales(cuda):
+    """f32 weights that an f16 scale cannot hold: too large ones show in the result, bf16 scales hold them."""
+    import torch_xdna
+
+    w = randn(4, 128, seed=1, dtype=torch.float32)
+    w[1] *= 1e6
+    x = randn(2, 128, seed=2, dtype=torch.float32)
+    y = torch_xdna.linear_w4(x, *torch_xdna.w4_pack(w, 64), 64)
+    assert not bool(torch.isfinite(y[:, 1]).any()) and bool(torch.isfinite(y[:, [0, 2, 3]]).all())
+    assert bool(torch.isfinite(torch_xdna.linear_w4(x, *torch_xdna.w4_pack(w, 64, torch.bfloat16), 64)).all())

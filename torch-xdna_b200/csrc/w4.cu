@@ -451,7 +451,8 @@ static int run_w4(W4Args& a, int group, int sms, cudaStream_t s) {
                  : nt == 2 ? launch_w4<XT, 2>(a, group, grid, smem, s) : launch_w4<XT, 4>(a, group, grid, smem, s);
 }
 
-// s = max |w| / 7 over the group, rounded to the scales' type; code = clamp(rint(w / s), -8, 7) + 8, 8 where s is 0.
+// s = max |w| / 7 over the group, rounded to the scales' type, NaN where a weight of it is not finite, which then shows
+// in the results; code = clamp(rint(w / s), -8, 7) + 8, 8 where s is 0 or NaN.
 // One warp per block of 128 columns: lane l takes columns 4 l .. 4 l + 3, so a group is group / 4 lanes.
 __global__ void __launch_bounds__(256) w4_pack_kernel(const void* w, int dt, int64_t N, int64_t K, int64_t ldw,
                                                       int group, uint8_t* codes, int64_t row_bytes, void* scales,
@@ -461,12 +462,17 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const void* w, int dt, int
   if (i >= N * blocks) return;
   const int64_t n = i / blocks, col = (i % blocks) * kW4Block + 4 * lane_id();
   float x[4], top = 0.f;
+  int odd = 0;
   for (int c = 0; c < 4; ++c) {
     x[c] = col + c < K ? load_f32(w, dt, n * ldw + col + c) : 0.f;
     top = fmaxf(top, fabsf(x[c]));
+    odd |= !(fabsf(x[c]) < INFINITY);
   }
-  for (int o = group / 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float s = top / 7.f;
+  for (int o = group / 8; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    odd |= __shfl_xor_sync(0xffffffffu, odd, o);
+  }
+  float s = odd ? NAN : top / 7.f;
   s = sdt == XDNA_BF16 ? __bfloat162float(__float2bfloat16_rn(s)) : __half2float(__float2half_rn(s));
   const int64_t g = col / group;
   if (lane_id() % (group / 4) == 0 && g < n_groups) store_f32(scales, sdt, n * n_groups + g, s);

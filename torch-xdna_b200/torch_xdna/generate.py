@@ -89,8 +89,8 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens,
 def w4_pack(w, group=128, scale_dtype=None):
     """A weight [N, K] (f32, bf16 or f16) in 4 bits: (codes uint8 [N, K' / 2], scales [N, ceil(K / group)]), K' = K
     rounded up to 128, w ~= (code - 8) * scale with scale = max |w| of the group / 7. group: 32, 64 or 128;
-    scale_dtype: bf16 or f16, by default w's where it is one of them, else f16. The layout of the codes is described
-    in include/xdna_b200.h."""
+    scale_dtype: bf16 or f16, by default w's where it is one of them, else f16 (groups of max |w| from 2e-7 to 4.5e5). A
+    group that is not finite has the scale NaN. The layout of the codes is described in include/xdna_b200.h."""
     t0 = _ready(w)
     bad = None
     if w.dim() != 2 or w.shape[1] < 1 or w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
