@@ -149,3 +149,13 @@ def test_w4_pack_past_the_range_of_f16_scales(cuda):
     y = torch_xdna.linear_w4(x, *torch_xdna.w4_pack(w, 64), 64)
     assert not bool(torch.isfinite(y[:, 1]).any()) and bool(torch.isfinite(y[:, [0, 2, 3]]).all())
     assert bool(torch.isfinite(torch_xdna.linear_w4(x, *torch_xdna.w4_pack(w, 64, torch.bfloat16), 64)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(65_536, 40, 130), (70_001, 17, 64), (2 ** 19 + 5, 5, 33)])
+def test_linear_w4_of_very_many_rows(cuda, dtype, m, n, k):
+    import torch_xdna
+
+    codes, scales = w4_inputs(n, k, 32, torch.float16 if dtype == torch.float16 else torch.bfloat16)
+    x, bias = randn(m, k, seed=2, dtype=dtype), randn(n, seed=3, dtype=torch.float32)
+    close(torch_xdna.linear_w4(x, codes, scales, 32, bias), *w4_want(x, codes, scales, 32, bias))

@@ -523,7 +523,7 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
                    void* y, int64_t ldy, void* stream) {
   int rc = check_w4("linear_w4", N, K, group, scale_dtype);
   if (rc != XDNA_OK) return rc;
-  XDNA_CHECK_ARG(M >= 0 && M < 65536 && ldx >= K && ldy >= N && is_float_dtype(x_dtype), "linear_w4: bad x or y");
+  XDNA_CHECK_ARG(M >= 0 && ldx >= K && ldy >= N && is_float_dtype(x_dtype), "linear_w4: bad x or y");
   XDNA_CHECK_ARG(bias == nullptr || is_float_dtype(bias_dtype), "linear_w4: bad bias type");
   int sms = 0;
   if ((rc = check_device(&sms)) != XDNA_OK) return rc;
@@ -531,14 +531,11 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
   XDNA_CHECK_ARG(x && codes && scales && y && aligned16(codes) && reinterpret_cast<uintptr_t>(scales) % 4 == 0,
                  "linear_w4: null pointer or unaligned codes or scales");
   W4Args a{};
-  a.x = x;
   a.ldx = ldx;
   a.codes = codes;
   a.scales = scales;
   a.bias = bias;
-  a.y = y;
   a.ldy = ldy;
-  a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
   a.blocks = static_cast<int>((K + kW4Block - 1) / kW4Block);
@@ -547,8 +544,15 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
   a.scale_dtype = scale_dtype;
   a.bias_dtype = bias_dtype;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return x_dtype == XDNA_F32 ? run_w4<XDNA_F32>(a, group, sms, s)
+  constexpr int64_t kRows = 1 << 19;  // of a launch: 52429 passes of f32, and a grid may have 65535
+  for (int64_t m = 0; m < M && rc == XDNA_OK; m += kRows) {
+    a.x = static_cast<const uint8_t*>(x) + m * ldx * dtype_size(x_dtype);
+    a.y = static_cast<uint8_t*>(y) + m * ldy * dtype_size(x_dtype);
+    a.M = static_cast<int>(std::min(kRows, M - m));
+    rc = x_dtype == XDNA_F32 ? run_w4<XDNA_F32>(a, group, sms, s)
                              : x_dtype == XDNA_BF16 ? run_w4<XDNA_BF16>(a, group, sms, s) : run_w4<XDNA_F16>(a, group, sms, s);
+  }
+  return rc;
 }
 
 }  // extern "C"
