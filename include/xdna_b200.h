@@ -366,7 +366,7 @@ int xdna_qwen3_stack(const xdna_qwen3_layer* layers, int n_layers, const float* 
  * cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (n_seqs + 1 ascending device words); a token attends to the tokens of its
  * sequence up to itself. Words outside [0, tokens] or out of order are clamped; tokens of no sequence give zeros,
  * and so do rows of which every score is -inf.
- * scale > 0. workspace: xdna_packed_attention_workspace bytes, 256-byte aligned. */
+ * 0 < scale <= 2.3e38. workspace: xdna_packed_attention_workspace bytes, 256-byte aligned. */
 size_t xdna_packed_attention_workspace(int64_t n_seqs, int64_t tokens, int64_t hq, int64_t hkv);
 int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                           const void* v, int64_t v_st, int64_t v_sh, const int32_t* cu_seqlens, int64_t n_seqs,

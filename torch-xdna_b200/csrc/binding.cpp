@@ -113,7 +113,7 @@ double scale_of(const char* name, const at::Tensor& q, const at::Tensor& kv, PyO
   if (scale == Py_None) return d == 64 ? 0.125 : 0.08838834764831845;
   const double s = PyFloat_AsDouble(scale);
   if (PyErr_Occurred()) throw Raised{};
-  REQUIRE(s > 0 && s <= 3.0e38, XDNA_ERR_INVALID, "scale " << s << " is not positive and finite");
+  REQUIRE(s > 0 && s <= 2.3e38, XDNA_ERR_INVALID, "scale " << s << " is not positive and at most 2.3e38");
   return s;
 }
 

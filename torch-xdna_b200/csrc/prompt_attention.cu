@@ -123,6 +123,7 @@ struct TileArgs {
   float2* part_ml; // [split][B * hq]: m (log2 units), l
 };
 
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kTaThreads = 384;  // three warpgroups: issue (TMA, MMA), softmax of tile A, of tile B
 // Registers per thread after setmaxnreg: together what the launch gives, 384 x 168. 16 prompts of up to 1900 tokens, and
 // one of 8191 with 16 heads of 64, with 56 for the issuing warps and 224 for the softmax: 125 and 248 us; 88 and 208: 111
@@ -1294,7 +1295,7 @@ static int check_heads(const char* what, int64_t hq, int64_t hkv, int64_t d, int
   XDNA_CHECK_ARG(hq >= 1 && hkv >= 1 && hq % hkv == 0 && hq / hkv <= 128,
                  "%s: %lld query heads over %lld key heads", what, (long long)hq, (long long)hkv);
   XDNA_CHECK_ARG(dtype == XDNA_BF16 || dtype == XDNA_F16, "%s: bf16 or f16", what);
-  XDNA_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", what);
+  XDNA_CHECK_ARG(scale > 0.f && scale * kLog2E < INFINITY, "%s: the scale must be positive and at most 2.3e38", what);
   if (d != 64 && d != 128) return fail(XDNA_ERR_UNSUPPORTED, "%s: head dimension %lld (64 or 128)", what, (long long)d);
   return XDNA_OK;
 }
@@ -1435,7 +1436,7 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
   a.hkv = static_cast<int>(hkv);
   a.group = static_cast<int>(group);
   a.tok = static_cast<int>(tok);
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2E;
   a.err = device_error_word();
   a.out = out;
   a.cu = cu_seqlens;
@@ -1499,7 +1500,7 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
     a.hkv = static_cast<int>(hkv);
     a.group = static_cast<int>(group);
     a.tok = static_cast<int>(tok);
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale * kLog2E;
     a.err = device_error_word();
     a.B = static_cast<int>(B);
     a.P = static_cast<int>(P);
@@ -1534,7 +1535,7 @@ int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void*
   o.group = static_cast<int>(group);
   o.parts = static_cast<int>(split.parts);
   o.splits = static_cast<int>(split.own);
-  o.scale_log2 = scale * 1.4426950408889634f;
+  o.scale_log2 = scale * kLog2E;
   o.part_o = part_o;
   o.part_ml = part_ml;
   o.out = out;
