@@ -19,3 +19,62 @@ def test_scales_whose_products_overflow_are_refused():
     entry = kernels.lib().xdna_packed_attention
     assert entry(None, 8, 8, None, 8, 8, None, 8, 8, None, 1, 5, 4, 2, 64, kernels.BF16, 2.4e38, None, None, 0, None) == -1
     assert b"scale" in kernels.lib().xdna_last_error()
+
+
+class _Fake:
+    """The binding's calls, answered with zeros of the right shape and without history, as it does."""
+
+    def launches(self):
+        return 1
+
+    def packed_attention(self, q, k, v, cu, scale):
+        return torch.zeros(q.shape, dtype=q.dtype)
+
+    def shared_prefix_attention(self, q, *rest):
+        return torch.zeros(q.shape, dtype=q.dtype)
+
+    def linear_w4(self, x, codes, scales, group, bias):
+        return torch.zeros(*x.shape[:-1], len(codes), dtype=x.dtype)
+
+    def process_logits(self, logits, *rest):
+        return torch.zeros(logits.shape, dtype=logits.dtype)
+
+
+def _calls():
+    def f(*shape):
+        return torch.zeros(*shape, dtype=torch.bfloat16, requires_grad=True)
+
+    n = torch.zeros(5, dtype=torch.int32)
+    codes = torch.zeros(9, 128, dtype=torch.uint8)
+    one = torch.zeros(3, requires_grad=True)
+    tokens = torch.zeros(3, 2, dtype=torch.int32)
+    plain = torch.zeros(3, 100)
+    q, c = torch.zeros(5, 4, 64).bfloat16(), torch.zeros(5, 3, 2, 64).bfloat16()
+    return [lambda ns: ns.packed_attention(f(5, 4, 64), f(5, 2, 64), f(5, 2, 64), n),
+            lambda ns: ns.packed_attention(q, q, f(5, 4, 64), n),
+            lambda ns: ns.shared_prefix_attention(f(5, 4, 64), f(7, 2, 64), f(7, 2, 64), c, c, n),
+            lambda ns: ns.shared_prefix_attention(q, f(7, 2, 64), f(7, 2, 64), f(5, 3, 2, 64), c, n),
+            lambda ns: ns.linear_w4(f(2, 200), codes, torch.zeros(9, 4).bfloat16(), 64),
+            lambda ns: ns.linear_w4(torch.zeros(2, 200), codes, f(9, 4), 64),
+            lambda ns: ns.linear_w4(torch.zeros(2, 200), codes, torch.zeros(9, 4).bfloat16(), 64, f(9)),
+            lambda ns: ns.process_logits(f(3, 100)),
+            lambda ns: ns.process_logits(plain, tokens, repetition=one),
+            lambda ns: ns.process_logits(plain, bias=torch.zeros(100, requires_grad=True))]
+
+
+def test_gradients_do_not_vanish_in_silence(monkeypatch):
+    """The operators have no backward pass. Where an input requires grad, the direct call's result does too and says so
+    in backward, as the custom op's; without grad mode both are as ever."""
+    from torch_xdna import generate
+
+    monkeypatch.setattr(generate, "_native", _Fake())
+    for call in _calls():
+        for ns in (torch_xdna, torch.ops.xdna):
+            y = call(ns)
+            assert y.requires_grad
+            with pytest.raises(RuntimeError, match="autograd"):
+                y.sum().backward()
+            with torch.no_grad():
+                assert not call(ns).requires_grad
+            with torch.inference_mode():
+                call(ns)

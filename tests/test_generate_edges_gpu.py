@@ -159,3 +159,23 @@ def test_linear_w4_of_very_many_rows(cuda, dtype, m, n, k):
     codes, scales = w4_inputs(n, k, 32, torch.float16 if dtype == torch.float16 else torch.bfloat16)
     x, bias = randn(m, k, seed=2, dtype=dtype), randn(n, seed=3, dtype=torch.float32)
     close(torch_xdna.linear_w4(x, codes, scales, 32, bias), *w4_want(x, codes, scales, 32, bias))
+
+
+def test_inputs_that_require_grad(cuda):
+    """The values are those without grad mode; backward raises."""
+    import torch_xdna
+
+    q, k, v = (randn(70, h, 64, seed=i) for i, h in enumerate((4, 2, 2)))
+    codes, scales = w4_inputs(33, 200, 64)
+    x, logits = randn(3, 200, seed=4), randn(3, 500, seed=5)
+    calls = [(q, lambda y: torch_xdna.packed_attention(y, k, v, cu_of((30, 40)))),
+             (q, lambda y: torch_xdna.shared_prefix_attention(y, k, v, k[:, None], v[:, None], cu_of([0] * 70)[:70])),
+             (x, lambda y: torch_xdna.linear_w4(y, codes, scales, 64)),
+             (logits, torch_xdna.process_logits)]
+    for value, call in calls:
+        want = call(value)
+        with torch.enable_grad():
+            got = call(value.clone().requires_grad_())
+            assert got.requires_grad and torch.equal(got, want)
+            with pytest.raises(RuntimeError, match="autograd"):
+                got.float().sum().backward()
