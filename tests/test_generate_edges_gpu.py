@@ -179,3 +179,37 @@ def test_inputs_that_require_grad(cuda):
             assert got.requires_grad and torch.equal(got, want)
             with pytest.raises(RuntimeError, match="autograd"):
                 got.float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d", [64, 128])
+def test_results_at_the_end_of_the_type(cuda, dtype, d):
+    """All values are the type's largest, and all weights but one round up: a mean of equal values is that value, to the
+    tolerance of two roundings, and not infinite."""
+    import torch_xdna
+
+    top = torch.finfo(dtype).max
+    size = top if dtype == torch.float16 else 2.0 ** 100   # bf16: sums over the keys have to stay within f32
+    x = torch.arange(0.25, 3.0, 2.0 ** -7, device="cuda").to(dtype).double()
+    p = torch.exp(-x)
+    x = float(x[((p.to(dtype).double() - p) / p).argmax()])
+    n, s = 600, 40
+    q = torch.zeros(n, 2, d, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(n, 1, d, dtype=dtype, device="cuda")
+    k[1:, 0, 0] = -x
+    v = torch.full_like(k, size)
+
+    def right(y, value=size):
+        return bool(torch.isfinite(y).all()) and bool(((y.double() - value).abs() <= 2 * U[dtype] * value).all())
+
+    assert right(torch_xdna.packed_attention(q, k, v, cu_of((n,)), 1.0))
+    if dtype == torch.bfloat16:                            # here the sums are summed again where they do not
+        assert right(torch_xdna.packed_attention(q, k, torch.full_like(k, top), cu_of((n,)), 1.0), top)
+    for b in (1, 3, 190):
+        ck, cv = k[1:s + 1].expand(b, s, 1, d).contiguous(), v[:s].expand(b, s, 1, d).contiguous()
+        lens = torch.full((b,), s, dtype=torch.int32, device="cuda")
+        wide = q[:1].expand(b, 2, d).contiguous()
+        for pk in (k, k[:0], torch.cat([k] * 12)):
+            assert right(torch_xdna.shared_prefix_attention(wide, pk, torch.full_like(pk, size), ck, cv, lens, 1.0))
+

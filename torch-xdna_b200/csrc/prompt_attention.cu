@@ -70,6 +70,27 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The larger magnitude of each of two 16-bit values, NaN where one is.
+template <typename T>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  if constexpr (__is_same(T, __half)) {
+    const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __nv_bfloat162 r =
+        __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+// x, or where it is finite the nearest value within T's range: a mean of values of T lies within it, and only the
+// roundings of the weights take it out.
+template <typename T>
+__device__ __forceinline__ float fit(float x) {
+  constexpr float kMax = __is_same(T, __half) ? 65504.f : 3.38953139e38f;
+  return fabsf(x) < INFINITY ? fminf(fmaxf(x, -kMax), kMax) : x;
+}
+
 // 2^x of two values on the FMA pipe, to relieve the MUFU unit, whose rate (16 a clock and SM) is as tight here as the
 // tensor core's: x = n + f with n whole and |f| <= 1/2, by adding and taking off 1.5 * 2^23; 2^f by the polynomial
 // 1 + c1 f + ... of least largest relative error on [-1/2, 1/2] (a linear program over 4001 points): 1.0e-4 of degree
@@ -218,8 +239,8 @@ __device__ __forceinline__ void unpack(const Raw<N>& u, float (&x)[N]) {
 //   infinite  the result is that infinity where it stands, and NaN where a weight was lost to 16 bits or a masked value
 //             came in: summed again. Where the row's scores are known to be sound, because another of its results is
 //             finite, the keys between the first and the last non-finite value are enough;
-//   0         the result is finite (a masked value came in, or sums overflowed) or a score is not: summed again over
-//             all keys.
+//   0         the result is finite (a masked value came in, sums overflowed, or it was rounded past the type's end) or
+//             a score is not: summed again over all keys.
 // The sums over V's non-finite values run on from row to row, so a warp reads V once for all of its rows, and up to
 // kRepairRows rows are summed again in one pass over K and V, 32 keys at a time, by running averages: with weights
 // divided by the sum of the weights so far they stay within the range of V.
@@ -443,7 +464,7 @@ __device__ __noinline__ void repair_rows(bool mine, int pos, const T* q, T* dst,
       T* row_dst = of_lane(dst, lane_of[r]);
 #pragma unroll
       for (int i = 0; i < kV; ++i)
-        if (redo[r] >> i & 1) row_dst[d0 + i] = from_f32<T>(o[r][i]);
+        if (redo[r] >> i & 1) row_dst[d0 + i] = from_f32<T>(fit<T>(o[r][i]));
     }
   }
 }
@@ -862,7 +883,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       uint32_t o[32];
       if constexpr (MODE == PACKED) {
         const float inv = l > 0.f || __isnanf(l) ? 1.f / l : 0.f;
-        float bad = 0.f;  // stays 0 over finite values
+        uint32_t most = 0;  // the largest magnitude written, of even and of odd dimensions
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
 #pragma unroll
@@ -874,16 +895,19 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             for (int e = 0; e < 32; e += 8) {
               float x[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                x[i] = __uint_as_float(o[e + i]) * inv;
-                bad = fmaf(x[i], 0.f, bad);
-              }
-              put(h * 4 + e / 8, make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])));
+              for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(o[e + i]) * inv;
+              const uint4 u = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+              most = max_abs2<T>(max_abs2<T>(max_abs2<T>(max_abs2<T>(most, u.x), u.y), u.z), u.w);
+              put(h * 4 + e / 8, u);
             }
           }
           flush(static_cast<uint8_t*>(args.out) + c * 128, D * 2);
         }
-        if (mine && !(bad == 0.f)) repair[warp - 4] = 1;
+        Raw<2> w;
+        float ends[2];
+        w.w[0] = most;
+        unpack<T>(w, ends);
+        if (mine && !(ends[0] < INFINITY && ends[1] < INFINITY)) repair[warp - 4] = 1;
       } else {
         const int64_t part = static_cast<int64_t>(it.split) * args.B * args.hq;
 #pragma unroll 1
@@ -1211,7 +1235,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnAr
     if (a.splits == 1) {
       const float inv = ll > 0.f || __isnanf(ll) ? 1.f / ll : 0.f;
       *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * D + d) =
-          make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          make_uint2(pack2<T>(fit<T>(acc.x * inv), fit<T>(acc.y * inv)), pack2<T>(fit<T>(acc.z * inv), fit<T>(acc.w * inv)));
     } else {
       const int64_t at = (a.parts + blockIdx.y) * n_rows + row;
       *reinterpret_cast<float4*>(a.part_o + at * D + d) = acc;
@@ -1259,7 +1283,7 @@ __global__ void __launch_bounds__(128) join_kernel(const float* part_o, const fl
 #pragma unroll
     for (int w = 0; w < 4; ++w) x += sums[w][d], y += sums[w][d + 1], l += sml[w].y;
     const float inv = l > 0.f || __isnanf(l) ? 1.f / l : 0.f;
-    reinterpret_cast<uint32_t*>(out + row * D)[threadIdx.x] = pack2<T>(x * inv, y * inv);
+    reinterpret_cast<uint32_t*>(out + row * D)[threadIdx.x] = pack2<T>(fit<T>(x * inv), fit<T>(y * inv));
   }
 }
 
