@@ -5,7 +5,8 @@ import math
 
 import pytest
 import torch
-from test_generate_gpu import U, _clean, close, cu_of, randn, unpack, w4_inputs, w4_want  # noqa: F401 (_clean: autouse)
+from test_generate_gpu import (U, _clean, close, cu_of, int32, prefix_inputs, prefix_want, randn, unpack,  # noqa: F401
+                               w4_inputs, w4_want)  # (_clean: autouse)
 
 pytestmark = pytest.mark.gpu
 HALF = [torch.bfloat16, torch.float16]
@@ -213,3 +214,69 @@ def test_results_at_the_end_of_the_type(cuda, dtype, d):
         for pk in (k, k[:0], torch.cat([k] * 12)):
             assert right(torch_xdna.shared_prefix_attention(wide, pk, torch.full_like(pk, size), ck, cv, lens, 1.0))
 
+
+
+# ------------------------------------------------------------------ how a prefix call is split
+@pytest.mark.parametrize("b,p,s,hq,hkv,d", [(190, 2500, 260, 8, 8, 64), (200, 3000, 300, 16, 8, 64), (180, 2000, 256, 6, 6, 128),
+                                            (20, 1500, 300, 8, 4, 128), (50, 1100, 300, 14, 2, 64)])
+def test_prefix_tiles_beside_split_caches_and_their_join(cuda, b, p, s, hq, hkv, d):
+    """Three launches (the prefix's tiles, the caches in pieces beside them, the join), among them batches of which many
+    caches wait for a place behind the tiles. Calls in a row use the same memory."""
+    import torch_xdna
+
+    x = prefix_inputs(b, p, s, hq, hkv, d)
+    y = [x[0].flip(0).contiguous(), x[2], x[1], x[4], x[3]]
+    lens = [(i * i * 31 + 5) % (s + 1) if i % 4 else 0 for i in range(b)]
+    a, z = int32(lens), int32(lens[::-1])
+    before = torch_xdna.stats.launches
+    first = torch_xdna.shared_prefix_attention(*x, a)
+    assert torch_xdna.stats.launches - before == 3
+    close(first, *prefix_want(*x, lens))
+    other = torch_xdna.shared_prefix_attention(*y, z)
+    close(other, *prefix_want(*y, lens[::-1]))
+    for _ in range(30):
+        got, got2 = torch_xdna.shared_prefix_attention(*x, a), torch_xdna.shared_prefix_attention(*y, z)
+        assert torch.equal(got, first) and torch.equal(got2, other)
+
+
+@pytest.mark.parametrize("b,p,s,hq,hkv,d", [(1, 700, 9000, 16, 8, 128), (3, 100, 20000, 4, 2, 64), (33, 3000, 9000, 4, 2, 64),
+                                            (64, 2100, 2000, 14, 2, 64), (130, 1500, 3000, 8, 4, 128)])
+def test_prefix_caches_with_room_to_spare(cuda, b, p, s, hq, hkv, d):
+    """Caches far longer than any sequence: most pieces of a cache are empty, and what lies past a length is not used."""
+    import torch_xdna
+
+    x = prefix_inputs(b, p, s, hq, hkv, d)
+    lens = [(i * 37) % 90 for i in range(b)]
+    for i, n in enumerate(lens):
+        x[3][i, n:], x[4][i, n:] = math.nan, math.inf
+    close(torch_xdna.shared_prefix_attention(*x, int32(lens)), *prefix_want(*x, lens))
+
+
+@pytest.mark.parametrize("b,p", [(1, 300), (3, 50), (90, 1000), (20, 1500)])
+def test_prefix_scores_of_minus_infinity_alone(cuda, b, p):
+    """They weigh nothing: a sequence that has no other keys is zero, and one that has is as without them."""
+    import torch_xdna
+
+    q, pk, pv, ck, cv = prefix_inputs(b, p, 40, 4, 2, 128)
+    q[..., 0] = -q[..., 0].abs() - 0.5
+    pk[..., 0] = math.inf
+    lens = [(i * 7) % 41 if i % 2 else 0 for i in range(b)]
+    want = prefix_want(q, pk[:0], pv[:0], ck, cv, lens)
+    got = torch_xdna.shared_prefix_attention(q, pk, pv, ck, cv, int32(lens))
+    close(got, *want)
+    assert not got[::2].any()
+
+
+@pytest.mark.parametrize("lens", [[i % 3 for i in range(2500)], [0] * 1100 + [700, 1, 0, 129] + [5] * 1030,
+                                  [1] * 1023 + [300], [1] * 1024 + [300], [2] * 1025])
+def test_packed_many_sequences(cuda, lens):
+    """The plan's block takes 1024 sequences at a time: fewer, just as many, more, empty ones among them."""
+    import torch_xdna
+
+    t = sum(lens)
+    q, k, v = (randn(t, h, 64, seed=i) for i, h in enumerate((4, 2, 2)))
+    got = torch_xdna.packed_attention(q, k, v, cu_of(lens))
+    start = torch.tensor([0] + lens).cumsum(0)[:-1].tolist()
+    rows = sorted({r for s, n in zip(start, lens) for r in (s, s + n // 2, s + n - 1) if n and s <= r < s + n})
+    rows = rows[::max(1, len(rows) // 400)] + [t - 1]
+    close(got[rows], *packed_rows(q, k, v, lens, rows))
