@@ -22,22 +22,19 @@ def test_scales_whose_products_overflow_are_refused():
 
 
 class _Fake:
-    """The binding's calls, answered with zeros of the right shape and without history, as it does."""
+    """The binding's calls: None where autograd would record them, else zeros of the right shape without history."""
 
     def launches(self):
         return 1
 
-    def packed_attention(self, q, k, v, cu, scale):
-        return torch.zeros(q.shape, dtype=q.dtype)
+    def __getattr__(self, name):
+        def call(*args):
+            if torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args):
+                return None
+            shape = (*args[0].shape[:-1], len(args[1])) if name == "linear_w4" else args[0].shape
+            return torch.zeros(shape, dtype=args[0].dtype)
 
-    def shared_prefix_attention(self, q, *rest):
-        return torch.zeros(q.shape, dtype=q.dtype)
-
-    def linear_w4(self, x, codes, scales, group, bias):
-        return torch.zeros(*x.shape[:-1], len(codes), dtype=x.dtype)
-
-    def process_logits(self, logits, *rest):
-        return torch.zeros(logits.shape, dtype=logits.dtype)
+        return call
 
 
 def _calls():
@@ -78,3 +75,31 @@ def test_gradients_do_not_vanish_in_silence(monkeypatch):
                 assert not call(ns).requires_grad
             with torch.inference_mode():
                 call(ns)
+
+
+def test_the_binding_hands_recorded_calls_back():
+    """Each input that may require grad, through the binding's own check (before it looks for a GPU)."""
+    from torch_xdna import generate
+
+    seen = []
+
+    class Spy:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append(getattr(binding, name)(*args))
+                return seen[-1]
+
+            return call
+
+    with pytest.raises(XdnaError):
+        torch_xdna.process_logits(torch.zeros(3))            # loads the binding
+    binding = generate._native
+    generate._native = Spy()
+    try:
+        for call in _calls():
+            with pytest.raises(torch_xdna.XdnaUnavailable):  # raised by the op's call, which is not recorded
+                call(torch_xdna)
+            assert seen == [None]
+            seen.clear()
+    finally:
+        generate._native = binding

@@ -172,7 +172,10 @@ def test_inputs_that_require_grad(cuda):
     calls = [(q, lambda y: torch_xdna.packed_attention(y, k, v, cu_of((30, 40)))),
              (q, lambda y: torch_xdna.shared_prefix_attention(y, k, v, k[:, None], v[:, None], cu_of([0] * 70)[:70])),
              (x, lambda y: torch_xdna.linear_w4(y, codes, scales, 64)),
-             (logits, torch_xdna.process_logits)]
+             (scales, lambda y: torch_xdna.linear_w4(x, codes, y, 64)),
+             (logits, torch_xdna.process_logits),
+             (logits[0].float(), lambda y: torch_xdna.process_logits(logits, bias=y)),
+             (logits[:, 0].float(), lambda y: torch_xdna.process_logits(logits, cu_of([1] * 8).view(3, 3), repetition=y + 1))]
     for value, call in calls:
         want = call(value)
         with torch.enable_grad():

@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -104,6 +105,15 @@ void check(const char* name, int rc) {
 
 const at::Tensor* in(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
 
+// Whether autograd would record a call with these inputs. The call then returns None, and the custom op makes it: its
+// result raises in backward, where one from here would have no history and the gradient would be missing without a word.
+bool tracked(std::initializer_list<const at::Tensor*> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : inputs)
+    if (t != nullptr && t->requires_grad()) return true;
+  return false;
+}
+
 double scale_of(const char* name, const at::Tensor& q, const at::Tensor& kv, PyObject* scale) {
   const int64_t hq = q.size(1), d = q.size(2), hkv = kv.size(-2);
   REQUIRE(half(q), XDNA_ERR_INVALID, "bf16 or f16, not " << type(q));
@@ -134,6 +144,7 @@ at::Tensor packed_attention(PyObject* const* a) {
   REQUIRE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) >= 1 && cu.is_contiguous(), XDNA_ERR_INVALID,
           "cu_seqlens: int32 [N + 1], contiguous");
   const double scale = scale_of(name, q0, k0, a[4]);
+  if (tracked({&q0, &k0, &v0})) return {};
   Place place(name, q0, {&k0, &v0, &cu});
   const at::Tensor q = rows(q0), k = rows(k0), v = rows(v0);
   const int64_t T = q.size(0), hq = q.size(1), d = q.size(2), hkv = k.size(1), n = cu.size(0) - 1;
@@ -163,6 +174,7 @@ at::Tensor shared_prefix_attention(PyObject* const* a) {
   REQUIRE(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == q0.size(0) && lens.is_contiguous(),
           XDNA_ERR_INVALID, "cache_lens: int32 [B], contiguous");
   const double scale = scale_of(name, q0, pk0, a[6]);
+  if (tracked({&q0, &pk0, &pv0, &ck0, &cv0})) return {};
   Place place(name, q0, {&pk0, &pv0, &ck0, &cv0, &lens});
   const at::Tensor q = rows(q0), pk = rows(pk0), pv = rows(pv0), ck = rows(ck0), cv = rows(cv0);
   const int64_t B = q.size(0), hq = q.size(1), d = q.size(2), P = pk.size(0), hkv = pk.size(1), S = ck.size(1);
@@ -199,6 +211,7 @@ at::Tensor linear_w4(PyObject* const* a) {
                                       << ": need contiguous bf16 or f16 [" << N << ", " << groups << "]");
   REQUIRE(!bias || (bias->dim() == 1 && bias->size(0) == N && code(bias->scalar_type()) >= 0), XDNA_ERR_INVALID,
           "bias: [N] in f32, bf16 or f16");
+  if (tracked({&x, &scales, in(bias)})) return {};
   Place place(name, x, {&codes, &scales, in(bias)});
   const at::Tensor sc = reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4 ? scales.clone() : scales;
   at::Tensor x2 = x.dim() == 2 ? x : x.reshape({x.numel() / K, K});
@@ -246,6 +259,7 @@ at::Tensor process_logits(PyObject* const* a) {
     REQUIRE(mask->scalar_type() == at::kInt && mask->dim() == 2 && mask->size(1) == words &&
                 (mask->size(0) == B || mask->size(0) == 1),
             XDNA_ERR_INVALID, "mask: int32 [B, " << words << "] or [1, " << words << "]");
+  if (tracked({&logits, in(row[2]), in(row[3]), in(row[4]), in(bias)})) return {};
   Place place(name, logits, {in(tokens), in(row[0]), in(row[1]), in(row[2]), in(row[3]), in(row[4]), in(bias), in(mask)});
   // rows contiguous
   for (at::Tensor* t : {&logits, tokens ? &*tokens : nullptr, bias ? &*bias : nullptr, mask ? &*mask : nullptr})

@@ -60,16 +60,6 @@ def _account(t0, launches=None):
     stats.seconds[DEVICE] += time.perf_counter() - t0
 
 
-def _tracked(*xs):
-    """Whether autograd would record this call. The custom op then makes it, whose result raises in backward; the
-    binding's would have no history, and the gradient would be missing without a word."""
-    if torch.is_grad_enabled():
-        for x in xs:
-            if getattr(x, "requires_grad", False):
-                return True
-    return False
-
-
 def packed_attention(q, k, v, cu_seqlens, scale=None):
     """Causal attention over packed sequences: softmax(scale q k^T) v per sequence and head, each token over the
     tokens of its sequence up to itself.
@@ -78,10 +68,10 @@ def packed_attention(q, k, v, cu_seqlens, scale=None):
     kernels cannot read them); cu_seqlens [N + 1] int32 on the GPU: sequence i is tokens cu_seqlens[i] ..
     cu_seqlens[i + 1] - 1. Tokens of no sequence (padding past the last one) give zeros. scale: 1 / sqrt(D) unless
     given. Returns [T, Hq, D]."""
-    if _tracked(q, k, v):
-        return torch.ops.xdna.packed_attention(q, k, v, cu_seqlens, scale)
     t0 = _ready(q)
     out = _native.packed_attention(q, k, v, cu_seqlens, scale)
+    if out is None:  # autograd records this call
+        return torch.ops.xdna.packed_attention(q, k, v, cu_seqlens, scale)
     _account(t0)
     return out
 
@@ -93,10 +83,10 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens,
     cache_lens[b] (int32 on the GPU, clamped to 0..S) are its own keys (bf16 or f16, D 64 or 128, Hq a multiple of
     Hkv; any strides, copied where the kernels cannot read them). Row b attends to the prefix and its own keys; with
     neither it is zero. scale: 1 / sqrt(D) unless given. Returns [B, Hq, D]."""
-    if _tracked(q, prefix_k, prefix_v, k_cache, v_cache):
-        return torch.ops.xdna.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
     t0 = _ready(q)
     out = _native.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
+    if out is None:  # autograd records this call
+        return torch.ops.xdna.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
     _account(t0)
     return out
 
@@ -134,10 +124,10 @@ def w4_pack(w, group=128, scale_dtype=None):
 def linear_w4(x, codes, scales, group, bias=None):
     """x [..., K] times a 4-bit weight (w4_pack) transposed, plus bias [N]: [..., N] in x's type (f32, bf16 or f16),
     summed in 32 bits and rounded once. Meant for the few rows of a decode step; any number is right."""
-    if _tracked(x, scales, bias):
-        return torch.ops.xdna.linear_w4(x, codes, scales, group, bias)
     t0 = _ready(x)
     y = _native.linear_w4(x, codes, scales, group, bias)
+    if y is None:  # autograd records this call
+        return torch.ops.xdna.linear_w4(x, codes, scales, group, bias)
     stats.macs[DEVICE] += x.numel() * len(codes)
     _account(t0)
     return y
@@ -153,9 +143,9 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=
     (taken off a generated token's logit once, and once for each time it occurs). bias: f32 [V] or [B, V], added.
     mask: int32 [B, ceil(V / 32)] or [1, ...], bit v % 32 of word v / 32 set where v is allowed; others become -inf,
     whatever stood there. Each may be None. Returns new logits in the same type."""
-    if _tracked(logits, repetition, presence, frequency, bias):
-        return torch.ops.xdna.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
     t0 = _ready(logits)
     out = _native.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
+    if out is None:  # autograd records this call
+        return torch.ops.xdna.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
     _account(t0)
     return out

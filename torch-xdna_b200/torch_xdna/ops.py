@@ -157,7 +157,8 @@ def _(x, mask, stack_id, cfg_id):
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      scale: Optional[float] = None) -> torch.Tensor:
     """Causal attention over packed sequences (generate.packed_attention)."""
-    return generate.packed_attention(q, k, v, cu_seqlens, scale)
+    with torch.no_grad():  # below autograd, whoever called
+        return generate.packed_attention(q, k, v, cu_seqlens, scale)
 
 
 @packed_attention.register_fake
@@ -170,7 +171,8 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
                             v_cache: torch.Tensor, cache_lens: torch.Tensor,
                             scale: Optional[float] = None) -> torch.Tensor:
     """A decode step's attention for a batch that shares a prefix (generate.shared_prefix_attention)."""
-    return generate.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
+    with torch.no_grad():  # below autograd, whoever called
+        return generate.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
 
 
 @shared_prefix_attention.register_fake
@@ -182,7 +184,8 @@ def _(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale=None):
 def linear_w4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int,
               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x times a 4-bit weight transposed (generate.linear_w4)."""
-    return generate.linear_w4(x, codes, scales, group, bias)
+    with torch.no_grad():  # below autograd, whoever called
+        return generate.linear_w4(x, codes, scales, group, bias)
 
 
 @linear_w4.register_fake
@@ -196,7 +199,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
                    presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
                    bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Penalties, bias and grammar mask on the next token's logits (generate.process_logits)."""
-    return generate.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
+    with torch.no_grad():  # below autograd, whoever called
+        return generate.process_logits(logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask)
 
 
 @process_logits.register_fake
