@@ -359,7 +359,8 @@ int xdna_qwen3_stack(const xdna_qwen3_layer* layers, int n_layers, const float* 
 /* ------------------------------------------------------------------ generation
  * From prompts to the next token (no reference counterpart: the reference answers with the logits of whole
  * sequences). Head dimensions 64 and 128, bf16 or f16, any number of query heads per key head up to 128;
- * strides are in elements, positive multiples of 8, bases 16-byte aligned. */
+ * strides are in elements, positive multiples of 8, bases 16-byte aligned. Scores, weights and sums are f32, weights
+ * enter the sums over V rounded to the operands' type. */
 
 /* Causal attention over packed sequences: out [tokens, hq, d] (contiguous) of q [tokens, hq, d], k and v
  * [tokens, hkv, d] with the strides *_st of a token and *_sh of a head. Sequence i is the tokens
@@ -375,7 +376,10 @@ int xdna_packed_attention(const void* q, int64_t q_st, int64_t q_sh, const void*
 
 /* One decode step's attention of B sequences that share a prefix: out [B, hq, d] (contiguous), row b's softmax over
  * the P prefix keys pk / pv [P, hkv, d] and the first lens[b] (clamped to 0..S) of its own ck / cv [B, S, hkv, d].
- * A row without any key gives zeros. workspace: xdna_prefix_attention_workspace bytes, 256-byte aligned. */
+ * A row without any key, or with scores of -inf alone, gives zeros. Sums over V are of weights up to 2^8 before the
+ * division by their sum: bf16 values for which they pass 3.4e38 overflow. How the work is split over the GPU goes by S,
+ * the lengths being on the device: a cache with much more room than it holds makes a call with a prefix slower, and is
+ * better passed cut to about its longest sequence. workspace: xdna_prefix_attention_workspace bytes, 256-byte aligned. */
 size_t xdna_prefix_attention_workspace(int64_t B, int64_t P, int64_t S, int64_t hq, int64_t hkv, int64_t d);
 int xdna_prefix_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* pk, int64_t pk_st, int64_t pk_sh,
                           const void* pv, int64_t pv_st, int64_t pv_sh, const void* ck, int64_t ck_sb, int64_t ck_st,
@@ -403,6 +407,7 @@ int xdna_linear_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
  * [0, V) count for nothing) and c = how often it is among those from prompt_lens[b] on:
  *   l = seen ? (l > 0 ? l / repetition[b] : l * repetition[b]) : l;  l -= frequency[b] * c + (c > 0) * presence[b];
  *   l += bias[b * ld_bias + v] (ld_bias 0: one for all rows);  l = bit v of mask[b * ld_mask + v / 32] ? l : -inf.
+ * At most 65535 rows; repetition at least 2^-126 (the quotient is a product with its reciprocal, one unit of f32 off).
  * Each of tokens, lens (then T), prompt_lens (then 0), repetition, presence, frequency, bias and mask may be NULL.
  * out must not overlap logits. */
 int xdna_process_logits(const void* logits, int dtype, int64_t B, int64_t V, int64_t ld_in, const void* tokens,

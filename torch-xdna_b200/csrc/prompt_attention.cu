@@ -25,13 +25,15 @@
 // Warps 2 and 3 only fill the first warpgroup: registers are moved between whole warpgroups.
 // TMEM: S_A | S_B | O_A | O_B, 128 columns each. Shared memory: Q 2 x 128 x D, a ring of K and V blocks of 128 x D (4 of
 // D = 128, 8 of 64), 32 KB through which outputs leave in whole lines.
-// Measured (bf16, 16 heads over 8 of 128, one causal prompt, the causal half counted): 4096 tokens 69 us, 990 TFLOP/s;
-// 8191 tokens 230 us, 1195 TFLOP/s, 0.72 of a large matrix product's rate. What bounds it is a tile's own chain, about
-// 2000 cycles of softmax and 1100 of its products per key block, with the other tile in antiphase: the tensor pipe and
-// the unit of the exponentials are each busy half of the time, and short prompts leave SMs idle at the end. Tried on an
-// earlier state of the kernel and left out: two threads per row (298 us against 289), an MMA thread per tile (their
-// products interleave, so each chain gets longer: 336 against 298), the row's maximum overlapped with its loads (239
-// against 236).
+// Measured (bf16, 16 heads over 8 of 128, one causal prompt, the causal half counted), in short replays of a graph with
+// warm operands at 1.9 GHz: 4096 tokens 69 us, 990 TFLOP/s; 8191 tokens 233 us, 1180 TFLOP/s, 0.71 of a large matrix
+// product's rate. The same call among others for a second, with other operands each time: 265 to 280 us, at the 1.7 GHz
+// that the power limit leaves. A tile's own chain is about 2000 cycles of softmax and 1100 of its products per key block,
+// with the other tile in antiphase: the tensor pipe and the unit of the exponentials are each busy half of the time, so
+// neither is the limit by itself, and short prompts leave SMs idle at the end and between items (one Q buffer for both
+// tiles). Tried on an earlier state of the kernel and left out: two threads per row (298 us against 289), an MMA thread
+// per tile (their products interleave, so each chain gets longer: 336 against 298), the row's maximum overlapped with its
+// loads (239 against 236).
 //
 // Keys that are masked for some rows of a tile but not for others carry p = 0; if their V holds an infinity or a NaN
 // the product is NaN. So it is where a weight that a row does see is too small for 16 bits, and sums of values near the
@@ -1069,8 +1071,9 @@ constexpr int kOwnMinSteps = 8;  // of a split, two per warp
 // 64 e + 8 g + 2 i (row g of product i) and 64 e + 8 g + 2 i + 1 (row g + 8). P^T is S^T's fragment, transposed by
 // movmatrix. Every lane reads back just what it copied, so no barrier is needed.
 // Keys past the length are not read and count as zeros with score -inf.
-// 190 sequences of 300 keys, 16 heads over 8 of 128, alone: 58 us for 247 MB, 4.2 TB/s, bound by the latency of the
-// copies that three CTAs per SM keep under way (the tensor pipe is busy 7 % of the time, the issue slots 25 %).
+// 190 sequences of 300 keys, 16 heads over 8 of 128, alone: 58 us for 247 MB, 4.2 TB/s; the tensor pipe is busy 7 % of
+// the time, the issue slots 25 %. 300 keys are 19 steps for four warps, so about five to a warp with two under way: the
+// copies are off most of the time, between a start that waits for the length and two barriers and a join at the end.
 // With one split the CTA also joins the prefix's parts and writes the output; else it leaves a part like theirs.
 template <typename T, int D>
 __global__ void __launch_bounds__(kOwnWarps * 32, 3) own_keys_kernel(const OwnArgs a) {
@@ -1380,8 +1383,9 @@ static int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtens
 
 static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { return tokens / (2 * (128 / group)) + n_seqs; }
 
-// How a prefix call is split. One sequence, and few with a short prefix, read the prefix themselves, before their own
-// keys (direct). With 8 key heads of 128, direct against the tile kernel: 2 sequences and a prefix of 3000 10.9 us and
+// How a prefix call is split (times: graph replays with warm operands; a call among others takes a few us more). One
+// sequence, and few with a short prefix, read the prefix themselves, before their own keys (direct). With 8 key heads of
+// 128, direct against the tile kernel: 2 sequences and a prefix of 3000 10.9 us and
 // 14.7, of 8000 22.1 and 17.1; 4 and 1000 8.7 and 9.2, and 2000 14.3 and 11.2; 8 and 500 8.7 and 10.4, and 1000 16.3 and
 // 11.3; with 2 of 64, 8 and 1000 6.3 and 8.0, 16 and 1500 8.8 and 9.5.
 // A sequence's keys, where the sequences and key heads alone are few CTAs for an SM, are split into pieces of at least
@@ -1397,6 +1401,10 @@ static int64_t plan_pairs(int64_t n_seqs, int64_t tokens, int64_t group) { retur
 // parts of one block 14.0, 8 parts 12.1; 100 sequences, prefix 1000, caches of 200: 8 parts of one block 26.3, 4 parts
 // 28.0. Split caches against whole ones: 300 sequences, prefix 9000, caches of 300: 81 us against 100; 190 and 16381:
 // 69 against 73; 190 and 4096: 49 against 51.)
+// The lengths are on the device, so half the cache stands for them. A cache with much more room than it holds makes the
+// parts too few: 32 sequences, prefix 4096, up to 600 keys of their own take 25 us in caches of 600, 31 of 1200, 64 of
+// 2400 and more; 190, prefix 16381, up to 301 keys: 71 in caches of 301, 93 of 602, 130 of 1204, 241 of 4096 and more. A
+// caller with long caches passes views of them that are about as long as the longest sequence.
 struct PrefixSplit {
   bool direct;
   int64_t pairs, parts, blocks_per_part, own;

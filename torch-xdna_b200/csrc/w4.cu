@@ -60,9 +60,11 @@ struct W4Args {
 // A CTA has an equal share of the tiles, to one, eight at a time; where fewer are left, or there are fewer from the
 // start, 2, 4 or 8 warps share one, each with a run of its blocks, and add their sums in shared memory in a fixed order.
 // (Whole rounds of eight alone left the 9496 tiles of a 151936-row head at 4.01 rounds: a fifth with three CTAs.)
-// 151936 x 1024, 8 x rows, groups of 128: 23 us for 82 MB, 3.6 TB/s; the copies alone take 19 us, and the rest is the
-// issue slots, busy 59 % of the time, mostly with taking codes apart (11 operations for the 8 codes of a word). 4096 x
-// 1024, one x row: 3.5 us, of which a kernel that does next to nothing takes 1.5.
+// 151936 x 1024, 8 x rows, groups of 128: 23 us for 82 MB, 3.6 TB/s. The copies alone take 19 us (16 warps to an SM, each
+// with two stages under way), and taking codes apart (11 operations for the 8 codes of a word; the issue slots are busy 59
+// % of the time) is not wholly hidden behind them. 4096 x 1024, one x row: 3.5 us, of which a kernel that does next to
+// nothing takes 1.5. (Short replays of a graph.)
+// A group's products are summed before its scale: |x| above 4e37 / group can overflow f32 there.
 // K split over the CTAs of a cluster, to give few tiles more SMs, was left out: 24.7 us became 18.3 where x is long (30
 // rows of 5001), but 4.1 became 6.0 for 1024 x 2048 (the cluster's launch and its two barriers).
 constexpr int kW4Blocks = 4;

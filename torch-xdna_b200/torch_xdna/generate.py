@@ -82,7 +82,8 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens,
     q [B, Hq, D]; prefix_k, prefix_v [P, Hkv, D]; k_cache, v_cache [B, S, Hkv, D], of which row b's first
     cache_lens[b] (int32 on the GPU, clamped to 0..S) are its own keys (bf16 or f16, D 64 or 128, Hq a multiple of
     Hkv; any strides, copied where the kernels cannot read them). Row b attends to the prefix and its own keys; with
-    neither it is zero. scale: 1 / sqrt(D) unless given. Returns [B, Hq, D]."""
+    neither it is zero. scale: 1 / sqrt(D) unless given. Returns [B, Hq, D]. The lengths stay on the GPU, and the work
+    is split by S: pass long caches cut to about the longest sequence (k_cache[:, :n], no copy)."""
     t0 = _ready(q)
     out = _native.shared_prefix_attention(q, prefix_k, prefix_v, k_cache, v_cache, cache_lens, scale)
     if out is None:  # autograd records this call
@@ -135,7 +136,7 @@ def linear_w4(x, codes, scales, group, bias=None):
 
 def process_logits(logits, tokens=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None,
                    bias=None, mask=None):
-    """Penalties, bias and grammar mask on the next token's logits [B, V] (f32, bf16 or f16), in one pass.
+    """Penalties, bias and grammar mask on the next token's logits [B, V] (f32, bf16 or f16; B up to 65535), in one pass.
 
     tokens [B, T] (int32 or int64): each row's tokens so far, the first lens[b] of them (all, unless given), of which
     the first prompt_lens[b] (none, unless given) are the prompt's; ids outside [0, V) count for nothing. Per row and
