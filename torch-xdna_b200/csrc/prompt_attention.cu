@@ -44,33 +44,9 @@
 
 #include "host_util.h"
 #include "sm100.cuh"
+#include "values.cuh"
 
 namespace xdna {
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T x);
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <>
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 // The larger magnitude of each of two 16-bit values, NaN where one is.
 template <typename T>
@@ -83,14 +59,6 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
         __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
-}
-
-// x, or where it is finite the nearest value within T's range: a mean of values of T lies within it, and only the
-// roundings of the weights take it out.
-template <typename T>
-__device__ __forceinline__ float fit(float x) {
-  constexpr float kMax = __is_same(T, __half) ? 65504.f : 3.38953139e38f;
-  return fabsf(x) < INFINITY ? fminf(fmaxf(x, -kMax), kMax) : x;
 }
 
 // 2^x of two values on the FMA pipe, to relieve the MUFU unit, whose rate (16 a clock and SM) is as tight here as the
@@ -146,7 +114,6 @@ struct TileArgs {
   float2* part_ml; // [split][B * hq]: m (log2 units), l
 };
 
-constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kTaThreads = 384;  // three warpgroups: issue (TMA, MMA), softmax of tile A, of tile B
 // Registers per thread after setmaxnreg: together what the launch gives, 384 x 168. 16 prompts of up to 1900 tokens, and
 // one of 8191 with 16 heads of 64, with 56 for the issuing warps and 224 for the softmax: 125 and 248 us; 88 and 208: 111
@@ -174,37 +141,6 @@ struct TileItem {
   int len, q_pos;          // PACKED: sequence length, tile A's first place in it
   int split;               // PREFIX
 };
-
-// A launch that may start while the kernel before it still runs (and waits for it itself, griddepcontrol.wait).
-template <typename... Params, typename... Args>
-static int launch_early(const char* what, void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  XDNA_CUDA(cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...));
-  return check_launch(what);
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // N consecutive values of T as they are (N * 2 bytes, aligned to as many) and as floats.
 template <int N>
@@ -1050,10 +986,6 @@ struct OwnArgs {
   float2* part_ml;
   void* out;
 };
-
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
 
 constexpr int kOwnWarps = 4;
 constexpr int kOwnStep = 16;   // keys of a warp's step
