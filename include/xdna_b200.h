@@ -44,6 +44,7 @@ extern "C" {
 #define XDNA_I32 3
 #define XDNA_I8 4
 #define XDNA_U8 5
+#define XDNA_E4M3 6
 
 /* ------------------------------------------------------------------ conv3x3 modes */
 #define XDNA_CONV_Q 0         /* q = sat((acc + 2^(shift-1)) >> shift) as int8, or uint8 [0,255] with relu, NCHW */
@@ -415,6 +416,69 @@ int xdna_process_logits(const void* logits, int dtype, int64_t B, int64_t V, int
                         const int32_t* prompt_lens, const float* repetition, const float* presence,
                         const float* frequency, const float* bias, int64_t ld_bias, const uint32_t* mask,
                         int64_t ld_mask, void* out, int64_t ld_out, void* stream);
+
+/* ------------------------------------------------------------------ a decoder layer around its products
+ * No reference counterpart. Strides are in elements unless said otherwise; norms' weights are f32, bf16 or f16. */
+
+/* out [T, H, D] (contiguous, x's type f32 / bf16 / f16) = x [T, H, D] with the first R = 2 * n_freq entries of each head
+ * turned: pairs (p, p + R / 2), or (2 p, 2 p + 1) with interleaved, by the angle positions[t] * inv_freq[p] (in 64 bits),
+ * times factor; the others stay. norm != NULL: each head is first divided by the root of its mean square (plus eps) and
+ * multiplied with the weights norm[h * norm_sh ..] (norm_sh 0: one for all heads). D a multiple of 8, up to 256; x_st,
+ * x_sh (of a token, of a head) and norm_sh multiples of 8; x, out and norm 16-byte aligned; positions 32 or 64 bits.
+ * Sums and products are f32, rounded once. */
+int xdna_rotary(const void* x, int dtype, int64_t T, int64_t H, int64_t D, int64_t x_st, int64_t x_sh,
+                const void* positions, int position_bytes, const float* inv_freq, int64_t n_freq, float factor,
+                int interleaved, const void* norm, int norm_dtype, int64_t norm_sh, float eps, void* out, void* stream);
+
+/* The norms around a block, its gate and its residual: for each of `rows` rows of D (up to 16384) entries, in f32,
+ *   z = post ? y / sqrt(mean y^2 + eps) * post : y;  x' = x + scale * gate * z;  h = x' / sqrt(mean x'^2 + eps) * weight
+ * x_out = x' in x's type, h in y's type (h is of x' before its rounding), both contiguous [rows, D] and apart from the
+ * inputs. post and gate may be NULL; ld_gate 0: one gate for all rows. Any row pitches and alignments; pieces of 16 bytes
+ * where all are multiples of 8 elements and 16-byte aligned. */
+int xdna_add_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_dtype, int64_t ldy, int64_t rows,
+                  int64_t D, const void* weight, int weight_dtype, const void* post, int post_dtype, const void* gate,
+                  int gate_dtype, int64_t ld_gate, float scale, float eps, void* x_out, void* h, void* stream);
+
+/* A cache of keys and values in pages and 8 bits: codes [pages][hkv][page][d] bytes (format XDNA_I8 or XDNA_E4M3; the
+ * last three dimensions contiguous, kc_sp / vc_sp bytes from page to page, multiples of 16; page 16, 32, 64 or 128; d 64
+ * or 128) and scales [pages][hkv] f32 (ks_sp / vs_sp elements from page to page): x = code * scale, one scale for a
+ * head's part of a page (a block), a power of two. table [n_seqs][max_pages] (int32, row pitch ld_table): the page of a
+ * sequence's tokens i * page .. ; an entry outside [0, pages) is no page.
+ *
+ * xdna_cache_append puts new tokens k, v [tokens, hkv, d] (bf16 / f16) behind the starts[i] that sequence i has in the
+ * cache: token i is sequence i's next one (cu_seqlens NULL, n_seqs == tokens), or tokens cu_seqlens[i] ..
+ * cu_seqlens[i + 1] - 1 are sequence i's next ones (ascending; words outside [0, tokens] are clamped). The keys, after
+ * k_norm where given, are turned to their place in the sequence as by xdna_rotary. A block's scale is the least 2^e >=
+ * 2^-126 with max |x| <= 127 * 2^e (int8) or 448 * 2^e (e4m3) over its tokens; where older tokens in it had a larger one
+ * that stays, where they had a smaller one their codes are rounded to the new one. A page whose first slot is written
+ * starts anew. A block that is given an infinity or a NaN has the scale NaN until then, and code 0 for the new tokens.
+ * Slots behind a sequence's last token, and all other pages, are left as they were. Tokens without a page, and sequences
+ * with starts[i] < 0, are not stored. No two sequences of a call may write to one page. q [tokens, hq, d] may be NULL;
+ * else q_out [tokens, hq, d] = q, after q_norm, turned to its tokens' places (zero where starts[i] < 0 and for tokens of
+ * no sequence). Rows of k, v and q as for xdna_rotary. */
+int xdna_cache_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
+                      int64_t tokens, int64_t hkv, int64_t d, void* k_codes, int64_t kc_sp, void* v_codes, int64_t vc_sp,
+                      int format, float* k_scales, int64_t ks_sp, float* v_scales, int64_t vs_sp, int64_t pages,
+                      int64_t page, const int32_t* table, int64_t ld_table, int64_t max_pages, const int32_t* starts,
+                      const int32_t* cu_seqlens, int64_t n_seqs, const float* inv_freq, int64_t n_freq, float factor,
+                      int interleaved, const void* k_norm, int k_norm_dtype, int64_t k_norm_sh, float eps, const void* q,
+                      int64_t q_st, int64_t q_sh, int64_t hq, const void* q_norm, int q_norm_dtype, int64_t q_norm_sh,
+                      void* q_out, void* stream);
+
+/* Attention over such a cache: out [B, T, hq, d] (contiguous) of q [B, T, hq, d] (bf16 / f16; strides q_sb, q_st, q_sh),
+ * the last T tokens of each sequence: token t attends to the first lens[b] - T + t + 1 tokens in the cache (lens clamped
+ * to 0 .. max_pages * page, which is below 2^30), without those that have no page. A row without any, or with scores of
+ * -inf alone, is zero. Scores and sums are f32; the weights that meet V are f16 with an exponent of their own per block
+ * (terms below 2^-25 of a row's largest are lost). How the work is split goes by the lengths, on the device; T is meant
+ * to be small: every 16 / (hq / hkv) tokens the cache is read once more. Codes of e4m3 are numbers. workspace: xdna_paged_attention_workspace
+ * bytes for most_keys = max_pages * page, 256-byte aligned. */
+size_t xdna_paged_attention_workspace(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys);
+int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, int64_t B, int64_t T,
+                         int64_t hq, int64_t hkv, int64_t d, const void* k_codes, int64_t kc_sp, const void* v_codes,
+                         int64_t vc_sp, int format, const float* k_scales, int64_t ks_sp, const float* v_scales,
+                         int64_t vs_sp, int64_t pages, int64_t page, const int32_t* table, int64_t ld_table,
+                         int64_t max_pages, const int32_t* lens, float scale, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

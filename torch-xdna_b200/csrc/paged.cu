@@ -1,0 +1,1044 @@
+// A cache of keys and values in pages and in 8 bits, and the two calls that a decode step makes of it: appending
+// (xdna_cache_append), with the norm and the rotation of the keys on the way, and attention (xdna_paged_attention).
+//
+// Codes lie as [pages][Hkv][page][D] bytes, int8 or e4m3, a page being 16, 32, 64 or 128 tokens; a block is one head's
+// part of a page, D * page contiguous bytes, and has one scale, a power of two: x = code * scale. table[b][i] is the
+// page of sequence b's tokens i * page .. (i + 1) * page - 1.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "host_util.h"
+#include "rotary.cuh"
+#include "rotary.h"
+
+namespace xdna {
+
+// ---------------------------------------------------------------------------- codes
+// A block's scale is the least 2^e, e >= -126, with max |x| <= top * 2^e (top 127 for int8, 448 for e4m3), so x / 2^e is
+// exact, no code is out of range, and a code whose block's scale grows is only halved, which loses nothing in e4m3 but at
+// its lowest values, and less than one step of the new scale in int8 however often it happens (1/2 + 1/4 + ...).
+// An infinity or a NaN makes the block's scale NaN.
+__device__ __forceinline__ int block_exponent(uint32_t top_bits, bool e4m3) {
+  const int e = static_cast<int>(top_bits >> 23) - 127;
+  const uint32_t mantissa = top_bits & 0x7fffffu;
+  return max(e4m3 ? e - 8 + (mantissa > 0x600000u) : e - 6 + (mantissa > 0x7e0000u), -126);
+}
+constexpr uint32_t kNotFinite = 0x7f800000u;
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }  // -126 .. 127
+
+// What an append makes of a block: the scale, 1 / scale for the new values, and the factor of the older codes.
+struct BlockChange {
+  float scale, inverse, older;  // inverse 0: not finite; older 1: they stay
+};
+__device__ __forceinline__ BlockChange change_block(uint32_t top_bits, bool has_older, uint32_t old_bits, bool e4m3) {
+  if (top_bits >= kNotFinite || (has_older && (old_bits & 0x7fffffffu) >= kNotFinite)) return {__uint_as_float(0x7fc00000u), 0.f, 1.f};
+  int e = block_exponent(top_bits, e4m3);
+  float older = 1.f;
+  if (has_older) {
+    const int old = max(static_cast<int>(old_bits >> 23 & 0xff) - 127, -126);
+    if (e > old)
+      older = power_of_two(max(old - e, -126));
+    else
+      e = old;
+  }
+  return {power_of_two(e), power_of_two(min(-e, 127)), older};
+}
+
+// Four values to codes; x is within the codes' range (0 where the block is not finite).
+__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d, bool e4m3) {
+  if (e4m3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    return lo | static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16;
+  }
+  auto byte = [](float x) { return static_cast<uint32_t>(__float2int_rn(x)) & 0xffu; };
+  return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(d) << 24;
+}
+// Two half pairs, exactly, of the four codes of a word, lowest first. int8: 1024 + (code + 128) is the half 0x6400 | byte.
+template <bool E4M3>
+__device__ __forceinline__ void to_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (E4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    const uint32_t u = w ^ 0x80808080u;
+    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    const __half2 p = __hsub2(*reinterpret_cast<const __half2*>(&x), off), q = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+    lo = *reinterpret_cast<const uint32_t*>(&p);
+    hi = *reinterpret_cast<const uint32_t*>(&q);
+  }
+}
+__device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float by, bool e4m3) {
+  uint32_t lo, hi;
+  if (e4m3)
+    to_halves<true>(w, lo, hi);
+  else
+    to_halves<false>(w, lo, hi);
+  const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&lo)), q = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return to_codes(p.x * by, p.y * by, q.x * by, q.y * by, e4m3);
+}
+// The first `bytes` (a multiple of 16) of a block, by `threads` threads of which this is number i.
+__device__ __forceinline__ void rescale_block(uint8_t* block, int bytes, float by, bool e4m3, int i, int threads) {
+#pragma unroll 4
+  for (int at = i * 16; at < bytes; at += threads * 16) {
+    uint4 u = *reinterpret_cast<const uint4*>(block + at);
+    u.x = rescale_codes(u.x, by, e4m3), u.y = rescale_codes(u.y, by, e4m3);
+    u.z = rescale_codes(u.z, by, e4m3), u.w = rescale_codes(u.w, by, e4m3);
+    *reinterpret_cast<uint4*>(block + at) = u;
+  }
+}
+
+// ---------------------------------------------------------------------------- append
+struct AppendArgs {
+  const void *k, *v, *q;  // q NULL: no queries
+  int64_t k_st, k_sh, v_st, v_sh, q_st, q_sh;
+  uint8_t *kc, *vc;       // codes
+  int64_t kc_sp, vc_sp;   // bytes from page to page
+  float *ks, *vs;         // scales
+  int64_t ks_sp, vs_sp;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t *starts, *cu;
+  const float* inv_freq;
+  const void *k_norm, *q_norm;
+  int64_t k_norm_sh, q_norm_sh;
+  void* q_out;
+  int64_t tokens;
+  float factor, eps;
+  int k_norm_dtype, q_norm_dtype;
+  int n_freq, n_seqs, hq, hkv, page, page_shift, pages, max_pages;
+  bool e4m3;
+  int heads;  // of a block of threads (packed)
+};
+
+template <int D, int V>
+struct RowShape {
+  static constexpr int kLanes = V == 8 ? D / 16 : 32, kUnits = V == 8 ? 1 : D / 64, kRows = 32 / kLanes;
+  static constexpr int kPerLane = 2 * V * kUnits;
+  static_assert(V == 8 || V == 1, "16-byte pieces, or single entries where pairs lie at odd distances");
+};
+
+template <typename T, int D, int V>
+struct RawRow {
+  Pack<T, V> p[RowShape<D, V>::kUnits][2];
+};
+template <typename T, int D, int V>
+__device__ __forceinline__ RawRow<T, D, V> load_row(const T* x, const UnitAt* u) {
+  RawRow<T, D, V> r;
+#pragma unroll
+  for (int k = 0; k < RowShape<D, V>::kUnits; ++k) r.p[k][0] = load_pack<T, V>(x + u[k].lo), r.p[k][1] = load_pack<T, V>(x + u[k].hi);
+  return r;
+}
+template <typename T, int D, int V>
+__device__ __forceinline__ void row_floats(const RawRow<T, D, V>& r, float (*f)[2 * V]) {
+#pragma unroll
+  for (int k = 0; k < RowShape<D, V>::kUnits; ++k) to_floats<T, V>(r.p[k][0], f[k]), to_floats<T, V>(r.p[k][1], f[k] + V);
+}
+// All lanes of the warp; norm NULL for rows without one.
+template <int D, int V>
+__device__ __forceinline__ void norm_row(float (*f)[2 * V], const UnitAt* u, const void* norm, int dtype, int64_t at, float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) ss = fmaf(f[k][i], f[k][i], ss);
+  }
+  ss = sum_of_lanes<RowShape<D, V>::kLanes>(ss);
+  if (norm == nullptr) return;
+  const float inv = rsqrtf(ss * (1.f / D) + eps);
+#pragma unroll
+  for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
+    float g[2 * V];
+    load_weights<V>(norm, dtype, at + u[k].lo, g);
+    load_weights<V>(norm, dtype, at + u[k].hi, g + V);
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) f[k][i] *= inv * g[i];
+  }
+}
+// The largest |x| of the lanes of a row, as bits: NaN is above infinity, and that above all numbers.
+template <int D, int V>
+__device__ __forceinline__ uint32_t row_top(const float (*f)[2 * V]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) top = max(top, __float_as_uint(f[k][i]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int o = RowShape<D, V>::kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  return top;
+}
+template <int D, int V>
+__device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V], const UnitAt* u, float inverse, bool e4m3) {
+#pragma unroll
+  for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
+    float x[2 * V];
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) x[i] = inverse == 0.f ? 0.f : f[k][i] * inverse;
+    if constexpr (V == 8) {
+      *reinterpret_cast<uint2*>(row + u[k].lo) = make_uint2(to_codes(x[0], x[1], x[2], x[3], e4m3), to_codes(x[4], x[5], x[6], x[7], e4m3));
+      *reinterpret_cast<uint2*>(row + u[k].hi) = make_uint2(to_codes(x[8], x[9], x[10], x[11], e4m3), to_codes(x[12], x[13], x[14], x[15], e4m3));
+    } else {
+      const uint32_t c = to_codes(x[0], x[1], 0.f, 0.f, e4m3);
+      row[u[k].lo] = static_cast<uint8_t>(c);
+      row[u[k].hi] = static_cast<uint8_t>(c >> 8);
+    }
+  }
+}
+
+constexpr int kAppendThreads = 256;
+
+// One token of each sequence: a block of threads per token, whose rows are its query heads, its keys and its values.
+// Latency is what counts: everything of a row is asked for at once, and only a block whose scale grows (a few times in a
+// page) is read and written again, by the whole warp.
+template <typename T, int D, int V, bool INTER>
+__global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const AppendArgs a) {
+  using S = RowShape<D, V>;
+  constexpr unsigned kAll = 0xffffffffu;
+  const int lane = lane_id(), r = lane / S::kLanes, j0 = lane % S::kLanes;
+  const int64_t token = blockIdx.x;
+  const int position = a.starts[token];
+  const bool there = position >= 0;
+  const int number = position >> a.page_shift, slot = position & (a.page - 1);
+  int page = -1;
+  if (there && number < a.max_pages) page = a.table[token * a.ld_table + number];
+  if (page >= a.pages) page = -1;
+  UnitAt u[S::kUnits];
+  float2 cs[S::kUnits][V];
+#pragma unroll
+  for (int k = 0; k < S::kUnits; ++k) {
+    u[k] = unit_at<V, INTER>(j0 + k * S::kLanes, a.n_freq);
+    constexpr int kPer = V / S::kRows;
+    float2 mine[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int p = (j0 + k * S::kLanes) * V + r * kPer + i;
+      mine[i] = p < a.n_freq ? turn_of(position, a.inv_freq[p], a.factor) : make_float2(1.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int src = (i / kPer) * S::kLanes + j0;
+      cs[k][i].x = __shfl_sync(kAll, mine[i % kPer].x, src);
+      cs[k][i].y = __shfl_sync(kAll, mine[i % kPer].y, src);
+    }
+  }
+  const int hq = a.q ? a.hq : 0, rows = hq + 2 * a.hkv;
+  for (int r0 = warp_id() * S::kRows; r0 < rows; r0 += kAppendThreads / 32 * S::kRows) {
+    const int row = r0 + r, kind = row < hq ? 0 : row < hq + a.hkv ? 1 : 2;  // query, key, value
+    const int h = kind == 0 ? row : kind == 1 ? row - hq : row - hq - a.hkv;
+    const bool mine = row < rows && there;
+    const T* src = kind == 0   ? static_cast<const T*>(a.q) + token * a.q_st + h * a.q_sh
+                   : kind == 1 ? static_cast<const T*>(a.k) + token * a.k_st + h * a.k_sh
+                               : static_cast<const T*>(a.v) + token * a.v_st + h * a.v_sh;
+    const bool cached = mine && kind > 0 && page >= 0;
+    float* scale = nullptr;
+    uint8_t* block = nullptr;
+    uint32_t old_bits = 0;
+    if (cached) {
+      scale = (kind == 1 ? a.ks + page * a.ks_sp : a.vs + page * a.vs_sp) + h;
+      block = (kind == 1 ? a.kc + page * a.kc_sp : a.vc + page * a.vc_sp) + static_cast<int64_t>(h) * a.page * D;
+      old_bits = __float_as_uint(*scale);
+    }
+    float f[S::kUnits][2 * V];
+    row_floats<T, D, V>(mine ? load_row<T, D, V>(src, u) : RawRow<T, D, V>{}, f);
+    norm_row<D, V>(f, u, !mine || kind == 2 ? nullptr : kind == 0 ? a.q_norm : a.k_norm, kind == 0 ? a.q_norm_dtype : a.k_norm_dtype,
+                   kind == 0 ? h * a.q_norm_sh : h * a.k_norm_sh, a.eps);
+    if (kind != 2) {
+#pragma unroll
+      for (int k = 0; k < S::kUnits; ++k) turn_unit<V, INTER>(f[k], cs[k], u[k].turning);
+    }
+    if (kind == 0 && row < rows) {
+      T* dst = static_cast<T*>(a.q_out) + (token * a.hq + h) * D;
+#pragma unroll
+      for (int k = 0; k < S::kUnits; ++k) {
+        store_pack<T, V>(dst + u[k].lo, mine ? from_floats<T, V>(f[k]) : Pack<T, V>{});
+        store_pack<T, V>(dst + u[k].hi, mine ? from_floats<T, V>(f[k] + V) : Pack<T, V>{});
+      }
+    }
+    const uint32_t top = row_top<D, V>(f);
+    BlockChange c{0.f, 0.f, 1.f};
+    if (cached) {
+      c = change_block(top, slot > 0, old_bits, a.e4m3);
+      store_codes<D, V>(block + slot * D, f, u, c.inverse, a.e4m3);
+      if (j0 == 0) *scale = c.scale;
+    }
+    unsigned grows = __ballot_sync(kAll, c.older != 1.f && j0 == 0);
+    while (grows) {
+      const int who = __ffs(grows) - 1;
+      grows &= grows - 1;
+      uint8_t* p = reinterpret_cast<uint8_t*>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(block), who));
+      rescale_block(p, slot * D, __shfl_sync(kAll, c.older, who), a.e4m3, lane, 32);
+    }
+  }
+}
+
+// Which page of which sequence this block of threads has: number `item` of those that the new tokens touch, sequence by
+// sequence. Every thread takes sequences in turn.
+struct PageItem {
+  int seq, number;           // the sequence and its page's number
+  int64_t first;             // the sequence's first new token
+  int64_t start, end;        // its first and behind its last new position
+};
+__device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t item, PageItem* found) {
+  __shared__ int sums[kAppendThreads / 32];
+  __shared__ PageItem it;
+  __shared__ int done;
+  if (threadIdx.x == 0) done = 0;
+  int64_t before = 0;
+  for (int base = 0; base < a.n_seqs; base += kAppendThreads) {
+    const int seq = base + static_cast<int>(threadIdx.x);
+    int64_t first = 0, start = -1, end = -1;
+    int count = 0;
+    if (seq < a.n_seqs) {
+      first = min(max(static_cast<int64_t>(a.cu[seq]), int64_t{0}), a.tokens);
+      const int64_t last = min(max(static_cast<int64_t>(a.cu[seq + 1]), first), a.tokens);
+      start = a.starts[seq];
+      end = min(start + (last - first), static_cast<int64_t>(a.max_pages) << a.page_shift);
+      if (start >= 0 && end > start) count = static_cast<int>(((end - 1) >> a.page_shift) - (start >> a.page_shift)) + 1;
+    }
+    int upto = count;  // of the warp's lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane_id() >= o) upto += y;
+    }
+    if (lane_id() == 31) sums[warp_id()] = upto;
+    __syncthreads();
+    int64_t all = 0, mine = before + upto - count;
+    for (int w = 0; w < kAppendThreads / 32; ++w) {
+      if (w < warp_id()) mine += sums[w];
+      all += sums[w];
+    }
+    if (item >= mine && item < mine + count) {
+      it = PageItem{seq, static_cast<int>((start >> a.page_shift) + (item - mine)), first, start, end};
+      done = 1;
+    }
+    before += all;
+    __syncthreads();
+    if (done) break;
+  }
+  *found = it;
+  return done != 0;
+}
+
+// The new tokens of packed sequences: a block of threads per page that they touch, K or V (blockIdx.z), and a.heads heads
+// (blockIdx.y). A head's part of the page lies in registers, at most 128 tokens, between the search for its largest value
+// and its codes; the angles' cosines and sines, which are those of all heads, are worked out once, in shared memory.
+template <typename T, int D, int V, bool INTER>
+__global__ void __launch_bounds__(kAppendThreads) append_packed_kernel(const AppendArgs a) {
+  using S = RowShape<D, V>;
+  constexpr int kWarps = kAppendThreads / 32, kAtOnce = kWarps * S::kRows, kMost = 128 / kAtOnce;  // rows at a time, times
+  constexpr int kSplit = D / (2 * V), kPitch = D / 2 + D / 16;  // of a token's turns; a lane's are kSplit apart
+  extern __shared__ __align__(16) float2 turns[];
+  __shared__ uint32_t tops[32];
+  PageItem it;
+  if (threadIdx.x < 32) tops[threadIdx.x] = 0;
+  if (!find_page(a, blockIdx.x, &it)) return;
+  const int page = a.table[it.seq * a.ld_table + it.number];
+  if (page < 0 || page >= a.pages) return;
+  const bool value = blockIdx.z != 0;
+  const int64_t page_first = static_cast<int64_t>(it.number) << a.page_shift;
+  const int lo = static_cast<int>(max(it.start - page_first, int64_t{0}));
+  const int n = static_cast<int>(min(it.end - page_first, static_cast<int64_t>(a.page))) - lo;  // new tokens, in slots lo ..
+  const int64_t token = it.first + (page_first + lo - it.start);
+  const int lane = lane_id(), r0 = warp_id() * S::kRows + lane / S::kLanes, j0 = lane % S::kLanes;
+  const int n_freq = value ? 0 : a.n_freq;
+  UnitAt u[S::kUnits];
+#pragma unroll
+  for (int k = 0; k < S::kUnits; ++k) u[k] = unit_at<V, INTER>(j0 + k * S::kLanes, n_freq);
+  for (int i = threadIdx.x; i < n * n_freq; i += kAppendThreads) {
+    const int t = i / n_freq, p = i % n_freq;
+    turns[t * kPitch + (p % V) * kSplit + p / V] = turn_of(page_first + lo + t, a.inv_freq[p], a.factor);
+  }
+  __syncthreads();
+  const int h0 = static_cast<int>(blockIdx.y) * a.heads, h1 = min(h0 + a.heads, a.hkv);
+  for (int h = h0; h < h1; ++h) {
+    const T* src = value ? static_cast<const T*>(a.v) + h * a.v_sh : static_cast<const T*>(a.k) + h * a.k_sh;
+    const int64_t st = value ? a.v_st : a.k_st;
+    float* scale = (value ? a.vs + page * a.vs_sp : a.ks + page * a.ks_sp) + h;
+    uint8_t* block = (value ? a.vc + page * a.vc_sp : a.kc + page * a.kc_sp) + static_cast<int64_t>(h) * a.page * D;
+    const uint32_t old_bits = __float_as_uint(*scale);
+    float f[kMost][S::kUnits][2 * V];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      const int t = r0 + i * kAtOnce;
+      row_floats<T, D, V>(t < n ? load_row<T, D, V>(src + (token + t) * st, u) : RawRow<T, D, V>{}, f[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      const int t = r0 + i * kAtOnce;
+      if (i * kAtOnce >= n) break;
+      if (!value) {
+        norm_row<D, V>(f[i], u, t < n ? a.k_norm : nullptr, a.k_norm_dtype, h * a.k_norm_sh, a.eps);
+#pragma unroll
+        for (int k = 0; k < S::kUnits; ++k) {
+          if (t < n && u[k].turning > 0) {
+            float2 cs[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) cs[e] = e < u[k].turning ? turns[t * kPitch + e * kSplit + j0 + k * S::kLanes] : make_float2(1.f, 0.f);
+            turn_unit<V, INTER>(f[i][k], cs, u[k].turning);
+          }
+        }
+      }
+      top = max(top, row_top<D, V>(f[i]));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) atomicMax(&tops[h - h0], top);
+    __syncthreads();
+    const BlockChange c = change_block(tops[h - h0], lo > 0, old_bits, a.e4m3);
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      const int t = r0 + i * kAtOnce;
+      if (t < n) store_codes<D, V>(block + (lo + t) * D, f[i], u, c.inverse, a.e4m3);
+    }
+    if (threadIdx.x == 0) *scale = c.scale;
+    if (c.older != 1.f) rescale_block(block, lo * D, c.older, a.e4m3, threadIdx.x, kAppendThreads);
+  }
+}
+
+template <typename T, int D, int V, bool INTER>
+static int launch_append_as(AppendArgs a, int sms, cudaStream_t s) {
+  if (a.cu == nullptr) {
+    append_token_kernel<T, D, V, INTER><<<static_cast<unsigned>(a.tokens), kAppendThreads, 0, s>>>(a);
+    return check_launch("append_token_kernel");
+  }
+  // pages that n tokens of N sequences can touch
+  const int64_t items = std::min(a.tokens, a.tokens / a.page + 2 * static_cast<int64_t>(a.n_seqs));
+  a.heads = std::min(a.hkv, 32);
+  while (a.heads > 1 && items * 2 * ((a.hkv + a.heads - 1) / a.heads) < 6 * sms) a.heads = (a.heads + 1) / 2;
+  const int smem = a.n_freq > 0 ? a.page * (D / 2 + D / 16) * static_cast<int>(sizeof(float2)) : 0;
+  auto kern = append_packed_kernel<T, D, V, INTER>;
+  static std::atomic<bool> allowed[64];
+  int rc = allow_shared(allowed, kern, 128 * (D / 2 + D / 16) * static_cast<int>(sizeof(float2)));
+  if (rc != XDNA_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>((a.hkv + a.heads - 1) / a.heads), 2);
+  kern<<<grid, kAppendThreads, smem, s>>>(a);
+  return check_launch("append_packed_kernel");
+}
+
+template <typename T>
+static int launch_append(const AppendArgs& a, int64_t d, bool interleaved, int sms, cudaStream_t s) {
+  if (interleaved) return d == 64 ? launch_append_as<T, 64, 8, true>(a, sms, s) : launch_append_as<T, 128, 8, true>(a, sms, s);
+  if (a.n_freq % 8 == 0) return d == 64 ? launch_append_as<T, 64, 8, false>(a, sms, s) : launch_append_as<T, 128, 8, false>(a, sms, s);
+  return d == 64 ? launch_append_as<T, 64, 1, false>(a, sms, s) : launch_append_as<T, 128, 1, false>(a, sms, s);
+}
+
+// ---------------------------------------------------------------------------- attention
+struct PagedArgs {
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  const uint8_t *kc, *vc;
+  int64_t kc_sp, vc_sp;
+  const float *ks, *vs;
+  int64_t ks_sp, vs_sp;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens;
+  float scale_log2;
+  int B, T, hkv, group, page_shift, pages, max_pages;
+  int col_groups, cols;  // columns: query heads of a key head times T; of an item 8 * NT of them
+  void* out;             // [B, T, hq, D]
+  int64_t* bases;        // [B + 1]: steps before each sequence, for one (key head, column group)
+  float* part_o;         // [2 * gridDim.x][8 * NT][D]
+  float4* part_ml;       // [2 * gridDim.x][8 * NT]: m, l, m'
+};
+
+constexpr int kPaWarps = 4;
+constexpr int kPaTile = 32;                  // keys of a warp's step
+constexpr int kPaStep = kPaWarps * kPaTile;  // keys of a CTA's step
+constexpr float kPaSlack = 8.f;              // how far (log2) a score may pass the reference before that is raised
+
+template <int D, int NT>
+struct PaShape {
+  static constexpr int kC = D / 64;                            // 16-byte pieces of a lane's key row
+  static constexpr int kVBytes = D / 8;                        // bytes of a lane's value row
+  static constexpr int kKeyBytes = 2 * 2 * kC * 512, kValueBytes = 2 * 4 * kVBytes * 32;
+  static constexpr int kStage = kKeyBytes + kValueBytes;       // D * 64: 8 or 4 KB
+  static constexpr int kCtas = NT == 1 ? 3 : 2;
+  static constexpr int kStages = (NT == 1 ? 16384 : 24576) / kStage;
+  static constexpr int kSmem = kPaWarps * kStages * kStage;
+  static_assert(kSmem >= kPaWarps * 8 * NT * (D + 4) * 4, "the warps' sums lie where the ring was");
+};
+
+__device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
+  return static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), static_cast<int64_t>(a.max_pages) << a.page_shift));
+}
+
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, int bytes) {
+  if (bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+}
+
+// Attention of B sequences with T query tokens each (the last T of the sequence) over the paged cache. Few rows, so its
+// time is the reading of the codes. The work is all steps of 128 keys of all (sequence, key head, 8 NT columns), in that
+// order, and every CTA takes an equal share of it, whatever the lengths are; they are read on the device. A share begins
+// and ends inside an item as it comes; parts of items go to the workspace and are joined by paged_join_kernel.
+// A warp takes 32 of a step's keys: every lane copies what it will read back itself (cp.async, kStages tiles under way),
+// and the products are mma.sync 16 x 8 x 16 with keys, then dimensions, as rows and the query rows as columns:
+// S^T = K Q^T, O^T = V^T P^T. Of K, lane (g, t) takes bytes 64 c + 16 t .. + 15 of keys g and g + 8: each word of it is,
+// as two half pairs, A fragments when the queries' B fragments are read in the same order. Of V, bytes g D / 8 .. of
+// keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, paired by byte permutes, are A fragments of output rows in the order of dimensions
+// g D / 8 + 2 i (row g of product i) and g D / 8 + 2 i + 1 (row g + 8). P^T is S^T's fragment, transposed by movmatrix.
+// Codes are exact in f16, and so are queries of either type after a power of two per row has brought them to about one
+// (bits below 2^-24 of the row's largest apart). The key block's scale goes into the scores. The value block's scale 2^e
+// goes into the exponent of the weights that meet V, 2^(s + e - m'), with a running maximum m' of its own, so that
+// weights of 16 bits are full where they count, whatever the blocks' scales; the softmax's sum has 2^(s - m). Both are
+// raised, and the sums rescaled, only when a score passes them by more than 2^8.
+template <typename T, int D, bool E4M3, int NT>
+__global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_kernel(const PagedArgs a) {
+  using S = PaShape<D, NT>;
+  constexpr unsigned kAll = 0xffffffffu;
+  constexpr int kCols = 8 * NT, kSteps = D / 16;
+  extern __shared__ __align__(16) uint8_t ring_all[];
+  __shared__ float scales[kPaWarps][S::kStages][4];  // key and value scales of a tile's two blocks; below zero: no page
+  __shared__ float sml[kPaWarps][kCols][3];
+  __shared__ int64_t sums[2][kPaWarps], found_base;
+  __shared__ int found_b;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
+  uint8_t* ring = ring_all + warp * (S::kStages * S::kStage);
+  float(*so)[kCols][D + 4] = reinterpret_cast<float(*)[kCols][D + 4]>(ring_all);
+
+  // ---- this CTA's share, and the sequence and step that it begins with
+  auto steps_of = [&](int b) { return b < a.B ? (paged_len(a, b) + kPaStep - 1) / kPaStep : 0; };
+  const int per_b = a.hkv * a.col_groups;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kPaWarps * 32) total += steps_of(b0 + static_cast<int>(threadIdx.x));
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
+  if (lane == 0) sums[0][warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < kPaWarps; ++w) total += sums[0][w];
+  const int64_t work = total * per_b;
+  int64_t at = blockIdx.x * work / gridDim.x;
+  const int64_t end = (blockIdx.x + 1) * work / gridDim.x;
+  const bool tells = blockIdx.x == 0;  // writes down where the sequences begin, for the join
+  if (at >= end && !tells) return;
+  int64_t base = 0;  // steps before sequence b, of one head
+  for (int b0 = 0, round = 1; b0 < a.B; b0 += kPaWarps * 32, round ^= 1) {
+    const int mine = steps_of(b0 + static_cast<int>(threadIdx.x));
+    int64_t upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(kAll, upto, o);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 31) sums[round][warp] = upto;
+    __syncthreads();
+    int64_t all = 0;
+    upto += base;
+    for (int w = 0; w < kPaWarps; ++w) {
+      if (w < warp) upto += sums[round][w];
+      all += sums[round][w];
+    }
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    if (tells && b < a.B) a.bases[b + 1] = upto;
+    if (at < end && at >= (upto - mine) * per_b && at < upto * per_b) found_b = b, found_base = upto - mine;
+    base += all;
+    if (!tells && base * per_b > at) break;
+  }
+  if (tells && threadIdx.x == 0) a.bases[0] = 0;
+  __syncthreads();
+  if (at >= end) return;
+  int b = found_b, len = paged_len(a, b);
+  base = found_base;
+  bool first = true;
+  while (at < end) {
+    while (len == 0 || at >= (base + (len + kPaStep - 1) / kPaStep) * per_b) {
+      base += (len + kPaStep - 1) / kPaStep;
+      len = paged_len(a, ++b);
+    }
+    const int steps = (len + kPaStep - 1) / kPaStep;
+    const int64_t in_b = at - base * per_b;
+    const int hc = static_cast<int>(in_b / steps), s0 = static_cast<int>(in_b % steps);
+    const int s1 = static_cast<int>(min(static_cast<int64_t>(steps), s0 + (end - at)));
+    const int h = hc / a.col_groups, c0 = (hc % a.col_groups) * kCols;
+    const uint8_t *kc = a.kc + ((static_cast<int64_t>(h) << a.page_shift) * D) + 16 * t, *vc = a.vc + ((static_cast<int64_t>(h) << a.page_shift) * D) + S::kVBytes * g;
+    const int32_t* table = a.table + b * a.ld_table;
+
+    int pages[2] = {-1, -1};  // of the two blocks of tile (lane) of 32
+    auto look = [&](int from) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = (s0 + from + lane) * kPaStep + warp * kPaTile + 16 * i;
+        int p = -1;
+        if (s0 + from + lane < s1 && key < len) p = table[key >> a.page_shift];
+        pages[i] = p < a.pages ? p : -1;
+      }
+    };
+    auto fetch = [&](int i, int st) {  // tile i of this warp
+      if (s0 + i < s1) {
+        const int key0 = (s0 + i) * kPaStep + warp * kPaTile;
+        const uint32_t dst = smem_u32(ring + st * S::kStage);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int page = __shfl_sync(kAll, pages[x], i & 31);
+          const int key = key0 + 16 * x, slot = key & ((1 << a.page_shift) - 1);
+          const int left = page < 0 ? 0 : len - key;
+          const uint8_t *kp = kc + max(page, 0) * a.kc_sp + slot * D, *vp = vc + max(page, 0) * a.vc_sp + slot * D;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int c = 0; c < S::kC; ++c)
+              cp_async(dst + ((x * 2 + r) * S::kC + c) * 512 + lane * 16, kp + (8 * r + g) * D + 64 * c, 8 * r + g < left, 16);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = 2 * t + (r & 1) + 8 * (r >> 1);
+            cp_async(dst + S::kKeyBytes + (x * 4 + r) * (S::kVBytes * 32) + lane * S::kVBytes, vp + row * D, row < left, S::kVBytes);
+          }
+          if (lane < 2) {
+            float* to = &scales[warp][st][2 * x + lane];
+            if (left > 0)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)),
+                           "l"(lane == 0 ? a.ks + page * a.ks_sp + h : a.vs + page * a.vs_sp + h)
+                           : "memory");
+            else
+              *to = -1.f;
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    look(0);
+#pragma unroll
+    for (int i = 0; i < S::kStages; ++i) fetch(i, i);
+
+    // the queries, brought to about one by a power of two per column, and what the products are to be multiplied with
+    uint32_t qf[NT][kSteps][2];
+    float by[NT][2];
+    int limit[NT][2];  // keys that columns 2 t, 2 t + 1 see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = c0 + 8 * n + g;
+      Pack<T, 4> raw[kSteps];
+      const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + (col / a.group) * a.q_st + (h * a.group + col % a.group) * a.q_sh + 16 * t;
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) raw[s] = col < a.cols ? load_pack<T, 4>(qp + 64 * (s / 4) + 4 * (s % 4)) : Pack<T, 4>{};
+      float f[4];
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        to_floats<T, 4>(raw[s], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+      }
+      top = max(top, __shfl_xor_sync(kAll, top, 1));
+      top = max(top, __shfl_xor_sync(kAll, top, 2));
+      const int e = top == 0 || top >= kNotFinite ? 0 : max(static_cast<int>(top >> 23) - 127, -126);
+      const float inverse = e == 127 ? 5.877471754e-39f : power_of_two(-e);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        to_floats<T, 4>(raw[s], f);
+        qf[n][s][0] = pack2<__half>(f[0] * inverse, f[1] * inverse);
+        qf[n][s][1] = pack2<__half>(f[2] * inverse, f[3] * inverse);
+      }
+      const float back = fminf(power_of_two(e) * a.scale_log2, 3.4e38f);
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        by[n][e2] = __shfl_sync(kAll, back, (2 * t + e2) * 4);
+        const int c = c0 + 8 * n + 2 * t + e2;
+        limit[n][e2] = c < a.cols ? len - a.T + c / a.group + 1 : 0;
+      }
+    }
+    const int seen_by_all = len - a.T + 1;
+
+    float o[NT][kSteps][4], m[NT][2], mv[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      m[n][0] = m[n][1] = mv[n][0] = mv[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+    }
+    int st = 0;
+    for (int i = 0; s0 + i < s1; ++i, st = st + 1 == S::kStages ? 0 : st + 1) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+      __syncwarp();
+      const uint8_t* mine = ring + st * S::kStage;
+      const int key0 = (s0 + i) * kPaStep + warp * kPaTile;
+      const float4 sc = *reinterpret_cast<const float4*>(scales[warp][st]);  // K, V of block 0, K, V of block 1
+      const float ks[2] = {sc.x, sc.z};
+      float ev[2];  // log2 of the value blocks' scales; NaN stays NaN
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t bits = __float_as_uint(x ? sc.w : sc.y);
+        ev[x] = (bits & 0x7fffffffu) >= kNotFinite ? __uint_as_float(0x7fc00000u) : static_cast<float>(static_cast<int>(bits >> 23 & 0xff) - 127);
+      }
+      // scores: s[n][x][e] is key 16 x + g (+ 8 for e >= 2) of the tile, column 2 t + (e & 1)
+      float s[NT][2][4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][x][0] = s[n][x][1] = s[n][x][2] = s[n][x][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < S::kC; ++c) {
+          const uint4 k0 = *reinterpret_cast<const uint4*>(mine + (x * 2 * S::kC + c) * 512 + lane * 16);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(mine + ((x * 2 + 1) * S::kC + c) * 512 + lane * 16);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t f[4];
+            to_halves<E4M3>(w0[w], f[0], f[2]);
+            to_halves<E4M3>(w1[w], f[1], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<false>(s[n][x], f, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
+          }
+        }
+      }
+      const bool whole = key0 + kPaTile <= seen_by_all && !(ks[0] < 0.f) && !(ks[1] < 0.f);
+      bool raise = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][x][e] = s[n][x][e] * ks[x] * by[n][e & 1];
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (ks[x] < 0.f || key0 + 16 * x + g + 8 * (e >> 1) >= limit[n][e & 1]) s[n][x][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float a0 = fmaxf(s[n][0][e], s[n][0][2 + e]), a1 = fmaxf(s[n][1][e], s[n][1][2 + e]);
+          raise |= fmaxf(a0, a1) > m[n][e] + kPaSlack || fmaxf(a0 + ev[0], a1 + ev[1]) > mv[n][e] + kPaSlack;
+        }
+      }
+      if (__any_sync(kAll, raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float a0 = fmaxf(s[n][0][e], s[n][0][2 + e]), a1 = fmaxf(s[n][1][e], s[n][1][2 + e]);
+            float top = fmaxf(a0, a1), tv = fmaxf(a0 + ev[0], a1 + ev[1]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(kAll, top, x));
+              tv = fmaxf(tv, __shfl_xor_sync(kAll, tv, x));
+            }
+            const float mn = fmaxf(m[n][e], top), vn = fmaxf(mv[n][e], tv);
+            l[n][e] *= mn == -INFINITY ? 1.f : fast_exp2(m[n][e] - mn);
+            f[e] = vn == -INFINITY ? 1.f : fast_exp2(mv[n][e] - vn);
+            m[n][e] = mn;
+            mv[n][e] = vn;
+          }
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) o[n][j][0] *= f[0], o[n][j][1] *= f[1], o[n][j][2] *= f[0], o[n][j][3] *= f[1];
+        }
+      }
+      uint32_t p[NT][2][2];  // B fragments of the weights
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+        const float v0 = mv[n][0] == -INFINITY ? 0.f : mv[n][0], v1 = mv[n][1] == -INFINITY ? 0.f : mv[n][1];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          l[n][0] += fast_exp2(s[n][x][0] - m0) + fast_exp2(s[n][x][2] - m0);
+          l[n][1] += fast_exp2(s[n][x][1] - m1) + fast_exp2(s[n][x][3] - m1);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            // masked weights are zero whatever the block's scale
+            float w0 = fast_exp2(s[n][x][2 * r] + ev[x] - v0), w1 = fast_exp2(s[n][x][2 * r + 1] + ev[x] - v1);
+            if (!whole) {
+              if (s[n][x][2 * r] == -INFINITY) w0 = 0.f;
+              if (s[n][x][2 * r + 1] == -INFINITY) w1 = 0.f;
+            }
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][x][r]) : "r"(pack2<__half>(w0, w1)));
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t v[4][S::kVBytes / 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint8_t* src = mine + S::kKeyBytes + (x * 4 + r) * (S::kVBytes * 32) + lane * S::kVBytes;
+          if constexpr (S::kVBytes == 16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(src);
+            v[r][0] = u.x, v[r][1] = u.y, v[r][2] = u.z, v[r][3] = u.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(src);
+            v[r][0] = u.x, v[r][1] = u.y;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < S::kVBytes / 4; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int sel = half ? 0x7362 : 0x5140;
+            uint32_t f[4];
+            to_halves<E4M3>(__byte_perm(v[0][w], v[1][w], sel), f[0], f[1]);
+            to_halves<E4M3>(__byte_perm(v[2][w], v[3][w], sel), f[2], f[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<false>(o[n][2 * w + half], f, p[n][x][0], p[n][x][1]);
+          }
+        }
+      }
+      if (((i + S::kStages) & 31) == 0) look(i + S::kStages);
+      __syncwarp();
+      fetch(i + S::kStages, st);  // into the stage just read
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    // ---- the warps' sums together
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[n][e] += __shfl_xor_sync(kAll, l[n][e], 4);
+        l[n][e] += __shfl_xor_sync(kAll, l[n][e], 8);
+        l[n][e] += __shfl_xor_sync(kAll, l[n][e], 16);
+        const int col = 8 * n + 2 * t + e;
+        if (g == 0) sml[warp][col][0] = m[n][e], sml[warp][col][1] = l[n][e], sml[warp][col][2] = mv[n][e];
+        float* dst = &so[warp][col][S::kVBytes * g];
+#pragma unroll
+        for (int j = 0; j < kSteps; j += 2)
+          *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
+      }
+    }
+    __syncthreads();
+    const bool alone = s0 == 0 && s1 == steps;
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
+    const int cols = min(kCols, a.cols - c0);
+    for (int i = threadIdx.x; i < cols * (D / 4); i += kPaWarps * 32) {
+      const int c = i / (D / 4), d = (i % (D / 4)) * 4;
+      float mm = -INFINITY, mmv = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPaWarps; ++w) mm = fmaxf(mm, sml[w][c][0]), mmv = fmaxf(mmv, sml[w][c][2]);
+      const float m0 = mm == -INFINITY ? 0.f : mm, v0 = mmv == -INFINITY ? 0.f : mmv;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kPaWarps; ++w) {
+        ll = fmaf(fast_exp2(sml[w][c][0] - m0), sml[w][c][1], ll);
+        const float f = fast_exp2(sml[w][c][2] - v0);
+        const float4 x = *reinterpret_cast<const float4*>(&so[w][c][d]);
+        acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+      }
+      if (alone) {
+        const float inv = ll > 0.f || __isnanf(ll) ? fast_exp2(v0 - m0) / ll : 0.f;
+        const int col = c0 + c;
+        T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(fit<T>(acc.x * inv), fit<T>(acc.y * inv)), pack2<T>(fit<T>(acc.z * inv), fit<T>(acc.w * inv)));
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (slot * kCols + c) * D + d) = acc;
+        if (d == 0) a.part_ml[slot * kCols + c] = make_float4(mm, ll, mmv, 0.f);
+      }
+    }
+    first = false;
+    at += s1 - s0;
+    __syncthreads();
+  }
+}
+
+// One block per (sequence, key head, column group): nothing where one CTA had all of it, zeros where there are no keys,
+// else the parts of the CTAs that shared it, in their order.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int ctas) {
+  constexpr int kCols = 8 * NT;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int per_b = a.hkv * a.col_groups;
+  const int b = static_cast<int>(blockIdx.x) / per_b, hc = static_cast<int>(blockIdx.x) % per_b;
+  const int h = hc / a.col_groups, c0 = (hc % a.col_groups) * kCols, cols = min(kCols, a.cols - c0);
+  const int64_t work = a.bases[a.B] * per_b, base = a.bases[b], steps = a.bases[b + 1] - base;
+  int64_t i0 = 0, i1 = -1;  // the CTAs
+  const int64_t s = base * per_b + hc * steps, e = s + steps;
+  if (steps > 0) {
+    i0 = ((s + 1) * ctas - 1) / work;
+    i1 = (e * ctas - 1) / work;
+    if (i0 == i1) return;
+  }
+  for (int i = threadIdx.x; i < cols * (D / 4); i += 128) {
+    const int c = i / (D / 4), d = (i % (D / 4)) * 4;
+    float mm = -INFINITY, mmv = -INFINITY, ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // a CTA's first item has its first slot: item s is CTA x's first one where x starts in it
+    auto slot = [&](int64_t x) { return 2 * x + (x * work / ctas >= s ? 0 : 1); };
+    for (int64_t x = i0; x <= i1; ++x) {
+      if (x * work / ctas == (x + 1) * work / ctas) continue;
+      const float4 ml = a.part_ml[slot(x) * kCols + c];
+      mm = fmaxf(mm, ml.x), mmv = fmaxf(mmv, ml.z);
+    }
+    const float m0 = mm == -INFINITY ? 0.f : mm, v0 = mmv == -INFINITY ? 0.f : mmv;
+    for (int64_t x = i0; x <= i1; ++x) {
+      if (x * work / ctas == (x + 1) * work / ctas) continue;
+      const float4 ml = a.part_ml[slot(x) * kCols + c];
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (slot(x) * kCols + c) * D + d);
+      ll = fmaf(fast_exp2(ml.x - m0), ml.y, ll);
+      const float f = fast_exp2(ml.z - v0);
+      acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y), acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
+    }
+    const float inv = ll > 0.f || __isnanf(ll) ? fast_exp2(v0 - m0) / ll : 0.f;
+    const int col = c0 + c;
+    T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(fit<T>(acc.x * inv), fit<T>(acc.y * inv)), pack2<T>(fit<T>(acc.z * inv), fit<T>(acc.w * inv)));
+  }
+}
+
+// CTAs of a call, and where its workspace's parts lie.
+struct PagedPlan {
+  int nt, col_groups;
+  int64_t ctas, ml_at, o_at, bytes;
+  PagedPlan(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys, int sms) {
+    const int64_t cols = hq / hkv * T;
+    nt = cols <= 8 ? 1 : 2;
+    col_groups = static_cast<int>((cols + 8 * nt - 1) / (8 * nt));
+    const int64_t most = B * hkv * col_groups * ((most_keys + kPaStep - 1) / kPaStep);
+    ctas = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sms) * (nt == 1 ? 3 : 2), most));
+    ml_at = ((B + 1) * 8 + 255) / 256 * 256;
+    o_at = ml_at + 2 * ctas * 8 * nt * 16;
+    bytes = o_at + 2 * ctas * 8 * nt * d * 4;
+  }
+};
+
+template <typename T, int D, bool E4M3, int NT>
+static int launch_paged_as(const PagedArgs& a, int ctas, cudaStream_t s) {
+  using S = PaShape<D, NT>;
+  auto kern = paged_kernel<T, D, E4M3, NT>;
+  static std::atomic<bool> allowed[64];
+  int rc = allow_shared(allowed, kern, S::kSmem);
+  if (rc != XDNA_OK) return rc;
+  kern<<<static_cast<unsigned>(ctas), kPaWarps * 32, S::kSmem, s>>>(a);
+  if ((rc = check_launch("paged_kernel")) != XDNA_OK) return rc;
+  const unsigned items = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.hkv * a.col_groups);
+  return launch_early("paged_join_kernel", paged_join_kernel<T, D, NT>, dim3(items), 128, 0, s, a, ctas);
+}
+
+template <typename T, int D>
+static int launch_paged(const PagedArgs& a, bool e4m3, int nt, int ctas, cudaStream_t s) {
+  if (e4m3) return nt == 1 ? launch_paged_as<T, D, true, 1>(a, ctas, s) : launch_paged_as<T, D, true, 2>(a, ctas, s);
+  return nt == 1 ? launch_paged_as<T, D, false, 1>(a, ctas, s) : launch_paged_as<T, D, false, 2>(a, ctas, s);
+}
+
+// ---------------------------------------------------------------------------- host
+static int check_cache(const char* what, int64_t pages, int64_t hkv, int64_t page, int64_t d, int format, int64_t max_pages) {
+  if (d != 64 && d != 128) return fail(XDNA_ERR_UNSUPPORTED, "%s: head dimension %lld (64 or 128)", what, (long long)d);
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(XDNA_ERR_UNSUPPORTED, "%s: pages of %lld tokens (16, 32, 64 or 128)", what, (long long)page);
+  XDNA_CHECK_ARG(format == XDNA_I8 || format == XDNA_E4M3, "%s: int8 or e4m3 codes", what);
+  XDNA_CHECK_ARG(pages >= 0 && pages < (1ll << 31) && hkv >= 1 && hkv < (1 << 16) && max_pages >= 0 && max_pages < (1ll << 30) / page,
+                 "%s: bad sizes", what);
+  return XDNA_OK;
+}
+static bool cache_ok(const void* codes, int64_t sp, const void* scales, int64_t ssp) {
+  return codes && scales && aligned16(codes) && sp >= 0 && sp % 16 == 0 && ssp >= 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
+}
+static bool rows_ok(const void* p, int64_t st, int64_t sh) { return p && aligned16(p) && st > 0 && sh > 0 && st % 8 == 0 && sh % 8 == 0; }
+static int shift_of(int64_t page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+}  // namespace xdna
+
+using namespace xdna;
+
+extern "C" {
+
+int xdna_cache_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
+                      int64_t tokens, int64_t hkv, int64_t d, void* k_codes, int64_t kc_sp, void* v_codes, int64_t vc_sp,
+                      int format, float* k_scales, int64_t ks_sp, float* v_scales, int64_t vs_sp, int64_t pages, int64_t page,
+                      const int32_t* table, int64_t ld_table, int64_t max_pages, const int32_t* starts,
+                      const int32_t* cu_seqlens, int64_t n_seqs, const float* inv_freq, int64_t n_freq, float factor,
+                      int interleaved, const void* k_norm, int k_norm_dtype, int64_t k_norm_sh, float eps, const void* q,
+                      int64_t q_st, int64_t q_sh, int64_t hq, const void* q_norm, int q_norm_dtype, int64_t q_norm_sh,
+                      void* q_out, void* stream) {
+  int rc = check_cache("cache_append", pages, hkv, page, d, format, max_pages);
+  if (rc != XDNA_OK) return rc;
+  XDNA_CHECK_ARG(dtype == XDNA_BF16 || dtype == XDNA_F16, "cache_append: bf16 or f16");
+  XDNA_CHECK_ARG(tokens >= 0 && tokens < (1ll << 31) && n_seqs >= 0 && n_seqs < (1 << 24) && hq >= 0 && hq < (1 << 16) &&
+                     (cu_seqlens || n_seqs == tokens),
+                 "cache_append: bad sizes");
+  XDNA_CHECK_ARG(n_freq >= 0 && 2 * n_freq <= d, "cache_append: %lld frequencies for heads of %lld", (long long)n_freq, (long long)d);
+  XDNA_CHECK_ARG((!k_norm || (is_float_dtype(k_norm_dtype) && aligned16(k_norm) && k_norm_sh >= 0 && k_norm_sh % 8 == 0)) &&
+                     (!q_norm || (is_float_dtype(q_norm_dtype) && aligned16(q_norm) && q_norm_sh >= 0 && q_norm_sh % 8 == 0)),
+                 "cache_append: the norms' weights are f32, bf16 or f16, aligned");
+  int sms = 0;
+  if ((rc = check_device(&sms)) != XDNA_OK) return rc;
+  if (tokens == 0) return XDNA_OK;
+  XDNA_CHECK_ARG(rows_ok(k, k_st, k_sh) && rows_ok(v, v_st, v_sh) && (!q || (rows_ok(q, q_st, q_sh) && q_out && aligned16(q_out) && hq >= 1)) &&
+                     cache_ok(k_codes, kc_sp, k_scales, ks_sp) && cache_ok(v_codes, vc_sp, v_scales, vs_sp) &&
+                     (table || max_pages == 0) && (starts || n_seqs == 0) && (n_freq == 0 || inv_freq),
+                 "cache_append: null pointer, unaligned rows or bad strides");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (q && cu_seqlens) {  // the queries of packed sequences
+    RotaryArgs r{};
+    r.x = q, r.x_st = q_st, r.x_sh = q_sh, r.out = q_out;
+    r.starts = starts, r.cu = cu_seqlens, r.n_seqs = static_cast<int>(n_seqs);
+    r.inv_freq = inv_freq, r.n_freq = static_cast<int>(n_freq), r.factor = factor;
+    r.norm = q_norm, r.norm_dtype = q_norm_dtype, r.norm_sh = q_norm_sh, r.eps = eps;
+    r.T = tokens, r.H = static_cast<int>(hq), r.D = static_cast<int>(d);
+    if ((rc = launch_rotary(r, dtype, interleaved != 0, sms, s)) != XDNA_OK) return rc;
+    q = nullptr;
+  }
+  if (n_seqs == 0) return XDNA_OK;
+  AppendArgs a{};
+  a.k = k, a.v = v, a.q = q;
+  a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh, a.q_st = q_st, a.q_sh = q_sh;
+  a.kc = static_cast<uint8_t*>(k_codes), a.vc = static_cast<uint8_t*>(v_codes), a.kc_sp = kc_sp, a.vc_sp = vc_sp;
+  a.ks = k_scales, a.vs = v_scales, a.ks_sp = ks_sp, a.vs_sp = vs_sp;
+  a.table = table, a.ld_table = ld_table, a.starts = starts, a.cu = cu_seqlens;
+  a.inv_freq = inv_freq, a.n_freq = static_cast<int>(n_freq), a.factor = factor, a.eps = eps;
+  a.k_norm = k_norm, a.k_norm_dtype = k_norm_dtype, a.k_norm_sh = k_norm_sh;
+  a.q_norm = q_norm, a.q_norm_dtype = q_norm_dtype, a.q_norm_sh = q_norm_sh;
+  a.q_out = q_out, a.tokens = tokens, a.n_seqs = static_cast<int>(n_seqs);
+  a.hq = static_cast<int>(hq), a.hkv = static_cast<int>(hkv), a.page = static_cast<int>(page), a.page_shift = shift_of(page);
+  a.pages = static_cast<int>(pages), a.max_pages = static_cast<int>(max_pages), a.e4m3 = format == XDNA_E4M3;
+  return dtype == XDNA_BF16 ? launch_append<__nv_bfloat16>(a, d, interleaved != 0, sms, s)
+                            : launch_append<__half>(a, d, interleaved != 0, sms, s);
+}
+
+size_t xdna_paged_attention_workspace(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys) {
+  int sms = 0;
+  if (B < 1 || T < 1 || hkv < 1 || hq < hkv || d < 1 || most_keys < 0 || check_device(&sms) != XDNA_OK) return 0;
+  return static_cast<size_t>(PagedPlan(B, T, hq, hkv, d, most_keys, sms).bytes);
+}
+
+int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, int64_t B, int64_t T, int64_t hq,
+                         int64_t hkv, int64_t d, const void* k_codes, int64_t kc_sp, const void* v_codes, int64_t vc_sp,
+                         int format, const float* k_scales, int64_t ks_sp, const float* v_scales, int64_t vs_sp,
+                         int64_t pages, int64_t page, const int32_t* table, int64_t ld_table, int64_t max_pages,
+                         const int32_t* lens, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_cache("paged_attention", pages, hkv, page, d, format, max_pages);
+  if (rc != XDNA_OK) return rc;
+  XDNA_CHECK_ARG(hq >= 1 && hq % hkv == 0 && hq / hkv <= 128, "paged_attention: %lld query heads over %lld key heads", (long long)hq, (long long)hkv);
+  XDNA_CHECK_ARG(dtype == XDNA_BF16 || dtype == XDNA_F16, "paged_attention: bf16 or f16");
+  XDNA_CHECK_ARG(scale > 0.f && scale * kLog2E < INFINITY, "paged_attention: the scale must be positive and at most 2.3e38");
+  XDNA_CHECK_ARG(B >= 0 && T >= 0 && B < (1ll << 24) && T < (1 << 24) && B * T < (1ll << 31) / hq, "paged_attention: bad sizes");
+  int sms = 0;
+  if ((rc = check_device(&sms)) != XDNA_OK) return rc;
+  if (B == 0 || T == 0) return XDNA_OK;
+  XDNA_CHECK_ARG(q && aligned16(q) && q_sb > 0 && q_st > 0 && q_sh > 0 && q_sb % 8 == 0 && q_st % 8 == 0 && q_sh % 8 == 0 && out && aligned16(out) && lens &&
+                     (table || max_pages == 0) && cache_ok(k_codes, kc_sp, k_scales, ks_sp) && cache_ok(v_codes, vc_sp, v_scales, vs_sp),
+                 "paged_attention: null pointer, unaligned rows or bad strides");
+  const PagedPlan plan(B, T, hq, hkv, d, max_pages * page, sms);
+  XDNA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_bytes >= static_cast<size_t>(plan.bytes),
+                 "paged_attention: workspace too small or unaligned");
+  PagedArgs a{};
+  a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
+  a.kc = static_cast<const uint8_t*>(k_codes), a.vc = static_cast<const uint8_t*>(v_codes), a.kc_sp = kc_sp, a.vc_sp = vc_sp;
+  a.ks = k_scales, a.vs = v_scales, a.ks_sp = ks_sp, a.vs_sp = vs_sp;
+  a.table = table, a.ld_table = ld_table, a.lens = lens, a.scale_log2 = scale * kLog2E;
+  a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.hkv = static_cast<int>(hkv), a.group = static_cast<int>(hq / hkv);
+  a.page_shift = shift_of(page), a.pages = static_cast<int>(pages), a.max_pages = static_cast<int>(max_pages);
+  a.col_groups = plan.col_groups, a.cols = static_cast<int>(a.group * T);
+  a.out = out;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.bases = reinterpret_cast<int64_t*>(ws);
+  a.part_ml = reinterpret_cast<float4*>(ws + plan.ml_at);
+  a.part_o = reinterpret_cast<float*>(ws + plan.o_at);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int ctas = static_cast<int>(plan.ctas);
+  const bool e4m3 = format == XDNA_E4M3;
+  if (dtype == XDNA_BF16)
+    return d == 64 ? launch_paged<__nv_bfloat16, 64>(a, e4m3, plan.nt, ctas, s) : launch_paged<__nv_bfloat16, 128>(a, e4m3, plan.nt, ctas, s);
+  return d == 64 ? launch_paged<__half, 64>(a, e4m3, plan.nt, ctas, s) : launch_paged<__half, 128>(a, e4m3, plan.nt, ctas, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,137 @@
+// One head of one token, spread over the lanes of a part of a warp, with its norm and its rotation.
+//
+//   u = x / sqrt(mean of x^2 over the head + eps) * w      (w: the norm's weights; without them u = x)
+//   pairs p = 0 .. R / 2 - 1 of u's first R entries, (p, p + R / 2) or interleaved (2 p, 2 p + 1), turned by
+//   the angle position * inv_freq[p]:   (a cos - b sin, b cos + a sin) * factor;   the entries from R on stay.
+//
+// A lane has V first and V second entries of pairs (of the entries past R: 2 V that follow one another), so that no
+// value crosses lanes; with interleaved pairs these are 2 V neighbouring entries.
+#pragma once
+
+#include "values.cuh"
+
+namespace xdna {
+
+// N values of T as they are; loads and stores take addresses aligned to the smaller of N * sizeof(T) and 16 bytes.
+template <typename T, int N>
+struct Pack {
+  static constexpr int kBytes = N * static_cast<int>(sizeof(T));
+  uint32_t w[kBytes >= 4 ? kBytes / 4 : 1];
+};
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  Pack<T, N> x;
+  if constexpr (Pack<T, N>::kBytes >= 16) {
+#pragma unroll
+    for (int i = 0; i < Pack<T, N>::kBytes / 16; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+      x.w[4 * i] = u.x, x.w[4 * i + 1] = u.y, x.w[4 * i + 2] = u.z, x.w[4 * i + 3] = u.w;
+    }
+  } else if constexpr (Pack<T, N>::kBytes == 8) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    x.w[0] = u.x, x.w[1] = u.y;
+  } else if constexpr (Pack<T, N>::kBytes == 4) {
+    x.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    x.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  }
+  return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& x) {
+  if constexpr (Pack<T, N>::kBytes >= 16) {
+#pragma unroll
+    for (int i = 0; i < Pack<T, N>::kBytes / 16; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(x.w[4 * i], x.w[4 * i + 1], x.w[4 * i + 2], x.w[4 * i + 3]);
+  } else if constexpr (Pack<T, N>::kBytes == 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(x.w[0], x.w[1]);
+  } else if constexpr (Pack<T, N>::kBytes == 4) {
+    *reinterpret_cast<uint32_t*>(p) = x.w[0];
+  } else {
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(x.w[0]);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void to_floats(const Pack<T, N>& u, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __uint_as_float(u.w[i]);
+    } else if constexpr (__is_same(T, __half)) {
+      const uint16_t h = static_cast<uint16_t>(u.w[i / 2] >> (16 * (i & 1)));
+      x[i] = __half2float(*reinterpret_cast<const __half*>(&h));
+    } else {
+      x[i] = __uint_as_float(i & 1 ? u.w[i / 2] & 0xffff0000u : u.w[i / 2] << 16);
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> from_floats(const float* x) {
+  Pack<T, N> u;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) u.w[i] = __float_as_uint(x[i]);
+  } else if constexpr (N == 1) {
+    u.w[0] = pack2<T>(x[0], 0.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) u.w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+  }
+  return u;
+}
+
+// N weights from place `at` on as floats, of any of the three types.
+template <int N>
+__device__ __forceinline__ void load_weights(const void* w, int dtype, int64_t at, float* x) {
+  if (dtype == XDNA_F32)
+    to_floats<float, N>(load_pack<float, N>(static_cast<const float*>(w) + at), x);
+  else if (dtype == XDNA_BF16)
+    to_floats<__nv_bfloat16, N>(load_pack<__nv_bfloat16, N>(static_cast<const __nv_bfloat16*>(w) + at), x);
+  else
+    to_floats<__half, N>(load_pack<__half, N>(static_cast<const __half*>(w) + at), x);
+}
+
+// cos and sin of position * inv_freq, times factor. The product is taken in turns and in 64 bits, and only its distance
+// from a whole turn is rounded to 32 (2^-26 of a turn, 9.4e-8 in the angle), so far positions lose nothing.
+__device__ __forceinline__ float2 turn_of(int64_t position, float inv_freq, float factor) {
+  const double turns = static_cast<double>(position) * (static_cast<double>(inv_freq) * 0.15915494309189533577);
+  float s, c;
+  sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+  return make_float2(c * factor, s * factor);
+}
+
+// Where a lane's unit j of a head lies and which of its pairs turn: V entries from lo and V from hi on, pairs
+// V j .. V j + turning - 1. n_freq = R / 2, a multiple of V where pairs are not interleaved.
+struct UnitAt {
+  int lo, hi, turning;
+};
+template <int V, bool INTER>
+__device__ __forceinline__ UnitAt unit_at(int j, int n_freq) {
+  const int turning = min(max(n_freq - V * j, 0), V);
+  if (!INTER && turning > 0) return {V * j, V * j + n_freq, V};
+  return {2 * V * j, 2 * V * j + V, turning};
+}
+
+// x: the unit's 2 V values, first those of lo, then those of hi.
+template <int V, bool INTER>
+__device__ __forceinline__ void turn_unit(float (&x)[2 * V], const float2 (&cs)[V], int turning) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float &a = x[INTER ? 2 * i : i], &b = x[INTER ? 2 * i + 1 : i + V];
+    if (i < turning) {
+      const float t = a * cs[i].x - b * cs[i].y;
+      b = b * cs[i].x + a * cs[i].y;
+      a = t;
+    }
+  }
+}
+
+// The sum over LANES neighbouring lanes, on all of them.
+template <int LANES>
+__device__ __forceinline__ float sum_of_lanes(float x) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+}  // namespace xdna

@@ -77,4 +77,17 @@ static int launch_early(const char* what, void (*kern)(Params...), dim3 grid, in
   return check_launch(what);
 }
 
+// Lets a kernel have that much dynamic shared memory on the current device; done: per device, whether it may already
+// (setting it twice from two threads is harmless).
+template <typename... Params>
+static int allow_shared(std::atomic<bool> (&done)[64], void (*kern)(Params...), int bytes) {
+  int dev = 0;
+  XDNA_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+    XDNA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+  }
+  return XDNA_OK;
+}
+
 }  // namespace xdna

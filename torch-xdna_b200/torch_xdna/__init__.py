@@ -9,7 +9,8 @@ xdna::linear_cat, xdna::linear_i8), 3x3 stride-1 convs run as an int8 implicit G
 requantise and ReLU in the epilogue (xdna::conv3x3), and a Qwen3-0.6B-shaped stack with its head
 runs as xdna::qwen3_stack. Integer results are bit-identical to the reference's CPU route.
 For generation there are packed_attention, shared_prefix_attention, linear_w4 (w4_pack) and
-process_logits (see generate.py). There is no CPU fallback: without a B200 the backend raises with the reason.
+process_logits (see generate.py), and for what a decoder layer does around its products rotary,
+add_norm, cache_append and paged_attention (see layer.py). There is no CPU fallback: without a B200 the backend raises with the reason.
 """
 
 import json
@@ -18,12 +19,14 @@ from . import kernels, ops  # noqa: F401  (registers the xdna:: ops)
 from .backend import offload_gemms, xdna_backend
 from .config import Config, set_config
 from .generate import linear_w4, packed_attention, process_logits, shared_prefix_attention, w4_pack
+from .layer import PagedCache, add_norm, cache_append, paged_attention, paged_cache, rotary, rotary_frequencies
 from .kernels import XdnaError, XdnaUnavailable
 from .runtime import XdnaResultMismatch, stats
 
 __all__ = ["Config", "set_config", "xdna_backend", "offload_gemms", "compile", "stats", "report",
            "npu_available", "gpu_available", "packed_attention", "shared_prefix_attention", "w4_pack", "linear_w4",
-           "process_logits", "XdnaError", "XdnaUnavailable", "XdnaResultMismatch"]
+           "process_logits", "rotary_frequencies", "rotary", "add_norm", "PagedCache", "paged_cache", "cache_append",
+           "paged_attention", "XdnaError", "XdnaUnavailable", "XdnaResultMismatch"]
 __version__ = "0.1.0+b200"
 
 

@@ -20,7 +20,7 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libxdna_b200.so"
 ABI_VERSION = 1
 
 # element types (XDNA_F32 ...)
-F32, BF16, F16, I32, I8, U8 = 0, 1, 2, 3, 4, 5
+F32, BF16, F16, I32, I8, U8, E4M3 = 0, 1, 2, 3, 4, 5, 6
 DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: I32, torch.int8: I8,
                torch.uint8: U8}
 # conv3x3 modes
@@ -97,6 +97,16 @@ def _load():
         "xdna_linear_w4": ([P, I, I64, I64, I64, P, P, I, I, I64, P, I, P, I64, P], I),
         "xdna_process_logits": ([P, I, I64, I64, I64, P, I, I64, I64, P, P, P, P, P, P, I64, P, I64, P, I64, P], I),
         "xdna_w4_pack": ([P, I, I64, I64, I64, I, P, P, I, P], I),
+        "xdna_rotary": ([P, I, I64, I64, I64, I64, I64, P, I, P, I64, ctypes.c_float, I, P, I, I64, ctypes.c_float, P,
+                         P], I),
+        "xdna_add_norm": ([P, I, I64, P, I, I64, I64, I64, P, I, P, I, P, I, I64, ctypes.c_float, ctypes.c_float, P, P,
+                           P], I),
+        "xdna_cache_append": ([P, I64, I64, P, I64, I64, I, I64, I64, I64, P, I64, P, I64, I, P, I64, P, I64, I64, I64,
+                               P, I64, I64, P, P, I64, P, I64, ctypes.c_float, I, P, I, I64, ctypes.c_float, P, I64,
+                               I64, I64, P, I, I64, P, P], I),
+        "xdna_paged_attention_workspace": ([I64, I64, I64, I64, I64, I64], ctypes.c_size_t),
+        "xdna_paged_attention": ([P, I64, I64, I64, I, I64, I64, I64, I64, I64, P, I64, P, I64, I, P, I64, P, I64, I64,
+                                  I64, P, I64, I64, P, ctypes.c_float, P, P, ctypes.c_size_t, P], I),
         "xdna_attention": ([P, P, I64, P, I64, I64, I, P, P, I, P], I),
         "xdna_qwen3_stack_workspace": ([I64, I64], ctypes.c_size_t),
         "xdna_qwen3_stack": ([P, I, P, P, I64, P, I, P, P, ctypes.c_float, P, I64, I64, I, P, P, I, P, I, I64, P,

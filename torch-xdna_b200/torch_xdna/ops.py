@@ -8,14 +8,15 @@ conv3x3_int8 as one op, because on the B200 those three steps are kernels of our
 graph ops for the CPU compiler to fuse; xdna::conv3x3_chain, the same for a conv inside a chain of
 convs whose activations between them stay int8 codes; and xdna::conv_int8, the same arithmetic for the
 1x1 and stride-2 convs the reference has no kernel for (offloaded with Config(conv_ext=True)).
-The ops at the end are the generation operators (generate.py), which the reference does not have.
+The ops at the end are the generation operators (generate.py) and those of a decoder layer around its products (layer.py),
+which the reference does not have.
 """
 
 from typing import Optional
 
 import torch
 
-from . import conv, generate, runtime, stack
+from . import conv, generate, kernels, layer, runtime, stack
 
 _configs = []  # cfg_id -> Config; op arguments must be plain values (R:torch_xdna/ops.py:14-22)
 
@@ -207,3 +208,68 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 def _(logits, tokens=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None, bias=None,
       mask=None):
     return logits.new_empty(logits.shape)
+
+
+# ------------------------------------------------------------------ a decoder layer around its products (layer.py)
+@torch.library.custom_op("xdna::rotary", mutates_args=())
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, factor: float = 1.0,
+           interleaved: bool = False, norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """Heads turned to their tokens' places (layer.rotary)."""
+    with torch.no_grad():  # below autograd, whoever called
+        return layer.rotary(x, positions, inv_freq, factor, interleaved, norm, eps)
+
+
+@rotary.register_fake
+def _(x, positions, inv_freq, factor=1.0, interleaved=False, norm=None, eps=1e-6):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op("xdna::add_norm", mutates_args=())
+def add_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: Optional[torch.Tensor] = None,
+             gate: Optional[torch.Tensor] = None, scale: float = 1.0,
+             eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """A block's result into the residual stream, and its norm (layer.add_norm)."""
+    with torch.no_grad():  # below autograd, whoever called
+        return layer.add_norm(x, y, weight, post, gate, scale, eps)
+
+
+@add_norm.register_fake
+def _(x, y, weight, post=None, gate=None, scale=1.0, eps=1e-6):
+    return x.new_empty(x.shape), y.new_empty(y.shape)
+
+
+@torch.library.custom_op("xdna::cache_append", mutates_args=("k_cache", "v_cache", "k_scales", "v_scales"))
+def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                 v_scales: torch.Tensor, table: torch.Tensor, starts: torch.Tensor,
+                 cu_seqlens: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                 factor: float = 1.0, interleaved: bool = False, k_norm: Optional[torch.Tensor] = None,
+                 q: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6) -> torch.Tensor:
+    """Keys and values into a paged cache (layer.cache_append); without q an empty tensor."""
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (k_norm is not None and k_norm.requires_grad)):
+        raise kernels.XdnaError("cache_append", generate.ERR_INVALID, "a cache keeps no gradients: keys and values that "
+                                "require grad are stored under torch.no_grad()")
+    with torch.no_grad():  # below autograd, whoever called
+        out = layer.cache_append(k, v, k_cache, v_cache, k_scales, v_scales, table, starts, cu_seqlens, inv_freq, factor,
+                                 interleaved, k_norm, q, q_norm, eps)
+    return k.new_empty(0) if out is None else out
+
+
+@cache_append.register_fake
+def _(k, v, k_cache, v_cache, k_scales, v_scales, table, starts, cu_seqlens=None, inv_freq=None, factor=1.0,
+      interleaved=False, k_norm=None, q=None, q_norm=None, eps=1e-6):
+    return k.new_empty(0) if q is None else q.new_empty(q.shape)
+
+
+@torch.library.custom_op("xdna::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                    v_scales: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                    scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of the newest tokens over a paged cache (layer.paged_attention)."""
+    with torch.no_grad():  # below autograd, whoever called
+        return layer.paged_attention(q, k_cache, v_cache, k_scales, v_scales, table, lens, scale)
+
+
+@paged_attention.register_fake
+def _(q, k_cache, v_cache, k_scales, v_scales, table, lens, scale=None):
+    return q.new_empty(q.shape)
