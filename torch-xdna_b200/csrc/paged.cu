@@ -433,200 +433,276 @@ static int launch_append(const AppendArgs& a, int64_t d, bool interleaved, int s
 struct PagedArgs {
   const void* q;
   int64_t q_sb, q_st, q_sh;
-  const uint8_t *kc, *vc;
-  int64_t kc_sp, vc_sp;
   const float *ks, *vs;
   int64_t ks_sp, vs_sp;
   const int32_t* table;
   int64_t ld_table;
   const int32_t* lens;
   float scale_log2;
+  int* err;
   int B, T, hkv, group, page_shift, pages, max_pages;
   int col_groups, cols;  // columns: query heads of a key head times T; of an item 8 * NT of them
   void* out;             // [B, T, hq, D]
-  int64_t* bases;        // [B + 1]: steps before each sequence, for one (key head, column group)
-  float* part_o;         // [2 * gridDim.x][8 * NT][D]
-  float4* part_ml;       // [2 * gridDim.x][8 * NT]: m, l, m'
+  int4* shared;          // per item: the first and the last warp that has a part of it, the first one's slot
+  float* part_o;         // [2 * warps][8 * NT][D]
+  float4* part_ml;       // [2 * warps][8 * NT]: m, l, m'
 };
 
 constexpr int kPaWarps = 4;
-constexpr int kPaTile = 32;                  // keys of a warp's step
-constexpr int kPaStep = kPaWarps * kPaTile;  // keys of a CTA's step
-constexpr float kPaSlack = 8.f;              // how far (log2) a score may pass the reference before that is raised
+constexpr int kPaTile = 32;      // keys of a warp's step
+constexpr int kPaSite = 70;      // of its waits, in the device error word
+constexpr int kPaShort = 1024;   // keys that the table can hold, up to which a share is of a warp
+constexpr float kPaSlack = 8.f;  // how far (log2) a score may pass the reference before that is raised
 
 template <int D, int NT>
 struct PaShape {
-  static constexpr int kC = D / 64;                            // 16-byte pieces of a lane's key row
-  static constexpr int kVBytes = D / 8;                        // bytes of a lane's value row
-  static constexpr int kKeyBytes = 2 * 2 * kC * 512, kValueBytes = 2 * 4 * kVBytes * 32;
-  static constexpr int kStage = kKeyBytes + kValueBytes;       // D * 64: 8 or 4 KB
+  static constexpr int kC = D / 64;                       // 16-byte pieces of a lane's key row
+  static constexpr int kVBytes = D / 8;                   // bytes of a lane's value row
+  static constexpr int kHalf = kPaTile * D;               // a tile's keys, and as much of values
   static constexpr int kCtas = NT == 1 ? 3 : 2;
-  static constexpr int kStages = (NT == 1 ? 16384 : 24576) / kStage;
-  static constexpr int kSmem = kPaWarps * kStages * kStage;
-  static_assert(kSmem >= kPaWarps * 8 * NT * (D + 4) * 4, "the warps' sums lie where the ring was");
+  static constexpr int kStages = (NT == 1 ? 16384 : 24576) / (2 * kHalf);
+  static constexpr int kRing = kPaWarps * kStages * 2 * kHalf, kSmem = kRing + 1024;  // aligned to 1024
+  static_assert(kRing >= kPaWarps * 8 * NT * (D + 4) * 4, "the warps' sums lie where the ring was");
+  // Tiles lie in shared memory row by row, swizzled by TMA: 16-byte piece p of row r is at p ^ turn(r). So that no load of
+  // a warp meets itself in a bank, row g of a fragment is key row(g) of its block, and lane group g takes part(g) of a
+  // value row.
+  static __device__ __forceinline__ constexpr int turn(int r) { return D == 128 ? r & 7 : (r >> 1) & 3; }
+  static __device__ __forceinline__ constexpr int row(int g) { return D == 128 ? (g & 1) << 2 | g >> 1 : g ^ g >> 1; }
+  static __device__ __forceinline__ constexpr int part(int g) { return D == 128 ? (g & 1) << 2 | g >> 1 : (g & 1) | (g & 2) << 1 | (g & 4) >> 1; }
 };
 
 __device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
   return static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), static_cast<int64_t>(a.max_pages) << a.page_shift));
 }
 
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool ok, int bytes) {
-  if (bytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+// All units (tiles, or steps of one tile for each of a CTA's warps) in order, shared out evenly: the first `more` shares
+// have one more than the others.
+struct Shares {
+  int64_t work, each, more;
+  __device__ __forceinline__ Shares(int64_t work, uint32_t shares) : work(work) {
+    each = work >> 31 ? work / shares : static_cast<uint32_t>(work) / shares;
+    more = work - each * shares;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ int owner(int64_t unit) const {  // the share that has it
+    const int64_t cut = more * (each + 1), from = unit < cut ? unit : unit - cut, by = unit < cut ? each + 1 : each;
+    const int64_t i = work >> 31 ? from / by : static_cast<uint32_t>(from) / static_cast<uint32_t>(by);
+    return static_cast<int>(unit < cut ? i : more + i);
+  }
+};
+
+// Where a place in the order of all units is: the sequence, its length and units, the units before it (of one head), the
+// (key head, column group), the unit in it, and the item's unit behind the last one of a share that ends at `end`.
+struct ItemAt {
+  int b, len, units, hc, unit, stop;
+  int64_t base;
+  __device__ __forceinline__ void load(const PagedArgs& a, int keys) {
+    len = paged_len(a, b);
+    units = (len + keys - 1) / keys;
+  }
+  __device__ __forceinline__ void go(const PagedArgs& a, int keys, int per_b, int64_t at, int64_t end) {
+    while (at >= (base + units) * per_b) {
+      base += units;
+      ++b;
+      load(a, keys);
+    }
+    const int64_t in_b = at - base * per_b;
+    hc = static_cast<int>(in_b >> 31 ? in_b / units : static_cast<uint32_t>(in_b) / static_cast<uint32_t>(units));
+    unit = static_cast<int>(in_b - static_cast<int64_t>(hc) * units);
+    stop = static_cast<int>(min(static_cast<int64_t>(units), unit + (end - at)));
+  }
+};
+
+__device__ __forceinline__ float sum_of_groups(float x) {  // over the lanes with the same lane & 3
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
 // Attention of B sequences with T query tokens each (the last T of the sequence) over the paged cache. Few rows, so its
-// time is the reading of the codes. The work is all steps of 128 keys of all (sequence, key head, 8 NT columns), in that
-// order, and every CTA takes an equal share of it, whatever the lengths are; they are read on the device. A share begins
-// and ends inside an item as it comes; parts of items go to the workspace and are joined by paged_join_kernel.
-// A warp takes 32 of a step's keys: every lane copies what it will read back itself (cp.async, kStages tiles under way),
-// and the products are mma.sync 16 x 8 x 16 with keys, then dimensions, as rows and the query rows as columns:
-// S^T = K Q^T, O^T = V^T P^T. Of K, lane (g, t) takes bytes 64 c + 16 t .. + 15 of keys g and g + 8: each word of it is,
-// as two half pairs, A fragments when the queries' B fragments are read in the same order. Of V, bytes g D / 8 .. of
-// keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, paired by byte permutes, are A fragments of output rows in the order of dimensions
-// g D / 8 + 2 i (row g of product i) and g D / 8 + 2 i + 1 (row g + 8). P^T is S^T's fragment, transposed by movmatrix.
+// time is the reading of the codes. The work is all tiles of 32 keys of all (sequence, key head, 8 NT columns), in that
+// order, shared out evenly, whatever the lengths are; they are read on the device. A share begins and ends inside an item
+// as it comes; parts of items go to the workspace and are joined by paged_join_kernel (joined by the last one to write a
+// part, 0.5 to 6 us slower: its loads wait for one another behind the whole item).
+// TOGETHER: a share is of a CTA, whose warps take the tiles of a unit of 128 keys and add up at an item's end, so there are few
+// parts. Otherwise a share is of a warp, whose copies run on across the borders of items, so that many short sequences
+// keep the memory as busy as a long one. Which one goes by the longest sequence that the table can hold (kPaShort) and
+// by whether there are enough items.
+// 200 sequences of up to 300 keys, 16 heads over 8 of 128, e4m3: 27.8 us with warps' shares, 40.3 with CTAs'; 32 of 1175 to
+// 4700: 41.1 us (4.8 TB/s) with CTAs' shares, 43 with warps'. One of 131071: 52 us, 5.1 TB/s; while it runs the memory is
+// busy throughout (7 TB/s and more over the tiles), the rest is the start (lengths, pages and tiles wait for one another,
+// 5 us) and the join (3 us).
+// A tile's codes come by TMA into the warp's own ring in shared memory, and the products are mma.sync 16 x 8 x 16 with keys, then dimensions, as rows and the query rows as columns: S^T = K Q^T,
+// O^T = V^T P^T. Of K, lane (g, t) reads bytes 64 c + 16 t .. + 15 of two keys: each word of them is, as two half pairs, A
+// fragments when the queries' B fragments are read in the same order. Of V, D / 8 bytes of four keys: bytes of two keys,
+// paired by byte permutes, are A fragments of output rows in the order of dimensions 2 i (row g of product i) and 2 i + 1
+// (row g + 8) of these D / 8. P^T is S^T's fragment, transposed by movmatrix.
 // Codes are exact in f16, and so are queries of either type after a power of two per row has brought them to about one
 // (bits below 2^-24 of the row's largest apart). The key block's scale goes into the scores. The value block's scale 2^e
 // goes into the exponent of the weights that meet V, 2^(s + e - m'), with a running maximum m' of its own, so that
 // weights of 16 bits are full where they count, whatever the blocks' scales; the softmax's sum has 2^(s - m). Both are
 // raised, and the sums rescaled, only when a score passes them by more than 2^8.
-template <typename T, int D, bool E4M3, int NT>
-__global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_kernel(const PagedArgs a) {
+template <typename T, int D, bool E4M3, int NT, bool TOGETHER>
+__global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
+    paged_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using S = PaShape<D, NT>;
   constexpr unsigned kAll = 0xffffffffu;
-  constexpr int kCols = 8 * NT, kSteps = D / 16;
-  extern __shared__ __align__(16) uint8_t ring_all[];
+  constexpr int kCols = 8 * NT, kSteps = D / 16, kKeys = TOGETHER ? kPaTile * kPaWarps : kPaTile;  // of a unit
+  extern __shared__ __align__(16) uint8_t paged_smem[];
+  __shared__ __align__(8) uint64_t bars[kPaWarps][S::kStages];
   __shared__ float scales[kPaWarps][S::kStages][4];  // key and value scales of a tile's two blocks; below zero: no page
   __shared__ float sml[kPaWarps][kCols][3];
-  __shared__ int64_t sums[2][kPaWarps], found_base;
-  __shared__ int found_b;
+  __shared__ int abort_flag;
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, t = lane & 3;
-  uint8_t* ring = ring_all + warp * (S::kStages * S::kStage);
+  uint8_t* ring_all = paged_smem + (1024 - (smem_u32(paged_smem) & 1023)) % 1024;
+  uint8_t* ring = ring_all + warp * (S::kStages * 2 * S::kHalf);
   float(*so)[kCols][D + 4] = reinterpret_cast<float(*)[kCols][D + 4]>(ring_all);
-
-  // ---- this CTA's share, and the sequence and step that it begins with
-  auto steps_of = [&](int b) { return b < a.B ? (paged_len(a, b) + kPaStep - 1) / kPaStep : 0; };
-  const int per_b = a.hkv * a.col_groups;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kPaWarps * 32) total += steps_of(b0 + static_cast<int>(threadIdx.x));
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
-  if (lane == 0) sums[0][warp] = total;
+  if (lane < S::kStages) mbar_init(&bars[warp][lane], 1);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
+  fence_mbar_init();
   __syncthreads();
-  total = 0;
-  for (int w = 0; w < kPaWarps; ++w) total += sums[0][w];
-  const int64_t work = total * per_b;
-  int64_t at = blockIdx.x * work / gridDim.x;
-  const int64_t end = (blockIdx.x + 1) * work / gridDim.x;
-  const bool tells = blockIdx.x == 0;  // writes down where the sequences begin, for the join
-  if (at >= end && !tells) return;
-  int64_t base = 0;  // steps before sequence b, of one head
-  for (int b0 = 0, round = 1; b0 < a.B; b0 += kPaWarps * 32, round ^= 1) {
-    const int mine = steps_of(b0 + static_cast<int>(threadIdx.x));
-    int64_t upto = mine;
+  const int key_row = S::row(g);
+  const int page_mask = (1 << a.page_shift) - 1;
+  const bool two_pages = a.page_shift == 4;  // a tile's two blocks of 16 keys lie in two pages
+
+  // ---- this warp's share, and the sequence that it begins in. Shares of warps: neighbouring ones go to neighbouring CTAs,
+  // so that few of them are spread over the SMs.
+  const int per_b = a.hkv * a.col_groups, grid = static_cast<int>(gridDim.x);
+  auto units_of = [&](int b) { return b < a.B ? (paged_len(a, b) + kKeys - 1) / kKeys : 0; };
+  int64_t units = 0;
+#pragma unroll 4
+  for (int b0 = 0; b0 < a.B; b0 += 32) units += __reduce_add_sync(kAll, units_of(b0 + lane));
+  const Shares all(units * per_b, TOGETHER ? grid : grid * kPaWarps);
+  const int share = TOGETHER ? static_cast<int>(blockIdx.x) : warp * grid + static_cast<int>(blockIdx.x);
+  const int64_t end = all.begin(share + 1);
+  const int64_t start = all.begin(share);
+  ItemAt it;  // what is worked on
+  it.b = 0, it.base = 0;
+  for (int64_t base = 0; start < end; it.b += 32) {
+    const int mine = units_of(it.b + lane);
+    int upto = mine;  // of the lanes up to this one
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(kAll, upto, o);
+      const int y = __shfl_up_sync(kAll, upto, o);
       if (lane >= o) upto += y;
     }
-    if (lane == 31) sums[round][warp] = upto;
-    __syncthreads();
-    int64_t all = 0;
-    upto += base;
-    for (int w = 0; w < kPaWarps; ++w) {
-      if (w < warp) upto += sums[round][w];
-      all += sums[round][w];
+    const unsigned here = __ballot_sync(kAll, start < (base + upto) * per_b);
+    if (here) {
+      const int who = __ffs(here) - 1;
+      it.b += who;
+      it.base = base + __shfl_sync(kAll, upto - mine, who);
+      break;
     }
-    const int b = b0 + static_cast<int>(threadIdx.x);
-    if (tells && b < a.B) a.bases[b + 1] = upto;
-    if (at < end && at >= (upto - mine) * per_b && at < upto * per_b) found_b = b, found_base = upto - mine;
-    base += all;
-    if (!tells && base * per_b > at) break;
+    base += __shfl_sync(kAll, upto, 31);
   }
-  if (tells && threadIdx.x == 0) a.bases[0] = 0;
-  __syncthreads();
-  if (at >= end) return;
-  int b = found_b, len = paged_len(a, b);
-  base = found_base;
-  bool first = true;
-  while (at < end) {
-    while (len == 0 || at >= (base + (len + kPaStep - 1) / kPaStep) * per_b) {
-      base += (len + kPaStep - 1) / kPaStep;
-      len = paged_len(a, ++b);
-    }
-    const int steps = (len + kPaStep - 1) / kPaStep;
-    const int64_t in_b = at - base * per_b;
-    const int hc = static_cast<int>(in_b / steps), s0 = static_cast<int>(in_b % steps);
-    const int s1 = static_cast<int>(min(static_cast<int64_t>(steps), s0 + (end - at)));
-    const int h = hc / a.col_groups, c0 = (hc % a.col_groups) * kCols;
-    const uint8_t *kc = a.kc + ((static_cast<int64_t>(h) << a.page_shift) * D) + 16 * t, *vc = a.vc + ((static_cast<int64_t>(h) << a.page_shift) * D) + S::kVBytes * g;
-    const int32_t* table = a.table + b * a.ld_table;
+  // sequences without keys
+  for (int b = warp * grid + static_cast<int>(blockIdx.x); b < a.B; b += grid * kPaWarps) {
+    if (units_of(b) > 0) continue;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.T * a.hkv * a.group * D);
+    for (int64_t i = lane; i < static_cast<int64_t>(a.T) * a.hkv * a.group * (D / 8); i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < per_b; i += 32) a.shared[static_cast<int64_t>(b) * per_b + i] = make_int4(0, 0, 0, 0);
+  }
+  if (start >= end) return;
 
-    int pages[2] = {-1, -1};  // of the two blocks of tile (lane) of 32
-    auto look = [&](int from) {
+  // ---- the copies
+  const int first_key = TOGETHER ? warp * kPaTile : 0;  // of this warp's tile of a unit
+  it.load(a, kKeys);
+  ItemAt next = it;                              // next.unit is to be copied next
+  next.unit = next.stop = 0;
+  int left = static_cast<int>(end - start), more = left;  // units to be worked on, and to be copied (not TOGETHER)
+  int looked = 0;                                // the number of next.unit among those whose pages the lanes have
+  int pages[2] = {-1, -1};                       // of a tile's two blocks
+  auto look = [&] {
+    looked = 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = (s0 + from + lane) * kPaStep + warp * kPaTile + 16 * i;
-        int p = -1;
-        if (s0 + from + lane < s1 && key < len) p = table[key >> a.page_shift];
-        pages[i] = p < a.pages ? p : -1;
+    for (int i = 0; i < 2; ++i) {
+      const int unit = next.unit + lane, key = unit * kKeys + first_key + 16 * i;
+      int p = -1;
+      if ((i == 0 || two_pages) && unit < next.stop && key < next.len) p = a.table[next.b * a.ld_table + (key >> a.page_shift)];
+      pages[i] = p < a.pages ? p : -1;
+    }
+  };
+  auto fetch = [&](int st) {
+    if (TOGETHER ? next.unit < next.stop : more > 0) {
+      if (!TOGETHER && next.unit == next.stop) {
+        next.go(a, kKeys, per_b, end - more, end);
+        look();
+      } else if (looked == 32) {
+        look();
       }
-    };
-    auto fetch = [&](int i, int st) {  // tile i of this warp
-      if (s0 + i < s1) {
-        const int key0 = (s0 + i) * kPaStep + warp * kPaTile;
-        const uint32_t dst = smem_u32(ring + st * S::kStage);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int page = __shfl_sync(kAll, pages[x], i & 31);
-          const int key = key0 + 16 * x, slot = key & ((1 << a.page_shift) - 1);
-          const int left = page < 0 ? 0 : len - key;
-          const uint8_t *kp = kc + max(page, 0) * a.kc_sp + slot * D, *vp = vc + max(page, 0) * a.vc_sp + slot * D;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-#pragma unroll
-            for (int c = 0; c < S::kC; ++c)
-              cp_async(dst + ((x * 2 + r) * S::kC + c) * 512 + lane * 16, kp + (8 * r + g) * D + 64 * c, 8 * r + g < left, 16);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = 2 * t + (r & 1) + 8 * (r >> 1);
-            cp_async(dst + S::kKeyBytes + (x * 4 + r) * (S::kVBytes * 32) + lane * S::kVBytes, vp + row * D, row < left, S::kVBytes);
-          }
-          if (lane < 2) {
-            float* to = &scales[warp][st][2 * x + lane];
-            if (left > 0)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)),
-                           "l"(lane == 0 ? a.ks + page * a.ks_sp + h : a.vs + page * a.vs_sp + h)
-                           : "memory");
-            else
-              *to = -1.f;
-          }
+      --more;
+      const int key0 = next.unit * kKeys + first_key, h = next.hc / a.col_groups;
+      const int p0 = __shfl_sync(kAll, pages[0], looked), p1 = two_pages ? __shfl_sync(kAll, pages[1], looked) : -1;
+      if (lane == 0) {
+        uint8_t* dst = ring + st * 2 * S::kHalf;
+        uint64_t* bar = &bars[warp][st];
+        const int block = two_pages ? S::kHalf / 2 : S::kHalf;
+        const int row = (h << a.page_shift) + (key0 & page_mask);
+        mbar_arrive_expect_tx(bar, ((p0 >= 0) + (p1 >= 0)) * 2 * block);
+        if (p0 >= 0) {
+          tma_load_3d(dst, &k_map, bar, 0, row, p0);
+          tma_load_3d(dst + S::kHalf, &v_map, bar, 0, row, p0);
+        }
+        if (p1 >= 0) {
+          tma_load_3d(dst + block, &k_map, bar, 0, row, p1);
+          tma_load_3d(dst + S::kHalf + block, &v_map, bar, 0, row, p1);
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    look(0);
-#pragma unroll
-    for (int i = 0; i < S::kStages; ++i) fetch(i, i);
+      if (lane < (two_pages ? 4 : 2)) {
+        const int page = lane < 2 ? p0 : p1;
+        float* to = &scales[warp][st][lane];
+        if (page >= 0)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)),
+                       "l"(lane & 1 ? a.vs + page * a.vs_sp + h : a.ks + page * a.ks_sp + h)
+                       : "memory");
+        else
+          *to = -1.f;
+      }
+      ++looked;
+      ++next.unit;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 
+  bool first = true;
+  int st = 0;  // the stage of the next tile, and the parity of its barrier
+  uint32_t parity = 0;
+  while (left > 0) {
+    it.go(a, kKeys, per_b, end - left, end);
+    const int len = it.len, begin = it.unit;
+    const int h = it.hc / a.col_groups, c0 = (it.hc % a.col_groups) * kCols;
+    Pack<T, 4> raw[NT][kSteps];  // the queries, on their way while the pages are looked up
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = c0 + 8 * n + g, q_t = col / a.group;
+      const T* qp = static_cast<const T*>(a.q) + it.b * a.q_sb + q_t * a.q_st + (h * a.group + col - q_t * a.group) * a.q_sh + 16 * t;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) raw[n][s] = col < a.cols ? load_pack<T, 4>(qp + 64 * (s / 4) + 4 * (s % 4)) : Pack<T, 4>{};
+    }
+    if constexpr (TOGETHER) {
+      next = it;
+      look();
+    }
+    if (TOGETHER || first) {
+#pragma unroll
+      for (int i = 0; i < S::kStages; ++i) fetch(st + i >= S::kStages ? st + i - S::kStages : st + i);
+    }
     // the queries, brought to about one by a power of two per column, and what the products are to be multiplied with
     uint32_t qf[NT][kSteps][2];
     float by[NT][2];
     int limit[NT][2];  // keys that columns 2 t, 2 t + 1 see
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int col = c0 + 8 * n + g;
-      Pack<T, 4> raw[kSteps];
-      const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + (col / a.group) * a.q_st + (h * a.group + col % a.group) * a.q_sh + 16 * t;
       uint32_t top = 0;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) raw[s] = col < a.cols ? load_pack<T, 4>(qp + 64 * (s / 4) + 4 * (s % 4)) : Pack<T, 4>{};
       float f[4];
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        to_floats<T, 4>(raw[s], f);
+        to_floats<T, 4>(raw[n][s], f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
       }
@@ -636,7 +712,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_ke
       const float inverse = e == 127 ? 5.877471754e-39f : power_of_two(-e);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        to_floats<T, 4>(raw[s], f);
+        to_floats<T, 4>(raw[n][s], f);
         qf[n][s][0] = pack2<__half>(f[0] * inverse, f[1] * inverse);
         qf[n][s][1] = pack2<__half>(f[2] * inverse, f[3] * inverse);
       }
@@ -658,30 +734,34 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_ke
       m[n][0] = m[n][1] = mv[n][0] = mv[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
     }
-    int st = 0;
-    for (int i = 0; s0 + i < s1; ++i, st = st + 1 == S::kStages ? 0 : st + 1) {
+    for (; it.unit < it.stop; ++it.unit) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
-      __syncwarp();
-      const uint8_t* mine = ring + st * S::kStage;
-      const int key0 = (s0 + i) * kPaStep + warp * kPaTile;
+      __syncwarp();  // the scales
+      if (!mbar_wait_warp(&bars[warp][st], parity, &abort_flag, a.err, kPaSite)) break;
+      const uint8_t* mine = ring + st * 2 * S::kHalf;
+      const int key0 = it.unit * kKeys + first_key;
       const float4 sc = *reinterpret_cast<const float4*>(scales[warp][st]);  // K, V of block 0, K, V of block 1
-      const float ks[2] = {sc.x, sc.z};
+      const float ks[2] = {sc.x, two_pages ? sc.z : sc.x};
       float ev[2];  // log2 of the value blocks' scales; NaN stays NaN
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t bits = __float_as_uint(x ? sc.w : sc.y);
+        const uint32_t bits = __float_as_uint(x && two_pages ? sc.w : sc.y);
         ev[x] = (bits & 0x7fffffffu) >= kNotFinite ? __uint_as_float(0x7fc00000u) : static_cast<float>(static_cast<int>(bits >> 23 & 0xff) - 127);
       }
-      // scores: s[n][x][e] is key 16 x + g (+ 8 for e >= 2) of the tile, column 2 t + (e & 1)
+      // scores: s[n][x][e] is key 16 x + key_row (+ 8 for e >= 2) of the tile, column 2 t + (e & 1)
       float s[NT][2][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
+        float odd[NT][4];  // two sums, so that the products are two chains
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][x][0] = s[n][x][1] = s[n][x][2] = s[n][x][3] = 0.f;
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][x][e] = odd[n][e] = 0.f;
+        }
 #pragma unroll
         for (int c = 0; c < S::kC; ++c) {
-          const uint4 k0 = *reinterpret_cast<const uint4*>(mine + (x * 2 * S::kC + c) * 512 + lane * 16);
-          const uint4 k1 = *reinterpret_cast<const uint4*>(mine + ((x * 2 + 1) * S::kC + c) * 512 + lane * 16);
+          const uint8_t* src = mine + (16 * x + key_row) * D + ((4 * c + t) ^ S::turn(key_row)) * 16;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(src), k1 = *reinterpret_cast<const uint4*>(src + 8 * D);
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -689,24 +769,36 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_ke
             to_halves<E4M3>(w0[w], f[0], f[2]);
             to_halves<E4M3>(w1[w], f[1], f[3]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816<false>(s[n][x], f, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
+            for (int n = 0; n < NT; ++n) mma_16816<false>(w & 1 ? odd[n] : s[n][x], f, qf[n][4 * c + w][0], qf[n][4 * c + w][1]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          // s = (sum * the block's scale) * what the column is to be multiplied with, two columns at a time
+          const float2 both = make_float2(ks[x], ks[x]), col = make_float2(by[n][0], by[n][1]);
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            float2 y = __fadd2_rn(make_float2(s[n][x][e], s[n][x][e + 1]), make_float2(odd[n][e], odd[n][e + 1]));
+            y = __fmul2_rn(__fmul2_rn(y, both), col);
+            s[n][x][e] = y.x, s[n][x][e + 1] = y.y;
           }
         }
       }
       const bool whole = key0 + kPaTile <= seen_by_all && !(ks[0] < 0.f) && !(ks[1] < 0.f);
+      if (!whole) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (ks[x] < 0.f || key0 + 16 * x + key_row + 8 * (e >> 1) >= limit[n][e & 1]) s[n][x][e] = -INFINITY;
+          }
+        }
+      }
       bool raise = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][x][e] = s[n][x][e] * ks[x] * by[n][e & 1];
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (ks[x] < 0.f || key0 + 16 * x + g + 8 * (e >> 1) >= limit[n][e & 1]) s[n][x][e] = -INFINITY;
-          }
-        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float a0 = fmaxf(s[n][0][e], s[n][0][2 + e]), a1 = fmaxf(s[n][1][e], s[n][1][2 + e]);
@@ -739,36 +831,49 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_ke
       uint32_t p[NT][2][2];  // B fragments of the weights
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-        const float v0 = mv[n][0] == -INFINITY ? 0.f : mv[n][0], v1 = mv[n][1] == -INFINITY ? 0.f : mv[n][1];
+        const float2 less = make_float2(m[n][0] == -INFINITY ? 0.f : -m[n][0], m[n][1] == -INFINITY ? 0.f : -m[n][1]);
+        const float2 less_v = make_float2(mv[n][0] == -INFINITY ? 0.f : -mv[n][0], mv[n][1] == -INFINITY ? 0.f : -mv[n][1]);
+        float2 sum = make_float2(l[n][0], l[n][1]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          l[n][0] += fast_exp2(s[n][x][0] - m0) + fast_exp2(s[n][x][2] - m0);
-          l[n][1] += fast_exp2(s[n][x][1] - m1) + fast_exp2(s[n][x][3] - m1);
+          const float2 less_x = __fadd2_rn(less_v, make_float2(ev[x], ev[x]));
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            // masked weights are zero whatever the block's scale
-            float w0 = fast_exp2(s[n][x][2 * r] + ev[x] - v0), w1 = fast_exp2(s[n][x][2 * r + 1] + ev[x] - v1);
-            if (!whole) {
-              if (s[n][x][2 * r] == -INFINITY) w0 = 0.f;
-              if (s[n][x][2 * r + 1] == -INFINITY) w1 = 0.f;
+            const float2 y = make_float2(s[n][x][2 * r], s[n][x][2 * r + 1]);
+            const float2 z = __fadd2_rn(y, less);
+            sum = __fadd2_rn(sum, make_float2(fast_exp2(z.x), fast_exp2(z.y)));
+            float2 w = __fadd2_rn(y, less_x);
+            w = make_float2(fast_exp2(w.x), fast_exp2(w.y));
+            if (!whole) {  // masked weights are zero whatever the block's scale
+              if (y.x == -INFINITY) w.x = 0.f;
+              if (y.y == -INFINITY) w.y = 0.f;
             }
-            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][x][r]) : "r"(pack2<__half>(w0, w1)));
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][x][r]) : "r"(pack2<__half>(w.x, w.y)));
           }
         }
+        l[n][0] = sum.x, l[n][1] = sum.y;
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         uint32_t v[4][S::kVBytes / 4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const uint8_t* src = mine + S::kKeyBytes + (x * 4 + r) * (S::kVBytes * 32) + lane * S::kVBytes;
+          // key of fragment place 2 t (+ 1), (+ 8)
+          const int row = S::row(2 * t + (r & 1)), at = S::part(g) * S::kVBytes;
+          const uint8_t* src = mine + S::kHalf + (16 * x + row + 8 * (r >> 1)) * D + ((at / 16) ^ S::turn(row)) * 16 + at % 16;
           if constexpr (S::kVBytes == 16) {
             const uint4 u = *reinterpret_cast<const uint4*>(src);
             v[r][0] = u.x, v[r][1] = u.y, v[r][2] = u.z, v[r][3] = u.w;
           } else {
             const uint2 u = *reinterpret_cast<const uint2*>(src);
             v[r][0] = u.x, v[r][1] = u.y;
+          }
+          if (!whole) {  // what lies behind the last key and in the place of a page that is none: any byte, also a NaN
+            const bool there = ks[x] >= 0.f || __isnanf(ks[x]);
+            if (!there || key0 + 16 * x + row + 8 * (r >> 1) >= len) {
+#pragma unroll
+              for (int w = 0; w < S::kVBytes / 4; ++w) v[r][w] = 0;
+            }
           }
         }
 #pragma unroll
@@ -784,139 +889,223 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas) paged_ke
           }
         }
       }
-      if (((i + S::kStages) & 31) == 0) look(i + S::kStages);
-      __syncwarp();
-      fetch(i + S::kStages, st);  // into the stage just read
+            __syncwarp();
+      fetch(st);  // into the stage just read
+      if (++st == S::kStages) st = 0, parity ^= 1;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    // ---- the warps' sums together
+    if (TOGETHER ? __syncthreads_or(it.unit < it.stop) : it.unit < it.stop) {  // a wait ran out: the copies still under way, and out
+      volatile int never = 0;
+      for (int n = TOGETHER ? next.unit - it.unit : left - (it.unit - begin) - more; n > 0; --n) {
+        mbar_wait(&bars[warp][st], parity, &never, a.err, kPaSite);
+        if (++st == S::kStages) st = 0, parity ^= 1;
+      }
+      return;
+    }
+    // ---- the item's sums, or a part of them; a share has at most two parts of items
+    const int64_t slot = 2 * static_cast<int64_t>(share) + (first ? 0 : 1), item = static_cast<int64_t>(it.b) * per_b + it.hc;
+    const bool whole_item = begin == 0 && it.stop == it.units;
+    if (begin == 0 && lane == 0 && (warp == 0 || !TOGETHER))
+      a.shared[item] = make_int4(share, whole_item ? share : all.owner(end - left + it.units - 1), static_cast<int>(slot), 0);
+    auto row_of = [&](int col) {
+      return static_cast<T*>(a.out) + ((static_cast<int64_t>(it.b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D;
+    };
+    auto inverse_of = [](float m, float sum, float mv) {
+      const float up = (mv == -INFINITY ? 0.f : mv) - (m == -INFINITY ? 0.f : m);
+      return sum > 0.f || __isnanf(sum) ? fast_exp2(up) / sum : 0.f;
+    };
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        l[n][e] += __shfl_xor_sync(kAll, l[n][e], 4);
-        l[n][e] += __shfl_xor_sync(kAll, l[n][e], 8);
-        l[n][e] += __shfl_xor_sync(kAll, l[n][e], 16);
-        const int col = 8 * n + 2 * t + e;
-        if (g == 0) sml[warp][col][0] = m[n][e], sml[warp][col][1] = l[n][e], sml[warp][col][2] = mv[n][e];
-        float* dst = &so[warp][col][S::kVBytes * g];
+        const float sum = sum_of_groups(l[n][e]);
+        const int c = 8 * n + 2 * t + e, col = c0 + c, d = S::kVBytes * S::part(g);
+        if (col >= a.cols) continue;
+        float x[2 * kSteps];
 #pragma unroll
-        for (int j = 0; j < kSteps; j += 2)
-          *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e], o[n][j + 1][2 + e]);
+        for (int j = 0; j < kSteps; ++j) x[2 * j] = o[n][j][e], x[2 * j + 1] = o[n][j][2 + e];
+        if constexpr (TOGETHER) {
+          if (g == 0) sml[warp][c][0] = m[n][e], sml[warp][c][1] = sum, sml[warp][c][2] = mv[n][e];
+          store_pack<float, 2 * kSteps>(&so[warp][c][d], from_floats<float, 2 * kSteps>(x));
+        } else if (whole_item) {
+          const float inv = inverse_of(m[n][e], sum, mv[n][e]);
+#pragma unroll
+          for (int j = 0; j < 2 * kSteps; ++j) x[j] = fit<T>(x[j] * inv);
+          store_pack<T, 2 * kSteps>(row_of(col) + d, from_floats<T, 2 * kSteps>(x));
+        } else {
+          store_pack<float, 2 * kSteps>(a.part_o + (slot * kCols + c) * D + d, from_floats<float, 2 * kSteps>(x));
+          if (g == 0) a.part_ml[slot * kCols + c] = make_float4(m[n][e], sum, mv[n][e], 0.f);
+        }
       }
     }
-    __syncthreads();
-    const bool alone = s0 == 0 && s1 == steps;
-    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
-    const int cols = min(kCols, a.cols - c0);
-    for (int i = threadIdx.x; i < cols * (D / 4); i += kPaWarps * 32) {
-      const int c = i / (D / 4), d = (i % (D / 4)) * 4;
-      float mm = -INFINITY, mmv = -INFINITY, ll = 0.f;
+    if constexpr (TOGETHER) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < min(kCols, a.cols - c0) * (D / 4); i += kPaWarps * 32) {
+        const int c = i / (D / 4), d = (i % (D / 4)) * 4;
+        float mm = -INFINITY, mmv = -INFINITY, ll = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPaWarps; ++w) mm = fmaxf(mm, sml[w][c][0]), mmv = fmaxf(mmv, sml[w][c][2]);
-      const float m0 = mm == -INFINITY ? 0.f : mm, v0 = mmv == -INFINITY ? 0.f : mmv;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kPaWarps; ++w) mm = fmaxf(mm, sml[w][c][0]), mmv = fmaxf(mmv, sml[w][c][2]);
+        const float m0 = mm == -INFINITY ? 0.f : mm, v0 = mmv == -INFINITY ? 0.f : mmv;
+        float acc[4] = {};
 #pragma unroll
-      for (int w = 0; w < kPaWarps; ++w) {
-        ll = fmaf(fast_exp2(sml[w][c][0] - m0), sml[w][c][1], ll);
-        const float f = fast_exp2(sml[w][c][2] - v0);
-        const float4 x = *reinterpret_cast<const float4*>(&so[w][c][d]);
-        acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+        for (int w = 0; w < kPaWarps; ++w) {
+          ll = fmaf(fast_exp2(sml[w][c][0] - m0), sml[w][c][1], ll);
+          const float f = fast_exp2(sml[w][c][2] - v0);
+          const float4 x = *reinterpret_cast<const float4*>(&so[w][c][d]);
+          acc[0] = fmaf(f, x.x, acc[0]), acc[1] = fmaf(f, x.y, acc[1]), acc[2] = fmaf(f, x.z, acc[2]), acc[3] = fmaf(f, x.w, acc[3]);
+        }
+        if (whole_item) {
+          const float inv = inverse_of(mm, ll, mmv);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * inv);
+          store_pack<T, 4>(row_of(c0 + c) + d, from_floats<T, 4>(acc));
+        } else {
+          store_pack<float, 4>(a.part_o + (slot * kCols + c) * D + d, from_floats<float, 4>(acc));
+          if (d == 0) a.part_ml[slot * kCols + c] = make_float4(mm, ll, mmv, 0.f);
+        }
       }
-      if (alone) {
-        const float inv = ll > 0.f || __isnanf(ll) ? fast_exp2(v0 - m0) / ll : 0.f;
-        const int col = c0 + c;
-        T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D + d;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(fit<T>(acc.x * inv), fit<T>(acc.y * inv)), pack2<T>(fit<T>(acc.z * inv), fit<T>(acc.w * inv)));
-      } else {
-        *reinterpret_cast<float4*>(a.part_o + (slot * kCols + c) * D + d) = acc;
-        if (d == 0) a.part_ml[slot * kCols + c] = make_float4(mm, ll, mmv, 0.f);
-      }
+      fence_async_smem();  // the sums, before TMA writes there again
+      __syncthreads();
     }
     first = false;
-    at += s1 - s0;
-    __syncthreads();
+    left -= it.stop - begin;
   }
 }
 
-// One block per (sequence, key head, column group): nothing where one CTA had all of it, zeros where there are no keys,
-// else the parts of the CTAs that shared it, in their order.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int ctas) {
-  constexpr int kCols = 8 * NT;
+// A row of an item (sequence, key head, column group): nothing where one share had all of it, else the parts of the shares,
+// joined in a fixed order. W = 1: a warp per row, for many rows; W = 4: a block per row, each warp with every fourth part. A
+// warp asks for 4 or 8 parts at once.
+template <typename T, int D, int NT, int W>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int64_t items) {
+  constexpr int kCols = 8 * NT, kV = D / 32, kAhead = W == 1 ? 4 : 8;
+  __shared__ float sums[W][D];
+  __shared__ float sml[W][3];
+  const int rows = min(kCols, a.cols), warp = W == 1 ? 0 : warp_id(), lane = lane_id();
+  const int64_t number = W == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + warp_id() : blockIdx.x;
+  const int64_t item = number / rows;
+  const int per_b = a.hkv * a.col_groups, hc = static_cast<int>(item % per_b), c = static_cast<int>(number - item * rows);
+  const int64_t b = item / per_b;
+  const int h = hc / a.col_groups, col = (hc % a.col_groups) * kCols + c;
+  if (item >= items || col >= a.cols) return;
+  T* dst = static_cast<T*>(a.out) + ((b * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int per_b = a.hkv * a.col_groups;
-  const int b = static_cast<int>(blockIdx.x) / per_b, hc = static_cast<int>(blockIdx.x) % per_b;
-  const int h = hc / a.col_groups, c0 = (hc % a.col_groups) * kCols, cols = min(kCols, a.cols - c0);
-  const int64_t work = a.bases[a.B] * per_b, base = a.bases[b], steps = a.bases[b + 1] - base;
-  int64_t i0 = 0, i1 = -1;  // the CTAs
-  const int64_t s = base * per_b + hc * steps, e = s + steps;
-  if (steps > 0) {
-    i0 = ((s + 1) * ctas - 1) / work;
-    i1 = (e * ctas - 1) / work;
-    if (i0 == i1) return;
-  }
-  for (int i = threadIdx.x; i < cols * (D / 4); i += 128) {
-    const int c = i / (D / 4), d = (i % (D / 4)) * 4;
-    float mm = -INFINITY, mmv = -INFINITY, ll = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    // a CTA's first item has its first slot: item s is CTA x's first one where x starts in it
-    auto slot = [&](int64_t x) { return 2 * x + (x * work / ctas >= s ? 0 : 1); };
-    for (int64_t x = i0; x <= i1; ++x) {
-      if (x * work / ctas == (x + 1) * work / ctas) continue;
-      const float4 ml = a.part_ml[slot(x) * kCols + c];
-      mm = fmaxf(mm, ml.x), mmv = fmaxf(mmv, ml.z);
+  const int4 it = a.shared[item];
+  if (it.x == it.y) return;
+  float mm = -INFINITY, mmv = -INFINITY, ll = 0.f, acc[kV] = {};
+  for (int x0 = it.x + warp; x0 <= it.y; x0 += W * kAhead) {
+    float4 ml[kAhead];
+    Pack<float, kV> y[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const int x = x0 + W * n;
+      ml[n] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);  // none
+      y[n] = Pack<float, kV>{};
+      if (x <= it.y) {
+        const int64_t from = (x == it.x ? it.z : 2 * static_cast<int64_t>(x)) * kCols + c;  // all but the first begin with it
+        ml[n] = a.part_ml[from];
+        y[n] = load_pack<float, kV>(a.part_o + from * D + lane * kV);
+      }
     }
-    const float m0 = mm == -INFINITY ? 0.f : mm, v0 = mmv == -INFINITY ? 0.f : mmv;
-    for (int64_t x = i0; x <= i1; ++x) {
-      if (x * work / ctas == (x + 1) * work / ctas) continue;
-      const float4 ml = a.part_ml[slot(x) * kCols + c];
-      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (slot(x) * kCols + c) * D + d);
-      ll = fmaf(fast_exp2(ml.x - m0), ml.y, ll);
-      const float f = fast_exp2(ml.z - v0);
-      acc.x = fmaf(f, y.x, acc.x), acc.y = fmaf(f, y.y, acc.y), acc.z = fmaf(f, y.z, acc.z), acc.w = fmaf(f, y.w, acc.w);
+    float m1 = mm, v1 = mmv;
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) m1 = fmaxf(m1, ml[n].x), v1 = fmaxf(v1, ml[n].z);
+    const float m0 = m1 == -INFINITY ? 0.f : m1, v0 = v1 == -INFINITY ? 0.f : v1, f0 = fast_exp2(mmv - v0);
+    ll *= fast_exp2(mm - m0);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] *= f0;
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      ll = fmaf(fast_exp2(ml[n].x - m0), ml[n].y, ll);
+      const float f = fast_exp2(ml[n].z - v0);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) acc[i] = fmaf(f, __uint_as_float(y[n].w[i]), acc[i]);
     }
-    const float inv = ll > 0.f || __isnanf(ll) ? fast_exp2(v0 - m0) / ll : 0.f;
-    const int col = c0 + c;
-    T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(fit<T>(acc.x * inv), fit<T>(acc.y * inv)), pack2<T>(fit<T>(acc.z * inv), fit<T>(acc.w * inv)));
+    mm = m1, mmv = v1;
   }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) sums[warp][lane * kV + i] = acc[i];
+    if (lane == 0) sml[warp][0] = mm, sml[warp][1] = ll, sml[warp][2] = mmv;
+    __syncthreads();
+    if (warp > 0) return;
+    const float wm = lane < W ? sml[lane % W][0] : -INFINITY, wl = lane < W ? sml[lane % W][1] : 0.f, wv = lane < W ? sml[lane % W][2] : -INFINITY;
+    mm = wm, mmv = wv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o)), mmv = fmaxf(mmv, __shfl_xor_sync(0xffffffffu, mmv, o));
+    ll = sum_of_lanes<32>(wl * fast_exp2(wm - (mm == -INFINITY ? 0.f : mm)));
+    const float f = fast_exp2(wv - (mmv == -INFINITY ? 0.f : mmv));
+#pragma unroll
+    for (int i = 0; i < kV; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float fw = __shfl_sync(0xffffffffu, f, w);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) acc[i] = fmaf(fw, sums[w][lane * kV + i], acc[i]);
+    }
+  }
+  const float inv = ll > 0.f || __isnanf(ll) ? fast_exp2((mmv == -INFINITY ? 0.f : mmv) - (mm == -INFINITY ? 0.f : mm)) / ll : 0.f;
+#pragma unroll
+  for (int i = 0; i < kV; ++i) acc[i] = fit<T>(acc[i] * inv);
+  store_pack<T, kV>(dst + lane * kV, from_floats<T, kV>(acc));
 }
 
 // CTAs of a call, and where its workspace's parts lie.
 struct PagedPlan {
   int nt, col_groups;
-  int64_t ctas, ml_at, o_at, bytes;
+  int64_t items, ctas, ml_at, o_at, bytes;
   PagedPlan(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys, int sms) {
     const int64_t cols = hq / hkv * T;
+    // tiles of eight columns that a warp takes at once. Heads of 64 have registers for four, but 24 sequences of up to 3001
+    // keys with 4 tokens and 7 heads per key head took 21.2 us with four and 20.3 with two (of up to 12000: 38.5 and 43.7)
     nt = cols <= 8 ? 1 : 2;
     col_groups = static_cast<int>((cols + 8 * nt - 1) / (8 * nt));
-    const int64_t most = B * hkv * col_groups * ((most_keys + kPaStep - 1) / kPaStep);
+    const int64_t most = B * hkv * col_groups * ((most_keys + kPaTile - 1) / kPaTile);
     ctas = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sms) * (nt == 1 ? 3 : 2), most));
-    ml_at = ((B + 1) * 8 + 255) / 256 * 256;
-    o_at = ml_at + 2 * ctas * 8 * nt * 16;
-    bytes = o_at + 2 * ctas * 8 * nt * d * 4;
+    items = B * hkv * col_groups;
+    ml_at = (items * 16 + 255) / 256 * 256;
+    o_at = ml_at + 2 * ctas * kPaWarps * 8 * nt * 16;
+    bytes = o_at + 2 * ctas * kPaWarps * 8 * nt * d * 4;
   }
 };
 
-template <typename T, int D, bool E4M3, int NT>
-static int launch_paged_as(const PagedArgs& a, int ctas, cudaStream_t s) {
+struct PagedMaps {
+  CUtensorMap k, v;
+};
+// Codes [pages][Hkv * page][d] as TMA reads them, 32 keys or a page at a time.
+static int codes_map(CUtensorMap* m, const void* codes, int64_t sp, int64_t pages, int64_t hkv, int64_t page, int64_t d) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(d), static_cast<uint64_t>(hkv * page), static_cast<uint64_t>(pages)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(d), static_cast<uint64_t>(pages > 1 ? sp : hkv * page * d)};
+  const uint32_t box[3] = {static_cast<uint32_t>(d), static_cast<uint32_t>(std::min<int64_t>(page, kPaTile)), 1};
+  return encode_tma(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, codes, dims, strides, box, "paged_attention codes",
+                    d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+template <typename T, int D, bool E4M3, int NT, bool TOGETHER>
+static int launch_paged_as(const PagedArgs& a, const PagedMaps& maps, int ctas, cudaStream_t s) {
   using S = PaShape<D, NT>;
-  auto kern = paged_kernel<T, D, E4M3, NT>;
+  auto kern = paged_kernel<T, D, E4M3, NT, TOGETHER>;
   static std::atomic<bool> allowed[64];
   int rc = allow_shared(allowed, kern, S::kSmem);
   if (rc != XDNA_OK) return rc;
-  kern<<<static_cast<unsigned>(ctas), kPaWarps * 32, S::kSmem, s>>>(a);
+  kern<<<static_cast<unsigned>(ctas), kPaWarps * 32, S::kSmem, s>>>(a, maps.k, maps.v);
   if ((rc = check_launch("paged_kernel")) != XDNA_OK) return rc;
-  const unsigned items = static_cast<unsigned>(static_cast<int64_t>(a.B) * a.hkv * a.col_groups);
-  return launch_early("paged_join_kernel", paged_join_kernel<T, D, NT>, dim3(items), 128, 0, s, a, ctas);
+  const int64_t items = static_cast<int64_t>(a.B) * a.hkv * a.col_groups;
+  const int64_t rows = items * std::min(8 * NT, a.cols);
+  return rows < 4 * 148
+             ? launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, s, a, items)
+             : launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, a, items);
+}
+
+template <typename T, int D, bool E4M3, int NT>
+static int launch_paged_as(const PagedArgs& a, const PagedMaps& m, int ctas, cudaStream_t s) {
+  const bool together = (static_cast<int64_t>(a.max_pages) << a.page_shift) > kPaShort || static_cast<int64_t>(a.B) * a.hkv * a.col_groups < ctas;
+  return together ? launch_paged_as<T, D, E4M3, NT, true>(a, m, ctas, s)
+                  : launch_paged_as<T, D, E4M3, NT, false>(a, m, ctas, s);
 }
 
 template <typename T, int D>
-static int launch_paged(const PagedArgs& a, bool e4m3, int nt, int ctas, cudaStream_t s) {
-  if (e4m3) return nt == 1 ? launch_paged_as<T, D, true, 1>(a, ctas, s) : launch_paged_as<T, D, true, 2>(a, ctas, s);
-  return nt == 1 ? launch_paged_as<T, D, false, 1>(a, ctas, s) : launch_paged_as<T, D, false, 2>(a, ctas, s);
+static int launch_paged(const PagedArgs& a, const PagedMaps& m, bool e4m3, int nt, int ctas, cudaStream_t s) {
+  if (nt == 1) return e4m3 ? launch_paged_as<T, D, true, 1>(a, m, ctas, s) : launch_paged_as<T, D, false, 1>(a, m, ctas, s);
+  return e4m3 ? launch_paged_as<T, D, true, 2>(a, m, ctas, s) : launch_paged_as<T, D, false, 2>(a, m, ctas, s);
 }
 
 // ---------------------------------------------------------------------------- host
@@ -929,8 +1118,8 @@ static int check_cache(const char* what, int64_t pages, int64_t hkv, int64_t pag
                  "%s: bad sizes", what);
   return XDNA_OK;
 }
-static bool cache_ok(const void* codes, int64_t sp, const void* scales, int64_t ssp) {
-  return codes && scales && aligned16(codes) && sp >= 0 && sp % 16 == 0 && ssp >= 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
+static bool cache_ok(const void* codes, int64_t sp, const void* scales, int64_t ssp, int64_t pages) {
+  return ((codes && scales) || pages == 0) && aligned16(codes) && sp >= 0 && sp % 16 == 0 && ssp >= 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
 }
 static bool rows_ok(const void* p, int64_t st, int64_t sh) { return p && aligned16(p) && st > 0 && sh > 0 && st % 8 == 0 && sh % 8 == 0; }
 static int shift_of(int64_t page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
@@ -963,7 +1152,7 @@ int xdna_cache_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, 
   if ((rc = check_device(&sms)) != XDNA_OK) return rc;
   if (tokens == 0) return XDNA_OK;
   XDNA_CHECK_ARG(rows_ok(k, k_st, k_sh) && rows_ok(v, v_st, v_sh) && (!q || (rows_ok(q, q_st, q_sh) && q_out && aligned16(q_out) && hq >= 1)) &&
-                     cache_ok(k_codes, kc_sp, k_scales, ks_sp) && cache_ok(v_codes, vc_sp, v_scales, vs_sp) &&
+                     cache_ok(k_codes, kc_sp, k_scales, ks_sp, pages) && cache_ok(v_codes, vc_sp, v_scales, vs_sp, pages) &&
                      (table || max_pages == 0) && (starts || n_seqs == 0) && (n_freq == 0 || inv_freq),
                  "cache_append: null pointer, unaligned rows or bad strides");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1015,30 +1204,35 @@ int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
   if ((rc = check_device(&sms)) != XDNA_OK) return rc;
   if (B == 0 || T == 0) return XDNA_OK;
   XDNA_CHECK_ARG(q && aligned16(q) && q_sb > 0 && q_st > 0 && q_sh > 0 && q_sb % 8 == 0 && q_st % 8 == 0 && q_sh % 8 == 0 && out && aligned16(out) && lens &&
-                     (table || max_pages == 0) && cache_ok(k_codes, kc_sp, k_scales, ks_sp) && cache_ok(v_codes, vc_sp, v_scales, vs_sp),
+                     (table || max_pages == 0) && cache_ok(k_codes, kc_sp, k_scales, ks_sp, pages) && cache_ok(v_codes, vc_sp, v_scales, vs_sp, pages),
                  "paged_attention: null pointer, unaligned rows or bad strides");
   const PagedPlan plan(B, T, hq, hkv, d, max_pages * page, sms);
+  XDNA_CHECK_ARG(plan.items < (1ll << 31) && plan.items * (max_pages * page / kPaTile + 1) / plan.ctas < (1ll << 31), "paged_attention: bad sizes");
   XDNA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_bytes >= static_cast<size_t>(plan.bytes),
                  "paged_attention: workspace too small or unaligned");
   PagedArgs a{};
   a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
-  a.kc = static_cast<const uint8_t*>(k_codes), a.vc = static_cast<const uint8_t*>(v_codes), a.kc_sp = kc_sp, a.vc_sp = vc_sp;
-  a.ks = k_scales, a.vs = v_scales, a.ks_sp = ks_sp, a.vs_sp = vs_sp;
+  a.ks = k_scales, a.vs = v_scales, a.ks_sp = ks_sp, a.vs_sp = vs_sp, a.err = device_error_word();
   a.table = table, a.ld_table = ld_table, a.lens = lens, a.scale_log2 = scale * kLog2E;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.hkv = static_cast<int>(hkv), a.group = static_cast<int>(hq / hkv);
   a.page_shift = shift_of(page), a.pages = static_cast<int>(pages), a.max_pages = static_cast<int>(max_pages);
   a.col_groups = plan.col_groups, a.cols = static_cast<int>(a.group * T);
   a.out = out;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  a.bases = reinterpret_cast<int64_t*>(ws);
+  a.shared = reinterpret_cast<int4*>(ws);
   a.part_ml = reinterpret_cast<float4*>(ws + plan.ml_at);
   a.part_o = reinterpret_cast<float*>(ws + plan.o_at);
+  PagedMaps maps{};
+  if (pages > 0) {  // without any, nothing is copied
+    if ((rc = codes_map(&maps.k, k_codes, kc_sp, pages, hkv, page, d)) != XDNA_OK) return rc;
+    if ((rc = codes_map(&maps.v, v_codes, vc_sp, pages, hkv, page, d)) != XDNA_OK) return rc;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int ctas = static_cast<int>(plan.ctas);
   const bool e4m3 = format == XDNA_E4M3;
   if (dtype == XDNA_BF16)
-    return d == 64 ? launch_paged<__nv_bfloat16, 64>(a, e4m3, plan.nt, ctas, s) : launch_paged<__nv_bfloat16, 128>(a, e4m3, plan.nt, ctas, s);
-  return d == 64 ? launch_paged<__half, 64>(a, e4m3, plan.nt, ctas, s) : launch_paged<__half, 128>(a, e4m3, plan.nt, ctas, s);
+    return d == 64 ? launch_paged<__nv_bfloat16, 64>(a, maps, e4m3, plan.nt, ctas, s) : launch_paged<__nv_bfloat16, 128>(a, maps, e4m3, plan.nt, ctas, s);
+  return d == 64 ? launch_paged<__half, 64>(a, maps, e4m3, plan.nt, ctas, s) : launch_paged<__half, 128>(a, maps, e4m3, plan.nt, ctas, s);
 }
 
 }  // extern "C"
