@@ -45,14 +45,17 @@ __device__ __forceinline__ BlockChange change_block(uint32_t top_bits, bool has_
   return {power_of_two(e), power_of_two(min(-e, 127)), older};
 }
 
-// Four values to codes; x is within the codes' range (0 where the block is not finite).
-__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d, bool e4m3) {
-  if (e4m3) {
+// Four values to codes; they are within the codes' range.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d) {
+  if constexpr (E4M3) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     return lo | static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16;
+  } else {
+    // 1.5 * 2^23 + x is x's rounding to whole numbers, in the lowest bits
+    auto whole = [](float x) { return __float_as_uint(x + 12582912.f); };
+    return __byte_perm(__byte_perm(whole(a), whole(b), 0x0040), __byte_perm(whole(c), whole(d), 0x0040), 0x5410);
   }
-  auto byte = [](float x) { return static_cast<uint32_t>(__float2int_rn(x)) & 0xffu; };
-  return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(d) << 24;
 }
 // Two half pairs, exactly, of the four codes of a word, lowest first. int8: 1024 + (code + 128) is the half 0x6400 | byte.
 template <bool E4M3>
@@ -73,24 +76,26 @@ __device__ __forceinline__ void to_halves(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = *reinterpret_cast<const uint32_t*>(&q);
   }
 }
-__device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float by, bool e4m3) {
+template <bool E4M3>
+__device__ __forceinline__ uint32_t rescale_codes(uint32_t w, float by) {
   uint32_t lo, hi;
-  if (e4m3)
-    to_halves<true>(w, lo, hi);
-  else
-    to_halves<false>(w, lo, hi);
+  to_halves<E4M3>(w, lo, hi);
   const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&lo)), q = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  return to_codes(p.x * by, p.y * by, q.x * by, q.y * by, e4m3);
+  return to_codes<E4M3>(p.x * by, p.y * by, q.x * by, q.y * by);
 }
 // The first `bytes` (a multiple of 16) of a block, by `threads` threads of which this is number i.
-__device__ __forceinline__ void rescale_block(uint8_t* block, int bytes, float by, bool e4m3, int i, int threads) {
+template <bool E4M3>
+__device__ __forceinline__ void rescale_block(uint8_t* block, int bytes, float by, int i, int threads) {
 #pragma unroll 4
   for (int at = i * 16; at < bytes; at += threads * 16) {
     uint4 u = *reinterpret_cast<const uint4*>(block + at);
-    u.x = rescale_codes(u.x, by, e4m3), u.y = rescale_codes(u.y, by, e4m3);
-    u.z = rescale_codes(u.z, by, e4m3), u.w = rescale_codes(u.w, by, e4m3);
+    u.x = rescale_codes<E4M3>(u.x, by), u.y = rescale_codes<E4M3>(u.y, by);
+    u.z = rescale_codes<E4M3>(u.z, by), u.w = rescale_codes<E4M3>(u.w, by);
     *reinterpret_cast<uint4*>(block + at) = u;
   }
+}
+__device__ __forceinline__ void rescale_block(uint8_t* block, int bytes, float by, bool e4m3, int i, int threads) {
+  e4m3 ? rescale_block<true>(block, bytes, by, i, threads) : rescale_block<false>(block, bytes, by, i, threads);
 }
 
 // ---------------------------------------------------------------------------- append
@@ -139,56 +144,77 @@ __device__ __forceinline__ void row_floats(const RawRow<T, D, V>& r, float (*f)[
 #pragma unroll
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) to_floats<T, V>(r.p[k][0], f[k]), to_floats<T, V>(r.p[k][1], f[k] + V);
 }
-// All lanes of the warp; norm NULL for rows without one.
+// 1 / sqrt(mean of x^2 + eps) of a row, on all its lanes.
 template <int D, int V>
-__device__ __forceinline__ void norm_row(float (*f)[2 * V], const UnitAt* u, const void* norm, int dtype, int64_t at, float eps) {
+__device__ __forceinline__ float row_inverse(const float (*f)[2 * V], float eps) {
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i) ss = fmaf(f[k][i], f[k][i], ss);
+    ss += squares<2 * V>(f[k]);
   }
-  ss = sum_of_lanes<RowShape<D, V>::kLanes>(ss);
-  if (norm == nullptr) return;
-  const float inv = rsqrtf(ss * (1.f / D) + eps);
+  return rsqrtf(sum_of_lanes<RowShape<D, V>::kLanes>(ss) * (1.f / D) + eps);
+}
+template <int D, int V>
+__device__ __forceinline__ void norm_row(float (*f)[2 * V], const UnitAt* u, const void* norm, int dtype, int64_t at, float inverse) {
 #pragma unroll
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
     float g[2 * V];
     load_weights<V>(norm, dtype, at + u[k].lo, g);
     load_weights<V>(norm, dtype, at + u[k].hi, g + V);
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i) f[k][i] *= inv * g[i];
+    scale_by<2 * V>(f[k], inverse, g);
   }
 }
-// The largest |x| of the lanes of a row, as bits: NaN is above infinity, and that above all numbers.
+// The largest |x| of a lane's share of a row, as bits, NaN where one is (above infinity, and that above all numbers); of
+// the row.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 template <int D, int V>
-__device__ __forceinline__ uint32_t row_top(const float (*f)[2 * V]) {
-  uint32_t top = 0;
+__device__ __forceinline__ uint32_t lane_top(const float (*f)[2 * V]) {
+  float top = 0.f;
 #pragma unroll
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) top = max(top, __float_as_uint(f[k][i]) & 0x7fffffffu);
+    for (int i = 0; i < 2 * V; i += 2) top = max_abs(top, f[k][i], f[k][i + 1]);
   }
+  return __float_as_uint(top) & 0x7fffffffu;
+}
+template <int D, int V>
+__device__ __forceinline__ uint32_t row_top(const float (*f)[2 * V]) {
+  uint32_t top = lane_top<D, V>(f);
 #pragma unroll
   for (int o = RowShape<D, V>::kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   return top;
 }
-template <int D, int V>
-__device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V], const UnitAt* u, float inverse, bool e4m3) {
+template <int D, int V, bool E4M3>
+__device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V], const UnitAt* u, float inverse) {
 #pragma unroll
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
     float x[2 * V];
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) x[i] = inverse == 0.f ? 0.f : f[k][i] * inverse;
+    for (int i = 0; i < 2 * V; i += 2) {
+      const float2 y = __fmul2_rn(make_float2(f[k][i], f[k][i + 1]), make_float2(inverse, inverse));
+      x[i] = y.x, x[i + 1] = y.y;
+    }
+    if (inverse == 0.f) {  // not finite
+#pragma unroll
+      for (int i = 0; i < 2 * V; ++i) x[i] = 0.f;
+    }
     if constexpr (V == 8) {
-      *reinterpret_cast<uint2*>(row + u[k].lo) = make_uint2(to_codes(x[0], x[1], x[2], x[3], e4m3), to_codes(x[4], x[5], x[6], x[7], e4m3));
-      *reinterpret_cast<uint2*>(row + u[k].hi) = make_uint2(to_codes(x[8], x[9], x[10], x[11], e4m3), to_codes(x[12], x[13], x[14], x[15], e4m3));
+      *reinterpret_cast<uint2*>(row + u[k].lo) = make_uint2(to_codes<E4M3>(x[0], x[1], x[2], x[3]), to_codes<E4M3>(x[4], x[5], x[6], x[7]));
+      *reinterpret_cast<uint2*>(row + u[k].hi) = make_uint2(to_codes<E4M3>(x[8], x[9], x[10], x[11]), to_codes<E4M3>(x[12], x[13], x[14], x[15]));
     } else {
-      const uint32_t c = to_codes(x[0], x[1], 0.f, 0.f, e4m3);
+      const uint32_t c = to_codes<E4M3>(x[0], x[1], 0.f, 0.f);
       row[u[k].lo] = static_cast<uint8_t>(c);
       row[u[k].hi] = static_cast<uint8_t>(c >> 8);
     }
   }
+}
+template <int D, int V>
+__device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V], const UnitAt* u, float inverse, bool e4m3) {
+  e4m3 ? store_codes<D, V, true>(row, f, u, inverse) : store_codes<D, V, false>(row, f, u, inverse);
 }
 
 constexpr int kAppendThreads = 256;
@@ -209,7 +235,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const Appe
   if (there && number < a.max_pages) page = a.table[token * a.ld_table + number];
   if (page >= a.pages) page = -1;
   UnitAt u[S::kUnits];
-  float2 cs[S::kUnits][V];
+  float cos_[S::kUnits][V], sin_[S::kUnits][V];
 #pragma unroll
   for (int k = 0; k < S::kUnits; ++k) {
     u[k] = unit_at<V, INTER>(j0 + k * S::kLanes, a.n_freq);
@@ -218,13 +244,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const Appe
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int p = (j0 + k * S::kLanes) * V + r * kPer + i;
-      mine[i] = p < a.n_freq ? turn_of(position, a.inv_freq[p], a.factor) : make_float2(1.f, 0.f);
+      mine[i] = p < a.n_freq ? turn_of(turns_of(a.inv_freq[p]) * static_cast<uint64_t>(static_cast<int64_t>(position)), a.factor) : make_float2(1.f, 0.f);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int src = (i / kPer) * S::kLanes + j0;
-      cs[k][i].x = __shfl_sync(kAll, mine[i % kPer].x, src);
-      cs[k][i].y = __shfl_sync(kAll, mine[i % kPer].y, src);
+      cos_[k][i] = __shfl_sync(kAll, mine[i % kPer].x, src);
+      sin_[k][i] = __shfl_sync(kAll, mine[i % kPer].y, src);
     }
   }
   const int hq = a.q ? a.hq : 0, rows = hq + 2 * a.hkv;
@@ -246,11 +272,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const Appe
     }
     float f[S::kUnits][2 * V];
     row_floats<T, D, V>(mine ? load_row<T, D, V>(src, u) : RawRow<T, D, V>{}, f);
-    norm_row<D, V>(f, u, !mine || kind == 2 ? nullptr : kind == 0 ? a.q_norm : a.k_norm, kind == 0 ? a.q_norm_dtype : a.k_norm_dtype,
-                   kind == 0 ? h * a.q_norm_sh : h * a.k_norm_sh, a.eps);
+    if (a.q_norm || a.k_norm) {  // every lane takes part in the sum
+      const float inverse = row_inverse<D, V>(f, a.eps);
+      const void* norm = kind == 0 ? a.q_norm : a.k_norm;
+      if (mine && kind != 2 && norm)
+        norm_row<D, V>(f, u, norm, kind == 0 ? a.q_norm_dtype : a.k_norm_dtype, kind == 0 ? h * a.q_norm_sh : h * a.k_norm_sh, inverse);
+    }
     if (kind != 2) {
 #pragma unroll
-      for (int k = 0; k < S::kUnits; ++k) turn_unit<V, INTER>(f[k], cs[k], u[k].turning);
+      for (int k = 0; k < S::kUnits; ++k) turn_unit<V, INTER>(f[k], cos_[k], sin_[k], u[k].turning);
     }
     if (kind == 0 && row < rows) {
       T* dst = static_cast<T*>(a.q_out) + (token * a.hq + h) * D;
@@ -277,21 +307,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const Appe
   }
 }
 
-// Which page of which sequence this block of threads has: number `item` of those that the new tokens touch, sequence by
-// sequence. Every thread takes sequences in turn.
+// Page number `item` of those that the new tokens touch, sequence by sequence: found by every warp for itself, a sequence
+// per lane.
 struct PageItem {
-  int seq, number;           // the sequence and its page's number
-  int64_t first;             // the sequence's first new token
-  int64_t start, end;        // its first and behind its last new position
+  int seq, number;     // the sequence and its page's number
+  int64_t first;       // the sequence's first new token
+  int64_t start, end;  // its first and behind its last new position
 };
 __device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t item, PageItem* found) {
-  __shared__ int sums[kAppendThreads / 32];
-  __shared__ PageItem it;
-  __shared__ int done;
-  if (threadIdx.x == 0) done = 0;
-  int64_t before = 0;
-  for (int base = 0; base < a.n_seqs; base += kAppendThreads) {
-    const int seq = base + static_cast<int>(threadIdx.x);
+  constexpr unsigned kAll = 0xffffffffu;
+  for (int base = 0; base < a.n_seqs; base += 32) {
+    const int seq = base + lane_id();
     int64_t first = 0, start = -1, end = -1;
     int count = 0;
     if (seq < a.n_seqs) {
@@ -301,105 +327,134 @@ __device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t item, Pag
       end = min(start + (last - first), static_cast<int64_t>(a.max_pages) << a.page_shift);
       if (start >= 0 && end > start) count = static_cast<int>(((end - 1) >> a.page_shift) - (start >> a.page_shift)) + 1;
     }
-    int upto = count;  // of the warp's lanes up to this one
+    int64_t upto = count;  // of the lanes up to this one
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      const int64_t y = __shfl_up_sync(kAll, upto, o);
       if (lane_id() >= o) upto += y;
     }
-    if (lane_id() == 31) sums[warp_id()] = upto;
-    __syncthreads();
-    int64_t all = 0, mine = before + upto - count;
-    for (int w = 0; w < kAppendThreads / 32; ++w) {
-      if (w < warp_id()) mine += sums[w];
-      all += sums[w];
+    const unsigned here = __ballot_sync(kAll, item < upto);
+    if (here) {
+      const int who = __ffs(here) - 1;
+      const int64_t mine = (start >> a.page_shift) + item - (upto - count);
+      *found = {base + who, static_cast<int>(__shfl_sync(kAll, mine, who)), __shfl_sync(kAll, first, who), __shfl_sync(kAll, start, who),
+                __shfl_sync(kAll, end, who)};
+      return true;
     }
-    if (item >= mine && item < mine + count) {
-      it = PageItem{seq, static_cast<int>((start >> a.page_shift) + (item - mine)), first, start, end};
-      done = 1;
-    }
-    before += all;
-    __syncthreads();
-    if (done) break;
+    item -= __shfl_sync(kAll, upto, 31);
   }
-  *found = it;
-  return done != 0;
+  return false;
 }
 
 // The new tokens of packed sequences: a block of threads per page that they touch, K or V (blockIdx.z), and a.heads heads
-// (blockIdx.y). A head's part of the page lies in registers, at most 128 tokens, between the search for its largest value
-// and its codes; the angles' cosines and sines, which are those of all heads, are worked out once, in shared memory.
-template <typename T, int D, int V, bool INTER>
+// (blockIdx.y). A head's part of the page, MOST tokens for each of a block's rows of lanes (pages of fewer tokens than rows:
+// several heads at once), stays in registers between the search for its largest value and its codes, while the next heads'
+// part is on its way. The angles' cosines and sines, which are those of all heads, are worked out once, in shared memory.
+template <typename T, int D, int V, bool INTER, int MOST>
 __global__ void __launch_bounds__(kAppendThreads) append_packed_kernel(const AppendArgs a) {
   using S = RowShape<D, V>;
-  constexpr int kWarps = kAppendThreads / 32, kAtOnce = kWarps * S::kRows, kMost = 128 / kAtOnce;  // rows at a time, times
+  constexpr int kAtOnce = kAppendThreads / 32 * S::kRows;       // rows of lanes
   constexpr int kSplit = D / (2 * V), kPitch = D / 2 + D / 16;  // of a token's turns; a lane's are kSplit apart
   extern __shared__ __align__(16) float2 turns[];
   __shared__ uint32_t tops[32];
   PageItem it;
-  if (threadIdx.x < 32) tops[threadIdx.x] = 0;
   if (!find_page(a, blockIdx.x, &it)) return;
   const int page = a.table[it.seq * a.ld_table + it.number];
   if (page < 0 || page >= a.pages) return;
+  if (threadIdx.x < 32) tops[threadIdx.x] = 0;
   const bool value = blockIdx.z != 0;
   const int64_t page_first = static_cast<int64_t>(it.number) << a.page_shift;
   const int lo = static_cast<int>(max(it.start - page_first, int64_t{0}));
   const int n = static_cast<int>(min(it.end - page_first, static_cast<int64_t>(a.page))) - lo;  // new tokens, in slots lo ..
   const int64_t token = it.first + (page_first + lo - it.start);
-  const int lane = lane_id(), r0 = warp_id() * S::kRows + lane / S::kLanes, j0 = lane % S::kLanes;
+  const int lane = lane_id(), row = warp_id() * S::kRows + lane / S::kLanes, j0 = lane % S::kLanes;
+  // the row's token and which of the heads at once it has, the same for a warp
+  const int t0 = MOST > 1 ? row : row & (a.page - 1), heads = MOST > 1 ? 1 : max(kAtOnce >> a.page_shift, 1);
+  const int mine = MOST > 1 ? 0 : row >> a.page_shift;
   const int n_freq = value ? 0 : a.n_freq;
   UnitAt u[S::kUnits];
 #pragma unroll
   for (int k = 0; k < S::kUnits; ++k) u[k] = unit_at<V, INTER>(j0 + k * S::kLanes, n_freq);
-  for (int i = threadIdx.x; i < n * n_freq; i += kAppendThreads) {
-    const int t = i / n_freq, p = i % n_freq;
-    turns[t * kPitch + (p % V) * kSplit + p / V] = turn_of(page_first + lo + t, a.inv_freq[p], a.factor);
+  const int h0 = static_cast<int>(blockIdx.y) * a.heads, h1 = min(h0 + a.heads, a.hkv);
+  const int64_t st = value ? a.v_st : a.k_st, sh = value ? a.v_sh : a.k_sh;
+  const T* src = static_cast<const T*>(value ? a.v : a.k) + (token + t0) * st;
+  float* scale = value ? a.vs + page * a.vs_sp : a.ks + page * a.ks_sp;
+  uint8_t* block = value ? a.vc + page * a.vc_sp : a.kc + page * a.kc_sp;
+  RawRow<T, D, V> later[MOST];
+  uint32_t later_bits = 0;
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) later[i] = t0 + i * kAtOnce < n && h < h1 ? load_row<T, D, V>(src + h * sh + i * kAtOnce * st, u) : RawRow<T, D, V>{};
+    if (lo > 0 && h < h1) later_bits = __float_as_uint(scale[h]);
+  };
+  load(h0 + mine);
+  if (n_freq > 0) {  // n_freq threads to a token
+    const int tokens = kAppendThreads / n_freq, p = static_cast<int>(threadIdx.x) % n_freq;
+    int t = static_cast<int>(threadIdx.x) / n_freq;
+    if (t < tokens) {
+      const uint64_t each = turns_of(a.inv_freq[p]);
+      uint64_t at = each * static_cast<uint64_t>(page_first + lo + t);
+      for (; t < n; t += tokens, at += each * tokens) turns[t * kPitch + (p % V) * kSplit + p / V] = turn_of(at, a.factor);
+    }
   }
   __syncthreads();
-  const int h0 = static_cast<int>(blockIdx.y) * a.heads, h1 = min(h0 + a.heads, a.hkv);
-  for (int h = h0; h < h1; ++h) {
-    const T* src = value ? static_cast<const T*>(a.v) + h * a.v_sh : static_cast<const T*>(a.k) + h * a.k_sh;
-    const int64_t st = value ? a.v_st : a.k_st;
-    float* scale = (value ? a.vs + page * a.vs_sp : a.ks + page * a.ks_sp) + h;
-    uint8_t* block = (value ? a.vc + page * a.vc_sp : a.kc + page * a.kc_sp) + static_cast<int64_t>(h) * a.page * D;
-    const uint32_t old_bits = __float_as_uint(*scale);
-    float f[kMost][S::kUnits][2 * V];
+  for (int first = h0; first < h1; first += heads) {
+    const int h = first + mine;
+    float f[MOST][S::kUnits][2 * V];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) row_floats<T, D, V>(later[i], f[i]);
+    const uint32_t old_bits = later_bits;
+    load(h + heads);
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      const int t = r0 + i * kAtOnce;
-      row_floats<T, D, V>(t < n ? load_row<T, D, V>(src + (token + t) * st, u) : RawRow<T, D, V>{}, f[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      const int t = r0 + i * kAtOnce;
-      if (i * kAtOnce >= n) break;
+    for (int i = 0; i < MOST; ++i) {
+      const int t = t0 + i * kAtOnce;
       if (!value) {
-        norm_row<D, V>(f[i], u, t < n ? a.k_norm : nullptr, a.k_norm_dtype, h * a.k_norm_sh, a.eps);
+        if (a.k_norm) {
+          const float inverse = row_inverse<D, V>(f[i], a.eps);
+          if (h < h1) norm_row<D, V>(f[i], u, a.k_norm, a.k_norm_dtype, h * a.k_norm_sh, inverse);
+        }
 #pragma unroll
         for (int k = 0; k < S::kUnits; ++k) {
           if (t < n && u[k].turning > 0) {
-            float2 cs[V];
+            float c[V], s[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) cs[e] = e < u[k].turning ? turns[t * kPitch + e * kSplit + j0 + k * S::kLanes] : make_float2(1.f, 0.f);
-            turn_unit<V, INTER>(f[i][k], cs, u[k].turning);
+            for (int e = 0; e < V; ++e) {
+              const float2 y = turns[t * kPitch + e * kSplit + j0 + k * S::kLanes];  // of no use from u.turning on
+              c[e] = y.x, s[e] = y.y;
+            }
+            turn_unit<V, INTER>(f[i][k], c, s, u[k].turning);
           }
         }
       }
-      top = max(top, row_top<D, V>(f[i]));
+      top = max(top, lane_top<D, V>(f[i]));
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) atomicMax(&tops[h - h0], top);
+    if (lane == 0 && h < h1) atomicMax(&tops[h - h0], top);
     __syncthreads();
+    if (h >= h1) continue;
     const BlockChange c = change_block(tops[h - h0], lo > 0, old_bits, a.e4m3);
+    uint8_t* to = block + static_cast<int64_t>(h) * a.page * D;
 #pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      const int t = r0 + i * kAtOnce;
-      if (t < n) store_codes<D, V>(block + (lo + t) * D, f[i], u, c.inverse, a.e4m3);
+    for (int i = 0; i < MOST; ++i) {
+      const int t = t0 + i * kAtOnce;
+      if (t < n) store_codes<D, V>(to + (lo + t) * D, f[i], u, c.inverse, a.e4m3);
     }
-    if (threadIdx.x == 0) *scale = c.scale;
-    if (c.older != 1.f) rescale_block(block, lo * D, c.older, a.e4m3, threadIdx.x, kAppendThreads);
+    if (j0 == 0 && t0 == 0) scale[h] = c.scale;
+    const int threads = kAppendThreads / heads;
+    if (c.older != 1.f) rescale_block(to, lo * D, c.older, a.e4m3, static_cast<int>(threadIdx.x) - mine * threads, threads);
   }
+}
+
+template <typename T, int D, int V, bool INTER, int MOST>
+static int launch_packed(const AppendArgs& a, dim3 grid, cudaStream_t s) {
+  auto kern = append_packed_kernel<T, D, V, INTER, MOST>;
+  constexpr int kTurn = (D / 2 + D / 16) * static_cast<int>(sizeof(float2));  // bytes of a token's turns
+  static std::atomic<bool> allowed[64];
+  int rc = allow_shared(allowed, kern, 128 * kTurn);
+  if (rc != XDNA_OK) return rc;
+  kern<<<grid, kAppendThreads, a.n_freq > 0 ? a.page * kTurn : 0, s>>>(a);
+  return check_launch("append_packed_kernel");
 }
 
 template <typename T, int D, int V, bool INTER>
@@ -412,14 +467,15 @@ static int launch_append_as(AppendArgs a, int sms, cudaStream_t s) {
   const int64_t items = std::min(a.tokens, a.tokens / a.page + 2 * static_cast<int64_t>(a.n_seqs));
   a.heads = std::min(a.hkv, 32);
   while (a.heads > 1 && items * 2 * ((a.hkv + a.heads - 1) / a.heads) < 6 * sms) a.heads = (a.heads + 1) / 2;
-  const int smem = a.n_freq > 0 ? a.page * (D / 2 + D / 16) * static_cast<int>(sizeof(float2)) : 0;
-  auto kern = append_packed_kernel<T, D, V, INTER>;
-  static std::atomic<bool> allowed[64];
-  int rc = allow_shared(allowed, kern, 128 * (D / 2 + D / 16) * static_cast<int>(sizeof(float2)));
-  if (rc != XDNA_OK) return rc;
+  constexpr int kAtOnce = kAppendThreads / 32 * RowShape<D, V>::kRows;
+  const int rounds = a.page / kAtOnce;  // tokens of a page for each row of lanes
   const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>((a.hkv + a.heads - 1) / a.heads), 2);
-  kern<<<grid, kAppendThreads, smem, s>>>(a);
-  return check_launch("append_packed_kernel");
+  if constexpr (V == 1)
+    return launch_packed<T, D, V, INTER, 16>(a, grid, s);
+  else if (rounds >= 4)
+    return launch_packed<T, D, V, INTER, 4>(a, grid, s);
+  else
+    return rounds >= 2 ? launch_packed<T, D, V, INTER, 2>(a, grid, s) : launch_packed<T, D, V, INTER, 1>(a, grid, s);
 }
 
 template <typename T>

@@ -91,12 +91,16 @@ __device__ __forceinline__ void load_weights(const void* w, int dtype, int64_t a
     to_floats<__half, N>(load_pack<__half, N>(static_cast<const __half*>(w) + at), x);
 }
 
-// cos and sin of position * inv_freq, times factor. The product is taken in turns and in 64 bits, and only its distance
-// from a whole turn is rounded to 32 (2^-26 of a turn, 9.4e-8 in the angle), so far positions lose nothing.
-__device__ __forceinline__ float2 turn_of(int64_t position, float inv_freq, float factor) {
-  const double turns = static_cast<double>(position) * (static_cast<double>(inv_freq) * 0.15915494309189533577);
+// Angles in turns, as 64-bit fractions: a frequency's turns per position, rounded to 2^-56 or better, times the position
+// leaves exactly the part within a turn, whatever the position, and only that is rounded to 32 bits (2^-26 of a turn, 9.4e-8
+// in the angle). cos and sin of it, times factor.
+__device__ __forceinline__ uint64_t turns_of(float inv_freq) {
+  const double turns = static_cast<double>(inv_freq) * 0.15915494309189533577;
+  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
+}
+__device__ __forceinline__ float2 turn_of(uint64_t turns, float factor) {
   float s, c;
-  sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
+  sincospif(static_cast<float>(static_cast<int32_t>(turns >> 32)) * 4.656612873e-10f, &s, &c);  // 2^-31: half turns
   return make_float2(c * factor, s * factor);
 }
 
@@ -112,18 +116,44 @@ __device__ __forceinline__ UnitAt unit_at(int j, int n_freq) {
   return {2 * V * j, 2 * V * j + V, turning};
 }
 
-// x: the unit's 2 V values, first those of lo, then those of hi.
+// x: the unit's 2 V values, first those of lo, then those of hi. Pairs that are not interleaved turn all or none, two at a
+// time.
 template <int V, bool INTER>
-__device__ __forceinline__ void turn_unit(float (&x)[2 * V], const float2 (&cs)[V], int turning) {
+__device__ __forceinline__ void turn_unit(float (&x)[2 * V], const float (&c)[V], const float (&s)[V], int turning) {
+  if (!INTER && turning == 0) return;
+  if constexpr (INTER || V == 1) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float &a = x[INTER ? 2 * i : i], &b = x[INTER ? 2 * i + 1 : i + V];
-    if (i < turning) {
-      const float t = a * cs[i].x - b * cs[i].y;
-      b = b * cs[i].x + a * cs[i].y;
-      a = t;
+    for (int i = 0; i < V; ++i) {
+      float &a = x[INTER ? 2 * i : i], &b = x[INTER ? 2 * i + 1 : i + V];
+      if (!INTER || i < turning) {
+        const float t = fmaf(a, c[i], -b * s[i]);
+        b = fmaf(b, c[i], a * s[i]);
+        a = t;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 a = make_float2(x[i], x[i + 1]), b = make_float2(x[i + V], x[i + 1 + V]);
+      const float2 cc = make_float2(c[i], c[i + 1]), ss = make_float2(s[i], s[i + 1]), minus = make_float2(-s[i], -s[i + 1]);
+      const float2 t = __ffma2_rn(a, cc, __fmul2_rn(b, minus)), y = __ffma2_rn(b, cc, __fmul2_rn(a, ss));
+      x[i] = t.x, x[i + 1] = t.y, x[i + V] = y.x, x[i + 1 + V] = y.y;
     }
   }
+}
+
+// x *= by * w.
+template <int N>
+__device__ __forceinline__ void scale_by(float* x, float by, const float* w) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] *= by * w[i];
+}
+template <int N>
+__device__ __forceinline__ float squares(const float* x) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s = fmaf(x[i], x[i], s);
+  return s;
 }
 
 // The sum over LANES neighbouring lanes, on all of them.
