@@ -16,7 +16,7 @@ from typing import Optional
 
 import torch
 
-from . import conv, generate, kernels, layer, runtime, stack
+from . import conv, generate, layer, runtime, stack
 
 _configs = []  # cfg_id -> Config; op arguments must be plain values (R:torch_xdna/ops.py:14-22)
 
@@ -246,9 +246,6 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                  q: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> torch.Tensor:
     """Keys and values into a paged cache (layer.cache_append); without q an empty tensor."""
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (k_norm is not None and k_norm.requires_grad)):
-        raise kernels.XdnaError("cache_append", generate.ERR_INVALID, "a cache keeps no gradients: keys and values that "
-                                "require grad are stored under torch.no_grad()")
     with torch.no_grad():  # below autograd, whoever called
         out = layer.cache_append(k, v, k_cache, v_cache, k_scales, v_scales, table, starts, cu_seqlens, inv_freq, factor,
                                  interleaved, k_norm, q, q_norm, eps)
