@@ -76,7 +76,7 @@ def parse():
     ap.add_argument("--kernel", default=None,
                     choices=["gemm_i8", "quant_rows", "conv3x3", "conv3x3_chain", "conv_quant_codes", "attention",
                              "gemm_bf16", "gemm_bf16_qkv", "packed_attention", "shared_prefix_attention", "linear_w4",
-                             "process_logits"],
+                             "process_logits", "rotary", "add_norm", "cache_append", "paged_attention"],
                     help="time one kernel on --shape instead of a workload (profiling)")
     ap.add_argument("--shape", default="8192,6144,1024", help="--kernel shape, comma-separated")
     return ap.parse_args()
@@ -1327,6 +1327,46 @@ def run_kernel(args):
         fn = lambda: torch_xdna.process_logits(x, tokens, repetition=one, presence=one, frequency=one, bias=bias,  # noqa
                                                mask=mask)
         work, unit = 4 * B * V + 4 * V + 4 * mask.numel() + 4 * B * T, "GB/s"
+    elif args.kernel == "rotary":                    # T, H, D: bf16 heads with a norm of their own each
+        import torch_xdna
+
+        T, H, D = shp
+        x, w = torch.randn(T, H, D, device=dev, generator=g).to(torch.bfloat16), torch.ones(H, D, device=dev)
+        freq, pos = torch_xdna.rotary_frequencies(D, 1e6, device=dev)[0], torch.arange(T, device=dev)
+        fn = lambda: torch_xdna.rotary(x, pos, freq, norm=w)  # noqa
+        work, unit = 4 * T * H * D, "GB/s"
+    elif args.kernel == "add_norm":                  # T, D: bf16, a norm behind the block and a gate for each entry
+        import torch_xdna
+
+        T, D = shp
+        x, y, gate = (torch.randn(T, D, device=dev, generator=g).to(torch.bfloat16) for _ in range(3))
+        w = torch.ones(D, device=dev)
+        fn = lambda: torch_xdna.add_norm(x, y, w, w, gate)  # noqa
+        work, unit = 10 * T * D, "GB/s"
+    elif args.kernel in ("cache_append", "paged_attention"):
+        # N, S, T, page: N sequences of S tokens, 16 q heads over 8 of 128, int8 codes, T new tokens of each (appended
+        # packed where T > 1)
+        import torch_xdna
+
+        N, S, T, page = shp
+        cache = torch_xdna.paged_cache(N * -(-S // page), 8, 128, page, device=dev)
+        for codes in cache[:2]:
+            codes.random_(-127, 128, generator=g)
+        for scales in cache[2:]:
+            scales.fill_(2.0 ** -5)
+        table = torch.randperm(len(cache.k), device=dev, generator=g).int().view(N, -1)
+        lens = torch.full((N,), S, dtype=torch.int32, device=dev)
+        qkv = torch.randn(N * T, 32, 128, device=dev, generator=g).to(torch.bfloat16)
+        if args.kernel == "paged_attention":
+            q = qkv[:, :16].reshape(N, T, 16, 128)
+            fn = lambda: torch_xdna.paged_attention(q, *cache, table, lens)  # noqa
+            work, unit = 2 * N * S * 1024 + 4 * N * T * 2048, "GB/s"
+        else:
+            freq, w = torch_xdna.rotary_frequencies(128, 1e6, device=dev)[0], torch.ones(128, device=dev)
+            cu = torch.arange(0, N * T + 1, T, dtype=torch.int32, device=dev) if T > 1 else None
+            fn = lambda: torch_xdna.cache_append(qkv[:, 16:24], qkv[:, 24:], *cache, table, lens - T, cu, freq,  # noqa
+                                                 k_norm=w, q=None if T > 1 else qkv[:, :16], q_norm=None if T > 1 else w)
+            work, unit = N * T * (3 * 2048 + (4 * 2048 if T == 1 else 0)), "GB/s"
     else:
         raise SystemExit(f"unknown kernel {args.kernel}")
     for _ in range(5):

@@ -841,3 +841,31 @@ def test_prompts_then_tokens(cuda, fmt):
                 want = torch.softmax(z, 0) @ kept[i][1][:, h // 2]
                 off = float((got[i, t - 1, h].double() - want).norm() / kept[i][1][:, h // 2].norm(dim=1).mean())
                 assert off < 0.05, (step, i, h, off)                # 8-bit codes: 1 to 3 % of a value each
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_example_generates(cuda, fmt):
+    """The example's model over its paged cache: whole prompts, then tokens, twice the same."""
+    import importlib.util
+    from pathlib import Path
+
+    at = Path(__file__).resolve().parent.parent / "examples" / "generate_paged.py"
+    spec = importlib.util.spec_from_file_location("generate_paged_example", at)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    gen = torch.Generator().manual_seed(5)
+    vocab = 704
+    prompts = [torch.randint(0, vocab, (n,), generator=gen).cuda() for n in (70, 1, 64)]
+    model = example.Model(2, vocab, torch.device("cuda"))
+    runs = []
+    for some in (prompts, prompts):
+        session = example.PagedSession(model, some, 6, fmt)
+        for _ in range(6):
+            assert torch.isfinite(session.logits.float()).all()
+            session.step(session.choose())
+        assert session.lens.tolist() == [76, 7, 70]
+        runs.append(session.tokens.clone())
+    assert torch.equal(*runs)
+    for i, n in enumerate((70, 1, 64)):
+        new = runs[0][i, n:n + 6]
+        assert ((new >= 0) & (new < vocab)).all() and torch.equal(runs[0][i, :n], prompts[i].int())

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 7) rotary_kernel(const Rota
       float ss = 0.f;
 #pragma unroll
       for (int k = 0; k < U; ++k) ss += squares<2 * V>(f[k]);
-      inv = rsqrtf(sum_of_lanes<LANES>(ss) / static_cast<float>(a.D) + a.eps);
+      inv = 1.f / sqrtf(sum_of_lanes<LANES>(ss) / static_cast<float>(a.D) + a.eps);
     }
     if (h >= a.H) continue;
     T* p = out + static_cast<int64_t>(h) * a.D;

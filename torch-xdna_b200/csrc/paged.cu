@@ -152,7 +152,7 @@ __device__ __forceinline__ float row_inverse(const float (*f)[2 * V], float eps)
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
     ss += squares<2 * V>(f[k]);
   }
-  return rsqrtf(sum_of_lanes<RowShape<D, V>::kLanes>(ss) * (1.f / D) + eps);
+  return 1.f / sqrtf(sum_of_lanes<RowShape<D, V>::kLanes>(ss) * (1.f / D) + eps);
 }
 template <int D, int V>
 __device__ __forceinline__ void norm_row(float (*f)[2 * V], const UnitAt* u, const void* norm, int dtype, int64_t at, float inverse) {
@@ -198,10 +198,6 @@ __device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V
       const float2 y = __fmul2_rn(make_float2(f[k][i], f[k][i + 1]), make_float2(inverse, inverse));
       x[i] = y.x, x[i + 1] = y.y;
     }
-    if (inverse == 0.f) {  // not finite
-#pragma unroll
-      for (int i = 0; i < 2 * V; ++i) x[i] = 0.f;
-    }
     if constexpr (V == 8) {
       *reinterpret_cast<uint2*>(row + u[k].lo) = make_uint2(to_codes<E4M3>(x[0], x[1], x[2], x[3]), to_codes<E4M3>(x[4], x[5], x[6], x[7]));
       *reinterpret_cast<uint2*>(row + u[k].hi) = make_uint2(to_codes<E4M3>(x[8], x[9], x[10], x[11]), to_codes<E4M3>(x[12], x[13], x[14], x[15]));
@@ -212,8 +208,14 @@ __device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V
     }
   }
 }
+// inverse 0: a block that is not finite, whose codes are 0.
 template <int D, int V>
 __device__ __forceinline__ void store_codes(uint8_t* row, const float (*f)[2 * V], const UnitAt* u, float inverse, bool e4m3) {
+  if (inverse == 0.f) {
+    const float zeros[RowShape<D, V>::kUnits][2 * V] = {};
+    store_codes<D, V, false>(row, zeros, u, 0.f);
+    return;
+  }
   e4m3 ? store_codes<D, V, true>(row, f, u, inverse) : store_codes<D, V, false>(row, f, u, inverse);
 }
 
@@ -351,7 +353,7 @@ __device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t item, Pag
 // several heads at once), stays in registers between the search for its largest value and its codes, while the next heads'
 // part is on its way. The angles' cosines and sines, which are those of all heads, are worked out once, in shared memory.
 template <typename T, int D, int V, bool INTER, int MOST>
-__global__ void __launch_bounds__(kAppendThreads) append_packed_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, V == 8 ? (MOST <= 2 ? 3 : 2) : 1) append_packed_kernel(const AppendArgs a) {
   using S = RowShape<D, V>;
   constexpr int kAtOnce = kAppendThreads / 32 * S::kRows;       // rows of lanes
   constexpr int kSplit = D / (2 * V), kPitch = D / 2 + D / 16;  // of a token's turns; a lane's are kSplit apart
@@ -466,7 +468,7 @@ static int launch_append_as(AppendArgs a, int sms, cudaStream_t s) {
   // pages that n tokens of N sequences can touch
   const int64_t items = std::min(a.tokens, a.tokens / a.page + 2 * static_cast<int64_t>(a.n_seqs));
   a.heads = std::min(a.hkv, 32);
-  while (a.heads > 1 && items * 2 * ((a.hkv + a.heads - 1) / a.heads) < 6 * sms) a.heads = (a.heads + 1) / 2;
+  while (a.heads > 1 && items * 2 * ((a.hkv + a.heads - 1) / a.heads) < 3 * sms) a.heads = (a.heads + 1) / 2;
   constexpr int kAtOnce = kAppendThreads / 32 * RowShape<D, V>::kRows;
   const int rounds = a.page / kAtOnce;  // tokens of a page for each row of lanes
   const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>((a.hkv + a.heads - 1) / a.heads), 2);

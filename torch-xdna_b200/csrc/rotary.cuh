@@ -92,16 +92,18 @@ __device__ __forceinline__ void load_weights(const void* w, int dtype, int64_t a
 }
 
 // Angles in turns, as 64-bit fractions: a frequency's turns per position, rounded to 2^-56 or better, times the position
-// leaves exactly the part within a turn, whatever the position, and only that is rounded to 32 bits (2^-26 of a turn, 9.4e-8
-// in the angle). cos and sin of it, times factor.
+// leaves exactly the part within a turn, whatever the position. cos and sin of it, times factor: of its upper 24 bits in 32
+// bits, turned on by what is left (below 2^-24 of half a turn, so to first order).
 __device__ __forceinline__ uint64_t turns_of(float inv_freq) {
   const double turns = static_cast<double>(inv_freq) * 0.15915494309189533577;
   return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
 }
 __device__ __forceinline__ float2 turn_of(uint64_t turns, float factor) {
+  const int32_t high = static_cast<int32_t>(turns >> 32), upper = high & ~0xff;
   float s, c;
-  sincospif(static_cast<float>(static_cast<int32_t>(turns >> 32)) * 4.656612873e-10f, &s, &c);  // 2^-31: half turns
-  return make_float2(c * factor, s * factor);
+  sincospif(static_cast<float>(upper) * 4.656612873e-10f, &s, &c);  // 2^-31: half turns
+  const float rest = (static_cast<float>(high & 0xff) + 0.5f) * 1.4629180792671596e-9f;  // to 2^-32, times pi 2^-31
+  return make_float2(fmaf(-s, rest, c) * factor, fmaf(c, rest, s) * factor);
 }
 
 // Where a lane's unit j of a head lies and which of its pairs turn: V entries from lo and V from hi on, pairs
