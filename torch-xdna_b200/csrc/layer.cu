@@ -246,14 +246,19 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const AddNormArgs a) {
   };
   Pack<TX, V> rx[C];
   Pack<TY, V> ry[C];
+  // a gate of 16 bits for each entry, with the others, not behind the first sum
+  const bool gated = V == 8 && a.gate && a.ld_gate > 0 && a.gate_dtype != XDNA_F32;
+  Pack<__half, V> rg[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int at = first + c * step;
     rx[c] = Pack<TX, V>{};
     ry[c] = Pack<TY, V>{};
+    rg[c] = Pack<__half, V>{};
     if (whole(at)) {
       ry[c] = load_pack<TY, V>(y + at);
       rx[c] = load_pack<TX, V>(x + at);
+      if (gated) rg[c] = load_pack<__half, V>(static_cast<const __half*>(a.gate) + row * a.ld_gate + at);
     } else if constexpr (SHIFT) {
       if (any(at)) {
         float f[V];
@@ -289,7 +294,14 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const AddNormArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] *= g[i];
     }
-    if (a.gate) {
+    if (gated && whole(at)) {
+      if (a.gate_dtype == XDNA_F16)
+        to_floats<__half, V>(rg[c], g);
+      else
+        to_floats<__nv_bfloat16, V>(*reinterpret_cast<const Pack<__nv_bfloat16, V>*>(&rg[c]), g);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] *= g[i];
+    } else if (a.gate) {
       if (SHIFT && a.ld_gate > 0) {
         if (a.gate_dtype == XDNA_F32)
           row_values(static_cast<const float*>(a.gate) + row * a.ld_gate, at, g);
