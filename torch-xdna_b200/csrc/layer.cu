@@ -38,6 +38,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 7) rotary_kernel(const Rota
       if (h < a.H && j0 + k * LANES < units) later[k][0] = load_pack<T, V>(p + u[k].lo), later[k][1] = load_pack<T, V>(p + u[k].hi);
     }
   };
+  const float inv_d = 1.f / static_cast<float>(a.D);
   int h = static_cast<int>(w % a.wpt) * kRows + r;
   load(h);
   const Place at = place_of(a, token);
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 7) rotary_kernel(const Rota
       float ss = 0.f;
 #pragma unroll
       for (int k = 0; k < U; ++k) ss += squares<2 * V>(f[k]);
-      inv = 1.f / sqrtf(sum_of_lanes<LANES>(ss) / static_cast<float>(a.D) + a.eps);
+      inv = inverse_root(fmaf(sum_of_lanes<LANES>(ss), inv_d, a.eps));
     }
     if (h >= a.H) continue;
     T* p = out + static_cast<int64_t>(h) * a.D;

@@ -152,7 +152,7 @@ __device__ __forceinline__ float row_inverse(const float (*f)[2 * V], float eps)
   for (int k = 0; k < RowShape<D, V>::kUnits; ++k) {
     ss += squares<2 * V>(f[k]);
   }
-  return 1.f / sqrtf(sum_of_lanes<RowShape<D, V>::kLanes>(ss) * (1.f / D) + eps);
+  return inverse_root(fmaf(sum_of_lanes<RowShape<D, V>::kLanes>(ss), 1.f / D, eps));
 }
 template <int D, int V>
 __device__ __forceinline__ void norm_row(float (*f)[2 * V], const UnitAt* u, const void* norm, int dtype, int64_t at, float inverse) {

@@ -144,7 +144,8 @@ __device__ __forceinline__ void turn_unit(float (&x)[2 * V], const float (&c)[V]
   }
 }
 
-// x *= by * w.
+// x *= by * w, and the sum of squares. (Two at a time, as in turn_unit, the registers cost more than the instructions saved:
+// cache_append of 12968 tokens 40.7 us instead of 32.3.)
 template <int N>
 __device__ __forceinline__ void scale_by(float* x, float by, const float* w) {
 #pragma unroll
@@ -156,6 +157,12 @@ __device__ __forceinline__ float squares(const float* x) {
 #pragma unroll
   for (int i = 0; i < N; ++i) s = fmaf(x[i], x[i], s);
   return s;
+}
+
+// 1 / sqrt(x): rsqrtf (2 ulp) and one step of Newton's method, y + y / 2 * (1 - x y^2), which leaves about one ulp.
+__device__ __forceinline__ float inverse_root(float x) {
+  const float y = rsqrtf(x);
+  return x > 1e-37f && x < 3e38f ? fmaf(0.5f * y, fmaf(-x * y, y, 1.f), y) : y;
 }
 
 // The sum over LANES neighbouring lanes, on all of them.
