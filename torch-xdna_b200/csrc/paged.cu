@@ -223,7 +223,8 @@ constexpr int kAppendThreads = 256;
 
 // One token of each sequence: a block of threads per token, whose rows are its query heads, its keys and its values.
 // Latency is what counts: everything of a row is asked for at once, and only a block whose scale grows (a few times in a
-// page) is read and written again, by the whole warp.
+// page) is read and written again, by the whole warp. One token with 16 query heads over 8 of 128: 3.0 us in a graph; 128
+// of them in pages of 16: 3.7.
 template <typename T, int D, int V, bool INTER>
 __global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const AppendArgs a) {
   using S = RowShape<D, V>;
@@ -352,6 +353,9 @@ __device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t item, Pag
 // (blockIdx.y). A head's part of the page, MOST tokens for each of a block's rows of lanes (pages of fewer tokens than rows:
 // several heads at once), stays in registers between the search for its largest value and its codes, while the next heads'
 // part is on its way. The angles' cosines and sines, which are those of all heads, are worked out once, in shared memory.
+// 12968 tokens of 16 prompts, 8 heads of 128 in bf16, pages of 64: 31 us, 3.0 TB/s (pages of 16: 33, of 128: 32). 60 % of
+// the issue slots are busy; without norm and rotation 26 us. Norm and rotation done twice, so that what was read stays in
+// 16 bits: 48 us; one kernel for all page sizes, with rounds for 128 tokens in each: 47 (pages of 16: 160).
 template <typename T, int D, int V, bool INTER, int MOST>
 __global__ void __launch_bounds__(kAppendThreads, V == 8 ? (MOST <= 2 ? 3 : 2) : 1) append_packed_kernel(const AppendArgs a) {
   using S = RowShape<D, V>;
