@@ -312,7 +312,7 @@ void check_freq(const char* name, const std::optional<at::Tensor>& f, int64_t d)
 
 // A norm's weights: [D], or [H, D] with one row per head.
 void check_norm(const char* name, const char* what, const std::optional<at::Tensor>& w, int64_t h, int64_t d) {
-  REQUIRE(!w || (code(w->scalar_type()) >= 0 && w->size(-1) == d && (w->dim() == 1 || (w->dim() == 2 && w->size(0) == h))), XDNA_ERR_INVALID,
+  REQUIRE(!w || (code(w->scalar_type()) >= 0 && (w->dim() == 1 || (w->dim() == 2 && w->size(0) == h)) && w->size(-1) == d), XDNA_ERR_INVALID,
           what << ": [" << d << "] or [" << h << ", " << d << "] in f32, bf16 or f16");
 }
 

@@ -503,6 +503,7 @@ struct PagedArgs {
   float scale_log2;
   int* err;
   int B, T, hkv, group, page_shift, pages, max_pages;
+  int splits;            // CLUSTER: CTAs of an item
   int col_groups, cols;  // columns: query heads of a key head times T; of an item 8 * NT of them
   void* out;             // [B, T, hq, D]
   int4* shared;          // per item: the first and the last warp that has a part of it, the first one's slot
@@ -513,7 +514,10 @@ struct PagedArgs {
 constexpr int kPaWarps = 4;
 constexpr int kPaTile = 32;      // keys of a warp's step
 constexpr int kPaSite = 70;      // of its waits, in the device error word
-constexpr int kPaShort = 1024;   // keys that the table can hold, up to which a share is of a warp
+constexpr int kMostSplits = 8;   // CTAs of a cluster
+// Units of 128 keys up to which items go to clusters, where those fit the SMs. One sequence, 16 heads over 8 of 128, with
+// clusters and without: of 764 keys 6.4 and 7.9 us, of 2000 8.1 and 8.6, of 4000 10.5 and 9.3; 16 of up to 300: 7.3 and 9.1.
+constexpr int kClusterUnits = 20;
 constexpr float kPaSlack = 8.f;  // how far (log2) a score may pass the reference before that is raised
 
 template <int D, int NT>
@@ -524,7 +528,7 @@ struct PaShape {
   static constexpr int kCtas = NT == 1 ? 3 : 2;
   static constexpr int kStages = (NT == 1 ? 16384 : 24576) / (2 * kHalf);
   static constexpr int kRing = kPaWarps * kStages * 2 * kHalf, kSmem = kRing + 1024;  // aligned to 1024
-  static_assert(kRing >= kPaWarps * 8 * NT * (D + 4) * 4, "the warps' sums lie where the ring was");
+  static_assert(kRing >= (kPaWarps + 1) * 8 * NT * (D + 4) * 4, "the warps' sums, and a cluster's part, lie where the ring was");
   // Tiles lie in shared memory row by row, swizzled by TMA: 16-byte piece p of row r is at p ^ turn(r). So that no load of
   // a warp meets itself in a bank, row g of a fragment is key row(g) of its block, and lane group g takes part(g) of a
   // value row.
@@ -581,15 +585,27 @@ __device__ __forceinline__ float sum_of_groups(float x) {  // over the lanes wit
   return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
+enum { PAGED_WARPS, PAGED_TOGETHER, PAGED_CLUSTER };  // how paged_kernel shares out its work
+
+__device__ __forceinline__ float4 load_remote(uint32_t cluster_address) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(cluster_address)
+               : "memory");
+  return x;
+}
+
 // Attention of B sequences with T query tokens each (the last T of the sequence) over the paged cache. Few rows, so its
 // time is the reading of the codes. The work is all tiles of 32 keys of all (sequence, key head, 8 NT columns), in that
 // order, shared out evenly, whatever the lengths are; they are read on the device. A share begins and ends inside an item
 // as it comes; parts of items go to the workspace and are joined by paged_join_kernel (joined by the last one to write a
 // part, 0.5 to 6 us slower: its loads wait for one another behind the whole item).
-// TOGETHER: a share is of a CTA, whose warps take the tiles of a unit of 128 keys and add up at an item's end, so there are few
-// parts. Otherwise a share is of a warp, whose copies run on across the borders of items, so that many short sequences
-// keep the memory as busy as a long one. Which one goes by the longest sequence that the table can hold (kPaShort) and
-// by whether there are enough items.
+// PAGED_TOGETHER: a share is of a CTA, whose warps take the tiles of a unit of 128 keys and add up at an item's end, so there
+// are few parts. PAGED_WARPS: a share is of a warp, whose copies run on across the borders of items, so that many short
+// sequences keep the memory as busy as a long one. PAGED_CLUSTER: few items of few keys, where a second launch costs more
+// than the work: a cluster of up to eight CTAs has one item, as together, and joins its parts in their shared memory. Which
+// one goes by the longest sequence that the table can hold and by the number of items (plan, below).
 // 200 sequences of up to 300 keys, 16 heads over 8 of 128, e4m3: 27.8 us with warps' shares, 40.3 with CTAs'; 32 of 1175 to
 // 4700: 41.1 us (4.8 TB/s) with CTAs' shares, 43 with warps'. One of 131071: 52 us, 5.1 TB/s; while it runs the memory is
 // busy throughout (7 TB/s and more over the tiles), the rest is the start (lengths, pages and tiles wait for one another,
@@ -604,11 +620,12 @@ __device__ __forceinline__ float sum_of_groups(float x) {  // over the lanes wit
 // goes into the exponent of the weights that meet V, 2^(s + e - m'), with a running maximum m' of its own, so that
 // weights of 16 bits are full where they count, whatever the blocks' scales; the softmax's sum has 2^(s - m). Both are
 // raised, and the sums rescaled, only when a score passes them by more than 2^8.
-template <typename T, int D, bool E4M3, int NT, bool TOGETHER>
+template <typename T, int D, bool E4M3, int NT, int MODE>
 __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
     paged_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using S = PaShape<D, NT>;
   constexpr unsigned kAll = 0xffffffffu;
+  constexpr bool TOGETHER = MODE != PAGED_WARPS, CLUSTER = MODE == PAGED_CLUSTER;
   constexpr int kCols = 8 * NT, kSteps = D / 16, kKeys = TOGETHER ? kPaTile * kPaWarps : kPaTile;  // of a unit
   extern __shared__ __align__(16) uint8_t paged_smem[];
   __shared__ __align__(8) uint64_t bars[kPaWarps][S::kStages];
@@ -638,14 +655,14 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
   auto units_of = [&](int b) { return b < a.B ? (paged_len(a, b) + kKeys - 1) / kKeys : 0; };
   int64_t units = 0;
 #pragma unroll 4
-  for (int b0 = 0; b0 < a.B; b0 += 32) units += __reduce_add_sync(kAll, units_of(b0 + lane));
+  for (int b0 = 0; b0 < a.B && !CLUSTER; b0 += 32) units += __reduce_add_sync(kAll, units_of(b0 + lane));
   const Shares all(units * per_b, TOGETHER ? grid : grid * kPaWarps);
   const int share = TOGETHER ? static_cast<int>(blockIdx.x) : warp * grid + static_cast<int>(blockIdx.x);
-  const int64_t end = all.begin(share + 1);
-  const int64_t start = all.begin(share);
+  int64_t end = all.begin(share + 1);
+  const int64_t start = CLUSTER ? 0 : all.begin(share);
   ItemAt it;  // what is worked on
   it.b = 0, it.base = 0;
-  for (int64_t base = 0; start < end; it.b += 32) {
+  for (int64_t base = 0; !CLUSTER && start < end; it.b += 32) {
     const int mine = units_of(it.b + lane);
     int upto = mine;  // of the lanes up to this one
 #pragma unroll
@@ -663,17 +680,26 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
     base += __shfl_sync(kAll, upto, 31);
   }
   // sequences without keys
-  for (int b = warp * grid + static_cast<int>(blockIdx.x); b < a.B; b += grid * kPaWarps) {
+  for (int b = warp * grid + static_cast<int>(blockIdx.x); b < a.B && !CLUSTER; b += grid * kPaWarps) {
     if (units_of(b) > 0) continue;
     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + static_cast<int64_t>(b) * a.T * a.hkv * a.group * D);
     for (int64_t i = lane; i < static_cast<int64_t>(a.T) * a.hkv * a.group * (D / 8); i += 32) dst[i] = make_uint4(0, 0, 0, 0);
     for (int i = lane; i < per_b; i += 32) a.shared[static_cast<int64_t>(b) * per_b + i] = make_int4(0, 0, 0, 0);
   }
-  if (start >= end) return;
+  if constexpr (CLUSTER) {  // this CTA's part of its cluster's item
+    const int item = static_cast<int>(blockIdx.x) / a.splits, rank = static_cast<int>(blockIdx.x) % a.splits;
+    it.b = item / per_b, it.hc = item % per_b;
+    it.load(a, kKeys);
+    it.unit = static_cast<int>(static_cast<int64_t>(rank) * it.units / a.splits);
+    it.stop = static_cast<int>(static_cast<int64_t>(rank + 1) * it.units / a.splits);
+    end = it.stop - it.unit;
+  } else if (start >= end) {
+    return;
+  }
 
   // ---- the copies
   const int first_key = TOGETHER ? warp * kPaTile : 0;  // of this warp's tile of a unit
-  it.load(a, kKeys);
+  if constexpr (!CLUSTER) it.load(a, kKeys);
   ItemAt next = it;                              // next.unit is to be copied next
   next.unit = next.stop = 0;
   int left = static_cast<int>(end - start), more = left;  // units to be worked on, and to be copied (not TOGETHER)
@@ -734,8 +760,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
   bool first = true;
   int st = 0;  // the stage of the next tile, and the parity of its barrier
   uint32_t parity = 0;
-  while (left > 0) {
-    it.go(a, kKeys, per_b, end - left, end);
+  for (bool once = true; CLUSTER ? once : left > 0; once = false) {
+    if constexpr (!CLUSTER) it.go(a, kKeys, per_b, end - left, end);
     const int len = it.len, begin = it.unit;
     const int h = it.hc / a.col_groups, c0 = (it.hc % a.col_groups) * kCols;
     Pack<T, 4> raw[NT][kSteps];  // the queries, on their way while the pages are looked up
@@ -961,12 +987,13 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
         mbar_wait(&bars[warp][st], parity, &never, a.err, kPaSite);
         if (++st == S::kStages) st = 0, parity ^= 1;
       }
-      return;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if constexpr (!CLUSTER) return;  // a cluster's CTAs still meet; what they write then is of no use
     }
     // ---- the item's sums, or a part of them; a share has at most two parts of items
     const int64_t slot = 2 * static_cast<int64_t>(share) + (first ? 0 : 1), item = static_cast<int64_t>(it.b) * per_b + it.hc;
-    const bool whole_item = begin == 0 && it.stop == it.units;
-    if (begin == 0 && lane == 0 && (warp == 0 || !TOGETHER))
+    const bool whole_item = !CLUSTER && begin == 0 && it.stop == it.units;
+    if (!CLUSTER && begin == 0 && lane == 0 && (warp == 0 || !TOGETHER))
       a.shared[item] = make_int4(share, whole_item ? share : all.owner(end - left + it.units - 1), static_cast<int>(slot), 0);
     auto row_of = [&](int col) {
       return static_cast<T*>(a.out) + ((static_cast<int64_t>(it.b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D;
@@ -1000,6 +1027,8 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
       }
     }
     if constexpr (TOGETHER) {
+      float* mine_o = &so[kPaWarps][0][0];  // CLUSTER: this CTA's part
+      float4* mine_ml = reinterpret_cast<float4*>(mine_o + kCols * D);
       __syncthreads();
       for (int i = threadIdx.x; i < min(kCols, a.cols - c0) * (D / 4); i += kPaWarps * 32) {
         const int c = i / (D / 4), d = (i % (D / 4)) * 4;
@@ -1015,7 +1044,10 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
           const float4 x = *reinterpret_cast<const float4*>(&so[w][c][d]);
           acc[0] = fmaf(f, x.x, acc[0]), acc[1] = fmaf(f, x.y, acc[1]), acc[2] = fmaf(f, x.z, acc[2]), acc[3] = fmaf(f, x.w, acc[3]);
         }
-        if (whole_item) {
+        if constexpr (CLUSTER) {
+          store_pack<float, 4>(&mine_o[c * D + d], from_floats<float, 4>(acc));
+          if (d == 0) mine_ml[c] = make_float4(mm, ll, mmv, 0.f);
+        } else if (whole_item) {
           const float inv = inverse_of(mm, ll, mmv);
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * inv);
@@ -1025,8 +1057,41 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
           if (d == 0) a.part_ml[slot * kCols + c] = make_float4(mm, ll, mmv, 0.f);
         }
       }
-      fence_async_smem();  // the sums, before TMA writes there again
-      __syncthreads();
+      if constexpr (CLUSTER) {
+        __syncwarp();
+        cluster_sync();
+        const int rank = static_cast<int>(blockIdx.x) % a.splits;
+        for (int i = rank * kPaWarps * 32 + static_cast<int>(threadIdx.x); i < min(kCols, a.cols - c0) * (D / 4); i += a.splits * kPaWarps * 32) {
+          const int c = i / (D / 4), d = (i % (D / 4)) * 4;
+          float4 ml[kMostSplits], x[kMostSplits];
+          float mm = -INFINITY, mmv = -INFINITY, ll = 0.f;
+#pragma unroll
+          for (int r = 0; r < kMostSplits; ++r) {
+            const int from = min(r, a.splits - 1);
+            ml[r] = load_remote(cluster_addr(mine_ml + c, from));
+            x[r] = load_remote(cluster_addr(mine_o + c * D + d, from));
+            mm = fmaxf(mm, ml[r].x), mmv = fmaxf(mmv, ml[r].z);
+          }
+          const float m0 = mm == -INFINITY ? 0.f : mm, v0 = mmv == -INFINITY ? 0.f : mmv;
+          float acc[4] = {};
+#pragma unroll
+          for (int r = 0; r < kMostSplits; ++r) {
+            if (r >= a.splits) break;
+            ll = fmaf(fast_exp2(ml[r].x - m0), ml[r].y, ll);
+            const float f = fast_exp2(ml[r].z - v0);
+            acc[0] = fmaf(f, x[r].x, acc[0]), acc[1] = fmaf(f, x[r].y, acc[1]), acc[2] = fmaf(f, x[r].z, acc[2]), acc[3] = fmaf(f, x[r].w, acc[3]);
+          }
+          const float inv = inverse_of(mm, ll, mmv);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * inv);
+          store_pack<T, 4>(row_of(c0 + c) + d, from_floats<T, 4>(acc));
+        }
+        __syncwarp();
+        cluster_sync();  // the others have read this CTA's part
+      } else {
+        fence_async_smem();  // the sums, before TMA writes there again
+        __syncthreads();
+      }
     }
     first = false;
     left -= it.stop - begin;
@@ -1110,9 +1175,9 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int6
   store_pack<T, kV>(dst + lane * kV, from_floats<T, kV>(acc));
 }
 
-// CTAs of a call, and where its workspace's parts lie.
+// How a call's work is shared out, its CTAs, and where its workspace's parts lie.
 struct PagedPlan {
-  int nt, col_groups;
+  int nt, col_groups, mode, splits;
   int64_t items, ctas, ml_at, o_at, bytes;
   PagedPlan(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys, int sms) {
     const int64_t cols = hq / hkv * T;
@@ -1120,9 +1185,18 @@ struct PagedPlan {
     // keys with 4 tokens and 7 heads per key head took 21.2 us with four and 20.3 with two (of up to 12000: 38.5 and 43.7)
     nt = cols <= 8 ? 1 : 2;
     col_groups = static_cast<int>((cols + 8 * nt - 1) / (8 * nt));
-    const int64_t most = B * hkv * col_groups * ((most_keys + kPaTile - 1) / kPaTile);
-    ctas = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sms) * (nt == 1 ? 3 : 2), most));
     items = B * hkv * col_groups;
+    const int64_t resident = static_cast<int64_t>(sms) * (nt == 1 ? 3 : 2), units = (most_keys + kPaTile * kPaWarps - 1) / (kPaTile * kPaWarps);
+    splits = static_cast<int>(std::min<int64_t>(kMostSplits, std::max<int64_t>(units, 1)));
+    if (units <= kClusterUnits && items * splits <= resident) {
+      mode = PAGED_CLUSTER;
+      ctas = items * splits;
+      ml_at = o_at = bytes = 0;
+      return;
+    }
+    mode = most_keys > 1024 || items < resident ? PAGED_TOGETHER : PAGED_WARPS;
+    splits = 0;
+    ctas = std::max<int64_t>(1, std::min(resident, items * ((most_keys + kPaTile - 1) / kPaTile)));
     ml_at = (items * 16 + 255) / 256 * 256;
     o_at = ml_at + 2 * ctas * kPaWarps * 8 * nt * 16;
     bytes = o_at + 2 * ctas * kPaWarps * 8 * nt * d * 4;
@@ -1141,33 +1215,50 @@ static int codes_map(CUtensorMap* m, const void* codes, int64_t sp, int64_t page
                     d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-template <typename T, int D, bool E4M3, int NT, bool TOGETHER>
+template <typename T, int D, bool E4M3, int NT, int MODE>
 static int launch_paged_as(const PagedArgs& a, const PagedMaps& maps, int ctas, cudaStream_t s) {
   using S = PaShape<D, NT>;
-  auto kern = paged_kernel<T, D, E4M3, NT, TOGETHER>;
+  auto kern = paged_kernel<T, D, E4M3, NT, MODE>;
   static std::atomic<bool> allowed[64];
   int rc = allow_shared(allowed, kern, S::kSmem);
   if (rc != XDNA_OK) return rc;
-  kern<<<static_cast<unsigned>(ctas), kPaWarps * 32, S::kSmem, s>>>(a, maps.k, maps.v);
-  if ((rc = check_launch("paged_kernel")) != XDNA_OK) return rc;
-  const int64_t items = static_cast<int64_t>(a.B) * a.hkv * a.col_groups;
-  const int64_t rows = items * std::min(8 * NT, a.cols);
-  return rows < 4 * 148
-             ? launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, s, a, items)
-             : launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, a, items);
+  if constexpr (MODE == PAGED_CLUSTER) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(kPaWarps * 32);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(a.splits);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    XDNA_CUDA(cudaLaunchKernelEx(&cfg, kern, a, maps.k, maps.v));
+    return check_launch("paged_kernel");
+  } else {
+    kern<<<static_cast<unsigned>(ctas), kPaWarps * 32, S::kSmem, s>>>(a, maps.k, maps.v);
+    if ((rc = check_launch("paged_kernel")) != XDNA_OK) return rc;
+    const int64_t items = static_cast<int64_t>(a.B) * a.hkv * a.col_groups;
+    const int64_t rows = items * std::min(8 * NT, a.cols);
+    return rows < 4 * 148
+               ? launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, s, a, items)
+               : launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, a, items);
+  }
 }
 
 template <typename T, int D, bool E4M3, int NT>
-static int launch_paged_as(const PagedArgs& a, const PagedMaps& m, int ctas, cudaStream_t s) {
-  const bool together = (static_cast<int64_t>(a.max_pages) << a.page_shift) > kPaShort || static_cast<int64_t>(a.B) * a.hkv * a.col_groups < ctas;
-  return together ? launch_paged_as<T, D, E4M3, NT, true>(a, m, ctas, s)
-                  : launch_paged_as<T, D, E4M3, NT, false>(a, m, ctas, s);
+static int launch_paged_as(const PagedArgs& a, const PagedMaps& m, const PagedPlan& plan, cudaStream_t s) {
+  const int ctas = static_cast<int>(plan.ctas);
+  if (plan.mode == PAGED_CLUSTER) return launch_paged_as<T, D, E4M3, NT, PAGED_CLUSTER>(a, m, ctas, s);
+  return plan.mode == PAGED_TOGETHER ? launch_paged_as<T, D, E4M3, NT, PAGED_TOGETHER>(a, m, ctas, s)
+                                     : launch_paged_as<T, D, E4M3, NT, PAGED_WARPS>(a, m, ctas, s);
 }
 
 template <typename T, int D>
-static int launch_paged(const PagedArgs& a, const PagedMaps& m, bool e4m3, int nt, int ctas, cudaStream_t s) {
-  if (nt == 1) return e4m3 ? launch_paged_as<T, D, true, 1>(a, m, ctas, s) : launch_paged_as<T, D, false, 1>(a, m, ctas, s);
-  return e4m3 ? launch_paged_as<T, D, true, 2>(a, m, ctas, s) : launch_paged_as<T, D, false, 2>(a, m, ctas, s);
+static int launch_paged(const PagedArgs& a, const PagedMaps& m, bool e4m3, const PagedPlan& plan, cudaStream_t s) {
+  if (plan.nt == 1) return e4m3 ? launch_paged_as<T, D, true, 1>(a, m, plan, s) : launch_paged_as<T, D, false, 1>(a, m, plan, s);
+  return e4m3 ? launch_paged_as<T, D, true, 2>(a, m, plan, s) : launch_paged_as<T, D, false, 2>(a, m, plan, s);
 }
 
 // ---------------------------------------------------------------------------- host
@@ -1270,7 +1361,7 @@ int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
                  "paged_attention: null pointer, unaligned rows or bad strides");
   const PagedPlan plan(B, T, hq, hkv, d, max_pages * page, sms);
   XDNA_CHECK_ARG(plan.items < (1ll << 31) && plan.items * (max_pages * page / kPaTile + 1) / plan.ctas < (1ll << 31), "paged_attention: bad sizes");
-  XDNA_CHECK_ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_bytes >= static_cast<size_t>(plan.bytes),
+  XDNA_CHECK_ARG(plan.bytes == 0 || (workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0 && workspace_bytes >= static_cast<size_t>(plan.bytes)),
                  "paged_attention: workspace too small or unaligned");
   PagedArgs a{};
   a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
@@ -1278,7 +1369,7 @@ int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
   a.table = table, a.ld_table = ld_table, a.lens = lens, a.scale_log2 = scale * kLog2E;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.hkv = static_cast<int>(hkv), a.group = static_cast<int>(hq / hkv);
   a.page_shift = shift_of(page), a.pages = static_cast<int>(pages), a.max_pages = static_cast<int>(max_pages);
-  a.col_groups = plan.col_groups, a.cols = static_cast<int>(a.group * T);
+  a.splits = plan.splits, a.col_groups = plan.col_groups, a.cols = static_cast<int>(a.group * T);
   a.out = out;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.shared = reinterpret_cast<int4*>(ws);
@@ -1290,11 +1381,10 @@ int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
     if ((rc = codes_map(&maps.v, v_codes, vc_sp, pages, hkv, page, d)) != XDNA_OK) return rc;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int ctas = static_cast<int>(plan.ctas);
   const bool e4m3 = format == XDNA_E4M3;
   if (dtype == XDNA_BF16)
-    return d == 64 ? launch_paged<__nv_bfloat16, 64>(a, maps, e4m3, plan.nt, ctas, s) : launch_paged<__nv_bfloat16, 128>(a, maps, e4m3, plan.nt, ctas, s);
-  return d == 64 ? launch_paged<__half, 64>(a, maps, e4m3, plan.nt, ctas, s) : launch_paged<__half, 128>(a, maps, e4m3, plan.nt, ctas, s);
+    return d == 64 ? launch_paged<__nv_bfloat16, 64>(a, maps, e4m3, plan, s) : launch_paged<__nv_bfloat16, 128>(a, maps, e4m3, plan, s);
+  return d == 64 ? launch_paged<__half, 64>(a, maps, e4m3, plan, s) : launch_paged<__half, 128>(a, maps, e4m3, plan, s);
 }
 
 }  // extern "C"
