@@ -73,6 +73,17 @@ def test_add_norm_refusals():
         f(x, x, w, w, w)
 
 
+def test_weights_of_no_dimension():
+    one, c, t, n = torch.tensor(1.0), cache(), z(3, 2, dtype=torch.int32), i32(3)
+    refuse(torch_xdna.rotary, z(5, 4, 64), i32(5), f32(32), norm=one, match="norm")
+    refuse(torch_xdna.rotary, z(5, 4, 64), i32(5), one, match="inv_freq")
+    refuse(torch_xdna.add_norm, z(3, 100), z(3, 100), one, match="weight")
+    refuse(torch_xdna.add_norm, z(3, 100), z(3, 100), f32(100), post=one, match="post")
+    refuse(torch_xdna.add_norm, z(3, 100), z(3, 100), f32(100), gate=one, match="gate")
+    refuse(torch_xdna.cache_append, z(3, 2, 64), z(3, 2, 64), *c, t, n, k_norm=one, match="k_norm")
+    refuse(torch_xdna.cache_append, z(3, 2, 64), z(3, 2, 64), *c, t, n, q=z(3, 4, 64), q_norm=one, match="q_norm")
+
+
 def test_paged_cache():
     for dtype in (torch.int8, E4):
         c = cache(3, 5, 32, 128, dtype)

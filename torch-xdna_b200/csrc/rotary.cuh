@@ -165,12 +165,20 @@ __device__ __forceinline__ float inverse_root(float x) {
   return x > 1e-37f && x < 3e38f ? fmaf(0.5f * y, fmaf(-x * y, y, 1.f), y) : y;
 }
 
-// The sum over LANES neighbouring lanes, on all of them.
+// The sum over LANES neighbouring lanes, from a multiple of LANES on, on all of them. All lanes of the warp.
 template <int LANES>
 __device__ __forceinline__ float sum_of_lanes(float x) {
+  if constexpr ((LANES & (LANES - 1)) == 0) {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  } else {
+    const int first = lane_id() / LANES * LANES;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) sum += __shfl_sync(0xffffffffu, x, (first + i) & 31);
+    return sum;
+  }
 }
 
 }  // namespace xdna
