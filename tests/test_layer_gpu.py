@@ -99,6 +99,19 @@ def test_rotary(cuda, dtype, interleaved, d, n):
         close(got, want, tol + rounding(want, dtype))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,n", [(48, 24), (64, 8), (80, 40), (96, 48), (112, 56)])
+def test_rotary_heads_of_a_few_lanes(cuda, d, n, interleaved):
+    """Rounds of as many heads as their lanes let into a warp, the last one part full, one warp per token and several."""
+    import torch_xdna
+
+    for t, h in ((2, 7), (5, 13), (4801, 11), (4801, 31)):
+        x, f, pos = randn(t, h, d, seed=d + h), freqs(n), torch.arange(t, device="cuda")
+        norm = randn(h, d, seed=2, dtype=torch.float32) if h != 13 else None
+        want, tol = turned(x, pos, f, 1.0, interleaved, norm)
+        close(torch_xdna.rotary(x, pos, f, 1.0, interleaved, norm), want, tol + rounding(want, x.dtype))
+
+
 def test_rotary_far_and_negative_positions(cuda):
     """Angles far out are those of the exact product, for either type of positions."""
     import torch_xdna
@@ -574,6 +587,19 @@ def test_paged_at_the_borders_of_its_manners(cuda, fmt, hq, hkv, d, t):
         table = table_of(counts, sum(counts) + 1)
         assert table.shape[1] * page == keys
         check_attention(randn(b, t, hq, d, seed=keys) if t > 1 else randn(b, hq, d, seed=keys), c, table, lens)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,t,d", [(2, 1, 128), (10, 2, 64)])
+@pytest.mark.parametrize("b,keys", [(370, 1024), (443, 256), (190, 896), (125, 960), (90, 1024), (77, 640), (60, 2048), (50, 2048), (40, 1920)])
+def test_paged_as_many_sequences_as_the_multiprocessors_hold(cuda, fmt, hq, t, d, b, keys):
+    """One to eight blocks of threads for each sequence, with lengths from none to the table's and parts without a key."""
+    g = torch.Generator().manual_seed(b)
+    lens = [keys, 0, 1, keys - 1] + torch.randint(0, keys, (b - 4,), generator=g).tolist()
+    counts = [-(-n // 64) for n in lens]
+    c = filled(sum(counts) + 1, 1, 64, d, fmt, seed=b)
+    table = table_of(counts, sum(counts) + 1)
+    check_attention(randn(b, t, hq, d, seed=keys), c, table, lens)
 
 
 def test_paged_lengths_and_pages_that_are_none(cuda):

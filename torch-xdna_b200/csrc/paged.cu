@@ -471,10 +471,13 @@ static int launch_append_as(AppendArgs a, int sms, cudaStream_t s) {
   }
   // pages that n tokens of N sequences can touch
   const int64_t items = std::min(a.tokens, a.tokens / a.page + 2 * static_cast<int64_t>(a.n_seqs));
+  // heads of a block: few enough that the SMs have blocks (pages of 128 as above: 31.7 us, all 8 heads in a block 40.8)
   a.heads = std::min(a.hkv, 32);
   while (a.heads > 1 && items * 2 * ((a.hkv + a.heads - 1) / a.heads) < 3 * sms) a.heads = (a.heads + 1) / 2;
   constexpr int kAtOnce = kAppendThreads / 32 * RowShape<D, V>::kRows;
-  const int rounds = a.page / kAtOnce;  // tokens of a page for each row of lanes
+  // tokens of a page for each row of lanes; registers for four at pages of 64, that need two: 42.8 us instead of 31.3, of 32:
+  // 64.8 instead of 32.4
+  const int rounds = a.page / kAtOnce;
   const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>((a.hkv + a.heads - 1) / a.heads), 2);
   if constexpr (V == 1)
     return launch_packed<T, D, V, INTER, 16>(a, grid, s);
@@ -506,18 +509,20 @@ struct PagedArgs {
   int splits;            // CLUSTER: CTAs of an item
   int col_groups, cols;  // columns: query heads of a key head times T; of an item 8 * NT of them
   void* out;             // [B, T, hq, D]
-  int4* shared;          // per item: the first and the last warp that has a part of it, the first one's slot
-  float* part_o;         // [2 * warps][8 * NT][D]
-  float4* part_ml;       // [2 * warps][8 * NT]: m, l, m'
+  int4* shared;          // per item: the first and the last share that has a part of it, the first one's slot
+  float* part_o;         // [2 * shares][8 * NT][D]
+  float4* part_ml;       // [2 * shares][8 * NT]: m, l, m'
 };
 
 constexpr int kPaWarps = 4;
 constexpr int kPaTile = 32;      // keys of a warp's step
 constexpr int kPaSite = 70;      // of its waits, in the device error word
 constexpr int kMostSplits = 8;   // CTAs of a cluster
-// Units of 128 keys up to which items go to clusters, where those fit the SMs. One sequence, 16 heads over 8 of 128, with
-// clusters and without: of 764 keys 6.4 and 7.9 us, of 2000 8.1 and 8.6, of 4000 10.5 and 9.3; 16 of up to 300: 7.3 and 9.1.
-constexpr int kClusterUnits = 20;
+// Units of 128 keys of one CTA up to which items go to clusters. 16 heads over 8 of 128, with clusters and without: one
+// sequence of 764 keys 6.4 and 7.9 us, of 2000 8.1 and 8.6; 16 of up to 300: 7.6 and 9.1; 50 of up to 900: 17.7 and 19.3; a
+// share longer than the average, one of 4000: 10.5 and 9.3. Shares of twelve units, whatever the average: 24 sequences of
+// up to 3001 with 28 columns 23.3 and 20.4.
+constexpr int kClusterUnits = 8;
 constexpr float kPaSlack = 8.f;  // how far (log2) a score may pass the reference before that is raised
 
 template <int D, int NT>
@@ -603,18 +608,20 @@ __device__ __forceinline__ float4 load_remote(uint32_t cluster_address) {
 // part, 0.5 to 6 us slower: its loads wait for one another behind the whole item).
 // PAGED_TOGETHER: a share is of a CTA, whose warps take the tiles of a unit of 128 keys and add up at an item's end, so there
 // are few parts. PAGED_WARPS: a share is of a warp, whose copies run on across the borders of items, so that many short
-// sequences keep the memory as busy as a long one. PAGED_CLUSTER: few items of few keys, where a second launch costs more
-// than the work: a cluster of up to eight CTAs has one item, as together, and joins its parts in their shared memory. Which
-// one goes by the longest sequence that the table can hold and by the number of items (plan, below).
+// sequences keep the memory as busy as a long one. PAGED_CLUSTER: items of few keys that the SMs hold all at once, where a
+// second launch costs more than an even share gains: a cluster of up to eight CTAs has one item, as together, and joins its
+// parts in their shared memory. Which one goes by the longest sequence that the table can hold and by the number of items
+// (plan, below).
 // 200 sequences of up to 300 keys, 16 heads over 8 of 128, e4m3: 27.8 us with warps' shares, 40.3 with CTAs'; 32 of 1175 to
 // 4700: 41.1 us (4.8 TB/s) with CTAs' shares, 43 with warps'. One of 131071: 52 us, 5.1 TB/s; while it runs the memory is
 // busy throughout (7 TB/s and more over the tiles), the rest is the start (lengths, pages and tiles wait for one another,
 // 5 us) and the join (3 us).
-// A tile's codes come by TMA into the warp's own ring in shared memory, and the products are mma.sync 16 x 8 x 16 with keys, then dimensions, as rows and the query rows as columns: S^T = K Q^T,
-// O^T = V^T P^T. Of K, lane (g, t) reads bytes 64 c + 16 t .. + 15 of two keys: each word of them is, as two half pairs, A
-// fragments when the queries' B fragments are read in the same order. Of V, D / 8 bytes of four keys: bytes of two keys,
-// paired by byte permutes, are A fragments of output rows in the order of dimensions 2 i (row g of product i) and 2 i + 1
-// (row g + 8) of these D / 8. P^T is S^T's fragment, transposed by movmatrix.
+// A tile's codes come by TMA into the warp's own ring in shared memory, and the products are mma.sync 16 x 8 x 16 with keys,
+// then dimensions, as rows and the query rows as columns: S^T = K Q^T, O^T = V^T P^T. Of K, lane (g, t) reads bytes
+// 64 c + 16 t .. + 15 of two keys: each word of them is, as two half pairs, A fragments when the queries' B fragments are
+// read in the same order. Of V, D / 8 bytes of four keys: bytes of two keys, paired by byte permutes, are A fragments of
+// output rows in the order of dimensions 2 i (row g of product i) and 2 i + 1 (row g + 8) of these D / 8. P^T is S^T's
+// fragment, transposed by movmatrix.
 // Codes are exact in f16, and so are queries of either type after a power of two per row has brought them to about one
 // (bits below 2^-24 of the row's largest apart). The key block's scale goes into the scores. The value block's scale 2^e
 // goes into the exponent of the weights that meet V, 2^(s + e - m'), with a running maximum m' of its own, so that
@@ -977,7 +984,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
           }
         }
       }
-            __syncwarp();
+      __syncwarp();
       fetch(st);  // into the stage just read
       if (++st == S::kStages) st = 0, parity ^= 1;
     }
@@ -1178,22 +1185,31 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int6
 // How a call's work is shared out, its CTAs, and where its workspace's parts lie.
 struct PagedPlan {
   int nt, col_groups, mode, splits;
-  int64_t items, ctas, ml_at, o_at, bytes;
-  PagedPlan(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys, int sms) {
-    const int64_t cols = hq / hkv * T;
-    // tiles of eight columns that a warp takes at once. Heads of 64 have registers for four, but 24 sequences of up to 3001
-    // keys with 4 tokens and 7 heads per key head took 21.2 us with four and 20.3 with two (of up to 12000: 38.5 and 43.7)
-    nt = cols <= 8 ? 1 : 2;
+  int64_t resident, items, ctas, ml_at, o_at, bytes;
+  void shape(int tiles, int64_t B, int64_t hkv, int64_t cols, int sms) {
+    nt = tiles;  // of eight columns that a warp takes at once
     col_groups = static_cast<int>((cols + 8 * nt - 1) / (8 * nt));
     items = B * hkv * col_groups;
-    const int64_t resident = static_cast<int64_t>(sms) * (nt == 1 ? 3 : 2), units = (most_keys + kPaTile * kPaWarps - 1) / (kPaTile * kPaWarps);
-    splits = static_cast<int>(std::min<int64_t>(kMostSplits, std::max<int64_t>(units, 1)));
-    if (units <= kClusterUnits && items * splits <= resident) {
-      mode = PAGED_CLUSTER;
+    resident = static_cast<int64_t>(sms) * (nt == 1 ? 3 : 2);
+  }
+  PagedPlan(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys, int sms) {
+    const int64_t cols = hq / hkv * T, units = (most_keys + kPaTile * kPaWarps - 1) / (kPaTile * kPaWarps);
+    ml_at = o_at = bytes = 0;
+    mode = PAGED_CLUSTER;
+    // as many CTAs per item as the SMs hold (clusters leave some of their places empty: with 288 of 296 taken by threes, 15.6 us
+    // instead of 12.7), where a share of the longest item is about one of all work
+    auto clusters = [&](int tiles) {
+      shape(tiles, B, hkv, cols, sms);
+      splits = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(kMostSplits), units, resident * 7 / 8 / items})));
       ctas = items * splits;
-      ml_at = o_at = bytes = 0;
-      return;
-    }
+      const int64_t longest = (units + splits - 1) / splits;
+      return items <= resident && longest <= kClusterUnits && longest <= (items * units + resident - 1) / resident + 1;
+    };
+    if (clusters(1)) return;
+    // two tiles of columns from nine columns on, which read the cache half as often (24 sequences of up to 12000 keys with 28
+    // columns: 44.3 us, with one tile 51.6; in a cluster, of up to 1000, 12.7 and 11.5). Heads of 64 have registers for
+    // four, but up to 3001 keys took 21.2 us with four and 20.3 with two (of up to 12000: 38.5 and 43.7)
+    if (cols > 8 && clusters(2)) return;
     mode = most_keys > 1024 || items < resident ? PAGED_TOGETHER : PAGED_WARPS;
     splits = 0;
     ctas = std::max<int64_t>(1, std::min(resident, items * ((most_keys + kPaTile - 1) / kPaTile)));
@@ -1241,6 +1257,8 @@ static int launch_paged_as(const PagedArgs& a, const PagedMaps& maps, int ctas, 
     if ((rc = check_launch("paged_kernel")) != XDNA_OK) return rc;
     const int64_t items = static_cast<int64_t>(a.B) * a.hkv * a.col_groups;
     const int64_t rows = items * std::min(8 * NT, a.cols);
+    // 16 rows of many parts (one sequence of 131071): 52.7 us with a block per row, 62.7 with a warp; 2048 rows of two or three
+    // (16 sequences of 680 to 2700 with 4 tokens): 22.0 and 20.3
     return rows < 4 * 148
                ? launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, s, a, items)
                : launch_early("paged_join_kernel", paged_join_kernel<T, D, NT, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, a, items);
