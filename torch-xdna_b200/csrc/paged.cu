@@ -11,6 +11,7 @@
 #include "host_util.h"
 #include "rotary.cuh"
 #include "rotary.h"
+#include "shares.h"
 
 namespace xdna {
 
@@ -507,6 +508,7 @@ struct PagedArgs {
   int* err;
   int B, T, hkv, group, page_shift, pages, max_pages;
   int splits;            // CLUSTER: CTAs of an item
+  int shares;            // else: shares of the work
   int col_groups, cols;  // columns: query heads of a key head times T; of an item 8 * NT of them
   void* out;             // [B, T, hq, D]
   int4* shared;          // per item: the first and the last share that has a part of it, the first one's slot
@@ -545,22 +547,6 @@ struct PaShape {
 __device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
   return static_cast<int>(min(static_cast<int64_t>(max(a.lens[b], 0)), static_cast<int64_t>(a.max_pages) << a.page_shift));
 }
-
-// All units (tiles, or steps of one tile for each of a CTA's warps) in order, shared out evenly: the first `more` shares
-// have one more than the others.
-struct Shares {
-  int64_t work, each, more;
-  __device__ __forceinline__ Shares(int64_t work, uint32_t shares) : work(work) {
-    each = work >> 31 ? work / shares : static_cast<uint32_t>(work) / shares;
-    more = work - each * shares;
-  }
-  __device__ __forceinline__ int64_t begin(int64_t i) const { return i * each + min(i, more); }
-  __device__ __forceinline__ int owner(int64_t unit) const {  // the share that has it
-    const int64_t cut = more * (each + 1), from = unit < cut ? unit : unit - cut, by = unit < cut ? each + 1 : each;
-    const int64_t i = work >> 31 ? from / by : static_cast<uint32_t>(from) / static_cast<uint32_t>(by);
-    return static_cast<int>(unit < cut ? i : more + i);
-  }
-};
 
 // Where a place in the order of all units is: the sequence, its length and units, the units before it (of one head), the
 // (key head, column group), the unit in it, and the item's unit behind the last one of a share that ends at `end`.
@@ -1124,6 +1110,13 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int6
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 it = a.shared[item];
   if (it.x == it.y) return;
+  if (!parts_exist(it.x, it.y, it.z, a.shares)) {  // a wait ran out, which the device error word says
+    float none[kV];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) none[i] = NAN;
+    if (warp == 0) store_pack<T, kV>(dst + lane * kV, from_floats<T, kV>(none));
+    return;
+  }
   float mm = -INFINITY, mmv = -INFINITY, ll = 0.f, acc[kV] = {};
   for (int x0 = it.x + warp; x0 <= it.y; x0 += W * kAhead) {
     float4 ml[kAhead];
@@ -1387,7 +1380,8 @@ int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
   a.table = table, a.ld_table = ld_table, a.lens = lens, a.scale_log2 = scale * kLog2E;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.hkv = static_cast<int>(hkv), a.group = static_cast<int>(hq / hkv);
   a.page_shift = shift_of(page), a.pages = static_cast<int>(pages), a.max_pages = static_cast<int>(max_pages);
-  a.splits = plan.splits, a.col_groups = plan.col_groups, a.cols = static_cast<int>(a.group * T);
+  a.splits = plan.splits, a.shares = static_cast<int>(plan.ctas) * (plan.mode == PAGED_WARPS ? kPaWarps : 1);
+  a.col_groups = plan.col_groups, a.cols = static_cast<int>(a.group * T);
   a.out = out;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.shared = reinterpret_cast<int4*>(ws);
