@@ -469,7 +469,7 @@ int xdna_cache_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, 
  * the last T tokens of each sequence: token t attends to the first lens[b] - T + t + 1 tokens in the cache (lens clamped
  * to 0 .. max_pages * page, which is below 2^30), without those that have no page. A row without any, or with scores of
  * -inf alone, is zero. Scores and sums are f32; the weights that meet V are f16 with an exponent of their own per block
- * (terms below 2^-25 of a row's largest are lost). The work is shared out by the lengths, on the device, in one of three
+ * (terms below 2^-26 of a row's largest lose bits, those below 2^-37 are lost). The work is shared out by the lengths, on the device, in one of three
  * manners by B, the heads and max_pages * page. T is meant to be small: every 16 / (hq / hkv) tokens the cache is read
  * once more. Codes of e4m3 are numbers. workspace: xdna_paged_attention_workspace bytes for most_keys = max_pages * page,
  * 256-byte aligned (0 bytes: NULL). */

@@ -525,7 +525,14 @@ constexpr int kMostSplits = 8;   // CTAs of a cluster
 // share longer than the average, one of 4000: 10.5 and 9.3. Shares of twelve units, whatever the average: 24 sequences of
 // up to 3001 with 28 columns 23.3 and 20.4.
 constexpr int kClusterUnits = 8;
-constexpr float kPaSlack = 8.f;  // how far (log2) a score may pass the reference before that is raised
+constexpr float kPaSlack = 8.f;  // how far (log2) a score may pass the running maximum before that is raised
+// The weights that meet V, rounded to f16, are between 2^12 and 2^15 for the largest (65504 is the most), so that they have
+// all of f16's bits down to 2^-26 of it and are lost from 2^-37 on: many small weights beside a large one count in full.
+// (From 1 on, with a slack of eight, they had all bits down to 2^-14 and were lost from 2^-25 on: a thousand keys of e^-15
+// beside a peak without a value were off by 2.6 %. From 2^14 on the slack is one, and the sums are rescaled more often: 24
+// sequences of up to 3001 with 28 columns 20.8 us instead of 20.4.)
+constexpr float kPaWeight = 12.f, kPaWeightSlack = 3.f;
+constexpr float kPaUnit = 2.44140625e-04f;  // 2^-kPaWeight
 
 template <int D, int NT>
 struct PaShape {
@@ -576,6 +583,13 @@ __device__ __forceinline__ float sum_of_groups(float x) {  // over the lanes wit
   return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
+// What a row's sums with V are to be multiplied with, after kPaUnit: 1 / the softmax's sum, brought from the weights'
+// reference to the scores'.
+__device__ __forceinline__ float inverse_of(float m, float sum, float mv) {
+  const float up = (mv == -INFINITY ? 0.f : mv + kPaWeight) - (m == -INFINITY ? 0.f : m);
+  return sum > 0.f || __isnanf(sum) ? fast_exp2(up) / sum : 0.f;
+}
+
 enum { PAGED_WARPS, PAGED_TOGETHER, PAGED_CLUSTER };  // how paged_kernel shares out its work
 
 __device__ __forceinline__ float4 load_remote(uint32_t cluster_address) {
@@ -610,9 +624,10 @@ __device__ __forceinline__ float4 load_remote(uint32_t cluster_address) {
 // fragment, transposed by movmatrix.
 // Codes are exact in f16, and so are queries of either type after a power of two per row has brought them to about one
 // (bits below 2^-24 of the row's largest apart). The key block's scale goes into the scores. The value block's scale 2^e
-// goes into the exponent of the weights that meet V, 2^(s + e - m'), with a running maximum m' of its own, so that
-// weights of 16 bits are full where they count, whatever the blocks' scales; the softmax's sum has 2^(s - m). Both are
-// raised, and the sums rescaled, only when a score passes them by more than 2^8.
+// goes into the exponent of the weights that meet V, 2^(s + e - m'), with a reference m' of its own, 12 below the largest
+// s + e, so that weights of 16 bits are full where they count, whatever the blocks' scales; the softmax's sum has
+// 2^(s - m). Both are raised, and the sums rescaled, only when a score passes m by more than 8 or the reference by more
+// than 15.
 template <typename T, int D, bool E4M3, int NT, int MODE>
 __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
     paged_kernel(const PagedArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -883,7 +898,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float a0 = fmaxf(s[n][0][e], s[n][0][2 + e]), a1 = fmaxf(s[n][1][e], s[n][1][2 + e]);
-          raise |= fmaxf(a0, a1) > m[n][e] + kPaSlack || fmaxf(a0 + ev[0], a1 + ev[1]) > mv[n][e] + kPaSlack;
+          raise |= fmaxf(a0, a1) > m[n][e] + kPaSlack || fmaxf(a0 + ev[0], a1 + ev[1]) > mv[n][e] + (kPaWeight + kPaWeightSlack);
         }
       }
       if (__any_sync(kAll, raise)) {
@@ -899,7 +914,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
               top = fmaxf(top, __shfl_xor_sync(kAll, top, x));
               tv = fmaxf(tv, __shfl_xor_sync(kAll, tv, x));
             }
-            const float mn = fmaxf(m[n][e], top), vn = fmaxf(mv[n][e], tv);
+            const float mn = fmaxf(m[n][e], top), vn = fmaxf(mv[n][e], tv - kPaWeight);
             l[n][e] *= mn == -INFINITY ? 1.f : fast_exp2(m[n][e] - mn);
             f[e] = vn == -INFINITY ? 1.f : fast_exp2(mv[n][e] - vn);
             m[n][e] = mn;
@@ -991,10 +1006,6 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
     auto row_of = [&](int col) {
       return static_cast<T*>(a.out) + ((static_cast<int64_t>(it.b) * a.T + col / a.group) * (a.hkv * a.group) + h * a.group + col % a.group) * D;
     };
-    auto inverse_of = [](float m, float sum, float mv) {
-      const float up = (mv == -INFINITY ? 0.f : mv) - (m == -INFINITY ? 0.f : m);
-      return sum > 0.f || __isnanf(sum) ? fast_exp2(up) / sum : 0.f;
-    };
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -1011,7 +1022,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
         } else if (whole_item) {
           const float inv = inverse_of(m[n][e], sum, mv[n][e]);
 #pragma unroll
-          for (int j = 0; j < 2 * kSteps; ++j) x[j] = fit<T>(x[j] * inv);
+          for (int j = 0; j < 2 * kSteps; ++j) x[j] = fit<T>(x[j] * kPaUnit * inv);
           store_pack<T, 2 * kSteps>(row_of(col) + d, from_floats<T, 2 * kSteps>(x));
         } else {
           store_pack<float, 2 * kSteps>(a.part_o + (slot * kCols + c) * D + d, from_floats<float, 2 * kSteps>(x));
@@ -1043,7 +1054,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
         } else if (whole_item) {
           const float inv = inverse_of(mm, ll, mmv);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * inv);
+          for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * kPaUnit * inv);
           store_pack<T, 4>(row_of(c0 + c) + d, from_floats<T, 4>(acc));
         } else {
           store_pack<float, 4>(a.part_o + (slot * kCols + c) * D + d, from_floats<float, 4>(acc));
@@ -1076,7 +1087,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
           }
           const float inv = inverse_of(mm, ll, mmv);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * inv);
+          for (int j = 0; j < 4; ++j) acc[j] = fit<T>(acc[j] * kPaUnit * inv);
           store_pack<T, 4>(row_of(c0 + c) + d, from_floats<T, 4>(acc));
         }
         __syncwarp();
@@ -1169,9 +1180,9 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int6
       for (int i = 0; i < kV; ++i) acc[i] = fmaf(fw, sums[w][lane * kV + i], acc[i]);
     }
   }
-  const float inv = ll > 0.f || __isnanf(ll) ? fast_exp2((mmv == -INFINITY ? 0.f : mmv) - (mm == -INFINITY ? 0.f : mm)) / ll : 0.f;
+  const float inv = inverse_of(mm, ll, mmv);
 #pragma unroll
-  for (int i = 0; i < kV; ++i) acc[i] = fit<T>(acc[i] * inv);
+  for (int i = 0; i < kV; ++i) acc[i] = fit<T>(acc[i] * kPaUnit * inv);
   store_pack<T, kV>(dst + lane * kV, from_floats<T, kV>(acc));
 }
 
