@@ -441,8 +441,8 @@ int xdna_add_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_
 
 /* A cache of keys and values in pages and 8 bits: codes [pages][hkv][page][d] bytes (format XDNA_I8 or XDNA_E4M3; the
  * last three dimensions contiguous, kc_sp / vc_sp bytes from page to page, multiples of 16; page 16, 32, 64 or 128; d 64
- * or 128) and scales [pages][hkv] f32 (ks_sp / vs_sp elements from page to page): x = code * scale, one scale for a
- * head's part of a page (a block), a power of two. table [n_seqs][max_pages] (int32, row pitch ld_table): the page of a
+ * or 128) and scales [pages][hkv] f32 (ks_sp / vs_sp elements from page to page): x = code * scale, one scale, zero or
+ * more, for a head's part of a page (a block). table [n_seqs][max_pages] (int32, row pitch ld_table): the page of a
  * sequence's tokens i * page .. ; an entry outside [0, pages) is no page.
  *
  * xdna_cache_append puts new tokens k, v [tokens, hkv, d] (bf16 / f16) behind the starts[i] that sequence i has in the

@@ -2,7 +2,8 @@
 
 import pytest
 import torch
-from test_layer_gpu import FORMATS, _clean, close, i32, rounding, step  # noqa: F401
+from test_layer_gpu import (FORMATS, _clean, check_attention, close, filled, i32, randn,  # noqa: F401
+                            rounding, step, table_of, values)
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +36,17 @@ def test_paged_a_peak_without_a_value(cuda, fmt, b, keys):
         p = torch.softmax(torch.where(torch.arange(keys, device="cuda") == at, 15.0, 0.0).double(), 0)
         want = (p @ vc[:, 0].reshape(-1, d)[:keys].double()).expand(b, 1, d)
         close(got, want, want * (2.0 ** -11 + 4 * 12 * 15 * 2.0 ** -23 + 2.0 ** -20) + rounding(want, torch.float16))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("b,keys,t", [(2, 700, 1), (3, 5000, 2), (230, 260, 1)])
+def test_paged_scales_that_are_no_powers_of_two(cuda, fmt, b, keys, t):
+    """Of a cache that something else has filled: keys and values are code * scale whatever the scale."""
+    page, hkv, d = 16, 2, 64
+    lens = [(keys * (i + 1)) // b for i in range(b)]
+    counts = [-(-n // page) for n in lens]
+    c = filled(sum(counts) + 1, hkv, page, d, fmt, seed=b)
+    g = torch.Generator(device="cuda").manual_seed(b)
+    for s in c[2:]:
+        s.mul_(1 + torch.rand(s.shape, generator=g, device="cuda"))
+    check_attention(randn(b, t, 4, d, seed=2, dtype=torch.float16), c, table_of(counts, sum(counts) + 1), lens)

@@ -2,8 +2,8 @@
 // (xdna_cache_append), with the norm and the rotation of the keys on the way, and attention (xdna_paged_attention).
 //
 // Codes lie as [pages][Hkv][page][D] bytes, int8 or e4m3, a page being 16, 32, 64 or 128 tokens; a block is one head's
-// part of a page, D * page contiguous bytes, and has one scale, a power of two: x = code * scale. table[b][i] is the
-// page of sequence b's tokens i * page .. (i + 1) * page - 1.
+// part of a page, D * page contiguous bytes, and has one scale: x = code * scale. An append writes powers of two.
+// table[b][i] is the page of sequence b's tokens i * page .. (i + 1) * page - 1.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -583,6 +583,14 @@ __device__ __forceinline__ float sum_of_groups(float x) {  // over the lanes wit
   return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
+// log2 of a value block's scale: NaN below zero, -inf of zero, else to 2^-22 of itself (of powers of two below one to 2^-23,
+// above whole, as measured), so that weights are off by 2^-20 at a scale of 2^-6 and by 2^-16 at 2^-126.
+__device__ __forceinline__ float log2_scale(float scale) {
+  float e;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(scale));
+  return e;
+}
+
 // What a row's sums with V are to be multiplied with, after kPaUnit: 1 / the softmax's sum, brought from the weights'
 // reference to the scores'.
 __device__ __forceinline__ float inverse_of(float m, float sum, float mv) {
@@ -637,7 +645,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
   constexpr int kCols = 8 * NT, kSteps = D / 16, kKeys = TOGETHER ? kPaTile * kPaWarps : kPaTile;  // of a unit
   extern __shared__ __align__(16) uint8_t paged_smem[];
   __shared__ __align__(8) uint64_t bars[kPaWarps][S::kStages];
-  __shared__ float scales[kPaWarps][S::kStages][4];  // key and value scales of a tile's two blocks; below zero: no page
+  __shared__ float scales[kPaWarps][S::kStages][4];  // key and value scales of a tile's two blocks; -inf: no page
   __shared__ float sml[kPaWarps][kCols][3];
   __shared__ int abort_flag;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -757,7 +765,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
                        "l"(lane & 1 ? a.vs + page * a.vs_sp + h : a.ks + page * a.ks_sp + h)
                        : "memory");
         else
-          *to = -1.f;
+          *to = -INFINITY;
       }
       ++looked;
       ++next.unit;
@@ -838,12 +846,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
       const int key0 = it.unit * kKeys + first_key;
       const float4 sc = *reinterpret_cast<const float4*>(scales[warp][st]);  // K, V of block 0, K, V of block 1
       const float ks[2] = {sc.x, two_pages ? sc.z : sc.x};
-      float ev[2];  // log2 of the value blocks' scales; NaN stays NaN
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t bits = __float_as_uint(x && two_pages ? sc.w : sc.y);
-        ev[x] = (bits & 0x7fffffffu) >= kNotFinite ? __uint_as_float(0x7fc00000u) : static_cast<float>(static_cast<int>(bits >> 23 & 0xff) - 127);
-      }
+      const float ev[2] = {log2_scale(sc.y), log2_scale(two_pages ? sc.w : sc.y)};
       // scores: s[n][x][e] is key 16 x + key_row (+ 8 for e >= 2) of the tile, column 2 t + (e & 1)
       float s[NT][2][4];
 #pragma unroll
@@ -880,7 +883,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
           }
         }
       }
-      const bool whole = key0 + kPaTile <= seen_by_all && !(ks[0] < 0.f) && !(ks[1] < 0.f);
+      const bool whole = key0 + kPaTile <= seen_by_all && ks[0] != -INFINITY && ks[1] != -INFINITY;
       if (!whole) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -888,7 +891,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
           for (int x = 0; x < 2; ++x) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (ks[x] < 0.f || key0 + 16 * x + key_row + 8 * (e >> 1) >= limit[n][e & 1]) s[n][x][e] = -INFINITY;
+              if (ks[x] == -INFINITY || key0 + 16 * x + key_row + 8 * (e >> 1) >= limit[n][e & 1]) s[n][x][e] = -INFINITY;
           }
         }
       }
@@ -965,8 +968,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaShape<D, NT>::kCtas)
             v[r][0] = u.x, v[r][1] = u.y;
           }
           if (!whole) {  // what lies behind the last key and in the place of a page that is none: any byte, also a NaN
-            const bool there = ks[x] >= 0.f || __isnanf(ks[x]);
-            if (!there || key0 + 16 * x + row + 8 * (r >> 1) >= len) {
+            if (ks[x] == -INFINITY || key0 + 16 * x + row + 8 * (r >> 1) >= len) {
 #pragma unroll
               for (int w = 0; w < S::kVBytes / 4; ++w) v[r][w] = 0;
             }

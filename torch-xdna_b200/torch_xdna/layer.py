@@ -88,7 +88,7 @@ def add_norm(x, y, weight, post=None, gate=None, scale=1.0, eps=1e-6):
 
 class PagedCache(NamedTuple):
     """Codes [pages, Hkv, page, D] (int8 or float8_e4m3fn) and scales f32 [pages, Hkv] of one layer's keys and values:
-    key = code * scale. A scale is of one head's part of a page and a power of two."""
+    key = code * scale. A scale is of one head's part of a page, zero or more; those of cache_append are powers of two."""
 
     k: torch.Tensor
     v: torch.Tensor
