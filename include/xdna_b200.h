@@ -450,8 +450,10 @@ int xdna_add_norm(const void* x, int x_dtype, int64_t ldx, const void* y, int y_
  * cu_seqlens[i + 1] - 1 are sequence i's next ones (ascending; words outside [0, tokens] are clamped). The keys, after
  * k_norm where given, are turned to their place in the sequence as by xdna_rotary. A block's scale is the least 2^e >=
  * 2^-126 with max |x| <= 127 * 2^e (int8) or 448 * 2^e (e4m3) over its tokens; where older tokens in it had a larger one
- * that stays, where they had a smaller one their codes are rounded to the new one. A page whose first slot is written
- * starts anew. A block that is given an infinity or a NaN has the scale NaN until then, and code 0 for the new tokens.
+ * that stays (one that is no power of two: the next above it, to which their codes are rounded), where they had a smaller
+ * one their codes are rounded to the new one. A page whose first slot is written starts anew. A block that is given an
+ * infinity or a NaN, or whose older scale is one, above 2^126 or below zero, has the scale NaN until then, and code 0 for
+ * the new tokens.
  * Slots behind a sequence's last token, and all other pages, are left as they were. Tokens without a page, and sequences
  * with starts[i] < 0, are not stored. No two sequences of a call may write to one page. q [tokens, hq, d] may be NULL;
  * else q_out [tokens, hq, d] = q, after q_norm, turned to its tokens' places (zero where starts[i] < 0 and for tokens of
@@ -469,10 +471,10 @@ int xdna_cache_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, 
  * the last T tokens of each sequence: token t attends to the first lens[b] - T + t + 1 tokens in the cache (lens clamped
  * to 0 .. max_pages * page, which is below 2^30), without those that have no page. A row without any, or with scores of
  * -inf alone, is zero. Scores and sums are f32; the weights that meet V are f16 with an exponent of their own per block
- * (terms below 2^-26 of a row's largest lose bits, those below 2^-37 are lost). The work is shared out by the lengths, on the device, in one of three
- * manners by B, the heads and max_pages * page. T is meant to be small: every 16 / (hq / hkv) tokens the cache is read
- * once more. Codes of e4m3 are numbers. workspace: xdna_paged_attention_workspace bytes for most_keys = max_pages * page,
- * 256-byte aligned (0 bytes: NULL). */
+ * (terms below 2^-26 of a row's largest lose bits, those below 2^-37 are lost). The work is shared out by the lengths, on
+ * the device, in one of three manners by B, the heads and max_pages * page. T is meant to be small: every 16 / (hq / hkv)
+ * tokens the cache is read once more. Codes of e4m3 are numbers. workspace: xdna_paged_attention_workspace bytes for
+ * most_keys = max_pages * page, 256-byte aligned (0 bytes: NULL). */
 size_t xdna_paged_attention_workspace(int64_t B, int64_t T, int64_t hq, int64_t hkv, int64_t d, int64_t most_keys);
 int xdna_paged_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, int64_t B, int64_t T,
                          int64_t hq, int64_t hkv, int64_t d, const void* k_codes, int64_t kc_sp, const void* v_codes,

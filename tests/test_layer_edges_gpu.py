@@ -2,8 +2,8 @@
 
 import pytest
 import torch
-from test_layer_gpu import (FORMATS, _clean, check_attention, close, filled, i32, randn,  # noqa: F401
-                            rounding, step, table_of, values)
+from test_layer_gpu import (E, FORMATS, _clean, check_attention, close, filled, i32,  # noqa: F401
+                            power, randn, rounding, step, table_of, values)
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,29 @@ def test_paged_scales_that_are_no_powers_of_two(cuda, fmt, b, keys, t):
     for s in c[2:]:
         s.mul_(1 + torch.rand(s.shape, generator=g, device="cuda"))
     check_attention(randn(b, t, 4, d, seed=2, dtype=torch.float16), c, table_of(counts, sum(counts) + 1), lens)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("packed", [False, True])
+def test_append_behind_scales_that_are_no_powers_of_two(cuda, fmt, packed):
+    """Older tokens of a block whose scale is no power of two keep their values, to half a step of the block's new scale: the
+    least power of two that holds it and the new tokens. (The product of a code and a factor is itself rounded, to 2^-24.)"""
+    import torch_xdna
+
+    page, hkv, d, lo = 32, 3, 64, 9
+    for factor, size in ((1.0, 1e-3), (1.37, 1e-3), (1.999, 1e-3), (1.37, 30.0), (1.5, 2000.0)):
+        c = filled(2, hkv, page, d, fmt, seed=3)
+        c.k_scales.mul_(factor), c.v_scales.mul_(factor)
+        old = [x.clone() for x in c]
+        n = 4 if packed else 1
+        k, v = randn(n, hkv, d, seed=4, scale=size), randn(n, hkv, d, seed=5, scale=size)
+        torch_xdna.cache_append(k, v, *c, i32(1).view(1, 1), i32(lo), i32(0, n) if packed else None)
+        for i, x in ((0, k), (1, v)):
+            new, was = x.double().transpose(0, 1), values(old[i][1], old[2 + i][1])[:, :lo]
+            mantissa, e = torch.frexp(old[2 + i][1].double())            # mantissas from 1/2 on
+            held = torch.ldexp(torch.ones_like(mantissa), e - (mantissa == 0.5).int())
+            scale = torch.maximum(power(new.abs().amax((1, 2)), fmt), held)
+            assert torch.equal(c[2 + i][1].double(), scale)
+            got, s = values(c[i][1], c[2 + i][1]), scale[:, None, None]
+            assert ((got[:, lo:lo + n] - new).abs() <= step(new, s, fmt)).all()
+            assert ((got[:, :lo] - was).abs() <= step(was, s, fmt) + was.abs() * E).all()

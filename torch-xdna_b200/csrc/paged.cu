@@ -26,6 +26,7 @@ __device__ __forceinline__ int block_exponent(uint32_t top_bits, bool e4m3) {
   return max(e4m3 ? e - 8 + (mantissa > 0x600000u) : e - 6 + (mantissa > 0x7e0000u), -126);
 }
 constexpr uint32_t kNotFinite = 0x7f800000u;
+constexpr uint32_t kMostScale = 0x7e800000u;  // 2^126; above it as bits: what is larger, not finite or below zero
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }  // -126 .. 127
 
 // What an append makes of a block: the scale, 1 / scale for the new values, and the factor of the older codes.
@@ -33,17 +34,14 @@ struct BlockChange {
   float scale, inverse, older;  // inverse 0: not finite; older 1: they stay
 };
 __device__ __forceinline__ BlockChange change_block(uint32_t top_bits, bool has_older, uint32_t old_bits, bool e4m3) {
-  if (top_bits >= kNotFinite || (has_older && (old_bits & 0x7fffffffu) >= kNotFinite)) return {__uint_as_float(0x7fc00000u), 0.f, 1.f};
+  if (top_bits >= kNotFinite || (has_older && old_bits > kMostScale)) return {__uint_as_float(0x7fc00000u), 0.f, 1.f};
   int e = block_exponent(top_bits, e4m3);
   float older = 1.f;
-  if (has_older) {
-    const int old = max(static_cast<int>(old_bits >> 23 & 0xff) - 127, -126);
-    if (e > old)
-      older = power_of_two(max(old - e, -126));
-    else
-      e = old;
+  if (has_older) {  // their scale is held by the least power of two from it on: itself, where an append wrote it
+    e = max(e, static_cast<int>(old_bits >> 23) - 127 + ((old_bits & 0x7fffffu) != 0));
+    older = __uint_as_float(old_bits) * power_of_two(-e);
   }
-  return {power_of_two(e), power_of_two(min(-e, 127)), older};
+  return {power_of_two(e), power_of_two(-e), older};
 }
 
 // Four values to codes; they are within the codes' range.
