@@ -485,7 +485,7 @@ at::Tensor paged_attention(PyObject* const* a) {
   const int64_t B = q4.size(0), T = q4.size(1), hq = q4.size(2);
   const double scale = scale_of(name, q4, hq, c.hkv, c.d, a[7]);
   const at::Tensor &table = table_of(name, a[5], B), &lens = counts_of(name, "lens", a[6], B);
-  if (tracked({&q0})) return {};
+  if (tracked({&q0, &c.k, &c.v, &c.ks, &c.vs})) return {};
   Place place(name, q0, {&c.k, &c.v, &c.ks, &c.vs, &table, &lens});
   const at::Tensor q = rows(q4);
   at::Tensor out = at::empty(q0.sizes(), q0.options());
