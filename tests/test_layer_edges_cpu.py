@@ -62,3 +62,16 @@ def test_attention_over_scales_that_require_grad_raises_in_backward(monkeypatch)
             assert y.requires_grad
             with pytest.raises(RuntimeError, match="autograd"):
                 y.sum().backward()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_cache_that_requires_grad_is_not_written(binding, fmt):
+    """What a call writes in place has no history: refused where autograd would want one, as keys that require grad are."""
+    for i in floats(cache(dtype=fmt)):
+        c = list(cache(dtype=fmt))
+        c[i].requires_grad_()
+        for more in ({}, dict(q=z(3, 4, 64).requires_grad_())):
+            with pytest.raises(XdnaError, match="no gradients"):
+                torch_xdna.cache_append(z(3, 2, 64), z(3, 2, 64), *c, i32(3, 2), i32(3), **more)
+        with torch.no_grad(), pytest.raises(XdnaUnavailable):
+            torch_xdna.cache_append(z(3, 2, 64), z(3, 2, 64), *c, i32(3, 2), i32(3))

@@ -454,7 +454,8 @@ PyObject* cache_append(PyObject* const* a) {
   check_norm(name, "k_norm", k_norm, c.hkv, c.d);
   REQUIRE(q0 || !q_norm, XDNA_ERR_INVALID, "q_norm without q");
   if (q0) check_norm(name, "q_norm", q_norm, q0->size(1), c.d);
-  REQUIRE(!tracked({&k0, &v0, in(k_norm)}), XDNA_ERR_INVALID, "a cache keeps no gradients: keys and values that require grad are stored under torch.no_grad()");
+  REQUIRE(!tracked({&k0, &v0, in(k_norm), &c.k, &c.v, &c.ks, &c.vs}), XDNA_ERR_INVALID,
+          "a cache keeps no gradients: keys and values that require grad, and into a cache that does, are stored under torch.no_grad()");
   if (tracked({in(q0), in(q_norm), in(freq)})) Py_RETURN_NONE;
   Place place(name, k0, {&v0, &c.k, &c.v, &c.ks, &c.vs, &table, &starts, in(cu), in(freq), in(q0), in(k_norm), in(q_norm)});
   const at::Tensor k = rows(k0), v = rows(v0);
