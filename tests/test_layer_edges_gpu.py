@@ -76,3 +76,27 @@ def test_append_behind_scales_that_are_no_powers_of_two(cuda, fmt, packed):
             got, s = values(c[i][1], c[2 + i][1]), scale[:, None, None]
             assert ((got[:, lo:lo + n] - new).abs() <= step(new, s, fmt)).all()
             assert ((got[:, :lo] - was).abs() <= step(was, s, fmt) + was.abs() * E).all()
+
+
+def test_append_says_that_it_wrote(cuda):
+    """A tensor of the cache that autograd saved before an append is noticed in backward, as with the custom op; caches of
+    inference mode, which count nothing, are written outside of it too."""
+    import torch_xdna
+
+    for ns in (torch_xdna, torch.ops.xdna):
+        c, k, table = filled(2, 2, 16, 64, torch.float8_e4m3fn), randn(1, 2, 64), i32(1).view(1, 1)
+        for t in c:
+            w = torch.ones((), device="cuda", requires_grad=True)
+            with torch.enable_grad():
+                y = (t.float() if t is c.k or t is c.v else t) * w       # saves scales themselves
+                versions = [x._version for x in c]
+                ns.cache_append(k, k, *c, table, i32(3))
+                assert all(x._version > n for x, n in zip(c, versions))
+                if t is c.k_scales or t is c.v_scales:
+                    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                        y.sum().backward()
+    with torch.inference_mode():
+        c = filled(2, 2, 16, 64, torch.int8)
+    before = c.k.clone()
+    torch_xdna.cache_append(k, k, *c, table, i32(3))
+    assert c.k.is_inference() and not torch.equal(c.k, before)

@@ -114,6 +114,12 @@ bool tracked(std::initializer_list<const at::Tensor*> inputs) {
   return false;
 }
 
+// Says to autograd that t has been written in place, so that backward notices where it was saved before. (Tensors of
+// inference mode keep no such count.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 double scale_of(const char* name, const at::Tensor& q, int64_t hq, int64_t hkv, int64_t d, PyObject* scale) {
   REQUIRE(half(q), XDNA_ERR_INVALID, "bf16 or f16, not " << type(q));
   REQUIRE(hq >= 1 && hkv >= 1 && hq % hkv == 0 && hq / hkv <= 128, XDNA_ERR_INVALID,
@@ -472,6 +478,7 @@ PyObject* cache_append(PyObject* const* a) {
                   freq ? freq->size(0) : 0, factor, interleaved, ptr(k_norm), dtype_of(k_norm), per_head(k_norm), eps,
                   q0 ? q.data_ptr() : nullptr, q0 ? pitch_of(q, 0) : 8, q0 ? pitch_of(q, 1) : 8, hq, ptr(q_norm), dtype_of(q_norm),
                   per_head(q_norm), q0 ? out.data_ptr() : nullptr, place.stream));
+  for (const at::Tensor* t : {&c.k, &c.v, &c.ks, &c.vs}) written(*t);
   if (!q0) Py_RETURN_FALSE;
   return THPVariable_Wrap(std::move(out));
 }
