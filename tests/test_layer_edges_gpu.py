@@ -2,8 +2,8 @@
 
 import pytest
 import torch
-from test_layer_gpu import (E, FORMATS, _clean, check_attention, close, filled, i32,  # noqa: F401
-                            power, randn, rounding, step, table_of, values)
+from test_layer_gpu import (E, FORMATS, _clean, check_attention, close, filled, freqs,  # noqa: F401
+                            i32, power, randn, rounding, step, table_of, values)
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,32 @@ def test_append_says_that_it_wrote(cuda):
     before = c.k.clone()
     torch_xdna.cache_append(k, k, *c, table, i32(3))
     assert c.k.is_inference() and not torch.equal(c.k, before)
+
+
+def test_rotary_angles_far_out(cuda):
+    """Positions beyond 32 bits against angles in exact arithmetic: the angle is good to the position times 2^-64 turns, at 2^40
+    2^-21.3, 6.5 units of 2^-24; cos and sin as ever 7; within the tolerance of near ones."""
+    from fractions import Fraction
+
+    import torch_xdna
+
+    two_pi = 2 * Fraction(314159265358979323846264338327950288419716939937510582097494459, 10 ** 62)
+    pos = [2 ** 31 - 1, 2 ** 33 + 12345, 2 ** 37 - 1, -(2 ** 37) + 99, 2 ** 40, 2 ** 40 - 7]
+    for base in (1e4, 1e6):
+        f = freqs(64, base)
+        x = torch.zeros(len(pos), 1, 128, device="cuda")
+        x[..., :64] = 1.0                                            # (1, 0) turns to (cos, sin)
+        angle = torch.empty(len(pos), 64, dtype=torch.float64)
+        for i, n in enumerate(pos):
+            for j, y in enumerate(f.tolist()):
+                turns = n * Fraction(y) / two_pi
+                angle[i, j] = float((turns - (turns.numerator // turns.denominator)) * two_pi)
+        want = torch.cat((angle.cos(), angle.sin()), 1)[:, None].cuda()
+        for interleaved in (False, True):
+            y = x.clone()
+            if interleaved:
+                y.zero_()[..., ::2] = 1.0
+            got = torch_xdna.rotary(y, torch.tensor(pos, device="cuda"), f, interleaved=interleaved)
+            if interleaved:
+                got = torch.cat((got[..., ::2], got[..., 1::2]), -1)
+            close(got, want, torch.full_like(want, 32 * E))

@@ -91,12 +91,15 @@ __device__ __forceinline__ void load_weights(const void* w, int dtype, int64_t a
     to_floats<__half, N>(load_pack<__half, N>(static_cast<const __half*>(w) + at), x);
 }
 
-// Angles in turns, as 64-bit fractions: a frequency's turns per position, rounded to 2^-56 or better, times the position
-// leaves exactly the part within a turn, whatever the position. cos and sin of it, times factor: of its upper 24 bits in 32
-// bits, turned on by what is left (below 2^-24 of half a turn, so to first order).
+// Angles in turns, as 64-bit fractions: a frequency's turns per position, to 2^-64 (1 / (2 pi) in two parts, and the first
+// product's rounding), times the position leaves the part within a turn, off by no more than position * 2^-64: 2^-24 radians
+// at 2^37. cos and sin of it, times factor: of its upper 24 bits in 32 bits, turned on by what is left (below 2^-24 of half a
+// turn, so to first order).
 __device__ __forceinline__ uint64_t turns_of(float inv_freq) {
-  const double turns = static_cast<double>(inv_freq) * 0.15915494309189533577;
-  return static_cast<uint64_t>((turns - floor(turns)) * 18446744073709551616.0);
+  constexpr double kHigh = 0.15915494309189535, kLow = -9.839338337591243e-18;
+  const double f = inv_freq, turns = __dmul_rn(f, kHigh), rest = fma(f, kLow, fma(f, kHigh, -turns));
+  return static_cast<uint64_t>(__double2ll_rn((turns - rint(turns)) * 18446744073709551616.0)) +
+         static_cast<uint64_t>(__double2ll_rn(rest * 18446744073709551616.0));
 }
 __device__ __forceinline__ float2 turn_of(uint64_t turns, float factor) {
   const int32_t high = static_cast<int32_t>(turns >> 32), upper = high & ~0xff;
