@@ -1,5 +1,7 @@
 """The operators around a decoder layer's products on the B200 where they are most easily wrong, against their definitions."""
 
+import math
+
 import pytest
 import torch
 from test_layer_gpu import (E, FORMATS, _clean, check_attention, close, filled, freqs,  # noqa: F401
@@ -129,3 +131,23 @@ def test_rotary_angles_far_out(cuda):
             if interleaved:
                 got = torch.cat((got[..., ::2], got[..., 1::2]), -1)
             close(got, want, torch.full_like(want, 32 * E))
+
+
+@pytest.mark.parametrize("d", [8, 64, 72, 80, 96, 112, 128, 200, 256])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_norm_of_non_finite_heads(cuda, d, interleaved):
+    """Heads with an infinity or a NaN leave the others of their token, which share a warp and its sums, as they were without."""
+    import torch_xdna
+
+    t, h = 5, 13
+    f, pos, w = freqs(d // 2), torch.arange(t, device="cuda"), randn(h, d, seed=2, dtype=torch.float32)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = randn(t, h, d, seed=d, dtype=dtype)
+        want = torch_xdna.rotary(x, pos, f, 1.0, interleaved, w)
+        bad = torch.zeros(t, h, dtype=torch.bool, device="cuda")
+        for i, (a, b, e, y) in enumerate(((0, 0, 0, math.inf), (1, 5, d - 1, math.nan), (1, 6, 3, -math.inf), (2, 12, d // 2, math.nan),
+                                          (4, 1, 5, math.inf))):
+            x[a, b, e], bad[a, b] = y, True
+        got = torch_xdna.rotary(x, pos, f, 1.0, interleaved, w)
+        assert torch.equal(torch.isfinite(got).all(-1), ~bad)
+        assert torch.equal(got[~bad], want[~bad])
