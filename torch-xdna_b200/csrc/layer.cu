@@ -15,10 +15,12 @@ constexpr int kRotaryWarps = 4;
 // next heads are asked for before those at hand are worked on, and the first ones before the angles are known. The token's
 // cosines and sines are worked out once, each by one lane, and handed round by shuffles; they then stay in registers. U
 // units of 2 V values per lane, U > 1 with V = 1 alone.
-// 16384 tokens of 24 heads of 128 in bf16 with norms of their own: 42 us, 4.8 TB/s (37 without the norm); 70 % of the issue
-// slots are busy, 270 to 320 instructions for four heads of a token, of which the norm, the turn and the 16-bit values take
-// about 150. Blocks of four warps, seven to an SM; of eight: 45.6 us; two rounds asked for ahead: 52, three: 51 (registers);
-// several tokens per warp, so that the start of one hides behind another: 47.
+// 16384 tokens of 24 heads of 128 in bf16 with norms of their own: 43.6 us, 4.6 TB/s (37.9 without the norm; 8192 in f32,
+// the same bytes: 38.5). 70 % of the issue slots are busy, 270 to 320 instructions for four heads of a token, of which the
+// norm, the turn and the 16-bit values take about 150; the norms' weights come through L1 for each token; and the 72
+// registers of seven blocks spill 8 to 28 bytes a thread in the 8-wide variants of 16 bits, 36 to 56 in those of f32.
+// Blocks of four warps, seven to an SM; of eight: 45.6 us; two rounds asked for ahead: 52, three: 51 (registers); several
+// tokens per warp, so that the start of one hides behind another: 47.
 template <typename T, int V, int LANES, int U, bool INTER>
 __global__ void __launch_bounds__(kRotaryWarps * 32, 7) rotary_kernel(const RotaryArgs a) {
   static_assert(U == 1 || (V == 1 && LANES == 32), "more units only where a lane has all of a warp's row");
@@ -203,7 +205,9 @@ __device__ __forceinline__ void load_shifted(const void* w, int dtype, int at, i
 // warp to a row, blockDim.y rows to a block. SHIFT: rows whose length is no multiple of V, in arrays that start at a
 // boundary of 16 bytes and whose pitches leave the same remainder. Pieces then begin at boundaries, `shift` entries before
 // the row's, and its ends are taken entry by entry. 8191 rows of 5003 in bf16 with a norm behind the block and a gate of
-// their own: 110 us (3.7 TB/s); entry by entry 436.
+// their own: 111 us (3.7 TB/s); entry by entry 436. Rows of 4096: 57.2 us (5.9 TB/s); with the gate in f32, which is read
+// behind the first sum, 74.7 (5.4). The inverse roots are rsqrtf's, off by 2 ulp at most, which is less than the
+// sums of a row's squares are off by.
 template <typename TX, typename TY, int V, int C, bool SHIFT>
 __global__ void __launch_bounds__(1024) add_norm_kernel(const AddNormArgs a) {
   __shared__ float parts[2][32];

@@ -352,9 +352,13 @@ __device__ __forceinline__ bool find_page(const AppendArgs& a, int64_t item, Pag
 // (blockIdx.y). A head's part of the page, MOST tokens for each of a block's rows of lanes (pages of fewer tokens than rows:
 // several heads at once), stays in registers between the search for its largest value and its codes, while the next heads'
 // part is on its way. The angles' cosines and sines, which are those of all heads, are worked out once, in shared memory.
-// 12968 tokens of 16 prompts, 8 heads of 128 in bf16, pages of 64: 31 us, 3.0 TB/s (pages of 16: 33, of 128: 32). 60 % of
-// the issue slots are busy; without norm and rotation 26 us. Norm and rotation done twice, so that what was read stays in
-// 16 bits: 48 us; one kernel for all page sizes, with rounds for 128 tokens in each: 47 (pages of 16: 160).
+// 12968 tokens of 16 prompts, 8 heads of 128 in bf16, pages of 64, e4m3: 31.3 us, 3.0 TB/s (int8 31.8; pages of 16: 33.1,
+// of 128: 31.3). Nothing is full: 60 % of the issue slots are busy, and without norm and rotation it is still 26.5 us.
+// There is one wave of blocks, whose start and end overlap with nothing, a barrier for each head, and those of keys have
+// more to do than those of values (an SM has 47300 cycles on average, 61129 at most). Many sequences cost the search for a
+// block's page: 1000 tokens of as many sequences beside a prompt of 1900 take 158 us, 100 of them 21, the prompt alone 8.8.
+// Norm and rotation done twice, so that what was read stays in 16 bits: 48 us; one kernel for all page sizes, with rounds
+// for 128 tokens in each: 47 (pages of 16: 160).
 template <typename T, int D, int V, bool INTER, int MOST>
 __global__ void __launch_bounds__(kAppendThreads, V == 8 ? (MOST <= 2 ? 3 : 2) : 1) append_packed_kernel(const AppendArgs a) {
   using S = RowShape<D, V>;
@@ -618,10 +622,10 @@ __device__ __forceinline__ float4 load_remote(uint32_t cluster_address) {
 // second launch costs more than an even share gains: a cluster of up to eight CTAs has one item, as together, and joins its
 // parts in their shared memory. Which one goes by the longest sequence that the table can hold and by the number of items
 // (plan, below).
-// 200 sequences of up to 300 keys, 16 heads over 8 of 128, e4m3: 27.8 us with warps' shares, 40.3 with CTAs'; 32 of 1175 to
-// 4700: 41.1 us (4.8 TB/s) with CTAs' shares, 43 with warps'. One of 131071: 52 us, 5.1 TB/s; while it runs the memory is
-// busy throughout (7 TB/s and more over the tiles), the rest is the start (lengths, pages and tiles wait for one another,
-// 5 us) and the join (3 us).
+// 200 sequences of up to 300 keys, 16 heads over 8 of 128, e4m3: 27.4 us with warps' shares, 35.1 with CTAs'; 32 of 1175 to
+// 4700: 40.2 us (4.9 TB/s) with CTAs' shares. One of 131071: 52.5 us, 5.1 TB/s; more keys of it are read at 6.4 TB/s (262144:
+// 95.7, 524288: 180.1), so that 10.5 us are the start (lengths, pages and tiles wait for one another), the ends of the SMs'
+// shares and the join.
 // A tile's codes come by TMA into the warp's own ring in shared memory, and the products are mma.sync 16 x 8 x 16 with keys,
 // then dimensions, as rows and the query rows as columns: S^T = K Q^T, O^T = V^T P^T. Of K, lane (g, t) reads bytes
 // 64 c + 16 t .. + 15 of two keys: each word of them is, as two half pairs, A fragments when the queries' B fragments are
@@ -1200,8 +1204,10 @@ struct PagedPlan {
     const int64_t cols = hq / hkv * T, units = (most_keys + kPaTile * kPaWarps - 1) / (kPaTile * kPaWarps);
     ml_at = o_at = bytes = 0;
     mode = PAGED_CLUSTER;
-    // as many CTAs per item as the SMs hold (clusters leave some of their places empty: with 288 of 296 taken by threes, 15.6 us
-    // instead of 12.7), where a share of the longest item is about one of all work
+    // as many CTAs per item as the SMs hold, where a share of the longest item is about one of all work. Clusters leave some
+    // of the places empty, so only seven eighths of them count: 72 items of up to 900 keys in clusters of five 8.9 us, in ones
+    // of six (432 of 444 places) 11.7; 144 of up to 500, twos and threes, 7.6 and 11.0; 96 in 296 places, twos and threes,
+    // 12.7 and 15.6. Clusters of two would always fit: 200 of up to 500 have one CTA each, 12.0 us, 8.6 with two.
     auto clusters = [&](int tiles) {
       shape(tiles, B, hkv, cols, sms);
       splits = static_cast<int>(std::max<int64_t>(1, std::min({static_cast<int64_t>(kMostSplits), units, resident * 7 / 8 / items})));
@@ -1214,6 +1220,8 @@ struct PagedPlan {
     // columns: 44.3 us, with one tile 51.6; in a cluster, of up to 1000, 12.7 and 11.5). Heads of 64 have registers for
     // four, but up to 3001 keys took 21.2 us with four and 20.3 with two (of up to 12000: 38.5 and 43.7)
     if (cols > 8 && clusters(2)) return;
+    // 200 sequences (the shorter ones from a quarter of the longest on) of up to 500, 1024 and 1600 keys, 8 key heads of 128:
+    // warps' shares 35.5, 56.1 and 77.3 us, CTAs' 42.5, 56.7 and 76.3; 100 of up to 4700: 110.2 and 105.6
     mode = most_keys > 1024 || items < resident ? PAGED_TOGETHER : PAGED_WARPS;
     splits = 0;
     ctas = std::max<int64_t>(1, std::min(resident, items * ((most_keys + kPaTile - 1) / kPaTile)));

@@ -245,7 +245,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                  factor: float = 1.0, interleaved: bool = False, k_norm: Optional[torch.Tensor] = None,
                  q: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> torch.Tensor:
-    """Keys and values into a paged cache (layer.cache_append); without q an empty tensor."""
+    """Keys and values into a paged cache (layer.cache_append); without q an empty tensor. An op cannot see whether a call
+    is recorded, so that keys and values that require grad, which the function refuses, are stored without a history."""
     with torch.no_grad():  # below autograd, whoever called
         out = layer.cache_append(k, v, k_cache, v_cache, k_scales, v_scales, table, starts, cu_seqlens, inv_freq, factor,
                                  interleaved, k_norm, q, q_norm, eps)
